@@ -33,8 +33,10 @@ typedef enum sb_status {
 /* Arithmetic classes of the GEMM inputs.  SB_F32 = fp32 storage, fp32 FMA
  * math (1e-5 class).  SB_TF32 = fp32 storage, TF32 tensor-core multiply, the
  * reference's own arithmetic (corecuda/wmma.spi:20,78-82).  SB_BF16 / SB_F16
- * = 16-bit storage.  Accumulation is always fp32. */
-typedef enum sb_dtype { SB_F32 = 0, SB_TF32 = 1, SB_BF16 = 2, SB_F16 = 3, SB_I32 = 4, SB_U8 = 5 } sb_dtype;
+ * = 16-bit storage.  Accumulation is always fp32.  SB_I64 names 64-bit token
+ * indices, SB_E4M3 8-bit floating-point codes (1 sign, 4 exponent and 3 mantissa
+ * bits, no infinities) that carry a scale per block. */
+typedef enum sb_dtype { SB_F32 = 0, SB_TF32 = 1, SB_BF16 = 2, SB_F16 = 3, SB_I32 = 4, SB_U8 = 5, SB_I64 = 6, SB_E4M3 = 7 } sb_dtype;
 
 /* Epilogue flags, OR-ed.  Order of application on one output row:
  *   v = alpha * acc + beta * C_old ; v += bias[col] ; v = relu(v) ;
@@ -455,6 +457,82 @@ int sb_mlp_train_step(int n_layers, const int* sizes, int batch, int in_dtype, c
                       const uint8_t* mask,
                       const float* target, float* probs, float* grads, int with_bias, float lr,
                       void* scratch, size_t scratch_bytes, float* loss, void* stream);
+
+/* ---- operators of nets that read tokens -------------------------------------
+ * A state that is a sequence of small integers (cards, actions, history) enters the net through an embedding table instead
+ * of a one-hot group; layer normalisation, AdamW and 8-bit products surround the same dense layers.  No counterparts in
+ * the reference.  Matrices are row-major with the element pitches ld*, which may exceed the columns; pointers need the
+ * alignment of their elements (SB_ERR_MISALIGNED), wider accesses are taken where pointers and pitches allow them.
+ * Outputs may not overlap inputs unless an entry says so. */
+
+/* out[i, :] = scale * table[tokens[i], :] for n tokens (index_dtype SB_I32 or SB_I64); a token outside [0, vocab) is no
+ * token and gives zeros, as an out-of-range field does in sb_encode_states.  table and out: SB_F32, SB_BF16 or SB_F16 each;
+ * the product is fp32, rounded once. */
+int sb_embedding(const void* tokens, int index_dtype, long long n, const void* table, long long ld_table, int table_dtype,
+                 int vocab, int dim, float scale, void* out, long long ld_out, int out_dtype, void* stream);
+/* Its gradient: dtable[v, :] = scale * (sum over i with tokens[i] == v of dout[i, :]), fp32 [vocab, dim], rows without a
+ * token zero; accumulate != 0 adds to dtable instead.  The sums are fp32 in the order of the positions (joined from
+ * pieces of equal length) and without atomics: equal inputs give equal bits.  dout: SB_F32, SB_BF16 or SB_F16.
+ * workspace: 16-byte aligned, at least sb_embedding_grad_workspace_bytes.  At most 2^30 tokens and rows. */
+int sb_embedding_grad_workspace_bytes(long long n, int vocab, int dim, size_t* bytes);
+int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const void* dout, long long ld_dout, int dout_dtype,
+                      float scale, float* dtable, long long ld_dtable, int vocab, int dim, int accumulate, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* y = (x - mean) * rstd * weight + bias over rows of `cols` values: mean and rstd = 1 / sqrt(var + eps) of each row (var
+ * divides by cols), fp32, left in mean / rstd [rows] where those are not NULL.  x and y: SB_F32, SB_BF16 or SB_F16, the
+ * same for both; y may be x.  weight, bias: fp32 [cols], NULL for ones / zeros. */
+int sb_layer_norm(const void* x, long long ldx, void* y, long long ldy, const float* weight, const float* bias, float eps,
+                  float* mean, float* rstd, long long rows, int cols, int dtype, void* stream);
+/* Its gradient from the same x, mean and rstd: dx (may be NULL) in the storage type, dweight and dbias (may be NULL) fp32
+ * [cols], added to their old values with accumulate != 0.  Column sums are taken in a fixed order without atomics.
+ * workspace: at least sb_layer_norm_grad_workspace_bytes where dweight or dbias is wanted. */
+int sb_layer_norm_grad_workspace_bytes(long long rows, int cols, size_t* bytes);
+int sb_layer_norm_grad(const void* dy, long long lddy, const void* x, long long ldx, const float* mean, const float* rstd,
+                       const float* weight, void* dx, long long lddx, float* dweight, float* dbias, int accumulate,
+                       long long rows, int cols, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step over many tensors:
+ *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * params fp32, grads of grad_dtype (SB_F32, SB_BF16, SB_F16), and where `copy` is not NULL the new parameters rounded to
+ * copy_dtype (SB_BF16, SB_F16, SB_TF32, SB_F32).  state_dtype SB_F32: exp_avg = m and exp_avg_sq = v, fp32 [n].  SB_E4M3:
+ * exp_avg = codes of m, exp_avg_sq = codes of sqrt(v), uint8 [n] each, value = code * scale, one fp32 scale per 256
+ * elements (exp_avg_scale, exp_avg_sq_scale: [ceil(n / 256)]; zero codes and any finite scale are a fresh state).  Codes are
+ * rounded with noise that is a hash of (element index, seed): give another seed every step.  Tensors may have any
+ * size and alignment; those of one call may not overlap.  `tensors` and `hyper` are HOST memory, read before the call
+ * returns; nothing is kept.  One launch per 400 tensors. */
+typedef struct sb_adamw_tensor {
+  float* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;          /* SB_E4M3 only */
+  float* exp_avg_sq_scale;       /* SB_E4M3 only */
+  void* copy;                    /* NULL: none */
+  long long n;
+} sb_adamw_tensor;
+typedef struct sb_adamw_hyper {
+  double lr, beta1, beta2, eps, weight_decay, grad_scale;
+  long long step;                /* counted from 1 */
+  uint32_t seed;
+} sb_adamw_hyper;
+int sb_adamw_step(int n_tensors, const sb_adamw_tensor* tensors, int state_dtype, int grad_dtype, int copy_dtype,
+                  const sb_adamw_hyper* hyper, void* stream);
+
+/* E4M3 codes of x [rows, cols] (SB_F32, SB_BF16, SB_F16) with a scale per block of block_rows x 128, block_rows 1
+ * (activations) or 128 (weights): scale = largest magnitude / 448 (of at least 2^-100), code = x * (448 / largest) rounded to
+ * nearest even.  A block that holds a NaN or an infinity has no finite values.  scales: for block_rows 1 fp32
+ * [ceil(cols / 128), rows] (the scales that a tile of rows needs together are neighbours), for 128 fp32
+ * [ceil(rows / 128), ceil(cols / 128)]. */
+int sb_quantize_fp8(const void* x, long long ldx, int dtype, long long rows, int cols, int block_rows, uint8_t* codes,
+                    long long ldc, float* scales, void* stream);
+/* C[m, n] = sum over blocks b of K of a_scales[b, m] * w_scales[n / 128, b] * (A[m, k in b] . W[n, k in b]): a dense layer in
+ * 8 bits, A [M, K] and W [N, K] codes with the scales that sb_quantize_fp8 leaves for block_rows 1 and 128.  fp32
+ * accumulation; C in SB_F32, SB_BF16 or SB_F16; epilogue: SB_EPI_BIAS (fp32 [N]), SB_EPI_RELU. */
+int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const uint8_t* w, long long ldw,
+                  const float* w_scales, void* c, long long ldc, int m, int n, int k, int out_dtype, int epilogue,
+                  const float* bias, void* stream);
 
 /* ---- data-parallel update over peer memory ---------------------------------
  * No reference counterpart (the reference is single-device, corecuda/base.spi:7);

@@ -9,4 +9,8 @@
 #include "mlp.cu"
 #include "mlp_fused.cu"
 #include "dp.cu"
+#include "embedding.cu"
+#include "layer_norm.cu"
+#include "adamw.cu"
+#include "gemm_fp8.cu"
 #include "selftest.cu"

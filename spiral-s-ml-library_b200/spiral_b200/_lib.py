@@ -17,8 +17,8 @@ STATUS_NAMES = {
 }
 
 # sb_dtype
-F32, TF32, BF16, F16, I32, U8 = 0, 1, 2, 3, 4, 5
-DTYPE_CODES = {"f32": F32, "tf32": TF32, "bf16": BF16, "f16": F16, "i32": I32, "u8": U8}
+F32, TF32, BF16, F16, I32, U8, I64, E4M3 = 0, 1, 2, 3, 4, 5, 6, 7
+DTYPE_CODES = {"f32": F32, "tf32": TF32, "bf16": BF16, "f16": F16, "i32": I32, "u8": U8, "i64": I64, "e4m3": E4M3}
 
 # epilogue flags
 EPI_NONE, EPI_BIAS, EPI_RELU, EPI_RELU_GRAD = 0, 1, 2, 4
@@ -60,6 +60,22 @@ class DecideArgs(ctypes.Structure):
                 ("sampling_prob_selected", c_void_p), ("sampling_prob_ensemble", c_void_p),
                 ("tile_counters", c_void_p)]
 
+
+
+class AdamwTensor(ctypes.Structure):
+    """sb_adamw_tensor of include/spiral_b200.h."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p),
+                ("exp_avg_scale", c_void_p), ("exp_avg_sq_scale", c_void_p), ("copy", c_void_p), ("n", ctypes.c_longlong)]
+
+
+class AdamwHyper(ctypes.Structure):
+    """sb_adamw_hyper of include/spiral_b200.h."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("grad_scale", ctypes.c_double), ("step", ctypes.c_longlong),
+                ("seed", ctypes.c_uint32)]
+
+
+_L = ctypes.c_longlong
 
 # name -> (restype, argtypes); every symbol include/spiral_b200.h declares.
 SIGNATURES = {
@@ -138,6 +154,15 @@ SIGNATURES = {
     "sb_mlp_backward": (_I, [_I, _IP, _I, _F, _I, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _P, _Z, _P, _P]),
     "sb_mlp_backward_dy_offset": (_I, [_I, _IP, _I, _I, _I, POINTER(c_size_t)]),
     "sb_mlp_backward_range": (_I, [_I, _IP, _I, _F, _I, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _P, _Z, _P, _I, _I, _P]),
+    "sb_embedding": (_I, [_P, _I, _L, _P, _L, _I, _I, _I, _F, _P, _L, _I, _P]),
+    "sb_embedding_grad_workspace_bytes": (_I, [_L, _I, _I, POINTER(c_size_t)]),
+    "sb_embedding_grad": (_I, [_P, _I, _L, _P, _L, _I, _F, _P, _L, _I, _I, _I, _P, _Z, _P]),
+    "sb_layer_norm": (_I, [_P, _L, _P, _L, _P, _P, _F, _P, _P, _L, _I, _I, _P]),
+    "sb_layer_norm_grad_workspace_bytes": (_I, [_L, _I, POINTER(c_size_t)]),
+    "sb_layer_norm_grad": (_I, [_P, _L, _P, _L, _P, _P, _P, _P, _L, _P, _P, _I, _L, _I, _I, _P, _Z, _P]),
+    "sb_adamw_step": (_I, [_I, POINTER(AdamwTensor), _I, _I, _I, POINTER(AdamwHyper), _P]),
+    "sb_quantize_fp8": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _P]),
+    "sb_matmul_fp8": (_I, [_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P]),
     "sb_sgd_update": (_I, [_P, _P, _P, ctypes.c_longlong, _F, _I, _P]),
     "sb_mlp_train_step": (_I, [_I, _IP, _I, _I, _P, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _F, _P, _Z, _P, _P]),
 }

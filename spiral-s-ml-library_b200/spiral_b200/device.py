@@ -14,9 +14,9 @@ import numpy as np
 from . import _lib
 from . import dtypes
 
-_ITEMSIZE = {"f32": 4, "tf32": 4, "bf16": 2, "f16": 2, "i32": 4, "u8": 1}
+_ITEMSIZE = {"f32": 4, "tf32": 4, "bf16": 2, "f16": 2, "i32": 4, "u8": 1, "i64": 8, "e4m3": 1}
 _NP_STORAGE = {"f32": np.float32, "tf32": np.float32, "bf16": np.uint16, "f16": np.float16,
-               "i32": np.int32, "u8": np.uint8}
+               "i32": np.int32, "u8": np.uint8, "i64": np.int64, "e4m3": np.uint8}
 
 
 def device_count():
@@ -85,7 +85,7 @@ class DeviceArray:
         """Uploads a host array; fp32 data is rounded to `dtype` on the host first."""
         array = np.asarray(array)
         if dtype is None:
-            dtype = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int32): "i32",
+            dtype = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int32): "i32", np.dtype(np.int64): "i64",
                      np.dtype(np.uint8): "u8", np.dtype(np.bool_): "u8",
                      np.dtype(np.float64): "f32"}.get(array.dtype)
             if dtype is None:
@@ -105,6 +105,9 @@ class DeviceArray:
             return np.ascontiguousarray(dtypes.f32_to_bf16_bits(np.asarray(array, np.float32)))
         if self.dtype == "tf32":
             return np.ascontiguousarray(dtypes.round_tf32(np.asarray(array, np.float32)))
+        if self.dtype == "e4m3":             # uint8 arrays hold codes, others values
+            array = np.asarray(array)
+            return np.ascontiguousarray(array if array.dtype == np.uint8 else dtypes.f32_to_e4m3_bits(array))
         return np.ascontiguousarray(np.asarray(array).astype(_NP_STORAGE[self.dtype], copy=False))
 
     def upload(self, array, stream=None):
@@ -121,7 +124,7 @@ class DeviceArray:
 
     # -- readback ----------------------------------------------------------
     def numpy(self, stream=None):
-        """Downloads; 16-bit float storage comes back widened to fp32."""
+        """Downloads; 8- and 16-bit float storage comes back widened to fp32."""
         host = np.empty(self.shape, dtype=_NP_STORAGE[self.dtype])
         _lib.call("sb_memcpy_d2h", host.ctypes.data, self.ptr, host.nbytes, stream_ptr(stream))
         # Synchronises, and raises SpiralError(SB_ERR_DEVICE_TIMEOUT) when a kernel gave up a bounded
@@ -131,6 +134,8 @@ class DeviceArray:
             return dtypes.bf16_bits_to_f32(host).reshape(self.shape)
         if self.dtype == "f16":
             return host.astype(np.float32)
+        if self.dtype == "e4m3":
+            return dtypes.e4m3_bits_to_f32(host).reshape(self.shape)
         return host
 
     def view(self, shape, dtype=None, offset_bytes=0):
@@ -186,10 +191,70 @@ def dtype_tag(obj):
         return _TAG_OF[dtype]
     except (KeyError, TypeError):
         name = str(dtype).replace("torch.", "")
-        tag = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "int32": "i32", "uint8": "u8", "bool": "u8"}.get(name, None)
+        tag = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "int32": "i32", "uint8": "u8", "bool": "u8",
+               "int64": "i64", "float8_e4m3fn": "e4m3"}.get(name, None)
         if tag is not None and type(dtype).__hash__ is not None:
             _TAG_OF[dtype] = tag                   # keyed by the dtype (torch, numpy, ...), of which there are a handful
         return tag
+
+
+def matrix_of(x, what):
+    """(rows, cols, pitch in elements) of a row-major device matrix: the last dimension is contiguous, the others make the
+    rows.  A pitch beyond the columns needs a two-dimensional array that knows its strides (torch, CuPy)."""
+    shape = x.shape
+    cols = shape[-1] if len(shape) else 1
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    if isinstance(x, DeviceArray):
+        return rows, cols, cols
+    strides = None
+    stride = getattr(x, "stride", None)
+    if callable(stride):
+        if len(shape) != 2 and x.is_contiguous():
+            return rows, cols, cols
+        strides = stride()
+    elif getattr(x, "strides", None) is not None:
+        strides = tuple(s // x.itemsize for s in x.strides)
+    if strides is None or rows == 0 or cols == 0 or not len(shape):
+        return rows, cols, cols
+    if cols > 1 and strides[-1] != 1:
+        raise ValueError("%s: the last dimension must be contiguous" % what)
+    if rows == 1:
+        return rows, cols, cols
+    if len(shape) == 2:
+        if strides[0] < cols:
+            raise ValueError("%s: rows may not overlap" % what)
+        return rows, cols, strides[0]
+    expect = cols
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n > 1 and s != expect:
+            raise ValueError("%s: an array of more than two dimensions must be contiguous" % what)
+        expect *= n
+    return rows, cols, cols
+
+
+def flat_size(x, what):
+    """Elements of a contiguous device array."""
+    rows, cols, pitch = matrix_of(x, what)
+    if rows > 1 and pitch != cols:
+        raise ValueError("%s must be contiguous" % what)
+    return rows * cols
+
+
+_WORKSPACES = {}
+
+
+def stream_workspace(nbytes, stream):
+    """Device memory for one call's intermediate results: kept per stream, grown on demand (the C ABI itself allocates
+    nothing), so calls on one stream share it in their order and calls on different streams never do."""
+    key = stream_ptr(stream) or 0
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.nbytes < nbytes:
+        if ws is not None:
+            _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
+        ws = _WORKSPACES[key] = DeviceArray((max(int(nbytes), 1 << 16),), "u8")
+    return ws
 
 
 def stream_ptr(stream):

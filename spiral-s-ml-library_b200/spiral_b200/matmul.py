@@ -7,7 +7,7 @@ updated in place: ``c <- alpha * op(a) @ op(b) + beta * c``.
 import ctypes
 
 from . import _lib
-from .device import DeviceArray, device_ptr, dtype_tag, stream_ptr
+from .device import DeviceArray, device_ptr, dtype_tag, flat_size, matrix_of, stream_ptr
 
 EPILOGUE_FLAGS = {
     "bias": _lib.EPI_BIAS, "relu": _lib.EPI_RELU, "relu_grad": _lib.EPI_RELU_GRAD,
@@ -157,3 +157,64 @@ def matmul_plan(a_trans, b_trans, m, n, k, in_dtype="tf32", epilogue=()):
     _lib.call("sb_matmul_plan", int(bool(a_trans)), int(bool(b_trans)), int(m), int(n), int(k),
               _lib.DTYPE_CODES[in_dtype], epi, plan)
     return dict(zip(("block_m", "block_n", "block_k", "stages", "grid"), list(plan)))
+
+
+_FP8_FLOATS = {"f32": _lib.F32, "tf32": _lib.F32, "bf16": _lib.BF16, "f16": _lib.F16}
+_FP8_EPILOGUES = {(): 0, ("bias",): _lib.EPI_BIAS, ("relu",): _lib.EPI_RELU, ("bias", "relu"): _lib.EPI_BIAS | _lib.EPI_RELU}
+
+
+def _fp8_scales(x, need, what):
+    if dtype_tag(x) != "f32" or flat_size(x, what) != need:
+        raise ValueError("%s must be %d contiguous fp32 values" % (what, need))
+    return device_ptr(x)
+
+
+def _fp8_codes(x, what):
+    if dtype_tag(x) not in ("e4m3", "u8"):
+        raise TypeError("%s must hold e4m3 codes, not %s" % (what, dtype_tag(x)))
+    return device_ptr(x)
+
+
+def quantize_fp8(x, codes, scales, block_rows=1, stream=None):
+    """E4M3 ``codes`` of the matrix ``x`` (fp32, bf16, f16) with a scale per block of ``block_rows`` x 128: scale = largest
+    magnitude / 448.  ``block_rows`` 1 is for activations, ``scales`` fp32 [ceil(cols / 128), rows]; 128 is for weights,
+    ``scales`` fp32 [ceil(rows / 128), ceil(cols / 128)].  Returns (codes, scales)."""
+    rows, cols, ldx = matrix_of(x, "x")
+    crows, ccols, ldc = matrix_of(codes, "codes")
+    if (crows, ccols) != (rows, cols):
+        raise ValueError("quantize_fp8: codes are %dx%d, x is %dx%d" % (crows, ccols, rows, cols))
+    if block_rows not in (1, 128):
+        raise ValueError("quantize_fp8: blocks are 1 x 128 or 128 x 128")
+    tag = dtype_tag(x)
+    if tag not in _FP8_FLOATS:
+        raise TypeError("quantize_fp8: x must hold f32, bf16 or f16, not %s" % tag)
+    across = -(-cols // 128)
+    _lib.call("sb_quantize_fp8", device_ptr(x), ldx, _FP8_FLOATS[tag], rows, cols, block_rows, _fp8_codes(codes, "codes"), ldc,
+              _fp8_scales(scales, across * (rows if block_rows == 1 else -(-rows // 128)), "scales"), stream_ptr(stream))
+    return codes, scales
+
+
+def matmul_fp8(a, a_scales, b, b_scales, c, epilogue=(), bias=None, stream=None):
+    """``c <- a @ b^T`` of E4M3 codes with their scales, fp32 accumulation: a dense layer in 8 bits.
+
+    ``a`` [m, k] with ``a_scales`` [ceil(k / 128), m] (``quantize_fp8`` with block_rows 1), ``b`` [n, k] with ``b_scales``
+    [ceil(n / 128), ceil(k / 128)] (block_rows 128), ``c`` [m, n] in fp32, bf16 or f16; ``epilogue``: "bias" (fp32 [n]),
+    "relu".  Rows may have a pitch; multiples of 16 run on the tensor cores."""
+    m, k, lda = matrix_of(a, "a")
+    n, kb, ldb = matrix_of(b, "b")
+    cm, cn, ldc = matrix_of(c, "c")
+    if kb != k or cm != m or cn != n:
+        raise ValueError("shape mismatch: a is %dx%d, b^T is %dx%d, c is %dx%d" % (m, k, kb, n, cm, cn))
+    tag = dtype_tag(c)
+    if tag not in _FP8_FLOATS:
+        raise TypeError("matmul_fp8: c must hold f32, bf16 or f16, not %s" % tag)
+    epi = _FP8_EPILOGUES.get(tuple(epilogue))
+    if epi is None:
+        raise ValueError("matmul_fp8: the epilogue is made of bias and relu, got %r" % (epilogue,))
+    if epi & _lib.EPI_BIAS and (bias is None or dtype_tag(bias) != "f32" or flat_size(bias, "bias") != n):
+        raise ValueError("matmul_fp8: bias must be %d fp32 values" % n)
+    across = -(-k // 128)
+    _lib.call("sb_matmul_fp8", _fp8_codes(a, "a"), lda, _fp8_scales(a_scales, across * m, "a_scales"), _fp8_codes(b, "b"), ldb,
+              _fp8_scales(b_scales, -(-n // 128) * across, "b_scales"), device_ptr(c), ldc, m, n, k, _FP8_FLOATS[tag], epi,
+              device_ptr(bias), stream_ptr(stream))
+    return c
