@@ -8,6 +8,8 @@
 #include "common.cuh"
 #include "vector_io.cuh"
 
+#include <math.h>
+
 namespace {
 
 constexpr int F8_BLOCK = 128;
@@ -208,36 +210,47 @@ __global__ void __launch_bounds__(256) gemm_fp8_simple_kernel(F8Args g) {
 }
 
 
-// The tensor-core form.  A tile of 128 x BN values per CTA, or of 256 x 256 per pair of CTAs (cta_group::2: each loads its
-// 128 rows of A and half of the rows of W); a stage of the ring is one 128-byte block of K of both operands, brought by TMA.
-// The scales change with every block of K, so every block's four MMAs start a fresh accumulator in TMEM, and eight warps
-// add it, times its two scales, to sums in registers (packed fp32 multiply-adds) while the MMAs of the next block run into
-// another accumulator.  A thread owns one row and half of the columns, which lie in one 128-block of N: the product of the
-// scales is one number per thread and block.
+// The tensor-core form: persistent CTAs, a tile of 128 x BN values each.  A stage of the ring is one 128-byte block of K of
+// both operands, brought by TMA.  The scales change with every block of K, so every block's MMAs start a fresh accumulator
+// in TMEM, and eight warps add it, times its two scales, to sums in registers (packed fp32 multiply-adds) while the MMAs of
+// the next block run into another accumulator.  A thread owns one row and half of the columns, which lie in one 128-block
+// of N: the product of the scales is one number per thread and block.  At BN = 256 the two halves of the columns are
+// products of their own with two accumulators each, so that the adding warps of a half wait for their own MMAs only.
+//
+// Bound by the operands' way from L2 into shared memory: at BN = 256 a block is 48 KB in 0.6 us per SM, 12 TB/s over the chip
+// (8192^3: 529 us, 2077 TFLOP/s, the same without the multiply-adds).  Pairs of CTAs (cta_group::2, 256 x 256) load a third
+// less and were slower, 320 us against 271 for 16384 x 4096 x 4096: the round trip from the MMAs over both CTAs' adding warps
+// back to the issuer is longer than two accumulators cover.  Four stages instead of three: 288 us; sixteen adding warps, whose
+// 112 registers spill: 327 us (in pairs).
 constexpr int F8_STAGES_MAX = 12;
-constexpr int F8_BUFFERS_MAX = 4;
 constexpr int F8_WARPS = 8;                                  // that add
-constexpr int F8_FIRST = 4;                                   // the first of them: warp 0 loads, warp 1 issues, a warpgroup adds as a whole
+constexpr int F8_FIRST = 4;                                  // the first of them: warp 0 loads, warp 1 issues
 constexpr int F8_THREADS = 32 * (F8_FIRST + F8_WARPS);
 constexpr int F8_SMEM = 225 * 1024;
 constexpr uint32_t F8_BOX = 4096;                            // a warp's staging box: 32 rows x 128 bytes
+constexpr int F8_AHEAD = 4;                                  // blocks whose scales are on their way or in use
+constexpr uint32_t F8_SCALES = F8_WARPS * 32 * 8;            // bytes of one block's: a pair per adding thread
 
-template <bool PAIR>
 __device__ __forceinline__ void f8_mma(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
                                        uint32_t accumulate, bool issue) {
-#define SB_F8_ASM(GROUP)                                                                                               \
-  "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"             \
-  "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t@q tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4"              \
-  " [%0], da, db, %5, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate),      \
-  "r"((uint32_t)issue) : "memory"
-  if (PAIR) asm volatile(SB_F8_ASM("2"));
-  else asm volatile(SB_F8_ASM("1"));
-#undef SB_F8_ASM
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"((uint32_t)issue) : "memory");
 }
+// One block of K: four MMAs of 32 elements into a fresh accumulator.
+__device__ __forceinline__ void f8_block(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                         bool issue) {
+  f8_mma(d, a_lo, a_hi, b_lo, b_hi, idesc, 0u, issue);
+  f8_mma(d, a_lo + 2u, a_hi, b_lo + 2u, b_hi, idesc, 1u, issue);
+  f8_mma(d, a_lo + 4u, a_hi, b_lo + 4u, b_hi, idesc, 1u, issue);
+  f8_mma(d, a_lo + 6u, a_hi, b_lo + 6u, b_hi, idesc, 1u, issue);
+}
+// kind::f8f6f4, E4M3 x E4M3 (formats 0), fp32 accumulator, M = 128; the fields are those of sb_umma_idesc.
+__host__ __device__ constexpr uint32_t f8_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24); }
 
 struct F8Plan {
-  int pair, block_n, stages, tiles_m, tiles_n, tiles;
-  uint32_t idesc;
+  int stages, tiles_m, tiles_n, tiles;
   int tma_store;
 };
 
@@ -253,18 +266,20 @@ __device__ __forceinline__ void f8_tile(const F8Plan& p, int tile, int& m_blk, i
 
 __shared__ int g_f8_abort;
 
-// 32 columns of an accumulator added to the sums: sum += scale * part.
-__device__ __forceinline__ void f8_add32(unsigned long long* sum, const uint32_t* part, unsigned long long scale) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    fma_f32x2(sum[j], pack_f32x2(__uint_as_float(part[2 * j]), __uint_as_float(part[2 * j + 1])), scale);
+__device__ __forceinline__ void f8_copy4(uint32_t dst, const float* src, uint32_t bytes) {   // bytes 0: a zero is written
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-
-// Arrival on another CTA's barrier without a release: what it announces, that an accumulator has been read, is ordered by
-// the wait for the loads and the tcgen05 fence before it.  (With a release it waits for the thread's earlier memory
-// operations once per block of K: 16384 x 4096 x 4096 took 516 us.)
-__device__ __forceinline__ void f8_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+__device__ __forceinline__ float f8_lds(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+// N columns of an accumulator added to the sums: sum += scale * part.
+template <int N>
+__device__ __forceinline__ void f8_add(unsigned long long* sum, const uint32_t* part, unsigned long long scale) {
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j)
+    fma_f32x2(sum[j], pack_f32x2(__uint_as_float(part[2 * j]), __uint_as_float(part[2 * j + 1])), scale);
 }
 
 // Finished values of this warp's 32 rows and COLS columns -> C, a box of 32 rows x 128 bytes at a time (64 bytes where the
@@ -336,30 +351,29 @@ __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tma
   }
 }
 
-template <bool PAIR, int BN>
+template <int BN>
 __global__ void __launch_bounds__(F8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                 const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ F8Args g, const __grid_constant__ F8Plan p) {
-  constexpr int BUFFERS = 512 / BN < F8_BUFFERS_MAX ? 512 / BN : F8_BUFFERS_MAX;
+  constexpr int PARTS = BN == 256 ? 2 : 1;                   // products with accumulators of their own
+  constexpr int PART_N = BN / PARTS;
+  constexpr int DEPTH = 4 / PARTS;                           // accumulators of each
   constexpr int COLS = BN / 2;                               // of a thread
-  constexpr int TILE_M = PAIR ? 256 : 128;
-  constexpr uint32_t A_BYTES = 128 * 128, W_ROWS = PAIR ? BN / 2 : BN, W_BYTES = W_ROWS * 128, STAGE = A_BYTES + W_BYTES;
+  constexpr uint32_t TMEM_COLS = PARTS * DEPTH * PART_N;
+  constexpr uint32_t A_BYTES = 128 * F8_BLOCK, W_BYTES = BN * F8_BLOCK, STAGE = A_BYTES + W_BYTES;
   extern __shared__ uint8_t f8_smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[F8_STAGES_MAX], bar_empty[F8_STAGES_MAX];
-  __shared__ __align__(8) uint64_t bar_acc_full[F8_BUFFERS_MAX], bar_acc_empty[F8_BUFFERS_MAX];
+  __shared__ __align__(8) uint64_t bar_full[F8_STAGES_MAX], bar_empty[F8_STAGES_MAX], bar_acc_full[4], bar_acc_empty[4];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
-  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
   const uint32_t stage0 = (smem_u32(f8_smem_raw) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
       mbar_init(smem_u32(&bar_full[i]), 1);
       mbar_init(smem_u32(&bar_empty[i]), 1);
     }
-    for (int i = 0; i < BUFFERS; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(smem_u32(&bar_acc_full[i]), 1);
-      mbar_init(smem_u32(&bar_acc_empty[i]), PAIR ? 2 * F8_WARPS : F8_WARPS);
+      mbar_init(smem_u32(&bar_acc_empty[i]), F8_WARPS / PARTS);
     }
     g_f8_abort = 0;
     fence_mbar_init();
@@ -367,16 +381,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tma_prefetch_desc(&tmap_w);
   }
   if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(smem_u32(&tmem_slot), BUFFERS * BN);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(smem_u32(&tmem_slot), BUFFERS * BN);
-      tmem_relinquish();
-    }
+    tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tmem_relinquish();
   }
   tc_fence_before_sync();
-  if (PAIR) cluster_sync_all(); else __syncthreads();
+  __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &g_f8_abort;
@@ -389,27 +398,19 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const uint32_t full_local = smem_u32(&bar_full[0]), full0 = PAIR ? map_to_cta(full_local, 0u) : full_local;
-    const uint32_t empty0 = smem_u32(&bar_empty[0]);
-    for (int tile = worker; ok && tile < p.tiles; tile += workers) {
+    const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       int m_blk, n_blk;
       f8_tile(p, tile, m_blk, n_blk);
-      const int m0 = m_blk * TILE_M + (int)rank * 128, n0 = n_blk * BN + (int)rank * (int)W_ROWS;
       for (int kb = 0; kb < g.k_blocks; ++kb) {
         if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) {
           ok = false;
           break;
         }
-        // In a pair the leader arms its barrier with the bytes of both CTAs.
-        if (one && rank == 0u) mbar_arrive_expect_tx(full_local + 8u * (uint32_t)stage, PAIR ? 2u * STAGE : STAGE);
         const uint32_t at = stage0 + (uint32_t)stage * STAGE, full = full0 + 8u * (uint32_t)stage;
-        if (PAIR) {
-          tma_load_2d_pair(at, &tmap_a, kb * F8_BLOCK, m0, full, one);
-          tma_load_2d_pair(at + A_BYTES, &tmap_w, kb * F8_BLOCK, n0, full, one);
-        } else {
-          tma_load_2d(at, &tmap_a, kb * F8_BLOCK, m0, full, one);
-          tma_load_2d(at + A_BYTES, &tmap_w, kb * F8_BLOCK, n0, full, one);
-        }
+        if (one) mbar_arrive_expect_tx(full, STAGE);
+        tma_load_2d(at, &tmap_a, kb * F8_BLOCK, m_blk * 128, full, one);
+        tma_load_2d(at + A_BYTES, &tmap_w, kb * F8_BLOCK, n_blk * BN, full, one);
         if (++stage == p.stages) {
           stage = 0;
           phase ^= 1u;
@@ -417,117 +418,106 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       }
     }
   } else if (warp == 1) {
-    if (rank == 0u) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      const uint64_t a_desc = umma_smem_desc(stage0, 16u, 1024u, 2u), w_desc = umma_smem_desc(stage0 + A_BYTES, 16u, 1024u, 2u);
-      const uint32_t a_hi = (uint32_t)(a_desc >> 32), w_hi = (uint32_t)(w_desc >> 32);
-      const uint32_t a_lo0 = (uint32_t)a_desc, w_lo0 = (uint32_t)w_desc;
-      const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
-      const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
-      uint32_t a_lo = a_lo0, w_lo = w_lo0;
-      for (int tile = worker; ok && tile < p.tiles; tile += workers) {
-        for (int kb = 0; kb < g.k_blocks; ++kb) {
-          if (!mbar_wait_warp(acc_empty0 + 8u * (uint32_t)buf, acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY) ||
-              !mbar_wait_warp(full0 + 8u * (uint32_t)stage, phase, abortp, SB_SITE_MMA_FULL)) {
-            ok = false;
-            break;
-          }
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    const uint64_t a_desc = umma_smem_desc(stage0, 16u, 1024u, 2u), w_desc = umma_smem_desc(stage0 + A_BYTES, 16u, 1024u, 2u);
+    const uint32_t a_hi = (uint32_t)(a_desc >> 32), w_hi = (uint32_t)(w_desc >> 32);
+    const uint32_t a_lo0 = (uint32_t)a_desc, w_lo0 = (uint32_t)w_desc;
+    const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+    const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
+    uint32_t a_lo = a_lo0, w_lo = w_lo0;
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+      for (int kb = 0; ok && kb < g.k_blocks; ++kb) {
+        ok = mbar_wait_warp(full0 + 8u * (uint32_t)stage, phase, abortp, SB_SITE_MMA_FULL);
+#pragma unroll
+        for (int h = 0; h < PARTS; ++h) {
+          const uint32_t at = (uint32_t)(PARTS * acc + h);
+          if (ok) ok = mbar_wait_warp(acc_empty0 + 8u * at, acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY);
+          if (!ok) break;
           tc_fence_after_sync();
-          const uint32_t d = tmem + (uint32_t)(buf * BN);
-          f8_mma<PAIR>(d, a_lo, a_hi, w_lo, w_hi, p.idesc, 0u, one);
-          f8_mma<PAIR>(d, a_lo + 2u, a_hi, w_lo + 2u, w_hi, p.idesc, 1u, one);
-          f8_mma<PAIR>(d, a_lo + 4u, a_hi, w_lo + 4u, w_hi, p.idesc, 1u, one);
-          f8_mma<PAIR>(d, a_lo + 6u, a_hi, w_lo + 6u, w_hi, p.idesc, 1u, one);
-          if (PAIR) {
-            tc_commit_pair(empty0 + 8u * (uint32_t)stage, (uint16_t)3, one);
-            tc_commit_pair(acc_full0 + 8u * (uint32_t)buf, (uint16_t)3, one);
-          } else {
-            tc_commit(empty0 + 8u * (uint32_t)stage, one);
-            tc_commit(acc_full0 + 8u * (uint32_t)buf, one);
-          }
-          a_lo += STAGE >> 4;
-          w_lo += STAGE >> 4;
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1u;
-            a_lo = a_lo0;
-            w_lo = w_lo0;
-          }
-          if (++buf == BUFFERS) {
-            buf = 0;
-            acc_phase ^= 1u;
-          }
+          f8_block(tmem + at * PART_N, a_lo, a_hi, w_lo + (uint32_t)h * (W_BYTES / PARTS >> 4), w_hi, f8_idesc(PART_N), one);
+          tc_commit(acc_full0 + 8u * at, one);
+        }
+        if (!ok) break;
+        tc_commit(empty0 + 8u * (uint32_t)stage, one);
+        a_lo += STAGE >> 4;
+        w_lo += STAGE >> 4;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+          a_lo = a_lo0;
+          w_lo = w_lo0;
+        }
+        if (++acc == DEPTH) {
+          acc = 0;
+          acc_phase ^= 1u;
         }
       }
     }
   } else if (warp >= F8_FIRST) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quad = warp & 3, half = (warp - F8_FIRST) >> 2;   // a warp reads the TMEM lanes of its number modulo 4
-    const uint32_t box = stage0 + (uint32_t)p.stages * STAGE + (uint32_t)(warp - F8_FIRST) * F8_BOX;
-    const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]);
-    const uint32_t acc_empty_local = smem_u32(&bar_acc_empty[0]), acc_empty0 = PAIR ? map_to_cta(acc_empty_local, 0u) : acc_empty_local;
-    int buf = 0;
+    const uint32_t boxes = stage0 + (uint32_t)p.stages * STAGE, box = boxes + (uint32_t)(warp - F8_FIRST) * F8_BOX;
+    const uint32_t scales = boxes + F8_WARPS * F8_BOX + (uint32_t)(threadIdx.x - 32 * F8_FIRST) * 8u;
+    const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
+    int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int tile = worker; ok && tile < p.tiles; tile += workers) {
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       int m_blk, n_blk;
       f8_tile(p, tile, m_blk, n_blk);
-      const long long row0 = (long long)m_blk * TILE_M + (int)rank * 128 + quad * 32;
+      const long long row0 = (long long)m_blk * 128 + quad * 32;
       const int col0 = n_blk * BN + half * COLS;
-      const bool row_ok = row0 + lane < g.m, col_ok = col0 < g.n;
-      const float* sa = g.sa + (row_ok ? row0 + lane : 0);
-      const float* sw = g.sw + (col_ok ? (long long)(col0 / F8_BLOCK) * g.k_blocks : 0);
+      const bool inside = row0 + lane < g.m && col0 < g.n;
+      const float* sa = g.sa + (inside ? row0 + lane : 0);
+      const float* sw = g.sw + (inside ? (long long)(col0 / F8_BLOCK) * g.k_blocks : 0);
       unsigned long long sum[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
-      // Scales four blocks ahead: the loads of the next four are on their way while these four are used.
-      float next[4];
-      auto fetch = [&](int kb0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kb = kb0 + i;
-          next[i] = kb < g.k_blocks && row_ok && col_ok ? __ldg(sa + (long long)kb * g.m) * __ldg(sw + kb) : 0.f;
+      // Each thread copies its own scales some blocks ahead, past the registers that the sums need.
+      int ahead = 0;
+      auto fetch = [&]() {
+        if (ahead < g.k_blocks) {
+          const uint32_t to = scales + (uint32_t)(ahead & (F8_AHEAD - 1)) * F8_SCALES;
+          f8_copy4(to, sa, inside ? 4u : 0u);
+          f8_copy4(to + 4u, sw, inside ? 4u : 0u);
+          sa += g.m;
+          ++sw;
+          ++ahead;
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      fetch(0);
-      for (int kb0 = 0; ok && kb0 < g.k_blocks; kb0 += 4) {
-        float scale[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) scale[i] = next[i];
-        fetch(kb0 + 4);
+      for (int i = 0; i < F8_AHEAD - 1; ++i) fetch();
+      for (int kb = 0; kb < g.k_blocks; ++kb) {
+        const uint32_t at = (uint32_t)(PARTS == 2 ? 2 * acc + half : acc);
+        fetch();
+        ok = mbar_wait_warp(acc_full0 + 8u * at, acc_phase, abortp, SB_SITE_EPI_TMEM_FULL);
+        if (!ok) break;
+        asm volatile("cp.async.wait_group %0;" ::"n"(F8_AHEAD - 1) : "memory");
+        const uint32_t from = scales + (uint32_t)(kb & (F8_AHEAD - 1)) * F8_SCALES;
+        const float scale = f8_lds(from) * f8_lds(from + 4u);
+        const unsigned long long scale2 = pack_f32x2(scale, scale);
+        tc_fence_after_sync();
+        const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + at * PART_N + (PARTS == 2 ? 0u : (uint32_t)(half * COLS));
+        uint32_t part[2][32];
+        tmem_ld32(t, part[0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kb0 + i < g.k_blocks && ok) {
-            ok = mbar_wait_warp(acc_full0 + 8u * (uint32_t)buf, acc_phase, abortp, SB_SITE_EPI_TMEM_FULL);
-            if (ok) {
-              tc_fence_after_sync();
-              const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
-              const unsigned long long s2 = pack_f32x2(scale[i], scale[i]);
-              uint32_t part[2][32];
-              tmem_ld32(t, part[0]);
-#pragma unroll
-              for (int c = 0; c < COLS / 32; ++c) {
-                tmem_ld_wait32(part[c & 1]);
-                if (c + 1 < COLS / 32) {
-                  tmem_ld32(t + (uint32_t)(c + 1) * 32u, part[(c + 1) & 1]);
-                } else {                                     // all of the accumulator is in registers
-                  tc_fence_before_sync();
-                  __syncwarp();
-                  if (lane == 0) {
-                    if (PAIR) f8_arrive_cluster(acc_empty0 + 8u * (uint32_t)buf);
-                    else mbar_arrive(acc_empty0 + 8u * (uint32_t)buf);
-                  }
-                }
-                f8_add32(sum + c * 16, part[c & 1], s2);
-              }
-              if (++buf == BUFFERS) {
-                buf = 0;
-                acc_phase ^= 1u;
-              }
-            }
+        for (int c = 0; c < COLS / 32; ++c) {
+          tmem_ld_wait32(part[c & 1]);
+          if (c + 1 < COLS / 32) {
+            tmem_ld32(t + (uint32_t)(c + 1) * 32u, part[(c + 1) & 1]);
+          } else {                                           // all of the accumulator is in registers
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty0 + 8u * at);
           }
+          f8_add<32>(sum + c * 16, part[c & 1], scale2);
+        }
+        if (++acc == DEPTH) {
+          acc = 0;
+          acc_phase ^= 1u;
         }
       }
       if (!ok) break;
@@ -540,23 +530,217 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
   }
-  // After an expired wait copies and MMAs in flight get time to land before shared and tensor memory are released; neither
-  // CTA of a pair leaves while the other can still reach it.
+  // After an expired wait copies and MMAs in flight get time to land before shared and tensor memory are released.
   tc_fence_before_sync();
-  if (PAIR) cluster_sync_all(); else __syncthreads();
+  __syncthreads();
   if (*abortp != 0) {
     const unsigned long long t0 = global_timer_ns();
     while (global_timer_ns() - t0 < 200000ull) { }
   }
-  if (PAIR) cluster_sync_all(); else __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem, BUFFERS * BN);
-    else tmem_dealloc(tmem, BUFFERS * BN);
+    tmem_dealloc(tmem, TMEM_COLS);
   }
 }
 
-// Row-major matrix -> tensor map with boxes of box_rows x box_bytes, swizzled by 128 bytes (64 where the box is no wider).
+// The form for few rows of A, and for products whose tiles would leave most of the chip without work: the operands change
+// places (M of the MMA is 128 rows of W, N is TN rows of A), and the blocks of K are shared by the CTAs of a cluster, each of
+// which loads its part of W at once.  Their sums meet in shared memory: CTA r gets every CTA's sums of the r-th part of the
+// columns and adds them in the order of the CTAs.  Bound by reading W, and by the launch.
+constexpr int F8_FEW_THREADS = 192;                          // warps 0-3 add, warp 4 loads, warp 5 issues
+constexpr int F8_FEW_BLOCKS = 64;                            // blocks of K per CTA at most: their scales are kept
+constexpr int F8_FEW_STAGES = 8;
+
+__device__ __forceinline__ void f8_prefetch(const CUtensorMap* tmap, int x, int y, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
+               "@q cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n\t}"
+               ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"((uint32_t)issue) : "memory");
+}
+// Floats of this thread in another CTA's shared memory, and back from its own.
+template <int N>
+__device__ __forceinline__ void f8_send(uint32_t cluster_addr, const float* v) {
+  if constexpr (N == 2) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr), "f"(v[0]), "f"(v[1]) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};"
+                   ::"r"(cluster_addr + 4u * (uint32_t)i), "f"(v[i]), "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]) : "memory");
+  }
+}
+
+template <int TN, int SPLITS>
+__global__ void __launch_bounds__(F8_FEW_THREADS, 1)
+gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ F8Args g,
+                    const int stages) {
+  constexpr int DEPTH = 4;
+  constexpr uint32_t TMEM_COLS = DEPTH * TN;
+  constexpr uint32_t W_BYTES = 128 * F8_BLOCK, A_BYTES = TN * F8_BLOCK, STAGE = W_BYTES + A_BYTES;
+  extern __shared__ uint8_t f8_smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[F8_FEW_STAGES], bar_empty[F8_FEW_STAGES], bar_acc_full[DEPTH], bar_acc_empty[DEPTH];
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float scales[F8_FEW_BLOCKS][TN];  // of A times of W
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int PER = TN / SPLITS;                           // columns that a CTA finishes
+  constexpr uint32_t PITCH = 4u * PER + (PER > 4 ? 16u : 0u);   // of a row's sums: 16-byte accesses without bank conflicts
+  const int rank = blockIdx.x;                               // a cluster is the splits of one tile
+  const int n0 = blockIdx.y * 128, m0 = blockIdx.z * TN;
+  const int kb0 = (int)((long long)g.k_blocks * rank / SPLITS), kb1 = (int)((long long)g.k_blocks * (rank + 1) / SPLITS);
+  const uint32_t stage0 = (smem_u32(f8_smem_raw) + 1023u) & ~1023u;
+  const uint32_t meet = stage0 + (uint32_t)stages * STAGE;   // [SPLITS][128 rows of W][PER] sums
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
+    }
+    for (int i = 0; i < DEPTH; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 1);
+      mbar_init(smem_u32(&bar_acc_empty[i]), 4);
+    }
+    g_f8_abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_w);
+  }
+  if (warp == 5) {
+    tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &g_f8_abort;
+  const bool one = elect_one_lane();
+  // The weights' way to L2 can begin while the kernel before this one, which may be making A, still runs: L2 is where all
+  // SMs meet, so a line that is written after the prefetch is not stale.
+  if (warp == 4)
+    for (int kb = kb0; kb < min(kb1, kb0 + stages); ++kb) f8_prefetch(&tmap_w, kb * F8_BLOCK, n0, one);
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  float sum[TN];
+  if (warp == 4) {
+    int stage = 0;
+    uint32_t phase = 0;
+    const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) break;
+      const uint32_t at = stage0 + (uint32_t)stage * STAGE, full = full0 + 8u * (uint32_t)stage;
+      if (one) mbar_arrive_expect_tx(full, STAGE);
+      tma_load_2d(at, &tmap_w, kb * F8_BLOCK, n0, full, one);
+      tma_load_2d(at + W_BYTES, &tmap_a, kb * F8_BLOCK, m0, full, one);
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  } else if (warp == 5) {
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    const uint64_t w_desc = umma_smem_desc(stage0, 16u, 1024u, 2u), a_desc = umma_smem_desc(stage0 + W_BYTES, 16u, 1024u, 2u);
+    const uint32_t w_hi = (uint32_t)(w_desc >> 32), a_hi = (uint32_t)(a_desc >> 32);
+    const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+    const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(acc_empty0 + 8u * (uint32_t)acc, acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY) ||
+          !mbar_wait_warp(full0 + 8u * (uint32_t)stage, phase, abortp, SB_SITE_MMA_FULL))
+        break;
+      tc_fence_after_sync();
+      const uint32_t step = (uint32_t)stage * (STAGE >> 4);
+      f8_block(tmem + (uint32_t)(acc * TN), (uint32_t)w_desc + step, w_hi, (uint32_t)a_desc + step, a_hi, f8_idesc(TN), one);
+      tc_commit(empty0 + 8u * (uint32_t)stage, one);
+      tc_commit(acc_full0 + 8u * (uint32_t)acc, one);
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+      if (++acc == DEPTH) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < (kb1 - kb0) * TN; i += 128) {
+      const int kb = i / TN, j = i % TN;
+      scales[kb][j] = m0 + j < g.m ? g.sa[(long long)(kb0 + kb) * g.m + m0 + j] * g.sw[(long long)blockIdx.y * g.k_blocks + kb0 + kb] : 0.f;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sum[j] = 0.f;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(acc_full0 + 8u * (uint32_t)acc, acc_phase, abortp, SB_SITE_EPI_TMEM_FULL)) break;
+      tc_fence_after_sync();
+      const uint32_t t = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(acc * TN);
+      uint32_t part[TN];
+#pragma unroll
+      for (int c = 0; c < TN; c += 16) tmem_ld16(t + (uint32_t)c, part + c);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < TN; ++j) asm volatile("" : "+r"(part[j]));   // not read above the wait
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty0 + 8u * (uint32_t)acc);
+      const float4* s4 = reinterpret_cast<const float4*>(scales[kb - kb0]);
+#pragma unroll
+      for (int j = 0; j < TN; j += 4) {
+        const float4 s = s4[j / 4];
+        sum[j] = fmaf(__uint_as_float(part[j]), s.x, sum[j]);
+        sum[j + 1] = fmaf(__uint_as_float(part[j + 1]), s.y, sum[j + 1]);
+        sum[j + 2] = fmaf(__uint_as_float(part[j + 2]), s.z, sum[j + 2]);
+        sum[j + 3] = fmaf(__uint_as_float(part[j + 3]), s.w, sum[j + 3]);
+      }
+      if (++acc == DEPTH) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+    const int n = n0 + threadIdx.x;
+    if (SPLITS == 1) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (n < g.n && m0 + j < g.m) f8_store(g, m0 + j, n, sum[j]);
+    } else {
+#pragma unroll
+      for (int to = 0; to < SPLITS; ++to)
+        f8_send<PER>(map_to_cta(meet + (uint32_t)(rank * 128 + (int)threadIdx.x) * PITCH, (uint32_t)to), sum + to * PER);
+    }
+  }
+  tc_fence_before_sync();
+  if (SPLITS > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    const int n = n0 + threadIdx.x;
+    if (warp < 4) {
+      float total[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) total[j] = 0.f;
+#pragma unroll
+      for (int r = 0; r < SPLITS; ++r)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) total[j] += f8_lds(meet + (uint32_t)(r * 128 + (int)threadIdx.x) * PITCH + 4u * (uint32_t)j);
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (n < g.n && m0 + rank * PER + j < g.m) f8_store(g, m0 + rank * PER + j, n, total[j]);
+    }
+  }
+  // As in gemm_fp8_kernel.
+  __syncthreads();
+  if (*abortp != 0) {
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) { }
+  }
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Row-major matrix -> tensor map with boxes of box_rows x box_cols, swizzled by 128 bytes (64 where the box is no wider).
 int f8_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int item, const void* base, long long rows, long long cols, long long pitch,
                   int box_rows, int box_cols) {
   EncodeTiledFn enc = get_encode_tiled();
@@ -570,47 +754,132 @@ int f8_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int item, const vo
   return SB_OK;
 }
 
-template <bool PAIR, int BN>
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once per device (again is harmless).
+template <typename K>
+int f8_allow_smem(K* kernel, int bytes, std::atomic<bool>* ready) {
+  int dev = 0;
+  SB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+    SB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+  }
+  return SB_OK;
+}
+
+template <int BN>
 int launch_fp8(const F8Args& g, cudaStream_t s) {
-  constexpr uint32_t STAGE = 128 * 128 + (PAIR ? BN / 2 : BN) * 128;
+  constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * F8_BOX + F8_AHEAD * F8_SCALES;
   F8Plan p;
   memset(&p, 0, sizeof(p));
-  p.pair = PAIR; p.block_n = BN;
-  p.tiles_m = (g.m + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128);
+  p.tiles_m = (g.m + 127) / 128;
   p.tiles_n = (g.n + BN - 1) / BN;
   p.tiles = p.tiles_m * p.tiles_n;
-  const int room = (int)((F8_SMEM - 1024 - F8_WARPS * F8_BOX) / STAGE);
-  p.stages = room < F8_STAGES_MAX ? room : F8_STAGES_MAX;
-  // kind::f8f6f4, E4M3 x E4M3 (formats 0), fp32 accumulator: see sb_umma_idesc for the fields.
-  p.idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((PAIR ? 256u : 128u) >> 4 << 24);
+  p.stages = BN == 256 ? 3 : (F8_SMEM - REST) / STAGE < F8_STAGES_MAX ? (F8_SMEM - REST) / STAGE : F8_STAGES_MAX;
   const int es = sb_dtype_size(g.out_dtype);
   // A TMA store cuts a box off at the row's end by whole 16-byte pieces only: rows of 70 bf16 in a pitch of 72 had the two
   // elements behind them overwritten.
   p.tma_store = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && (g.ldc * es) % 16 == 0 && ((long long)g.n * es) % 16 == 0;
   CUtensorMap ta, tw, tc;
   memset(&tc, 0, sizeof(tc));
-  int rc = f8_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, 128, 128);
-  if (rc == SB_OK) rc = f8_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, PAIR ? BN / 2 : BN, 128);
+  int rc = f8_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, 128, F8_BLOCK);
+  if (rc == SB_OK) rc = f8_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, BN, F8_BLOCK);
   if (rc == SB_OK && p.tma_store) {
     const int cols = (BN / 2) * es >= 128 ? 128 / es : BN / 2;
     rc = f8_tensor_map(&tc, g.out_dtype == SB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                             : g.out_dtype == SB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                        es, g.c, g.m, g.n, g.ldc, 32, cols);
   }
-  if (rc != SB_OK) return rc;
-  const size_t smem = 1024 + (size_t)p.stages * STAGE + F8_WARPS * F8_BOX;
   static std::atomic<bool> ready[64];
-  int dev = 0;
-  SB_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {   // setting it twice is harmless
-    SB_CUDA(cudaFuncSetAttribute(gemm_fp8_kernel<PAIR, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, F8_SMEM));
-    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
-  }
-  const int most = PAIR ? sb_sm_count() / 2 : sb_sm_count();
-  const int workers = p.tiles < most ? p.tiles : most;
-  SB_CUDA(sb_launch(gemm_fp8_kernel<PAIR, BN>, dim3(PAIR ? 2 * workers : workers), dim3(F8_THREADS), smem, s, PAIR ? 2 : 1, ta, tw, tc, g, p));
+  if (rc == SB_OK) rc = f8_allow_smem(gemm_fp8_kernel<BN>, F8_SMEM, ready);
+  if (rc != SB_OK) return rc;
+  const int workers = p.tiles < sb_sm_count() ? p.tiles : sb_sm_count();
+  SB_CUDA(sb_launch(gemm_fp8_kernel<BN>, dim3(workers), dim3(F8_THREADS), (size_t)(REST + p.stages * STAGE), s, 1, ta, tw, tc, g, p));
   SB_COUNT_LAUNCH();
   return SB_OK;
+}
+
+// Shared memory of the form for few rows: dynamic bytes and stages; scales and barriers are static (4 to 17 KB).
+struct F8FewSize {
+  int stages, bytes, fixed;
+};
+constexpr int F8_FEW_SMEM = F8_SMEM - 20 * 1024;
+F8FewSize f8_few_size(int tn, int splits, int k_blocks) {
+  const int stage = (128 + tn) * F8_BLOCK, blocks = (k_blocks + splits - 1) / splits;
+  const int rest = 1024 + (splits > 1 ? splits * 128 * (4 * (tn / splits) + 16) : 0);
+  int stages = (F8_FEW_SMEM - rest) / stage;
+  if (stages > F8_FEW_STAGES) stages = F8_FEW_STAGES;
+  if (stages > blocks) stages = blocks;
+  return {stages, rest + stages * stage, tn * F8_FEW_BLOCKS * 4 + 512};
+}
+
+template <int TN, int SPLITS>
+int launch_fp8_few(const F8Args& g, cudaStream_t s) {
+  const F8FewSize size = f8_few_size(TN, SPLITS, g.k_blocks);
+  CUtensorMap ta, tw;
+  int rc = f8_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, TN, F8_BLOCK);
+  if (rc == SB_OK) rc = f8_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, 128, F8_BLOCK);
+  static std::atomic<bool> ready[64];
+  if (rc == SB_OK) rc = f8_allow_smem(gemm_fp8_few_kernel<TN, SPLITS>, F8_FEW_SMEM, ready);
+  if (rc != SB_OK) return rc;
+  const dim3 grid(SPLITS, (g.n + 127) / 128, (g.m + TN - 1) / TN);
+  SB_CUDA(sb_launch(gemm_fp8_few_kernel<TN, SPLITS>, grid, dim3(F8_FEW_THREADS), (size_t)size.bytes, s, SPLITS, ta, tw, g, size.stages));
+  SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+template <int TN>
+int launch_fp8_few(const F8Args& g, int splits, cudaStream_t s) {
+  switch (splits) {
+    case 1: return launch_fp8_few<TN, 1>(g, s);
+    case 2: return launch_fp8_few<TN, 2>(g, s);
+    case 4: return launch_fp8_few<TN, 4>(g, s);
+    default: return launch_fp8_few<TN, 8>(g, s);
+  }
+}
+
+// Which form a product takes: the least of rounds over the SMs x (time of a tile + blocks of K x time of a block), in us as
+// measured.  Times of back-to-back launches on operands beyond L2, tiles of 256 / 128 / 64 columns: 16384 x 4096 x 4096 296 / 342 /
+// 580, 4000 x 3000 x 1008 25.5 / 27.0 / 39.5, 1024^3 9.3 / 6.2 / 5.6.  Few rows, 16 x 4096 x 4096 with K over 1 / 2 / 4 / 8 CTAs: 11.4 /
+// 8.1 / 6.4 / 5.7, and 13.6 as 64-column tiles; 64 x 4096 x 4096 20.2 / 12.6 / 9.9 / 21.0 (two rounds), 12.9; 512 x 512 x 4096 18.2 / 11.3 /
+// 8.9 / 20.0, 12.3.
+struct F8Choice {
+  int few, tile, splits;
+};
+F8Choice f8_choose(int m, int n, int k_blocks) {
+  const int sms = sb_sm_count();
+  F8Choice best = {0, 256, 1};
+  double least = 1e30;
+  const struct { int bn; double block, tile; } forms[] = {{256, 0.60, 2.0}, {128, 0.37, 2.0}, {64, 0.35, 1.8}};
+  for (const auto& f : forms) {
+    const double tiles = (double)((m + 127) / 128) * ((n + f.bn - 1) / f.bn);
+    const double t = ceil(tiles / sms) * (k_blocks * f.block + f.tile);
+    if (t < least) {
+      least = t;
+      best = {0, f.bn, 1};
+    }
+  }
+  for (int tn = 16; tn <= 64; tn *= 2) {
+    const long long across = (n + 127) / 128, down = (m + tn - 1) / tn;
+    if (across > 65535 || down > 65535) continue;
+    const double block = tn == 16 ? 0.28 : tn == 32 ? 0.36 : 0.50;
+    const double weights = 128e-6 * 128.0 * across * k_blocks / 5.0;           // on their way from DRAM
+    for (int splits = 1; splits <= 8; splits *= 2) {
+      const int blocks = (k_blocks + splits - 1) / splits;
+      if (blocks > F8_FEW_BLOCKS || (splits > 1 && k_blocks < 2 * splits)) continue;
+      const F8FewSize size = f8_few_size(tn, splits, k_blocks);
+      int resident = 227 * 1024 / (size.bytes + size.fixed + 1024);
+      if (resident > 2) resident = 2;
+      const double ctas = (double)across * down * splits;
+      // Clusters do not fill every SM, and a second round of them costs more than it brings.
+      if (splits > 1 && ctas > 0.9 * resident * sms) continue;
+      const double t = ceil(ctas / (resident * sms)) * (2.2 + blocks * block) + weights;
+      if (t < least) {
+        least = t;
+        best = {1, tn, splits};
+      }
+    }
+  }
+  return best;
 }
 
 bool f8_aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -663,15 +932,9 @@ int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const 
   cudaStream_t s = (cudaStream_t)stream;
   // TMA takes rows that begin on 16-byte boundaries.
   if (k > 0 && f8_aligned(a, 16) && f8_aligned(w, 16) && lda % 16 == 0 && ldw % 16 == 0) {
-    const long long sms = sb_sm_count();
-    const long long pairs = ((m + 255) / 256LL) * ((n + 255) / 256LL), singles = ((m + 127) / 128LL) * ((n + 127) / 128LL);
-    if (getenv("F8V")) {
-      const int v = atoi(getenv("F8V"));
-      return v == 0 ? launch_fp8<true, 256>(g, s) : v == 1 ? launch_fp8<false, 128>(g, s) : launch_fp8<false, 64>(g, s);
-    }
-    if (pairs >= sms / 2) return launch_fp8<true, 256>(g, s);
-    if (singles >= sms / 2) return launch_fp8<false, 128>(g, s);
-    return launch_fp8<false, 64>(g, s);
+    const F8Choice c = f8_choose(m, n, g.k_blocks);
+    if (c.few) return c.tile == 16 ? launch_fp8_few<16>(g, c.splits, s) : c.tile == 32 ? launch_fp8_few<32>(g, c.splits, s) : launch_fp8_few<64>(g, c.splits, s);
+    return c.tile == 256 ? launch_fp8<256>(g, s) : c.tile == 128 ? launch_fp8<128>(g, s) : launch_fp8<64>(g, s);
   }
   const dim3 grid((unsigned)((m + 63) / 64), (unsigned)((n + 63) / 64));
   SB_CUDA(sb_launch(gemm_fp8_simple_kernel, grid, dim3(256), 0, s, 1, g));
