@@ -35,6 +35,7 @@ struct QuantArgs {
   float* scales;
   long long rows, ldx, ldc;
   int cols;
+  unsigned across;               // blocks of 128 columns
 };
 
 // ------------------------------ quantisation -------------------------------------
@@ -51,8 +52,11 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const int lane = threadIdx.x % L, r0 = threadIdx.x / L;
-  const long long row0 = (long long)blockIdx.x * ROWS;
-  const int col0 = blockIdx.y * F8_BLOCK;
+  // Tiles that are neighbours in a row run at the same time: their pieces of x are neighbours in memory.
+  const long long up = blockIdx.x / a.across;
+  const int over = (int)(blockIdx.x - up * a.across);
+  const long long row0 = up * ROWS;
+  const int col0 = over * F8_BLOCK;
   SbPack<T, V> in[PASSES][STEPS];
   uint32_t all = 0u;
   uint32_t largest[PASSES];
@@ -84,7 +88,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; ++w) all = max(all, warp_max[w]);
-    if (threadIdx.x == 0) a.scales[(long long)blockIdx.x * gridDim.y + blockIdx.y] = __fdiv_rn(__uint_as_float(all), F8_TOP);
+    if (threadIdx.x == 0) a.scales[blockIdx.x] = __fdiv_rn(__uint_as_float(all), F8_TOP);
   }
   const float square_inv = __fdiv_rn(F8_TOP, __uint_as_float(all));
 #pragma unroll
@@ -114,15 +118,16 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
   if (!SQUARE) {
     __syncthreads();
     for (int r = threadIdx.x; r < ROWS; r += 256)
-      if (row0 + r < a.rows) a.scales[(long long)blockIdx.y * a.rows + row0 + r] = row_scale[r];
+      if (row0 + r < a.rows) a.scales[over * a.rows + row0 + r] = row_scale[r];
   }
 }
 
 template <typename T, int V>
 int launch_quantize(const QuantArgs& a, int block_rows, cudaStream_t s) {
-  const int across = (a.cols + F8_BLOCK - 1) / F8_BLOCK;
   const int rows = block_rows == 1 ? 64 : 128;
-  const dim3 grid((unsigned)((a.rows + rows - 1) / rows), (unsigned)across);
+  const long long tiles = (a.rows + rows - 1) / rows * a.across;
+  if (tiles > 0x7fffffffLL) return sb_fail(SB_ERR_TOO_LARGE, "sb_quantize_fp8: more than 2^31 - 1 tiles");
+  const dim3 grid((unsigned)tiles);
   if (block_rows == 1) SB_CUDA(sb_launch(quantize_fp8_kernel<T, V, 64, false>, grid, dim3(256), 0, s, 1, a));
   else SB_CUDA(sb_launch(quantize_fp8_kernel<T, V, 128, true>, grid, dim3(256), 0, s, 1, a));
   SB_COUNT_LAUNCH();
@@ -282,11 +287,11 @@ __device__ __forceinline__ void f8_add(unsigned long long* sum, const uint32_t* 
     fma_f32x2(sum[j], pack_f32x2(__uint_as_float(part[2 * j]), __uint_as_float(part[2 * j + 1])), scale);
 }
 
-// Finished values of this warp's 32 rows and COLS columns -> C, a box of 32 rows x 128 bytes at a time (64 bytes where the
+// Finished values of this warp's 32 rows and COLS columns (their biases in shared memory) -> C, a box of 32 rows x 128 bytes at a time (64 bytes where the
 // columns are no more): by a TMA store, or by coalesced stores where C's rows are not whole 16-byte pieces.
 template <typename O, int COLS>
 __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tmap_c, bool tma, const unsigned long long* sum,
-                                         long long row0, int col0, uint32_t box, int lane) {
+                                         long long row0, int col0, uint32_t box, uint32_t bias, int lane) {
   constexpr int BOX_COLS = COLS * sizeof(O) >= 128 ? 128 / sizeof(O) : COLS;
   constexpr int ROW_BYTES = BOX_COLS * sizeof(O), PIECES = ROW_BYTES / 16, PER = 16 / sizeof(O);
 #pragma unroll
@@ -304,10 +309,7 @@ __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tma
       for (int t = 0; t < PER; t += 2) unpack_f32x2(sum[(b * BOX_COLS + q * PER + t) / 2], v[t], v[t + 1]);
       if (g.bias) {
 #pragma unroll
-        for (int t = 0; t < PER; ++t) {
-          const int col = first + q * PER + t;
-          if (col < g.n) v[t] += __ldg(g.bias + col);
-        }
+        for (int t = 0; t < PER; ++t) v[t] += f8_lds(bias + 4u * (uint32_t)(b * BOX_COLS + q * PER + t));
       }
       if (g.relu) {
 #pragma unroll
@@ -459,7 +461,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quad = warp & 3, half = (warp - F8_FIRST) >> 2;   // a warp reads the TMEM lanes of its number modulo 4
     const uint32_t boxes = stage0 + (uint32_t)p.stages * STAGE, box = boxes + (uint32_t)(warp - F8_FIRST) * F8_BOX;
-    const uint32_t scales = boxes + F8_WARPS * F8_BOX + (uint32_t)(threadIdx.x - 32 * F8_FIRST) * 8u;
+    const uint32_t scales = boxes + F8_WARPS * F8_BOX + (uint32_t)(threadIdx.x - 32 * F8_FIRST) * 4u;
+    const uint32_t bias = boxes + F8_WARPS * F8_BOX + F8_AHEAD * F8_SCALES + (uint32_t)(warp - F8_FIRST) * 512u;
     const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -475,13 +478,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       unsigned long long sum[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
+      // The columns' biases, for when the sums are done.  (Read there one by one they took 33 of 374 us at 16384 x 4096 x 4096.)
+      if (g.bias)
+#pragma unroll
+        for (int j = lane; j < COLS; j += 32) f8_copy4(bias + 4u * (uint32_t)j, g.bias + (col0 + j < g.n ? col0 + j : 0), col0 + j < g.n ? 4u : 0u);
       // Each thread copies its own scales some blocks ahead, past the registers that the sums need.
       int ahead = 0;
       auto fetch = [&]() {
         if (ahead < g.k_blocks) {
           const uint32_t to = scales + (uint32_t)(ahead & (F8_AHEAD - 1)) * F8_SCALES;
           f8_copy4(to, sa, inside ? 4u : 0u);
-          f8_copy4(to + 4u, sw, inside ? 4u : 0u);
+          f8_copy4(to + F8_SCALES / 2, sw, inside ? 4u : 0u);
           sa += g.m;
           ++sw;
           ++ahead;
@@ -497,7 +504,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (!ok) break;
         asm volatile("cp.async.wait_group %0;" ::"n"(F8_AHEAD - 1) : "memory");
         const uint32_t from = scales + (uint32_t)(kb & (F8_AHEAD - 1)) * F8_SCALES;
-        const float scale = f8_lds(from) * f8_lds(from + 4u);
+        const float scale = f8_lds(from) * f8_lds(from + F8_SCALES / 2);
         const unsigned long long scale2 = pack_f32x2(scale, scale);
         tc_fence_after_sync();
         const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + at * PART_N + (PARTS == 2 ? 0u : (uint32_t)(half * COLS));
@@ -521,11 +528,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
       }
       if (!ok) break;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
       if (row0 < g.m) {
-        if (g.out_dtype == SB_F32) f8_write<float, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, lane);
-        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, lane);
-        else f8_write<__half, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, lane);
+        if (g.out_dtype == SB_F32) f8_write<float, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+        else f8_write<__half, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
       }
+      __syncwarp();                                          // the biases have been read
     }
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
@@ -768,7 +778,7 @@ int f8_allow_smem(K* kernel, int bytes, std::atomic<bool>* ready) {
 
 template <int BN>
 int launch_fp8(const F8Args& g, cudaStream_t s) {
-  constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * F8_BOX + F8_AHEAD * F8_SCALES;
+  constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * (F8_BOX + 512) + F8_AHEAD * F8_SCALES;
   F8Plan p;
   memset(&p, 0, sizeof(p));
   p.tiles_m = (g.m + 127) / 128;
@@ -905,6 +915,7 @@ int sb_quantize_fp8(const void* x, long long ldx, int dtype, long long rows, int
   QuantArgs a;
   memset(&a, 0, sizeof(a));
   a.x = x; a.codes = codes; a.scales = scales; a.rows = rows; a.ldx = ldx; a.ldc = ldc; a.cols = cols;
+  a.across = (unsigned)((cols + F8_BLOCK - 1) / F8_BLOCK);
   cudaStream_t s = (cudaStream_t)stream;
   return dtype == SB_F32 ? launch_quantize_width<float>(a, block_rows, s)
          : dtype == SB_BF16 ? launch_quantize_width<__nv_bfloat16>(a, block_rows, s) : launch_quantize_width<__half>(a, block_rows, s);

@@ -26,6 +26,411 @@ struct NormArgs {
   float eps, inv_cols;
 };
 
+// Rows that fit into registers.  LANES threads share a row (a part of a warp, a warp, or W warps), each with NV packs of V
+// elements, R rows at a time.  In the backward pass the running column sums stay in registers over all rows of a thread.
+// The arithmetic is packed, two fp32 operations per instruction: with 12 operations per element and 16 warps per SM the
+// scalar form was bound by issue (65536 x 1024 bf16: 97 us forward, 107 backward).
+constexpr int LN_THREADS = 512;                              // of a block at most
+struct NormShape {
+  int warps;                     // per row; 1: `lanes` threads of a warp
+  int lanes;                     // threads per row
+  int groups;                    // of threads with rows of their own, per block
+};
+typedef unsigned long long Pair; // two fp32 values
+__device__ __forceinline__ Pair ln_pair(float v) { return pack_f32x2(v, v); }
+__device__ __forceinline__ float ln_both(Pair v) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return lo + hi;
+}
+
+// K sums over the threads that share a row; the two buffers of `slots` take turns, so that one barrier per call is enough.
+template <int K>
+__device__ __forceinline__ void ln_row_sums(float (&v)[K], const NormShape& s, int group, float4* slots) {
+  static_assert(K <= 4, "");
+  const int from = s.warps > 1 ? 16 : s.lanes >> 1;
+  for (int o = from; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
+  if (s.warps > 1) {
+    const int warp = threadIdx.x >> 5, first = group * s.warps;
+    if ((threadIdx.x & 31) == 0) slots[warp] = make_float4(v[0], K > 1 ? v[K > 1 ? 1 : 0] : 0.f, K > 2 ? v[K > 2 ? 2 : 0] : 0.f, K > 3 ? v[K > 3 ? 3 : 0] : 0.f);
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(s.warps * 32) : "memory");
+    float4 t = slots[first];
+    for (int w = 1; w < s.warps; ++w) {
+      const float4 u = slots[first + w];
+      t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+    }
+    v[0] = t.x;
+    if (K > 1) v[K > 1 ? 1 : 0] = t.y;
+    if (K > 2) v[K > 2 ? 2 : 0] = t.z;
+    if (K > 3) v[K > 3 ? 3 : 0] = t.w;
+  }
+}
+
+// Rows on their way.  Packs of 4 bytes and more travel by cp.async, DEPTH turns of R rows ahead: every thread copies what it
+// will itself read into its own places in shared memory, so nothing needs a barrier, and the rows in flight need no
+// registers.  Packs of 2 bytes (16-bit rows whose pitch or base is odd), which cp.async does not take, are loaded one turn
+// ahead into registers.
+template <typename T, int V, int NV, int R, int MATRICES, int DEPTH>
+struct LnAhead {
+  static constexpr bool RING = sizeof(T) * V >= 4;
+  static constexpr uint32_t PACK = sizeof(T) * V, TURN = MATRICES * R * NV;   // packs per thread and turn
+  SbPack<T, V> held[RING ? 1 : TURN];
+  uint32_t mine, stride;         // this thread's first place; bytes between its places
+  int slot;
+
+  static __host__ __device__ constexpr size_t bytes(int threads) { return RING ? (size_t)DEPTH * TURN * PACK * threads : 0; }
+  __device__ __forceinline__ void start(uint32_t smem) {
+    stride = blockDim.x * PACK;
+    mine = smem + threadIdx.x * PACK;
+    slot = 0;
+  }
+  // Rows `row` .. `row` + R - 1; `from` points at this thread's first element of the first.
+  __device__ __forceinline__ void fetch(int matrix, const T* from, long long row, long long ld, const NormArgs& a, int lane, int lanes, int to) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = row + r < a.rows && (lane + i * lanes) * V < a.cols;
+        const T* at = in ? from + r * ld + i * lanes * V : from;
+        const int k = (matrix * R + r) * NV + i;
+        if constexpr (RING) {
+          const uint32_t dst = mine + (uint32_t)(to * (int)TURN + k) * stride;
+          if constexpr (PACK == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? at : (const T*)a.x), "r"(in ? 16u : 0u) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(in ? at : (const T*)a.x), "r"(in ? 4u : 0u) : "memory");
+        } else {
+          held[k] = in ? sb_load_pack<T, V>(at) : sb_zero_pack<T, V>();
+        }
+      }
+  }
+  __device__ __forceinline__ void read(int matrix, int r, int i, float* x) const {
+    static_assert(!RING || PACK == 4 || PACK == 16, "");
+    const int k = (matrix * R + r) * NV + i;
+    SbPack<T, V> p;
+    if constexpr (RING) {
+      const uint32_t src = mine + (uint32_t)(slot * (int)TURN + k) * stride;
+      if constexpr (PACK == 16) {
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+        p = *reinterpret_cast<const SbPack<T, V>*>(&v);
+      } else {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(src) : "memory");
+        p = *reinterpret_cast<const SbPack<T, V>*>(&v);
+      }
+    } else {
+      p = held[k];
+    }
+    sb_unpack<T, V>(p, x);
+  }
+  __device__ __forceinline__ void next() {
+    if (++slot == DEPTH) slot = 0;
+  }
+};
+
+// V weights from column `col` on (16-byte loads where V allows them); `other` where there are none or the row has ended.
+template <int V>
+__device__ __forceinline__ void ln_weights(const float* w, int col, int cols, float other, float* to) {
+  if (!w || col >= cols) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) to[k] = other;
+  } else if constexpr (V >= 4) {
+#pragma unroll
+    for (int k = 0; k < V; k += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(w + col + k));
+      to[k] = f.x; to[k + 1] = f.y; to[k + 2] = f.z; to[k + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) to[k] = __ldg(w + col + k);
+  }
+}
+
+// NV x V values of a thread as pairs.
+template <typename A, int V, int NV>
+__device__ __forceinline__ void ln_read(const A& rows, int matrix, int r, Pair* x) {
+  float v[NV * V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) rows.read(matrix, r, i, v + i * V);
+#pragma unroll
+  for (int j = 0; j < NV * V / 2; ++j) x[j] = pack_f32x2(v[2 * j], v[2 * j + 1]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void ln_store(T* to, const Pair* x, int i) {
+  float v[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    float lo, hi;
+    unpack_f32x2(x[(i * V + k) / 2], lo, hi);
+    v[k] = (i * V + k) & 1 ? hi : lo;
+  }
+  sb_store_f32<T, V>(to, v);
+}
+
+constexpr int LN_DEPTH = 3;
+
+// Weights are read for every row, from L1: in registers they would cost half of the warps.
+template <typename T, int V, int NV, int R>
+__global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, NormShape s) {
+  constexpr int E = NV * V;
+  __shared__ float4 slots[2][LN_THREADS / 32];
+  extern __shared__ __align__(16) uint8_t ln_smem[];
+  const int group = threadIdx.x / s.lanes, lane = threadIdx.x % s.lanes;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const long long step = (long long)R * gridDim.x * s.groups;
+  long long row = (long long)R * ((long long)blockIdx.x * s.groups + group);
+  // All groups of a warp stay together: they end when the last has no row left.
+  const long long last = s.warps > 1 ? row : row - (long long)R * (group % (32 / s.lanes));
+  LnAhead<T, V, NV, R, 1, LN_DEPTH> rows;
+  constexpr bool RING = decltype(rows)::RING;
+  rows.start(smem_u32(ln_smem));
+  const T* x_at = (const T*)a.x + row * a.ldx + lane * V;
+  T* y_at = (T*)a.out + row * a.ldout + lane * V;
+  constexpr int FIRST = RING ? LN_DEPTH - 1 : 1;
+#pragma unroll
+  for (int d = 0; d < FIRST; ++d) {
+    rows.fetch(0, x_at + d * step * a.ldx, row + d * step, a.ldx, a, lane, s.lanes, d);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  const bool full = a.cols == s.lanes * E;
+  for (long long at = last; at < a.rows; at += step, row += step, x_at += step * a.ldx, y_at += step * a.ldout) {
+    if (RING) {
+      rows.fetch(0, x_at + (LN_DEPTH - 1) * step * a.ldx, row + (LN_DEPTH - 1) * step, a.ldx, a, lane, s.lanes,
+                 rows.slot == 0 ? LN_DEPTH - 1 : rows.slot - 1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(LN_DEPTH - 1) : "memory");
+    }
+    Pair x[R][E / 2];
+    float v[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      ln_read<decltype(rows), V, NV>(rows, 0, r, x[r]);
+      Pair t = x[r][0];
+#pragma unroll
+      for (int j = 1; j < E / 2; ++j) t = add_f32x2(t, x[r][j]);
+      v[r] = ln_both(t);
+    }
+    if (!RING) rows.fetch(0, x_at + step * a.ldx, row + step, a.ldx, a, lane, s.lanes, 0);
+    rows.next();
+    ln_row_sums<R>(v, s, group, slots[0]);
+    float mean[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = v[r] * a.inv_cols;
+      const Pair m = ln_pair(mean[r]);
+      Pair t = 0ull;
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) x[r][j] = sub_f32x2(x[r][j], m);
+      if (!full) {                                           // what lies behind the row's end deviates by nothing
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+          float lo, hi;
+          unpack_f32x2(x[r][j], lo, hi);
+          if ((lane + 2 * j / V * s.lanes) * V >= a.cols) lo = 0.f;
+          if ((lane + (2 * j + 1) / V * s.lanes) * V >= a.cols) hi = 0.f;
+          x[r][j] = pack_f32x2(lo, hi);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) fma_f32x2(t, x[r][j], x[r][j]);
+      v[r] = ln_both(t);
+    }
+    ln_row_sums<R>(v, s, group, slots[1]);
+    float rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      rstd[r] = 1.f / sqrtf(v[r] * a.inv_cols + a.eps);
+      const Pair f = ln_pair(rstd[r]);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) x[r][j] = mul_f32x2(x[r][j], f);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i += V == 1 ? 2 : 1) {           // pairs of packs where a pack is one element
+      constexpr int P = V == 1 ? 2 : 1;
+      float w[P * V], b[P * V];
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        ln_weights<V>(a.weight, (lane + (i + q) * s.lanes) * V, a.cols, 1.f, w + q * V);
+        ln_weights<V>(a.bias, (lane + (i + q) * s.lanes) * V, a.cols, 0.f, b + q * V);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int k = 0; k < P * V; k += 2) {
+          Pair y = pack_f32x2(b[k], b[k + 1]);
+          fma_f32x2(y, x[r][(i * V + k) / 2], pack_f32x2(w[k], w[k + 1]));
+          x[r][(i * V + k) / 2] = y;
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          if (row + r < a.rows && (lane + (i + q) * s.lanes) * V < a.cols)
+            ln_store<T, V>(y_at + r * a.ldout + (i + q) * s.lanes * V, x[r], i + q);
+      }
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row + r < a.rows) {
+          if (a.mean) a.mean[row + r] = mean[r];
+          if (a.rstd) a.rstd[row + r] = rstd[r];
+        }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The backward pass: x and dy are read once for dx and the column sums together.
+template <typename T, int V, int NV, int R>
+__global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a, NormShape s) {
+  constexpr int E = NV * V;
+  __shared__ float4 slots[2][LN_THREADS / 32];
+  __shared__ float stats[LN_DEPTH][LN_THREADS / 4][2 * R];   // mean and rstd of the rows on their way, per warp or group
+  extern __shared__ __align__(16) uint8_t ln_smem[];
+  float* columns = reinterpret_cast<float*>(ln_smem);        // [2][cols], where several groups of a block add up at the end
+  const int group = threadIdx.x / s.lanes, lane = threadIdx.x % s.lanes;
+  const int unit = s.warps > 1 ? threadIdx.x >> 5 : group, place = s.warps > 1 ? threadIdx.x & 31 : lane;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const long long step = (long long)R * gridDim.x * s.groups;
+  long long row = (long long)R * ((long long)blockIdx.x * s.groups + group);
+  const long long last = s.warps > 1 ? row : row - (long long)R * (group % (32 / s.lanes));
+  LnAhead<T, V, NV, R, 2, LN_DEPTH> rows;
+  constexpr bool RING = decltype(rows)::RING;
+  rows.start(smem_u32(ln_smem));
+  const T* x_at = (const T*)a.x + row * a.ldx + lane * V;
+  const T* dy_at = (const T*)a.dy + row * a.lddy + lane * V;
+  T* dx_at = (T*)a.out + row * a.ldout + lane * V;
+  auto fetch = [&](int turns, int to) {
+    const long long at = row + turns * step;
+    rows.fetch(0, x_at + turns * step * a.ldx, at, a.ldx, a, lane, s.lanes, RING ? to : 0);
+    rows.fetch(1, dy_at + turns * step * a.lddy, at, a.lddy, a, lane, s.lanes, RING ? to : 0);
+    if (place < 2 * R) {
+      const bool in = at + place % R < a.rows;
+      const float* from = (place < R ? a.mean : a.rstd) + (in ? at + place % R : 0);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&stats[to][unit][place])), "l"(from), "r"(in ? 4u : 0u) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  constexpr int FIRST = RING ? LN_DEPTH - 1 : 1;
+#pragma unroll
+  for (int d = 0; d < FIRST; ++d) fetch(d, d);
+  Pair w[E / 2], dw[E / 2], db[E / 2];
+  {
+    float f[E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) ln_weights<V>(a.weight, (lane + i * s.lanes) * V, a.cols, 1.f, f + i * V);
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+      w[j] = pack_f32x2(f[2 * j], f[2 * j + 1]);
+      dw[j] = db[j] = 0ull;
+    }
+  }
+  int turn = 0;
+  for (long long at = last; at < a.rows; at += step, turn ^= 1) {
+    if (RING) {
+      fetch(LN_DEPTH - 1, rows.slot == 0 ? LN_DEPTH - 1 : rows.slot - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(LN_DEPTH - 1) : "memory");
+    } else {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    __syncwarp();                                            // the statistics were copied by other lanes
+    Pair h[R][E / 2], g[R][E / 2];
+    float v[2 * R], rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float mean = *(volatile float*)&stats[rows.slot][unit][r];
+      rstd[r] = *(volatile float*)&stats[rows.slot][unit][R + r];
+      const Pair m = ln_pair(mean), f = ln_pair(rstd[r]);
+      ln_read<decltype(rows), V, NV>(rows, 0, r, h[r]);
+      ln_read<decltype(rows), V, NV>(rows, 1, r, g[r]);
+      Pair s1 = 0ull, s2 = 0ull;
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        h[r][j] = mul_f32x2(sub_f32x2(h[r][j], m), f);
+        fma_f32x2(dw[j], g[r][j], h[r][j]);
+        db[j] = add_f32x2(db[j], g[r][j]);
+        g[r][j] = mul_f32x2(g[r][j], w[j]);
+        s1 = add_f32x2(s1, g[r][j]);
+        fma_f32x2(s2, g[r][j], h[r][j]);
+      }
+      v[2 * r] = ln_both(s1);
+      v[2 * r + 1] = ln_both(s2);
+    }
+    __syncwarp();                                            // the statistics have been read
+    rows.next();
+    if (!RING) fetch(1, rows.slot);
+    if (a.out) {
+      ln_row_sums<2 * R>(v, s, group, slots[turn]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const Pair s1 = ln_pair(-v[2 * r] * a.inv_cols), s2 = ln_pair(-v[2 * r + 1] * a.inv_cols), f = ln_pair(rstd[r]);
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+          Pair t = add_f32x2(g[r][j], s1);
+          fma_f32x2(t, h[r][j], s2);
+          g[r][j] = mul_f32x2(t, f);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (row + r < a.rows && (lane + i * s.lanes) * V < a.cols) ln_store<T, V>(dx_at + r * a.ldout + i * s.lanes * V, g[r], i);
+      }
+    }
+    row += step;
+    x_at += step * a.ldx;
+    dy_at += step * a.lddy;
+    dx_at += step * a.ldout;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!a.partial) return;
+  float sums[2][E];
+#pragma unroll
+  for (int j = 0; j < E / 2; ++j) {
+    unpack_f32x2(dw[j], sums[0][2 * j], sums[0][2 * j + 1]);
+    unpack_f32x2(db[j], sums[1][2 * j], sums[1][2 * j + 1]);
+  }
+  float* part = a.partial + (long long)blockIdx.x * 2 * a.cols;
+  if (s.groups == 1) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int col = (lane + j / V * s.lanes) * V + j % V;
+      if (col < a.cols) {
+        part[col] = sums[0][j];
+        part[a.cols + col] = sums[1][j];
+      }
+    }
+    return;
+  }
+  // Groups of one warp add up by shuffles, then the block's in their order through shared memory.
+  for (int o = 16; o >= s.lanes; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      sums[0][j] += __shfl_xor_sync(0xffffffffu, sums[0][j], o);
+      sums[1][j] += __shfl_xor_sync(0xffffffffu, sums[1][j], o);
+    }
+  const bool mine = s.warps > 1 || (threadIdx.x & 31) < s.lanes;
+  const int turns = s.warps > 1 ? s.groups : blockDim.x / 32, my_turn = s.warps > 1 ? group : threadIdx.x >> 5;
+  __syncthreads();                                           // every group's rows have been read
+  for (int t = 0; t < turns; ++t) {
+    if (t == my_turn && mine) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int col = (lane + j / V * s.lanes) * V + j % V;
+        if (col < a.cols) {
+          columns[col] = (t ? columns[col] : 0.f) + sums[0][j];
+          columns[a.cols + col] = (t ? columns[a.cols + col] : 0.f) + sums[1][j];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * a.cols; i += blockDim.x) part[i] = columns[i];
+}
+
 __device__ __forceinline__ float ln_warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -143,9 +548,12 @@ layer_norm_partials_kernel(const float* __restrict__ partial, int parts, int col
   }
 }
 
+// Blocks with partial column sums, at most.
+constexpr int LN_BLOCKS_PER_SM = 8;
+constexpr int LN_SMEM = 200 * 1024;
 int ln_columns_blocks(long long rows) {
-  const long long want = (rows + 31) / 32, most = 4LL * sb_sm_count();
-  return (int)(want < 1 ? 1 : want < most ? want : most);
+  const long long most = LN_BLOCKS_PER_SM * (long long)sb_sm_count();
+  return (int)(rows < 1 ? 1 : rows < most ? rows : most);
 }
 
 int norm_args_ok(const char* who, long long rows, int cols, int dtype, const void* x, long long ldx) {
@@ -165,20 +573,126 @@ int norm_element_aligned(const char* who, const void* p, int dtype) {
   return SB_OK;
 }
 
-template <typename T>
-cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
-  const int threads = a.cols >= 1024 ? 1024 : (a.cols + 31) / 32 * 32;
-  const long long most = 16LL * sb_sm_count();
-  const int grid = (int)(a.rows < most ? a.rows : most);
-  return sb_launch(layer_norm_wide_kernel<T>, dim3(grid), dim3(threads), 0, s, 1, a);
+// How many threads share a row, for packs of v elements and nv of them per thread; false: the row does not fit.
+bool norm_shape(int cols, int v, int nv, NormShape* s) {
+  const int packs = (cols + v - 1) / v, most = LN_THREADS * nv;
+  if (packs > most) return false;
+  s->warps = (packs + 32 * nv - 1) / (32 * nv);
+  s->lanes = 32 * s->warps;
+  if (s->warps == 1) {
+    s->lanes = 4;
+    while (s->lanes * nv < packs) s->lanes *= 2;
+  }
+  s->groups = s->lanes < 256 ? 256 / s->lanes : 1;
+  return true;
+}
+
+// Blocks of KERNEL that are resident on the device at a time (at most LN_BLOCKS_PER_SM per SM), asked once per device and
+// block size; the kernel may use `smem` bytes of shared memory.
+template <auto KERNEL>
+cudaError_t norm_resident(int threads, size_t smem, int* blocks) {
+  static std::atomic<int> known[64][LN_THREADS / 32 + 1];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool keep = dev >= 0 && dev < 64;
+  int per_sm = keep ? known[dev][threads / 32].load(std::memory_order_acquire) : 0;
+  if (per_sm == 0) {
+    if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, LN_SMEM)) != cudaSuccess) return e;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, threads, smem)) != cudaSuccess) return e;
+    per_sm = per_sm < 1 ? 1 : per_sm > LN_BLOCKS_PER_SM ? LN_BLOCKS_PER_SM : per_sm;
+    if (keep) known[dev][threads / 32].store(per_sm, std::memory_order_release);
+  }
+  *blocks = per_sm * sb_sm_count();
+  return cudaSuccess;
+}
+
+int norm_grid(const NormArgs& a, const NormShape& s, int r, int most) {
+  const long long at_once = (long long)r * s.groups, want = (a.rows + at_once - 1) / at_once;
+  return (int)(want < most ? want : most);
+}
+
+template <typename T, int V, int NV, int R>
+bool try_norm(const NormArgs& a, cudaStream_t s, cudaError_t* e) {
+  NormShape shape;
+  if (!norm_shape(a.cols, V, NV, &shape)) return false;
+  const int threads = shape.lanes * shape.groups;
+  const size_t smem = LnAhead<T, V, NV, R, 1, LN_DEPTH>::bytes(threads);
+  int blocks = 0;
+  if ((*e = norm_resident<layer_norm_kernel<T, V, NV, R>>(threads, smem, &blocks)) == cudaSuccess)
+    *e = sb_launch(layer_norm_kernel<T, V, NV, R>, dim3(norm_grid(a, shape, R, blocks)), dim3(threads), smem, s, 1, a, shape);
+  return true;
+}
+
+// Pack width of rows and weights: 16 bytes, 4 bytes, or one element.
+int norm_width(int v, int item, const NormArgs& a) {
+  if (v * item == 16 && (reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) % 16 == 0) return v;
+  return v * item >= 4 ? 4 / item : 1;
 }
 
 template <typename T>
-cudaError_t launch_norm_grad(const NormArgs& a, cudaStream_t s) {
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
+  constexpr int MOST = 16 / sizeof(T), WORD = 4 / sizeof(T);
+  int v = sb_vector_width(a.x, a.ldx, a.cols, sizeof(T), MOST);
+  v = norm_width(sb_vector_width(a.out, a.ldout, a.cols, sizeof(T), v), sizeof(T), a);
+  cudaError_t e = cudaSuccess;
+  if (v == MOST) {
+    if (a.cols <= 32 * MOST && try_norm<T, MOST, 1, 2>(a, s, &e)) return e;
+    if (try_norm<T, MOST, 4, 1>(a, s, &e)) return e;
+  } else if (v == WORD && WORD > 1) {
+    if (a.cols <= 128 * WORD && try_norm<T, WORD, 4, 2>(a, s, &e)) return e;
+    if (try_norm<T, WORD, 16, 1>(a, s, &e)) return e;
+  } else {
+    if (a.cols <= 128 && try_norm<T, 1, 4, 2>(a, s, &e)) return e;
+    if (try_norm<T, 1, 16, 1>(a, s, &e)) return e;
+  }
   const int threads = a.cols >= 1024 ? 1024 : (a.cols + 31) / 32 * 32;
   const long long most = 16LL * sb_sm_count();
-  const int grid = (int)(a.rows < most ? a.rows : most);
-  return sb_launch(layer_norm_grad_wide_kernel<T>, dim3(grid), dim3(threads), 0, s, 1, a);
+  return sb_launch(layer_norm_wide_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(threads), 0, s, 1, a);
+}
+
+// Writes the partial sums' number to *parts where the row fits into registers.
+template <typename T, int V, int NV, int R>
+bool try_norm_grad(const NormArgs& a, cudaStream_t s, cudaError_t* e, int* parts) {
+  NormShape shape;
+  if (!norm_shape(a.cols, V, NV, &shape)) return false;
+  const int threads = shape.lanes * shape.groups;
+  const size_t ahead = LnAhead<T, V, NV, R, 2, LN_DEPTH>::bytes(threads);
+  const size_t sums = shape.groups > 1 ? 2 * sizeof(float) * (size_t)a.cols : 0;   // at most 16 KB: two groups share 256 threads
+  const size_t smem = ahead > sums ? ahead : sums;
+  int blocks = 0;
+  if ((*e = norm_resident<layer_norm_grad_kernel<T, V, NV, R>>(threads, smem, &blocks)) != cudaSuccess) return true;
+  *parts = norm_grid(a, shape, R, blocks);
+  *e = sb_launch(layer_norm_grad_kernel<T, V, NV, R>, dim3(*parts), dim3(threads), smem, s, 1, a, shape);
+  return true;
+}
+
+template <typename T>
+cudaError_t launch_norm_grad(const NormArgs& a, cudaStream_t s, int* parts) {
+  constexpr int MOST = 16 / sizeof(T), WORD = 4 / sizeof(T);
+  int v = sb_vector_width(a.x, a.ldx, a.cols, sizeof(T), MOST);
+  v = sb_vector_width(a.dy, a.lddy, a.cols, sizeof(T), v);
+  if (a.out) v = sb_vector_width(a.out, a.ldout, a.cols, sizeof(T), v);
+  v = norm_width(v, sizeof(T), a);
+  cudaError_t e = cudaSuccess;
+  // Short rows two at a time (65536 x 1024 fp32 147 -> 127 us, bf16 82 -> 80, against one pack per thread and more warps per row).
+  if (v == MOST) {
+    if (a.cols <= 64 * MOST && try_norm_grad<T, MOST, 1, 2>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, MOST, 2, 1>(a, s, &e, parts)) return e;
+  } else if (v == WORD && WORD > 1) {
+    if (try_norm_grad<T, WORD, 4, 1>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, WORD, 8, 1>(a, s, &e, parts)) return e;
+  } else {
+    if (try_norm_grad<T, 1, 8, 1>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, 1, 16, 1>(a, s, &e, parts)) return e;
+  }
+  *parts = 0;
+  if (!a.out) return cudaSuccess;
+  const int threads = a.cols >= 1024 ? 1024 : (a.cols + 31) / 32 * 32;
+  const long long most = 16LL * sb_sm_count();
+  e = sb_launch(layer_norm_grad_wide_kernel<T>, dim3((unsigned)(a.rows < most ? a.rows : most)), dim3(threads), 0, s, 1, a);
+  SB_COUNT_LAUNCH();
+  return e;
 }
 
 }  // namespace
@@ -248,20 +762,22 @@ int sb_layer_norm_grad(const void* dy, long long lddy, const void* x, long long 
   a.x = x; a.dy = dy; a.out = dx; a.weight = weight; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
   a.partial = (float*)workspace; a.rows = rows; a.ldx = ldx; a.lddy = lddy; a.ldout = lddx; a.cols = cols;
   a.inv_cols = 1.f / (float)cols;
-  if (dx) {
-    cudaError_t e = dtype == SB_F32 ? launch_norm_grad<float>(a, s)
-                                    : dtype == SB_BF16 ? launch_norm_grad<__nv_bfloat16>(a, s) : launch_norm_grad<__half>(a, s);
-    SB_COUNT_LAUNCH();
-    SB_CUDA(e);
-  }
+  if (!columns) a.partial = nullptr;
+  int parts = 0;
+  cudaError_t e = dtype == SB_F32 ? launch_norm_grad<float>(a, s, &parts)
+                                  : dtype == SB_BF16 ? launch_norm_grad<__nv_bfloat16>(a, s, &parts) : launch_norm_grad<__half>(a, s, &parts);
+  SB_CUDA(e);
+  if (parts > 0) SB_COUNT_LAUNCH();
   if (columns) {
-    const int parts = ln_columns_blocks(rows);
-    const dim3 grid((cols + 255) / 256, parts);
-    cudaError_t e = dtype == SB_F32 ? sb_launch(layer_norm_columns_kernel<float>, grid, dim3(256), 0, s, 1, a)
-                    : dtype == SB_BF16 ? sb_launch(layer_norm_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, 1, a)
-                                       : sb_launch(layer_norm_columns_kernel<__half>, grid, dim3(256), 0, s, 1, a);
-    SB_COUNT_LAUNCH();
-    SB_CUDA(e);
+    if (parts == 0) {
+      parts = ln_columns_blocks(rows);
+      const dim3 grid((cols + 255) / 256, parts);
+      e = dtype == SB_F32 ? sb_launch(layer_norm_columns_kernel<float>, grid, dim3(256), 0, s, 1, a)
+          : dtype == SB_BF16 ? sb_launch(layer_norm_columns_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, 1, a)
+                             : sb_launch(layer_norm_columns_kernel<__half>, grid, dim3(256), 0, s, 1, a);
+      SB_COUNT_LAUNCH();
+      SB_CUDA(e);
+    }
     e = sb_launch(layer_norm_partials_kernel, dim3((cols + 31) / 32, 2), dim3(1024), 0, s, 1, (const float*)workspace, parts, cols,
                   dweight, dbias, accumulate);
     SB_COUNT_LAUNCH();
