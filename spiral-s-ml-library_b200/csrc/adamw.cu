@@ -59,8 +59,6 @@ struct AdamwTable {
   AdamwHyper h;
 };
 
-typedef unsigned long long Pair2;   // two fp32 values
-
 __device__ __forceinline__ uint32_t aw_noise(uint32_t index, uint32_t salted_seed) {
   uint32_t u = index * AW_K1 + salted_seed;
   u = (u ^ (u >> 16)) * AW_K3;
@@ -86,20 +84,33 @@ __device__ __forceinline__ void aw_update(const AdamwHyper& h, float& p, float g
   p = __fsub_rn(__fmul_rn(p, h.keep), __fmul_rn(d, h.step));
 }
 
-// The same for two neighbours, two products or sums per instruction (each half rounds as the scalar form).
+// The same for two neighbours, two products per instruction; the sums stay scalar, because the assembler joins packed products
+// and packed sums into multiply-adds, which round once instead of twice.
+__device__ __forceinline__ void aw_scale2(float* x, const float* a, float b) {
+  unpack_f32x2(mul_f32x2(pack_f32x2(a[0], a[1]), pack_f32x2(b, b)), x[0], x[1]);
+}
 __device__ __forceinline__ void aw_update2(const AdamwHyper& h, float* p, float* g, float* m, float* v, float* r) {
-  const Pair2 b1 = pack_f32x2(h.b1, h.b1), c1 = pack_f32x2(h.c1, h.c1), b2 = pack_f32x2(h.b2, h.b2), c2 = pack_f32x2(h.c2, h.c2);
-  const Pair2 g2 = mul_f32x2(pack_f32x2(g[0], g[1]), pack_f32x2(h.grad_scale, h.grad_scale));
-  const Pair2 m2 = add_f32x2(mul_f32x2(pack_f32x2(m[0], m[1]), b1), mul_f32x2(g2, c1));
-  const Pair2 v2 = add_f32x2(mul_f32x2(pack_f32x2(v[0], v[1]), b2), mul_f32x2(mul_f32x2(g2, c2), g2));
-  unpack_f32x2(m2, m[0], m[1]);
-  unpack_f32x2(v2, v[0], v[1]);
-  r[0] = __fsqrt_rn(v[0]);
-  r[1] = __fsqrt_rn(v[1]);
-  float den[2];
-  unpack_f32x2(add_f32x2(mul_f32x2(pack_f32x2(r[0], r[1]), pack_f32x2(h.unbias, h.unbias)), pack_f32x2(h.eps, h.eps)), den[0], den[1]);
-  const Pair2 d2 = pack_f32x2(__fdiv_rn(m[0], den[0]), __fdiv_rn(m[1], den[1]));
-  unpack_f32x2(sub_f32x2(mul_f32x2(pack_f32x2(p[0], p[1]), pack_f32x2(h.keep, h.keep)), mul_f32x2(d2, pack_f32x2(h.step, h.step))), p[0], p[1]);
+  float a[2], b[2], d[2];
+  aw_scale2(g, g, h.grad_scale);
+  aw_scale2(a, m, h.b1);
+  aw_scale2(b, g, h.c1);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) m[k] = __fadd_rn(a[k], b[k]);
+  aw_scale2(a, v, h.b2);
+  aw_scale2(b, g, h.c2);
+  unpack_f32x2(mul_f32x2(pack_f32x2(b[0], b[1]), pack_f32x2(g[0], g[1])), b[0], b[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    v[k] = __fadd_rn(a[k], b[k]);
+    r[k] = __fsqrt_rn(v[k]);
+  }
+  aw_scale2(a, r, h.unbias);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) d[k] = __fdiv_rn(m[k], __fadd_rn(a[k], h.eps));
+  aw_scale2(a, p, h.keep);
+  aw_scale2(b, d, h.step);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) p[k] = __fsub_rn(a[k], b[k]);
 }
 
 __device__ __forceinline__ float aw_round_tf32(float v) {

@@ -201,6 +201,17 @@ def test_sizes_of_nothing_need_no_device(sb):
     _lib.call("sb_matmul_fp8", None, 0, None, None, 0, None, None, 0, 0, 8, 16, 0, 0, None, None)
 
 
+def test_workspaces_of_any_size(sb):
+    """Nothing, one of a kind, the limits: an answer, and for more a refusal."""
+    p = sb.primitives
+    for n, vocab, dim in ((0, 5, 8), (3, 0, 8), (3, 5, 0), (1, 1, 1), (5, 3, 100000), (1 << 30, 1, 1), (1, 1 << 30, 1), (1 << 30, 1 << 30, 1)):
+        assert p.embedding_grad_workspace(n, vocab, dim) >= 0
+    for rows, cols in ((0, 5), (5, 0), (1, 1), (1 << 40, 3), (1, 1 << 30)):
+        assert p.layer_norm_grad_workspace(rows, cols) >= 0
+    with pytest.raises(sb.SpiralError):
+        p.embedding_grad_workspace((1 << 30) + 1, 4, 4)
+
+
 def test_e4m3_conversions(sb):
     """All codes there and back; halves go to even; beyond the range the largest value."""
     from spiral_b200 import dtypes
