@@ -58,8 +58,7 @@ SortPlan sort_plan(long long n, int vocab) {
   while (bits < 31 && (1LL << bits) <= vocab) ++bits;
   p.passes = (bits + ES_MAX_BITS - 1) / ES_MAX_BITS;
   p.bits = (bits + p.passes - 1) / p.passes;
-  // Chunks of 1024 tokens until there are several per SM, then of 4096.
-  p.rounds = n > 1024LL * 4 * sb_sm_count() ? 16 : 4;
+  p.rounds = 16;
   p.chunk = ES_THREADS * p.rounds;
   p.chunks = (int)((n + p.chunk - 1) / p.chunk);
   return p;
@@ -71,17 +70,63 @@ struct SortArgs {
   const int* pos_in;
   int* keys_out;
   int* pos_out;
-  int* counts;                   // [bins][chunks], turned into the bin's running sums by the scan
+  int* counts;                   // [chunks][bins], turned into the bins' running sums by the scan
   int* totals;                   // [bins]
   int n, vocab, shift, bits, chunks, chunk;
   int index64;
 };
 
-template <bool FIRST>
-__device__ __forceinline__ int sort_key(const SortArgs& a, int i) {
-  if (!FIRST) return a.keys_in[i];
-  const long long t = a.index64 ? ((const long long*)a.tokens)[i] : (long long)((const int*)a.tokens)[i];
-  return t >= 0 && t < a.vocab ? (int)t : a.vocab;
+// N tokens of a thread, `stride` apart, all on their way before the first is looked at (loads and comparisons in turn follow
+// one another: 4096 tokens per block took 14 us, nearly all of it 16 latencies): -1 behind the end, vocab for no token.
+struct TokenWords {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ void load_token(TokenWords& w, const void* tokens, long long i, bool index64, bool issue) {
+  w.lo = w.hi = 0u;
+  if (index64)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t@p ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
+                 : "+r"(w.lo), "+r"(w.hi) : "l"((const char*)tokens + i * 8), "r"((uint32_t)issue));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}"
+                 : "+r"(w.lo) : "l"((const char*)tokens + i * 4), "r"((uint32_t)issue));
+}
+// The token, or `none` for one outside [0, vocab).
+__device__ __forceinline__ int token_of(const TokenWords& w, bool index64, int vocab, int none) {
+  return w.lo < (uint32_t)vocab && (!index64 || w.hi == 0u) ? (int)w.lo : none;
+}
+template <int N>
+__device__ __forceinline__ void load_keys(int (&key)[N], const SortArgs& a, int first, int stride, int end) {
+  TokenWords w[N];
+  if (a.index64) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) load_token(w[k], a.tokens, first + k * stride, true, first + k * stride < end);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) load_token(w[k], a.tokens, first + k * stride, false, first + k * stride < end);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) key[k] = first + k * stride < end ? token_of(w[k], a.index64 != 0, a.vocab, a.vocab) : -1;
+}
+// The same of an earlier pass's keys or positions (not through the read-only path: the kernel may have written them).
+template <int N>
+__device__ __forceinline__ void load_pairs(int (&v)[N], const int* from, int first, int stride, int end) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    v[k] = -1;
+    const bool issue = first + k * stride < end;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.cg.b32 %0, [%1];\n\t}"
+                 : "+r"(v[k]) : "l"(from + (issue ? first + k * stride : 0)), "r"((uint32_t)issue) : "memory");
+  }
+}
+
+// The lanes of a warp whose digit of `bits` bits is this one's (a lane without a token has digit 1 << bits): a vote per bit.
+__device__ __forceinline__ unsigned same_digit(int digit, int bits) {
+  unsigned same = 0xffffffffu;
+  for (int b = 0; b <= bits; ++b) {
+    const unsigned set = __ballot_sync(0xffffffffu, (digit >> b) & 1);
+    same &= (digit >> b) & 1 ? set : ~set;
+  }
+  return same;
 }
 
 template <bool FIRST>
@@ -94,14 +139,17 @@ __global__ void __launch_bounds__(ES_THREADS) token_count_kernel(SortArgs a) {
   __syncthreads();
   // Equal digits of a warp are added as one: with the 53 tokens of a deck most lanes of a warp meet in a few words.
   const int first = blockIdx.x * a.chunk, last = min(a.n - first, a.chunk) + first;
-  for (int i0 = first; i0 < last; i0 += ES_THREADS) {
-    const int i = i0 + threadIdx.x;
-    const int digit = i < last ? (sort_key<FIRST>(a, i) >> a.shift) & (bins - 1) : bins;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+  int key[16];                   // all on their way at once
+  if (FIRST) load_keys<16>(key, a, first + (int)threadIdx.x, ES_THREADS, last);
+  else load_pairs<16>(key, a.keys_in, first + (int)threadIdx.x, ES_THREADS, last);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int digit = key[k] < 0 ? bins : (key[k] >> a.shift) & (bins - 1);
+    const unsigned same = same_digit(digit, a.bits);
     if (digit < bins && (same & ((1u << (threadIdx.x & 31)) - 1u)) == 0u) atomicAdd(&hist[digit], __popc(same));
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += ES_THREADS) a.counts[(long long)b * a.chunks + blockIdx.x] = hist[b];
+  for (int b = threadIdx.x; b < bins; b += ES_THREADS) a.counts[(long long)blockIdx.x * bins + b] = hist[b];
 }
 
 __device__ __forceinline__ int warp_inclusive(int v) {
@@ -114,25 +162,33 @@ __device__ __forceinline__ int warp_inclusive(int v) {
   return v;
 }
 
-// A warp per bin: running sums of its counts over the chunks, and its total.
-__global__ void __launch_bounds__(256) token_scan_kernel(SortArgs a) {
+// Running sums of the bins' counts over the chunks, and their totals: 32 neighbouring bins per block, each of its 32 warps a
+// run of chunks.
+__global__ void __launch_bounds__(1024) token_scan_kernel(SortArgs a) {
+  __shared__ int part[32][33];
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const int bin = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (bin >= (1 << a.bits)) return;
-  int* c = a.counts + (long long)bin * a.chunks;
+  const int bins = 1 << a.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bin = blockIdx.x * 32 + lane;
+  const int per = (a.chunks + 31) / 32, from = min(a.chunks, warp * per), to = min(a.chunks, from + per);
+  int sum = 0;
+  if (bin < bins)
+    for (int c = from; c < to; ++c) sum += a.counts[(long long)c * bins + bin];
+  part[warp][lane] = sum;
+  __syncthreads();
   int before = 0;
-  for (int i0 = 0; i0 < a.chunks; i0 += 32) {
-    const int v = i0 + lane < a.chunks ? c[i0 + lane] : 0;
-    const int up = warp_inclusive(v);
-    if (i0 + lane < a.chunks) c[i0 + lane] = before + up - v;
-    before += __shfl_sync(0xffffffffu, up, 31);
+  for (int w = 0; w < warp; ++w) before += part[w][lane];
+  if (bin >= bins) return;
+  for (int c = from; c < to; ++c) {
+    int* at = a.counts + (long long)c * bins + bin;
+    const int here = *at;
+    *at = before;
+    before += here;
   }
-  if (lane == 0) a.totals[bin] = before;
+  if (warp == 31) a.totals[bin] = before;
 }
 
 // Puts a chunk's (token, position) pairs where they belong by this digit, those of equal digits in their order: a warp
-// takes a run of consecutive tokens 32 at a time; equal digits within the 32 find each other by a match.
+// takes a run of consecutive tokens 32 at a time; equal digits within the 32 find each other by votes.
 template <bool FIRST, int ROUNDS>
 __global__ void __launch_bounds__(ES_THREADS) token_scatter_kernel(SortArgs a) {
   extern __shared__ int s_scatter[];
@@ -144,38 +200,41 @@ __global__ void __launch_bounds__(ES_THREADS) token_scatter_kernel(SortArgs a) {
   for (int b = threadIdx.x; b < bins * ES_WARPS; b += ES_THREADS) seen[b] = 0;
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  // Exclusive sums of the bins' totals: each thread a run of bins.
+  // Exclusive sums of the bins' totals: each thread a run of at most 8 bins.
+  constexpr int PER = ES_MAX_BINS / ES_THREADS;
   const int per = (bins + ES_THREADS - 1) / ES_THREADS;
-  int mine = 0;
-  for (int k = 0; k < per; ++k) {
+  int total[PER], before_me[PER], mine = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
     const int b = threadIdx.x * per + k;
-    if (b < bins) mine += a.totals[b];
+    const bool in = k < per && b < bins;
+    total[k] = in ? a.totals[b] : 0;
+    before_me[k] = in ? a.counts[(long long)blockIdx.x * bins + b] : 0;
+    mine += total[k];
   }
   const int incl = warp_inclusive(mine);
   if (lane == 31) warp_total[warp] = incl;
   __syncthreads();
   int run = incl - mine;
   for (int w = 0; w < warp; ++w) run += warp_total[w];
-  for (int k = 0; k < per; ++k) {
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
     const int b = threadIdx.x * per + k;
-    if (b < bins) {
-      base[b] = run + a.counts[(long long)b * a.chunks + blockIdx.x];
-      run += a.totals[b];
-    }
+    if (k < per && b < bins) base[b] = run + before_me[k];
+    run += total[k];
   }
   const int first = blockIdx.x * a.chunk + warp * (32 * ROUNDS);
   int key[ROUNDS];
   unsigned short rank[ROUNDS];
   unsigned short* mine_seen = seen + warp * bins;
-#pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int i = first + k * 32 + lane;
-    key[k] = i >= 0 && i < a.n ? sort_key<FIRST>(a, i) : -1;
-  }
+  if (FIRST) load_keys<ROUNDS>(key, a, first + lane, 32, a.n);
+  else load_pairs<ROUNDS>(key, a.keys_in, first + lane, 32, a.n);
+  int pos[ROUNDS];
+  if (!FIRST) load_pairs<ROUNDS>(pos, a.pos_in, first + lane, 32, a.n);
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
     const int digit = key[k] < 0 ? bins : (key[k] >> a.shift) & (bins - 1);
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    const unsigned same = same_digit(digit, a.bits);
     const int before = __popc(same & ((1u << lane) - 1u));
     if (digit < bins) rank[k] = (unsigned short)(mine_seen[digit] + before);
     __syncwarp();
@@ -200,85 +259,124 @@ __global__ void __launch_bounds__(ES_THREADS) token_scatter_kernel(SortArgs a) {
     const int digit = (key[k] >> a.shift) & (bins - 1);
     const int to = base[digit] + mine_seen[digit] + rank[k];
     a.keys_out[to] = key[k];
-    a.pos_out[to] = FIRST ? i : a.pos_in[i];
+    a.pos_out[to] = FIRST ? i : pos[k];
   }
 }
 
-// Up to ES_SMALL tokens: one block sorts them in shared memory, 8 bits at a time.
+// Up to ES_CLUSTER (98304) tokens in one launch: the blocks of a cluster hold the tokens in registers, at most 10 bits at a time;
+// their counts meet in shared memory across the cluster, the pairs go through the workspace (L2).  The whole gradient of 64
+// fp32 columns, 16384 / 65537 tokens of 50001: 27 / 37 us, 42 / 46 with two passes of three launches; 131072 of 2000 41 us, 34 with one
+// such pass.  Up to ES_SMALL tokens a single block.
 constexpr int ES_SMALL = 4096;
-constexpr int ES_SMALL_THREADS = 1024;
-__global__ void __launch_bounds__(ES_SMALL_THREADS) token_sort_small_kernel(SortArgs a, int bits) {
-  constexpr int BINS = 256, WARPS = ES_SMALL_THREADS / 32, ROUNDS = ES_SMALL / ES_SMALL_THREADS;
-  extern __shared__ int s_sort[];
-  int* keys = s_sort;
-  unsigned short* pos = reinterpret_cast<unsigned short*>(keys + ES_SMALL);
-  unsigned short* seen = pos + ES_SMALL;                     // [warps][bins]
-  __shared__ int base[BINS], warp_total[BINS / 32];
+constexpr int ES_BLOCKS = 16;                                // more than the 8 that every GPU takes; B200 does
+constexpr int ES_ROUNDS = 6;
+constexpr int ES_CLUSTER_THREADS = 1024;
+constexpr int ES_CLUSTER_BITS = 10;                          // of a digit, at most: a bin per thread
+constexpr int ES_CLUSTER = ES_BLOCKS * ES_ROUNDS * ES_CLUSTER_THREADS;
+__global__ void __launch_bounds__(ES_CLUSTER_THREADS) token_sort_kernel(SortArgs a, int* keys, int* pos, int bits, int rounds) {
+  constexpr int WARPS = ES_CLUSTER_THREADS / 32;
+  __shared__ int totals[ES_CLUSTER_THREADS], base[ES_CLUSTER_THREADS], here[ES_CLUSTER_THREADS], warp_total[2][WARPS];
+  extern __shared__ int s_pairs[];                           // this block's pairs in the order of the digit
+  int* s_key = s_pairs;
+  int* s_pos = s_pairs + ES_CLUSTER_THREADS * rounds;
+  const int bins = 1 << a.bits;                              // a thread each
+  unsigned short* seen = reinterpret_cast<unsigned short*>(s_pos + ES_CLUSTER_THREADS * rounds);   // [warps][bins]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned short* mine = seen + warp * bins;
+  const int rank = blockIdx.x, blocks = gridDim.x;           // the grid is one cluster
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  int key[ROUNDS], at[ROUNDS];
-#pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    at[k] = warp * (32 * ROUNDS) + k * 32 + lane;
-    key[k] = at[k] < a.n ? sort_key<true>(a, at[k]) : -1;
-  }
-  for (int shift = 0; shift < bits; shift += 8) {
-    for (int b = threadIdx.x; b < BINS * WARPS / 2; b += ES_SMALL_THREADS) reinterpret_cast<int*>(seen)[b] = 0;
+  const int first = (rank * ES_CLUSTER_THREADS + warp * 32) * rounds + lane;
+  int key[ES_ROUNDS];
+  unsigned short rank_in[ES_ROUNDS];
+  int turn = 0;
+  for (int shift = 0; shift < bits; shift += a.bits, turn ^= 1) {
+    const int* pos_in = pos + (turn ? 0 : a.n);
+    int* keys_out = keys + (turn ? a.n : 0);
+    int* pos_out = pos + (turn ? a.n : 0);
+    const int end = min(a.n, first - lane + 32 * rounds);
+    if (shift == 0) load_keys<ES_ROUNDS>(key, a, first, 32, end);
+    else load_pairs<ES_ROUNDS>(key, keys + (turn ? 0 : a.n), first, 32, end);
+    for (int b = threadIdx.x; b < bins * WARPS / 2; b += ES_CLUSTER_THREADS) reinterpret_cast<int*>(seen)[b] = 0;
     __syncthreads();
-    unsigned short rank[ROUNDS];
-    unsigned short* mine = seen + warp * BINS;
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-      const int digit = key[k] < 0 ? BINS : (key[k] >> shift) & (BINS - 1);
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
+    for (int k = 0; k < ES_ROUNDS; ++k) {
+      if (k >= rounds) break;
+      const int digit = key[k] < 0 ? bins : (key[k] >> shift) & (bins - 1);
+      const unsigned same = same_digit(digit, a.bits);
       const int before = __popc(same & ((1u << lane) - 1u));
-      if (digit < BINS) rank[k] = (unsigned short)(mine[digit] + before);
+      if (digit < bins) rank_in[k] = (unsigned short)(mine[digit] + before);
       __syncwarp();
-      if (digit < BINS && before == 0) mine[digit] = (unsigned short)(mine[digit] + __popc(same));
+      if (digit < bins && before == 0) mine[digit] = (unsigned short)(mine[digit] + __popc(same));
       __syncwarp();
     }
     __syncthreads();
-    int total = 0, incl = 0;
-    if (threadIdx.x < BINS) {
+    if ((int)threadIdx.x < bins) {
+      int total = 0;
 #pragma unroll 8
       for (int w = 0; w < WARPS; ++w) {
-        const int c = seen[w * BINS + threadIdx.x];
-        seen[w * BINS + threadIdx.x] = (unsigned short)total;
+        const int c = seen[w * bins + threadIdx.x];
+        seen[w * bins + threadIdx.x] = (unsigned short)total;
         total += c;
       }
-      incl = warp_inclusive(total);
-      if (lane == 31) warp_total[warp] = incl;
+      totals[threadIdx.x] = total;
     }
-    __syncthreads();
-    if (threadIdx.x < BINS) {
-      int run = incl - total;
-      for (int w = 0; w < warp; ++w) run += warp_total[w];
-      base[threadIdx.x] = run;
-    }
-    __syncthreads();
+    __syncwarp();
+    if (blocks > 1) cluster_sync_all(); else __syncthreads();
+    // Where this block's tokens of each digit begin: among all (base) and among its own (here).
+    int all = 0, before = 0, own = 0, incl = 0, own_incl = 0;
+    if ((int)threadIdx.x < bins) {
+      all = own = totals[threadIdx.x];
+      if (blocks > 1) {
+        int c[ES_BLOCKS];
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k)
+        for (int r = 0; r < ES_BLOCKS; ++r)
+          asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c[r]) : "r"(map_to_cta(smem_u32(&totals[threadIdx.x]), (uint32_t)r)) : "memory");
+        all = 0;
+#pragma unroll
+        for (int r = 0; r < ES_BLOCKS; ++r) {
+          before += r < rank ? c[r] : 0;
+          all += c[r];
+        }
+      }
+    }
+    incl = warp_inclusive(all);
+    own_incl = warp_inclusive(own);
+    if (lane == 31) {
+      warp_total[0][warp] = incl;
+      warp_total[1][warp] = own_incl;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < bins) {
+      int run = incl - all, own_run = own_incl - own;
+      for (int w = 0; w < warp; ++w) {
+        run += warp_total[0][w];
+        own_run += warp_total[1][w];
+      }
+      base[threadIdx.x] = run + before - own_run;
+      here[threadIdx.x] = own_run;
+    }
+    __syncthreads();
+    int at[ES_ROUNDS];
+    if (shift != 0) load_pairs<ES_ROUNDS>(at, pos_in, first, 32, end);
+    // Through shared memory, so that tokens of one digit leave side by side: a scattered 4-byte store costs a clock per lane.
+#pragma unroll
+    for (int k = 0; k < ES_ROUNDS; ++k)
       if (key[k] >= 0) {
-        const int digit = (key[k] >> shift) & (BINS - 1), to = base[digit] + mine[digit] + rank[k];
-        keys[to] = key[k];
-        pos[to] = (unsigned short)at[k];
+        const int i = first + k * 32, digit = (key[k] >> shift) & (bins - 1), to = here[digit] + mine[digit] + rank_in[k];
+        s_key[to] = key[k];
+        s_pos[to] = shift == 0 ? i : at[k];
       }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < ROUNDS; ++k) {
-      const int i = warp * (32 * ROUNDS) + k * 32 + lane;
-      key[k] = i < a.n ? keys[i] : -1;
-      at[k] = i < a.n ? pos[i] : 0;
+    const int block_first = rank * ES_CLUSTER_THREADS * rounds, count = min(a.n - block_first, ES_CLUSTER_THREADS * rounds);
+    for (int j = threadIdx.x; j < count; j += ES_CLUSTER_THREADS) {
+      const int k = s_key[j], to = base[(k >> shift) & (bins - 1)] + j;
+      keys_out[to] = k;
+      pos_out[to] = s_pos[j];
     }
-  }
-#pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) {
-    const int i = warp * (32 * ROUNDS) + k * 32 + lane;
-    if (i < a.n) {
-      a.keys_out[i] = key[k];
-      a.pos_out[i] = at[k];
-    }
+    // The pairs are where the next pass reads them, and nobody reads this block's totals any more.
+    __syncwarp();
+    if (blocks > 1) cluster_sync_all(); else __syncthreads();
   }
 }
 
@@ -288,11 +386,12 @@ struct GradArgs {
   const int* pos;
   const void* dout;
   float* dtable;
-  float* carry;                  // [runs][dim]: what a run adds to the row that it leaves unfinished
-  int* run_key;                  // [runs + 1]: tokens consumed where a run begins
+  float* carry;                  // [parts][dim]: what a block's part of the walk adds to the row that it leaves unfinished
+  int* part_key;                 // [parts + 1]: tokens consumed where a part begins
   long long ld_dout, ld_dtable;
   int n, vocab, dim;
-  int run_len, runs;             // steps (rows read + rows written) per run
+  int run_len;                   // steps (rows read + rows written) per run
+  int parts, part_len;           // blocks, and steps of each
   int group;                     // threads that share a run
   float scale;
   int accumulate;
@@ -321,21 +420,29 @@ __device__ __forceinline__ int walk_split(const int* __restrict__ keys, int n, i
 // while the ones before are added.  (Every group searching the sorted tokens for itself, 17 dependent loads twice, and
 // reading token and position from global memory in the loop: 50001 x 1000 fp32 213 us.)
 template <typename T, int V>
-__global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a) {
+__global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
   constexpr int UNROLL = 8;
-  extern __shared__ int s_walk[];
+  extern __shared__ __align__(16) int s_walk[];
   __shared__ int ends[2];
   const int groups = blockDim.x / a.group;
   const int steps = groups * a.run_len;
-  int* s_key = s_walk;
-  int* s_pos = s_walk + steps;
+  float* s_carry = reinterpret_cast<float*>(s_walk);         // [256][V]: what each run leaves behind
+  int* s_end = s_walk + 256 * V;                             // [groups]: the row that the run ends in
+  int* s_key = s_end + groups;
+  int* s_pos = s_key + steps;
   const long long first = (long long)blockIdx.x * steps, all = (long long)a.n + a.vocab;
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   if (threadIdx.x < 64) {
     const int which = threadIdx.x >> 5;
-    const int k = walk_split(a.keys, a.n, a.vocab, which == 0 ? first : min(first + steps, all));
-    if ((threadIdx.x & 31) == 0) ends[which] = k;
+    const int k = walk_split(a.keys, a.n, a.vocab, min(which == 0 ? first : first + steps, all));
+    if ((threadIdx.x & 31) == 0) {
+      ends[which] = k;
+      if (blockIdx.y == 0) {                                 // of this block's part, and the next one's begin
+        if (which == 0) a.part_key[blockIdx.x] = k;
+        else if (blockIdx.x == gridDim.x - 1) a.part_key[gridDim.x] = k;
+      }
+    }
   }
   __syncthreads();
   const int k_first = ends[0], count = ends[1] - k_first;
@@ -344,10 +451,8 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a) {
     s_pos[i] = a.pos[k_first + i];
   }
   __syncthreads();
-  const int in_group = threadIdx.x % a.group;
-  const int run = blockIdx.x * groups + threadIdx.x / a.group;
+  const int in_group = threadIdx.x % a.group, g = threadIdx.x / a.group;
   const int col = (blockIdx.y * a.group + in_group) * V;
-  if (run >= a.runs) return;
   // The run's own part, by halves.
   auto split = [&](long long d) {
     int lo = (int)max(0LL, d - a.vocab - k_first), hi = (int)min((long long)count, d - k_first);
@@ -358,17 +463,13 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a) {
     }
     return lo;
   };
-  const long long d0 = (long long)run * a.run_len, d1 = min(d0 + a.run_len, all);
+  const long long d0 = min(first + (long long)g * a.run_len, all), d1 = min(d0 + a.run_len, all);
   int k = split(d0);
   const int k_end = split(d1);
-  if (blockIdx.y == 0 && in_group == 0) {
-    a.run_key[run] = k_first + k;
-    if (run == a.runs - 1) a.run_key[a.runs] = k_first + k_end;
-  }
-  if (col >= a.dim) return;
-  int row = (int)(d0 - (k_first + k));
-  const int row_end = (int)(d1 - (k_first + k_end));
-  const T* dout = (const T*)a.dout + col;
+  const int row0 = (int)(d0 - (k_first + k)), row_end = (int)(d1 - (k_first + k_end));
+  const bool active = col < a.dim;
+  int row = row0;
+  const T* dout = (const T*)a.dout + (active ? col : 0);
   float* to = a.dtable + (long long)row * a.ld_dtable + col;
   float acc[V];
 #pragma unroll
@@ -391,35 +492,62 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(GradArgs a) {
     to += a.ld_dtable;
     ++row;
   };
-  while (k < k_end) {
-    SbPack<T, V> in[UNROLL];
-    int key[UNROLL];
+  if (active) {
+    while (k < k_end) {
+      SbWords<sizeof(T) * V> in[UNROLL] = {};
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      key[u] = k + u < k_end ? s_key[k + u] : a.vocab;
-      if (key[u] < a.vocab) in[u] = sb_load_pack<T, V>(dout + (long long)s_pos[k + u] * a.ld_dout);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      if (key[u] < a.vocab) {
-        while (row < key[u]) finish();
-        float v[V];
-        sb_unpack<T, V>(in[u], v);
-#pragma unroll
-        for (int t = 0; t < V; ++t) acc[t] += v[t];
+      for (int u = 0; u < UNROLL; ++u) {
+        const bool issue = k + u < k_end && s_key[k + u] < a.vocab;
+        sb_load_words(in[u], dout + (long long)(issue ? s_pos[k + u] : 0) * a.ld_dout, issue);
       }
-    }
-    k += UNROLL;
-  }
-  while (row < row_end) finish();
-  float* carry = a.carry + (long long)run * a.dim + col;
 #pragma unroll
-  for (int t = 0; t < V; ++t) carry[t] = acc[t];
+      for (int u = 0; u < UNROLL; ++u) {
+        const int key = k + u < k_end ? s_key[k + u] : a.vocab;
+        if (key < a.vocab) {
+          while (row < key) finish();
+          float v[V];
+          sb_unpack_words<T, V>(in[u], v);
+#pragma unroll
+          for (int t = 0; t < V; ++t) acc[t] += v[t];
+        }
+      }
+      k += UNROLL;
+    }
+    while (row < row_end) finish();
+  }
+  // What is left belongs to the row that the next run begins in.  Where a run finishes the row that it begins in, it adds
+  // what the block's runs before it left for that row, in their order; the block's last leftover goes to the workspace.
+#pragma unroll
+  for (int t = 0; t < V; ++t) s_carry[threadIdx.x * V + t] = acc[t];
+  if (in_group == 0) s_end[g] = row_end;
+  __syncthreads();
+  if (!active) return;
+  auto leftover = [&](int last, int r, float* sum) {         // of the runs up to `last` that end in row r
+    int from = last;
+    while (from > 0 && s_end[from - 1] == r) --from;
+#pragma unroll
+    for (int t = 0; t < V; ++t) sum[t] = 0.f;
+    for (int h = from; h <= last; ++h)
+#pragma unroll
+      for (int t = 0; t < V; ++t) sum[t] += s_carry[(h * a.group + in_group) * V + t];
+  };
+  float sum[V];
+  if (g > 0 && row_end > row0) {
+    leftover(g - 1, row0, sum);
+    float* at = a.dtable + (long long)row0 * a.ld_dtable + col;
+#pragma unroll
+    for (int t = 0; t < V; ++t) at[t] += sum[t] * a.scale;
+  }
+  if (g == groups - 1) {
+    leftover(g, row_end, sum);
+#pragma unroll
+    for (int t = 0; t < V; ++t) a.carry[(long long)blockIdx.x * a.dim + col + t] = sum[t];
+  }
 }
 
 // A table of few rows needs no sort: every warp (or part of one) adds its share of the positions, in their order, to a table of
 // its own in shared memory, V columns per thread and G x V per block; the block adds its tables up, and the blocks' sums are
-// added in their order by a second launch.  Bound by reading dout: 524288 x 64 bf16 over 53 tokens, PLACEHOLDER.
+// added in their order by a second launch.  Bound by reading dout: 524288 x 64 bf16 over 53 tokens 28 us (floor 11).
 constexpr int EF_THREADS = 512;
 constexpr int EF_SMEM = 200 * 1024;
 struct FewArgs {
@@ -437,50 +565,56 @@ struct FewArgs {
 
 template <typename T, int V>
 __global__ void __launch_bounds__(EF_THREADS) embedding_few_kernel(FewArgs a) {
-  constexpr int UNROLL = 8;
-  extern __shared__ __align__(16) float s_tables[];          // [copies][vocab][lanes * V]
-  const int width = a.lanes * V, table = a.vocab * width;
+  constexpr int UNROLL = 16;                                 // at most `lanes`: as many tokens as one load of the group brings
+  extern __shared__ __align__(16) float s_tables[];          // [copies][vocab + 1][lanes * V]; the last row is for no token
+  const int width = a.lanes * V, table = (a.vocab + 1) * width;
   const int copy = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes;
-  for (int i = threadIdx.x; i < a.copies * table; i += blockDim.x) s_tables[i] = 0.f;
+  for (int i = threadIdx.x; i < a.copies * table / 4; i += EF_THREADS) reinterpret_cast<float4*>(s_tables)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   __syncthreads();
   const int col = (blockIdx.y * a.lanes + lane) * V;
   const long long first = ((long long)blockIdx.x * a.copies + copy) * a.per;
   const int count = (int)max(0LL, min((long long)a.per, a.n - first));
-  if (copy < a.copies && col < a.dim) {
-    float* mine = s_tables + copy * table + lane * V;
-    const T* dout = (const T*)a.dout + first * a.ld_dout + col;
-    for (int i = 0; i < count; i += UNROLL) {
-      SbPack<T, V> in[UNROLL];
-      int token[UNROLL];
+  // Rows do not wait for their tokens, and the next UNROLL of both are on their way while these are added.
+  float* mine = s_tables + copy * table + lane * V;
+  const bool active = col < a.dim;
+  const T* dout = (const T*)a.dout + (active ? first * a.ld_dout + col : 0);
+  struct Ahead {
+    SbWords<sizeof(T) * V> row[UNROLL];
+    TokenWords token;            // lane u holds row u's, as it was read: looking at it would wait for it
+  };
+  auto fetch = [&](Ahead& x, int i) {
+    load_token(x.token, a.tokens, first + i + lane, a.index64 != 0, lane < UNROLL && i + lane < count);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        token[u] = -1;
-        if (i + u < count) {
-          const long long t = a.index64 ? ((const long long*)a.tokens)[first + i + u] : (long long)((const int*)a.tokens)[first + i + u];
-          if (t >= 0 && t < a.vocab) token[u] = (int)t;
-        }
-      }
+    for (int u = 0; u < UNROLL; ++u)
+      sb_load_words(x.row[u], dout + (active ? (long long)(i + u) * a.ld_dout : 0), active && i + u < count);
+  };
+  auto add = [&](const Ahead& x, int i) {
+    const int token = i + lane < count ? token_of(x.token, a.index64 != 0, a.vocab, a.vocab) : a.vocab;
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u)
-        if (token[u] >= 0) in[u] = sb_load_pack<T, V>(dout + u * a.ld_dout);
+    for (int u = 0; u < UNROLL; ++u) {
+      float v[V], t[V];
+      sb_unpack_words<T, V>(x.row[u], v);
+      float* to = mine + __shfl_sync(0xffffffffu, token, u, a.lanes) * width;
+      sb_unpack<float, V>(sb_load_pack<float, V>(to), t);
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u)
-        if (token[u] >= 0) {
-          float v[V], t[V];
-          sb_unpack<T, V>(in[u], v);
-          float* to = mine + token[u] * width;
-          sb_unpack<float, V>(sb_load_pack<float, V>(to), t);
-#pragma unroll
-          for (int k = 0; k < V; ++k) t[k] += v[k];
-          sb_store_f32<float, V>(to, t);
-        }
-      dout += UNROLL * a.ld_dout;
+      for (int k = 0; k < V; ++k) t[k] += v[k];
+      sb_store_f32<float, V>(to, t);
+    }
+  };
+  if (copy < a.copies) {         // whole warps; the others help before and after
+    Ahead x = {}, y = {};        // by turns: a copy from one to the other would wait for the loads
+    fetch(x, 0);
+    for (int i = 0; i < a.per; i += 2 * UNROLL) {            // the same for all
+      fetch(y, i + UNROLL);
+      add(x, i);
+      fetch(x, i + 2 * UNROLL);
+      add(y, i + UNROLL);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < table; i += blockDim.x) {
+  for (int i = threadIdx.x; i < a.vocab * width; i += EF_THREADS) {
     const int row = i / width, c = blockIdx.y * width + i % width;
     if (c >= a.dim) continue;
     float total = 0.f;
@@ -515,41 +649,82 @@ __global__ void __launch_bounds__(1024) embedding_few_join_kernel(FewArgs a, int
   }
 }
 
-// Adds what runs left unfinished to the row that a later run finished: a block of 8 warps per such run and 32 columns; every
-// warp takes a part of the runs before it, in order, and the warps' sums meet in shared memory.
+// Adds what parts of the walk left unfinished to the row that a later part finished.  A warp looks at a part each; where few
+// parts lead up to it, as with all but the commonest tokens, it adds them itself, and the block's warps share the others: every
+// warp a run of the parts, in order, and their sums meet in shared memory.
+template <int V>
+__device__ __forceinline__ void join_add(float* s, const float* from) {
+  float v[V];
+  sb_unpack<float, V>(sb_load_pack<float, V>(from), v);
+#pragma unroll
+  for (int t = 0; t < V; ++t) s[t] += v[t];
+}
+template <int V>
 __global__ void __launch_bounds__(256) embedding_join_kernel(GradArgs a) {
-  __shared__ float sums[8][32];
+  constexpr int FEW = 8;
+  __shared__ float sums[8][32 * V];
+  __shared__ int shared_from[8], shared_to[8], shared_row[8];
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long all = (long long)a.n + a.vocab;
-  for (int run = blockIdx.x + 1; run < a.runs; run += gridDim.x) {
-    const long long d0 = (long long)run * a.run_len, d1 = min(d0 + a.run_len, all);
-    const int k0 = a.run_key[run], row = (int)(d0 - k0), row_end = (int)(d1 - a.run_key[run + 1]);
-    // Only where this run finishes a row that tokens of earlier runs have been added to.
-    if (row >= a.vocab || row_end == row || k0 == 0 || a.keys[k0 - 1] != row) continue;
-    int lo = 0, hi = run;        // the first run that ends in this row
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if ((long long)(mid + 1) * a.run_len - a.run_key[mid + 1] >= row) hi = mid;
-      else lo = mid + 1;
+  const int part = blockIdx.x * 8 + warp + 1;
+  int from = part, row = 0;      // parts from .. part - 1 lead up to it
+  if (part < a.parts) {
+    const long long d0 = (long long)part * a.part_len, d1 = min(d0 + a.part_len, all);
+    const int k0 = a.part_key[part], row_end = (int)(d1 - a.part_key[part + 1]);
+    const int row_before = (int)((long long)(part - 1) * a.part_len - a.part_key[part - 1]);
+    row = (int)(d0 - k0);
+    // Only where this part finishes a row that tokens of earlier parts have been added to.
+    if (row < a.vocab && row_end > row && k0 > 0 && a.keys[k0 - 1] == row) {
+      from = part - 1;
+      if (row_before == row) {   // the part before begins in the same row: look for the first that ends in it
+        int lo = 0, hi = part - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if ((long long)(mid + 1) * a.part_len - a.part_key[mid + 1] >= row) hi = mid;
+          else lo = mid + 1;
+        }
+        from = lo;
+      }
     }
-    const int parts = run - lo, per = (parts + 7) / 8;
-    const int from = lo + warp * per, to = min(run, from + per);
-    for (int c = blockIdx.y * 32 + lane; c < (a.dim + 31) / 32 * 32; c += 32 * gridDim.y) {
-      float s = 0.f;
+  }
+  const bool many = part - from > FEW;
+  if (lane == 0) {
+    shared_from[warp] = many ? from : part;
+    shared_to[warp] = part;
+    shared_row[warp] = row;
+  }
+  if (!many && from < part)
+    for (int c = (blockIdx.y * 32 + lane) * V; c < a.dim; c += 32 * V * gridDim.y) {
+      float s[V] = {};
+      for (int r = from; r < part; ++r) join_add<V>(s, a.carry + (long long)r * a.dim + c);
+      float* to = a.dtable + (long long)row * a.ld_dtable + c;
+#pragma unroll
+      for (int t = 0; t < V; ++t) to[t] += s[t] * a.scale;
+    }
+  __syncthreads();
+  for (int w = 0; w < 8; ++w) {
+    const int begin = shared_from[w], end = shared_to[w], share = (end - begin + 7) / 8;
+    if (begin >= end) continue;
+    const int mine = begin + warp * share, last = min(end, mine + share);
+    for (int c0 = blockIdx.y * 32 * V; c0 < a.dim; c0 += 32 * V * gridDim.y) {
+      const int c = c0 + lane * V;
+      float s[V] = {};
       if (c < a.dim) {
 #pragma unroll 4
-        for (int r = from; r < to; ++r) s += a.carry[(long long)r * a.dim + c];
+        for (int r = mine; r < last; ++r) join_add<V>(s, a.carry + (long long)r * a.dim + c);
       }
-      sums[warp][lane] = s;
-      __syncthreads();
-      if (warp == 0 && c < a.dim) {
-        float total = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) total += sums[w][lane];
-        a.dtable[(long long)row * a.ld_dtable + c] += total * a.scale;
-      }
+      for (int t = 0; t < V; ++t) sums[warp][lane * V + t] = s[t];
+      __syncthreads();
+      for (int i = threadIdx.x; i < 32 * V; i += 256)
+        if (c0 + i < a.dim) {
+          float total = 0.f;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) total += sums[v][i];
+          a.dtable[(long long)shared_row[w] * a.ld_dtable + c0 + i] += total * a.scale;
+        }
       __syncthreads();
     }
   }
@@ -559,18 +734,20 @@ struct FewPlan {
   int v, lanes, copies, per, blocks, slabs;
 };
 
-// A table of at most 100 rows or so: six or more copies of 64 columns (two per thread; 32 or fewer, one per thread, where dout does not
-// allow pairs) fit into a block's shared memory.
+// Copies of 64 columns of the table (two per thread; 32 or 16, one per thread, of shorter rows and where dout does not allow
+// pairs) in a block's shared memory: nine or more of them, up to 85 rows or so.  524288 tokens, 64 columns bf16, 53 / 120 rows: 28 /
+// 56 us (14 / 6 copies), sorted 42.  256 tokens of 53 / 256: 6 / 19 us (14 / 3 copies), sorted 17.
 bool few_plan(long long n, int vocab, int dim, int v, FewPlan* p) {
   p->v = dim >= 64 ? v : 1;
   p->lanes = 32;
   if (p->v == 1)
-    while (p->lanes > 4 && p->lanes / 2 >= dim) p->lanes /= 2;
-  const long long table = 4LL * vocab * p->lanes * p->v;
-  if (table * 6 > EF_SMEM) return false;
+    while (p->lanes > 16 && p->lanes / 2 >= dim) p->lanes /= 2;
+  const long long table = 4LL * (vocab + 1LL) * p->lanes * p->v;
+  if (table * 9 > EF_SMEM) return false;
   const long long room = EF_SMEM / table, threads = EF_THREADS / p->lanes;
   p->copies = (int)(room < threads ? room : threads);
   if (n < 32LL * p->copies) p->copies = (int)((n + 31) / 32);
+  if (p->lanes < 32) p->copies = p->copies < 2 ? 2 : p->copies / 2 * 2;        // whole warps
   p->slabs = (dim + p->lanes * p->v - 1) / (p->lanes * p->v);
   if (p->slabs > 65535) return false;
   // One wave of blocks, at least 32 positions per table.
@@ -586,8 +763,8 @@ bool few_plan(long long n, int vocab, int dim, int v, FewPlan* p) {
 
 struct GradPlan {
   SortPlan sort;
-  int run_len, runs, group;
-  size_t keys, pos, counts, totals, run_key, carry, bytes;    // byte offsets
+  int run_len, parts, part_len, group;
+  size_t keys, pos, counts, totals, part_key, carry, bytes;   // byte offsets
 };
 
 GradPlan grad_plan(long long n, int vocab, int dim, int v) {
@@ -595,14 +772,16 @@ GradPlan grad_plan(long long n, int vocab, int dim, int v) {
   p.sort = sort_plan(n, vocab);
   p.group = 1;
   while (p.group < (dim + v - 1) / v && p.group < 256) p.group *= 2;
-  // About two waves of runs (of 1024 threads per SM), none shorter than 32 steps.
-  const long long steps = n + vocab, waves = 2LL * sb_sm_count() * (1024 / p.group);
+  // Runs of 8 to 512 steps: one wave of 768 threads per SM, whose blocks share the search for their part; two and a half where a
+  // run has most of a block (524288 tokens of 2000, 64 columns 50 us against 63; 65537 of 50001, 1000 columns 132 against 123).
+  const long long steps = n + vocab, waves = (long long)sb_sm_count() * (p.group >= 128 ? 2048 : 768) / p.group;
   long long len = (steps + waves - 1) / waves;
-  len = len < 32 ? 32 : len > 512 ? 512 : len;
-  const long long fit = 5120 / (256 / p.group);              // the block's tokens and positions in 40 KB
+  len = len < 8 ? 8 : len > 512 ? 512 : len;
+  const long long fit = 4096 / (256 / p.group);              // the block's tokens and positions in 32 KB
   if (len > fit) len = fit;
   p.run_len = (int)len;
-  p.runs = (int)((steps + len - 1) / len);
+  p.part_len = (int)(len * (256 / p.group));
+  p.parts = (int)((steps + p.part_len - 1) / p.part_len);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -613,8 +792,8 @@ GradPlan grad_plan(long long n, int vocab, int dim, int v) {
   p.pos = take(2 * sizeof(int) * (size_t)n);
   p.counts = take(sizeof(int) * ((size_t)1 << p.sort.bits) * (size_t)p.sort.chunks);
   p.totals = take(sizeof(int) * ((size_t)1 << p.sort.bits));
-  p.run_key = take(sizeof(int) * ((size_t)p.runs + 1));
-  p.carry = take(sizeof(float) * (size_t)p.runs * (size_t)dim);
+  p.part_key = take(sizeof(int) * ((size_t)p.parts + 1));
+  p.carry = take(sizeof(float) * (size_t)p.parts * (size_t)dim);
   p.bytes = at;
   return p;
 }
@@ -624,11 +803,10 @@ int launch_sort_pass(const SortArgs& a, const SortPlan& p, cudaStream_t s) {
   const int bins = 1 << p.bits;
   SB_CUDA(sb_launch(token_count_kernel<FIRST>, dim3(p.chunks), dim3(ES_THREADS), 0, s, 1, a));
   SB_COUNT_LAUNCH();
-  SB_CUDA(sb_launch(token_scan_kernel, dim3((bins + 7) / 8), dim3(256), 0, s, 1, a));
+  SB_CUDA(sb_launch(token_scan_kernel, dim3((bins + 31) / 32), dim3(1024), 0, s, 1, a));
   SB_COUNT_LAUNCH();
   const size_t smem = sizeof(int) * bins + sizeof(unsigned short) * bins * ES_WARPS;   // at most 40 KB
-  if (p.rounds == 16) SB_CUDA(sb_launch(token_scatter_kernel<FIRST, 16>, dim3(p.chunks), dim3(ES_THREADS), smem, s, 1, a));
-  else SB_CUDA(sb_launch(token_scatter_kernel<FIRST, 4>, dim3(p.chunks), dim3(ES_THREADS), smem, s, 1, a));
+  SB_CUDA(sb_launch(token_scatter_kernel<FIRST, 16>, dim3(p.chunks), dim3(ES_THREADS), smem, s, 1, a));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
@@ -636,8 +814,9 @@ int launch_sort_pass(const SortArgs& a, const SortPlan& p, cudaStream_t s) {
 template <typename T, int V>
 int launch_grad(GradArgs& a, cudaStream_t s) {
   const int threads = (a.dim + V - 1) / V, groups = 256 / a.group;
-  const dim3 grid((a.runs + groups - 1) / groups, (threads + a.group - 1) / a.group);
-  SB_CUDA(sb_launch(embedding_grad_kernel<T, V>, grid, dim3(256), 2 * sizeof(int) * (size_t)(groups * a.run_len), s, 1, a));
+  const dim3 grid(a.parts, (threads + a.group - 1) / a.group);
+  const size_t smem = sizeof(int) * (size_t)(256 * V + groups + 2 * a.part_len);   // at most 41 KB
+  SB_CUDA(sb_launch(embedding_grad_kernel<T, V>, grid, dim3(256), smem, s, 1, a));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
@@ -660,7 +839,7 @@ int launch_grad_type(GradArgs& a, int v, cudaStream_t s) {
 
 template <typename T>
 int launch_few(const FewArgs& a, const FewPlan& p, cudaStream_t s) {
-  const size_t smem = sizeof(float) * (size_t)p.copies * a.vocab * p.lanes * p.v;
+  const size_t smem = sizeof(float) * (size_t)p.copies * (size_t)(a.vocab + 1) * p.lanes * p.v;
   static std::atomic<bool> ready[64];
   int dev = 0;
   SB_CUDA(cudaGetDevice(&dev));
@@ -670,9 +849,8 @@ int launch_few(const FewArgs& a, const FewPlan& p, cudaStream_t s) {
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
   const dim3 grid(p.blocks, p.slabs);
-  const int threads = (p.copies * p.lanes + 31) / 32 * 32;
-  if (p.v == 2) SB_CUDA(sb_launch(embedding_few_kernel<T, 2>, grid, dim3(threads), smem, s, 1, a));
-  else SB_CUDA(sb_launch(embedding_few_kernel<T, 1>, grid, dim3(threads), smem, s, 1, a));
+  if (p.v == 2) SB_CUDA(sb_launch(embedding_few_kernel<T, 2>, grid, dim3(EF_THREADS), smem, s, 1, a));
+  else SB_CUDA(sb_launch(embedding_few_kernel<T, 1>, grid, dim3(EF_THREADS), smem, s, 1, a));
   SB_COUNT_LAUNCH();
   if (p.blocks > 1) {
     const long long size = (long long)a.vocab * a.dim;
@@ -814,12 +992,27 @@ int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const vo
   int* keys = (int*)(ws + p.keys);
   int* pos = (int*)(ws + p.pos);
   a.keys_out = keys; a.pos_out = pos;
-  if (n <= ES_SMALL) {
+  if (n <= ES_CLUSTER) {
     int bits = 1;
     while (bits < 31 && (1LL << bits) <= vocab) ++bits;
-    const size_t smem = 6 * ES_SMALL + sizeof(unsigned short) * 256 * (ES_SMALL_THREADS / 32);   // 40 KB
-    SB_CUDA(sb_launch(token_sort_small_kernel, dim3(1), dim3(ES_SMALL_THREADS), smem, s, 1, a, bits));
+    const int passes = (bits + ES_CLUSTER_BITS - 1) / ES_CLUSTER_BITS;
+    a.bits = (bits + passes - 1) / passes;
+    const int blocks = n <= ES_SMALL ? 1 : ES_BLOCKS;
+    const int rounds = (int)((n + (long long)blocks * ES_CLUSTER_THREADS - 1) / ((long long)blocks * ES_CLUSTER_THREADS));
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    SB_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {   // setting it twice is harmless
+      SB_CUDA(cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
+      SB_CUDA(cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
+    }
+    // At most 112 KB: the pairs, and every warp's counts.
+    const size_t smem = 2 * sizeof(int) * (size_t)(ES_CLUSTER_THREADS * rounds) + (sizeof(short) * ES_CLUSTER_THREADS / 32 << a.bits);
+    SB_CUDA(sb_launch(token_sort_kernel, dim3(blocks), dim3(ES_CLUSTER_THREADS), smem, s, blocks, a, keys, pos, bits, rounds));
     SB_COUNT_LAUNCH();
+    a.keys_out = keys + (passes & 1 ? 0 : n);
+    a.pos_out = pos + (passes & 1 ? 0 : n);
   } else {
     for (int pass = 0; pass < p.sort.passes; ++pass) {
       a.shift = pass * p.sort.bits;
@@ -832,15 +1025,17 @@ int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const vo
   GradArgs g;
   memset(&g, 0, sizeof(g));
   g.keys = a.keys_out; g.pos = a.pos_out; g.dout = dout; g.dtable = dtable;
-  g.carry = (float*)(ws + p.carry); g.run_key = (int*)(ws + p.run_key);
+  g.carry = (float*)(ws + p.carry); g.part_key = (int*)(ws + p.part_key);
   g.ld_dout = ld_dout; g.ld_dtable = ld_dtable; g.n = (int)n; g.vocab = vocab; g.dim = dim;
-  g.group = p.group; g.run_len = p.run_len; g.runs = p.runs; g.scale = scale; g.accumulate = accumulate;
+  g.group = p.group; g.run_len = p.run_len; g.parts = p.parts; g.part_len = p.part_len; g.scale = scale; g.accumulate = accumulate;
   rc = dout_dtype == SB_F32 ? launch_grad_type<float>(g, v, s)
        : dout_dtype == SB_BF16 ? launch_grad_type<__nv_bfloat16>(g, v, s) : launch_grad_type<__half>(g, v, s);
   if (rc != SB_OK) return rc;
-  if (p.runs > 1) {
-    const int most = 32 * sb_sm_count();
-    SB_CUDA(sb_launch(embedding_join_kernel, dim3(p.runs - 1 < most ? p.runs - 1 : most, dim > 256 ? 4 : 1), dim3(256), 0, s, 1, g));
+  if (p.parts > 1) {
+    const int wide = v >= 4 ? 128 : 32, slabs = (dim + wide - 1) / wide;   // columns of a warp
+    const dim3 grid((p.parts + 6) / 8, slabs < 8 ? slabs : 8);
+    if (v >= 4) SB_CUDA(sb_launch(embedding_join_kernel<4>, grid, dim3(256), 0, s, 1, g));
+    else SB_CUDA(sb_launch(embedding_join_kernel<1>, grid, dim3(256), 0, s, 1, g));
     SB_COUNT_LAUNCH();
   }
   return SB_OK;

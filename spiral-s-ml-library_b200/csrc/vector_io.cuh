@@ -32,6 +32,43 @@ template <typename T, int V>
 __device__ __forceinline__ SbPack<T, V> sb_load_pack(const T* p) {
   return *reinterpret_cast<const SbPack<T, V>*>(p);
 }
+// The same as the bytes that were read, where `issue` is set (else `w` keeps what it holds), at this place of the program: an
+// ordinary load whose value is used in a branch is moved into that branch by the compiler, and a pack is taken apart right
+// behind its load; loads that were to be on their way together then follow one another.  Read-only data, not kept in L1.
+template <int BYTES>
+struct SbWords;
+template <>
+struct SbWords<2> { uint16_t v; };
+template <>
+struct SbWords<4> { uint32_t v; };
+template <>
+struct SbWords<8> { uint2 v; };
+template <>
+struct SbWords<16> { uint4 v; };
+__device__ __forceinline__ void sb_load_words(SbWords<16>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(w.v.x), "+r"(w.v.y), "+r"(w.v.z), "+r"(w.v.w) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_words(SbWords<8>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t@q ld.global.nc.L1::no_allocate.v2.b32 {%0, %1}, [%2];\n\t}"
+               : "+r"(w.v.x), "+r"(w.v.y) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_words(SbWords<4>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.L1::no_allocate.b32 %0, [%1];\n\t}"
+               : "+r"(w.v) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_words(SbWords<2>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.L1::no_allocate.b16 %0, [%1];\n\t}"
+               : "+h"(w.v) : "l"(from), "r"((uint32_t)issue));
+}
+template <typename T, int V>
+__device__ __forceinline__ void sb_unpack_words(const SbWords<sizeof(T) * V>& w, float* x) {
+  SbPack<T, V> p;
+  memcpy(&p, &w, sizeof(p));
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = sb_to_f32<T>(p.v[i]);
+}
+
 template <typename T, int V>
 __device__ __forceinline__ SbPack<T, V> sb_zero_pack() {
   SbPack<T, V> r;

@@ -166,10 +166,11 @@ def device_ptr(obj):
         return None
     if isinstance(obj, DeviceArray):
         return obj.ptr
+    data_ptr = getattr(obj, "data_ptr", None)
+    if data_ptr is not None:
+        return int(data_ptr())
     if isinstance(obj, int):
         return obj
-    if hasattr(obj, "data_ptr"):
-        return int(obj.data_ptr())
     cai = getattr(obj, "__cuda_array_interface__", None)
     if cai is not None:
         return int(cai["data"][0])
@@ -201,21 +202,27 @@ def dtype_tag(obj):
 def matrix_of(x, what):
     """(rows, cols, pitch in elements) of a row-major device matrix: the last dimension is contiguous, the others make the
     rows.  A pitch beyond the columns needs a two-dimensional array that knows its strides (torch, CuPy)."""
-    shape = x.shape
+    if type(x) is not DeviceArray:
+        stride = getattr(x, "stride", None)
+        if callable(stride):
+            shape = x.shape
+            if len(shape) == 2:
+                rows, cols = shape
+                pitch, step = stride()
+                if step == 1 and pitch >= cols:
+                    return rows, cols, pitch
+            return _matrix_of(x, shape, stride(), what)
+        strides = getattr(x, "strides", None)
+        if strides is not None:
+            return _matrix_of(x, x.shape, tuple(s // x.itemsize for s in strides), what)
+    return _matrix_of(x, x.shape, None, what)
+
+
+def _matrix_of(x, shape, strides, what):
     cols = shape[-1] if len(shape) else 1
     rows = 1
     for n in shape[:-1]:
         rows *= n
-    if isinstance(x, DeviceArray):
-        return rows, cols, cols
-    strides = None
-    stride = getattr(x, "stride", None)
-    if callable(stride):
-        if len(shape) != 2 and x.is_contiguous():
-            return rows, cols, cols
-        strides = stride()
-    elif getattr(x, "strides", None) is not None:
-        strides = tuple(s // x.itemsize for s in x.strides)
     if strides is None or rows == 0 or cols == 0 or not len(shape):
         return rows, cols, cols
     if cols > 1 and strides[-1] != 1:
@@ -236,10 +243,23 @@ def matrix_of(x, what):
 
 def flat_size(x, what):
     """Elements of a contiguous device array."""
+    if type(x) is not DeviceArray:
+        numel = getattr(x, "numel", None)
+        if numel is not None and x.is_contiguous():
+            return numel()
     rows, cols, pitch = matrix_of(x, what)
     if rows > 1 and pitch != cols:
         raise ValueError("%s must be contiguous" % what)
     return rows * cols
+
+
+def values_ptr(x, n, what):
+    """Address of n contiguous fp32 values (None -> NULL)."""
+    if x is None:
+        return None
+    if dtype_tag(x) != "f32" or flat_size(x, what) != n:
+        raise ValueError("%s must be %d contiguous fp32 values" % (what, n))
+    return device_ptr(x)
 
 
 _WORKSPACES = {}

@@ -7,7 +7,7 @@ updated in place: ``c <- alpha * op(a) @ op(b) + beta * c``.
 import ctypes
 
 from . import _lib
-from .device import DeviceArray, device_ptr, dtype_tag, flat_size, matrix_of, stream_ptr
+from .device import DeviceArray, device_ptr, dtype_tag, matrix_of, stream_ptr, values_ptr
 
 EPILOGUE_FLAGS = {
     "bias": _lib.EPI_BIAS, "relu": _lib.EPI_RELU, "relu_grad": _lib.EPI_RELU_GRAD,
@@ -163,12 +163,6 @@ _FP8_FLOATS = {"f32": _lib.F32, "tf32": _lib.F32, "bf16": _lib.BF16, "f16": _lib
 _FP8_EPILOGUES = {(): 0, ("bias",): _lib.EPI_BIAS, ("relu",): _lib.EPI_RELU, ("bias", "relu"): _lib.EPI_BIAS | _lib.EPI_RELU}
 
 
-def _fp8_scales(x, need, what):
-    if dtype_tag(x) != "f32" or flat_size(x, what) != need:
-        raise ValueError("%s must be %d contiguous fp32 values" % (what, need))
-    return device_ptr(x)
-
-
 def _fp8_codes(x, what):
     if dtype_tag(x) not in ("e4m3", "u8"):
         raise TypeError("%s must hold e4m3 codes, not %s" % (what, dtype_tag(x)))
@@ -190,7 +184,7 @@ def quantize_fp8(x, codes, scales, block_rows=1, stream=None):
         raise TypeError("quantize_fp8: x must hold f32, bf16 or f16, not %s" % tag)
     across = -(-cols // 128)
     _lib.call("sb_quantize_fp8", device_ptr(x), ldx, _FP8_FLOATS[tag], rows, cols, block_rows, _fp8_codes(codes, "codes"), ldc,
-              _fp8_scales(scales, across * (rows if block_rows == 1 else -(-rows // 128)), "scales"), stream_ptr(stream))
+              values_ptr(scales, across * (rows if block_rows == 1 else -(-rows // 128)), "scales"), stream_ptr(stream))
     return codes, scales
 
 
@@ -211,10 +205,10 @@ def matmul_fp8(a, a_scales, b, b_scales, c, epilogue=(), bias=None, stream=None)
     epi = _FP8_EPILOGUES.get(tuple(epilogue))
     if epi is None:
         raise ValueError("matmul_fp8: the epilogue is made of bias and relu, got %r" % (epilogue,))
-    if epi & _lib.EPI_BIAS and (bias is None or dtype_tag(bias) != "f32" or flat_size(bias, "bias") != n):
+    if epi & _lib.EPI_BIAS and bias is None:
         raise ValueError("matmul_fp8: bias must be %d fp32 values" % n)
     across = -(-k // 128)
-    _lib.call("sb_matmul_fp8", _fp8_codes(a, "a"), lda, _fp8_scales(a_scales, across * m, "a_scales"), _fp8_codes(b, "b"), ldb,
-              _fp8_scales(b_scales, -(-n // 128) * across, "b_scales"), device_ptr(c), ldc, m, n, k, _FP8_FLOATS[tag], epi,
-              device_ptr(bias), stream_ptr(stream))
+    _lib.call("sb_matmul_fp8", _fp8_codes(a, "a"), lda, values_ptr(a_scales, across * m, "a_scales"), _fp8_codes(b, "b"), ldb,
+              values_ptr(b_scales, -(-n // 128) * across, "b_scales"), device_ptr(c), ldc, m, n, k, _FP8_FLOATS[tag], epi,
+              values_ptr(bias, n, "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
     return c

@@ -3,7 +3,7 @@ operators in front of the dense layers of a net that reads tokens (embedding, la
 import ctypes
 
 from . import _lib
-from .device import device_ptr, dtype_tag, flat_size, matrix_of, stream_ptr, stream_workspace
+from .device import device_ptr, dtype_tag, flat_size, matrix_of, stream_ptr, stream_workspace, values_ptr
 
 
 def _rows_cols(x):
@@ -141,13 +141,6 @@ def _code(x, what, table=_FLOATS):
         raise TypeError("%s must hold %s, not %s" % (what, " / ".join(table), tag)) from None
 
 
-def _columns(x, cols, what):
-    """A vector of fp32 values, one per column."""
-    if x is not None and (_code(x, what) != _lib.F32 or flat_size(x, what) != cols):
-        raise ValueError("%s must be %d fp32 values" % (what, cols))
-    return device_ptr(x)
-
-
 def embedding(tokens, table, out, scale=1.0, stream=None):
     """``out[i, :] = scale * table[tokens[i], :]``.
 
@@ -206,8 +199,8 @@ def layer_norm(x, out=None, weight=None, bias=None, eps=1e-5, mean=None, rstd=No
     code = _code(x, "x")
     if out_rows != rows or out_cols != cols or _code(out, "out") != code:
         raise ValueError("layer_norm: out must be like x, %dx%d" % (rows, cols))
-    _lib.call("sb_layer_norm", device_ptr(x), ldx, device_ptr(out), ldy, _columns(weight, cols, "weight"),
-              _columns(bias, cols, "bias"), eps, _columns(mean, rows, "mean"), _columns(rstd, rows, "rstd"), rows, cols, code,
+    _lib.call("sb_layer_norm", device_ptr(x), ldx, device_ptr(out), ldy, values_ptr(weight, cols, "weight"),
+              values_ptr(bias, cols, "bias"), eps, values_ptr(mean, rows, "mean"), values_ptr(rstd, rows, "rstd"), rows, cols, code,
               stream_ptr(stream))
     return out
 
@@ -233,9 +226,9 @@ def layer_norm_grad(dy, x, mean, rstd, dx=None, weight=None, dweight=None, dbias
     elif dweight is not None or dbias is not None:
         nbytes = layer_norm_grad_workspace(rows, cols)
         workspace = stream_workspace(nbytes, stream)
-    _lib.call("sb_layer_norm_grad", device_ptr(dy), lddy, device_ptr(x), ldx, _columns(mean, rows, "mean"),
-              _columns(rstd, rows, "rstd"), _columns(weight, cols, "weight"), device_ptr(dx), lddx,
-              _columns(dweight, cols, "dweight"), _columns(dbias, cols, "dbias"), int(bool(accumulate)), rows, cols, code,
+    _lib.call("sb_layer_norm_grad", device_ptr(dy), lddy, device_ptr(x), ldx, values_ptr(mean, rows, "mean"),
+              values_ptr(rstd, rows, "rstd"), values_ptr(weight, cols, "weight"), device_ptr(dx), lddx,
+              values_ptr(dweight, cols, "dweight"), values_ptr(dbias, cols, "dbias"), int(bool(accumulate)), rows, cols, code,
               device_ptr(workspace), nbytes, stream_ptr(stream))
     return dx
 
