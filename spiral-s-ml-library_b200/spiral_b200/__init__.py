@@ -9,7 +9,7 @@ from .device import (DeviceArray, Event, Stream, wait_event, GemmProfile, launch
                      synchronize)
 from .matmul import head_spec, matmul, matmul_fp8, matmul_head, matmul_plan, matmul_tf32, quantize_fp8  # noqa: F401
 from . import primitives  # noqa: F401
-from .models import EnsemblePolicyMLP, PolicyMLP, param_offsets, to_storage  # noqa: F401
+from .models import EnsemblePolicyMLP, PolicyMLP, TokenPolicy, param_offsets, to_storage  # noqa: F401
 from . import layers  # noqa: F401
 from .optim import AdamW  # noqa: F401
 from .parallel import DataParallel, PeerUpdate, shard_rows, bucket_ranges, update_slice  # noqa: F401

@@ -10,9 +10,11 @@ import ctypes
 
 import numpy as np
 
-from . import _lib
+from . import _lib, primitives
 from .device import DeviceArray, device_ptr, stream_ptr
 from . import dtypes
+from .matmul import matmul, matmul_fp8, quantize_fp8
+from .optim import AdamW
 
 HEAD_FLAGS = {"masked_softmax": _lib.EPI_MASKED_SOFTMAX, "regret_matching": _lib.EPI_REGRET_MATCHING,
               "argmax": _lib.EPI_ARGMAX}
@@ -386,3 +388,105 @@ class EnsemblePolicyMLP:
                                  "output_indices")}
         out["output_probs"] = self.probs
         return out
+
+
+class TokenPolicy:
+    """A policy net whose states are sequences of ``n_tokens`` small integers (cards, actions, history; anything outside the
+    vocabulary means "none"): embedding -> layer normalisation over the whole state -> a ``PolicyMLP`` with a masked-softmax
+    head.  ``train_step`` is one AdamW step on the mean cross-entropy; ``forward_8bit`` answers with the dense layers in
+    8-bit floating point (``quantize`` first, and after every change of the weights).
+
+    Buffers: ``table`` fp32 [vocab, dim], ``norm_weight`` and ``norm_bias`` fp32 [n_tokens * dim], ``mlp.params``; all are
+    stepped by one ``AdamW`` (``optimizer``, states in fp32 or 'e4m3')."""
+
+    def __init__(self, vocab, n_tokens, dim, hidden, n_actions, batch, in_dtype="bf16", training=False, state="f32"):
+        if in_dtype not in ("bf16", "f16"):
+            raise ValueError("in_dtype must be 'bf16' or 'f16'")
+        self.vocab, self.n_tokens, self.dim, self.batch = int(vocab), int(n_tokens), int(dim), int(batch)
+        self.width = self.n_tokens * self.dim
+        self.in_dtype = in_dtype
+        self.scale = self.dim ** -0.5
+        self.mlp = PolicyMLP([self.width] + list(hidden) + [n_actions], batch, in_dtype=in_dtype, training=training)
+        self.table = DeviceArray.zeros((self.vocab, self.dim), "f32")
+        self.norm_weight = DeviceArray.from_numpy(np.ones(self.width, np.float32))
+        self.norm_bias = DeviceArray.zeros((self.width,), "f32")
+        self.embedded = DeviceArray((self.batch, self.width), in_dtype)
+        self.x = DeviceArray((self.batch, self.width), in_dtype)
+        self.mean, self.rstd = DeviceArray((self.batch,), "f32"), DeviceArray((self.batch,), "f32")
+        self.optimizer = None
+        self._codes = None
+        if training:
+            self.dx = DeviceArray((self.batch, self.width), in_dtype)
+            self.dembedded = DeviceArray((self.batch, self.width), in_dtype)
+            self.dtable = DeviceArray((self.vocab, self.dim), "f32")
+            self.dnorm_weight, self.dnorm_bias = DeviceArray((self.width,), "f32"), DeviceArray((self.width,), "f32")
+            self.optimizer = AdamW([self.mlp.params, self.table, self.norm_weight, self.norm_bias],
+                                   [self.mlp.grads, self.dtable, self.dnorm_weight, self.dnorm_bias],
+                                   copies=[self.mlp.w_compute.view((self.mlp.n_params,)), None, None, None], state=state)
+
+    def load_weights(self, table, weights, biases=None, norm_weight=None, norm_bias=None):
+        """Uploads fp32 host weights: the table, the layers' [out, in] matrices (and biases), the normalisation's vectors."""
+        self.table.upload(np.asarray(table, np.float32))
+        self.mlp.load_weights(weights, biases)
+        if norm_weight is not None:
+            self.norm_weight.upload(np.asarray(norm_weight, np.float32))
+        if norm_bias is not None:
+            self.norm_bias.upload(np.asarray(norm_bias, np.float32))
+        return self
+
+    def _input(self, tokens, stream):
+        by_token = (self.batch * self.n_tokens, self.dim)
+        primitives.embedding(tokens, self.table, self.embedded.view(by_token), scale=self.scale, stream=stream)
+        primitives.layer_norm(self.embedded, self.x, self.norm_weight, self.norm_bias, mean=self.mean, rstd=self.rstd, stream=stream)
+
+    def forward(self, tokens, mask=None, stream=None):
+        """Action probabilities fp32 [batch, n_actions] for ``tokens`` (int32 or int64, [batch, n_tokens])."""
+        self._input(tokens, stream)
+        return self.mlp.forward(self.x, mask, stream=stream)
+
+    def gradients(self, tokens, mask, target, stream=None):
+        """Forward and backward pass: fills ``mlp.grads``, ``dtable``, ``dnorm_weight`` and ``dnorm_bias`` with the gradient of
+        the mean cross-entropy and adds that to ``mlp.loss``."""
+        self.forward(tokens, mask, stream=stream)
+        self.mlp.backward(self.x, mask, target, stream=stream)
+        # Into the input: what the first layer left behind times its weights (rows padded alike to multiples of 8).
+        dy = self.mlp.layer_dy(0)
+        w = self.mlp.w_compute.view((dy.shape[1], self.width), self.in_dtype, self.mlp.offsets[0] * 2)
+        matmul(False, False, 1.0, dy, w, 0.0, self.dx, stream=stream)
+        primitives.layer_norm_grad(self.dx, self.embedded, self.mean, self.rstd, self.dembedded, self.norm_weight,
+                                   self.dnorm_weight, self.dnorm_bias, stream=stream)
+        primitives.embedding_grad(tokens, self.dembedded.view((self.batch * self.n_tokens, self.dim)), self.dtable,
+                                  scale=self.scale, stream=stream)
+
+    def train_step(self, tokens, mask, target, lr, weight_decay=0.01, stream=None):
+        """One AdamW step on this batch."""
+        self.gradients(tokens, mask, target, stream=stream)
+        self.optimizer.step(lr, weight_decay=weight_decay, stream=stream)
+
+    def quantize(self, stream=None):
+        """E4M3 codes of the dense layers' weights, a scale per block of 128 x 128, for ``forward_8bit``."""
+        sizes = self.mlp.sizes
+        if self._codes is None:
+            self._codes = [(DeviceArray((o, i), "e4m3"), DeviceArray((-(-o // 128), -(-i // 128)), "f32"),
+                            DeviceArray((self.batch, i), "e4m3"), DeviceArray((-(-i // 128), self.batch), "f32"))
+                           for i, o in zip(sizes, sizes[1:])]
+        for layer, (codes, scales, _, _) in enumerate(self._codes):
+            w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
+            quantize_fp8(w, codes, scales, block_rows=128, stream=stream)
+        return self
+
+    def forward_8bit(self, tokens, mask=None, stream=None):
+        """``forward`` with the dense layers in 8 bits: activations quantised per row and 128 columns, products of codes."""
+        if self._codes is None:
+            raise ValueError("quantize() the weights first")
+        self._input(tokens, stream)
+        x = self.x
+        for layer, (codes, scales, x_codes, x_scales) in enumerate(self._codes):
+            last = layer == self.mlp.n_layers - 1
+            out = self.mlp.probs if last else self.mlp.activations[layer]
+            bias = self.mlp.params.view((self.mlp.sizes[layer + 1],), "f32", self.mlp.offsets[2 * layer + 1] * 4)
+            quantize_fp8(x, x_codes, x_scales, stream=stream)
+            matmul_fp8(x_codes, x_scales, codes, scales, out, epilogue=("bias",) if last else ("bias", "relu"), bias=bias,
+                       stream=stream)
+            x = out
+        return primitives.softmax(self.mlp.probs, mask=mask, stream=stream)
