@@ -39,6 +39,34 @@ struct QuantArgs {
 };
 
 // ------------------------------ quantisation -------------------------------------
+// The bits of the largest magnitude in a pack: as integers, so that a NaN is the largest and stays; 16-bit types two at a
+// time.  fp32 bits come back from `f8_largest_bits`.
+template <typename T, int V>
+__device__ __forceinline__ uint32_t f8_larger(const SbPack<T, V>& p, uint32_t largest) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    uint32_t w[V / 2];
+    memcpy(w, &p, sizeof(w));
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) asm("max.u16x2 %0, %0, %1;" : "+r"(largest) : "r"(w[k] & 0x7fff7fffu));
+    return largest;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) largest = max(largest, __float_as_uint(sb_to_f32<T>(p.v[k])) & 0x7fffffffu);
+    return largest;
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ uint32_t f8_largest_bits(uint32_t largest) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    const uint16_t h = (uint16_t)max(largest & 0xffffu, largest >> 16);
+    T v;
+    memcpy(&v, &h, sizeof(v));
+    return __float_as_uint(sb_to_f32<T>(v));
+  } else {
+    return largest;
+  }
+}
+
 // A block of 256 threads per ROWS x 128 tile of x, which stays in registers between the search for its largest magnitude
 // and the rounding; L lanes share a row, V neighbouring elements each.  SQUARE: one scale for the tile, else one per row.
 template <typename T, int V, int ROWS, bool SQUARE>
@@ -70,12 +98,8 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
       in[p][s] = row < a.rows && col < a.cols ? sb_load_pack<T, V>((const T*)a.x + row * a.ldx + col) : sb_zero_pack<T, V>();
     }
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      float v[V];
-      sb_unpack<T, V>(in[p][s], v);
-#pragma unroll
-      for (int k = 0; k < V; ++k) mx = max(mx, __float_as_uint(v[k]) & 0x7fffffffu);   // a NaN is the largest and stays
-    }
+    for (int s = 0; s < STEPS; ++s) mx = f8_larger<T, V>(in[p][s], mx);
+    mx = f8_largest_bits<T, V>(mx);
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     largest[p] = max(mx, __float_as_uint(F8_FLOOR));
@@ -108,8 +132,13 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
           *to = (uint8_t)f8_pack2(v[0] * inv, 0.f);
         } else {
           SbPack<uint16_t, V / 2> c;
+          const unsigned long long inv2 = pack_f32x2(inv, inv);
 #pragma unroll
-          for (int k = 0; k < V; k += 2) c.v[k / 2] = (uint16_t)f8_pack2(v[k] * inv, v[k + 1] * inv);
+          for (int k = 0; k < V; k += 2) {
+            float lo, hi;
+            unpack_f32x2(mul_f32x2(pack_f32x2(v[k], v[k + 1]), inv2), lo, hi);
+            c.v[k / 2] = (uint16_t)f8_pack2(lo, hi);
+          }
           *reinterpret_cast<SbPack<uint16_t, V / 2>*>(to) = c;
         }
       }
