@@ -14,28 +14,36 @@
 namespace {
 
 // ------------------------------- lookup -----------------------------------------
-// A thread per V neighbouring elements of the output.  Tables are stored with a row pitch.
-template <typename I, typename T, typename O, int V>
+// `lanes` threads per row (a power of two), PACKS packs of V neighbouring elements each at a time, all loads before the first
+// store; the next row's token is on its way meanwhile.
+template <typename I, typename T, typename O, int V, int PACKS>
 __global__ void __launch_bounds__(256)
 embedding_kernel(const I* __restrict__ tokens, const T* __restrict__ table, O* __restrict__ out, long long n, int vocab, int dim,
-                 long long ld_table, long long ld_out, float scale) {
+                 long long ld_table, long long ld_out, float scale, int lanes) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const int pieces = dim / V;
-  const long long total = n * pieces, step = (long long)gridDim.x * blockDim.x;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-    const long long r = i / pieces;
-    const int c = (int)(i - r * pieces) * V;
-    const long long t = (long long)tokens[r];
-    float v[V];
+  const unsigned lane = threadIdx.x & (lanes - 1), stride = lanes * V;
+  const long long step = (long long)gridDim.x * (blockDim.x / lanes);
+  long long r = (long long)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+  long long t = r < n ? (long long)tokens[r] : 0;
+  for (; r < n; r += step) {
+    const bool known = t >= 0 && t < vocab;
+    const T* from = table + (known ? t : 0) * ld_table;
+    O* to = out + r * ld_out;
+    if (r + step < n) t = (long long)tokens[r + step];
+    for (unsigned c = lane * V; c < (unsigned)dim; c += PACKS * stride) {
+      SbWords<sizeof(T) * V> in[PACKS] = {};
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
-    if (t >= 0 && t < vocab) {
-      sb_unpack<T, V>(sb_load_pack<T, V>(table + t * ld_table + c), v);
+      for (int i = 0; i < PACKS; ++i) sb_load_kept(in[i], from + c + i * stride, known && c + i * stride < (unsigned)dim);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] *= scale;
+      for (int i = 0; i < PACKS; ++i) {
+        float v[V];
+        sb_unpack_words<T, V>(in[i], v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] *= scale;
+        if (c + i * stride < (unsigned)dim) sb_store_f32<O, V>(to + c + i * stride, v);
+      }
     }
-    sb_store_f32<O, V>(out + r * ld_out + c, v);
   }
 }
 
@@ -860,12 +868,15 @@ int launch_few(const FewArgs& a, const FewPlan& p, cudaStream_t s) {
   return SB_OK;
 }
 
-template <typename I, typename T, typename O, int V>
+template <typename I, typename T, typename O, int V, int PACKS>
 cudaError_t launch_lookup(const void* tokens, const void* table, void* out, long long n, int vocab, int dim, long long ld_table,
                           long long ld_out, float scale, cudaStream_t s) {
-  const long long blocks = (n * (dim / V) + 255) / 256, most = 16LL * sb_sm_count();
-  return sb_launch(embedding_kernel<I, T, O, V>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, (const I*)tokens,
-                   (const T*)table, (O*)out, n, vocab, dim, ld_table, ld_out, scale);
+  const int packs = (dim + V * PACKS - 1) / (V * PACKS);
+  int lanes = 1;
+  while (lanes < packs && lanes < 256) lanes *= 2;
+  const long long blocks = (n * lanes + 255) / 256, most = 16LL * sb_sm_count();
+  return sb_launch(embedding_kernel<I, T, O, V, PACKS>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, (const I*)tokens,
+                   (const T*)table, (O*)out, n, vocab, dim, ld_table, ld_out, scale, lanes);
 }
 
 template <typename I, typename T, typename O>
@@ -875,10 +886,10 @@ cudaError_t launch_lookup_width(const void* tokens, const void* table, void* out
   constexpr int MOST = SMALL == 4 ? 4 : (sizeof(T) == sizeof(O) ? 8 : 4);
   int v = sb_vector_width(table, ld_table, dim, sizeof(T), MOST);
   v = sb_vector_width(out, ld_out, dim, sizeof(O), v);
-  if (v == 8) return launch_lookup<I, T, O, MOST>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  if (v == 4) return launch_lookup<I, T, O, 4>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  if (v == 2) return launch_lookup<I, T, O, 2>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  return launch_lookup<I, T, O, 1>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 8) return launch_lookup<I, T, O, MOST, 1>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 4) return launch_lookup<I, T, O, 4, 1>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 2) return launch_lookup<I, T, O, 2, 2>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  return launch_lookup<I, T, O, 1, 4>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
 }
 
 template <typename I, typename T>

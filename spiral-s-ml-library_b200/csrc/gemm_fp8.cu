@@ -316,6 +316,40 @@ __device__ __forceinline__ void f8_add(unsigned long long* sum, const uint32_t* 
     fma_f32x2(sum[j], pack_f32x2(__uint_as_float(part[2 * j]), __uint_as_float(part[2 * j + 1])), scale);
 }
 
+// A box of 32 rows -> C with plain stores.  Lane l has columns l, l + 32, ... of a row; the places of 8 rows (4 where a row is
+// 64 bytes: two rows share a 128-byte line) repeat with the swizzle, so the loop over rows knows them as constants.
+template <typename O, int BOX_COLS>
+__device__ __forceinline__ void f8_write_rows(O* to, long long ldc, int rows, int cols, uint32_t box, int lane) {
+  constexpr int PER = 16 / sizeof(O), ROW_BYTES = BOX_COLS * sizeof(O), PIECES = ROW_BYTES / 16;
+  constexpr int EACH = (BOX_COLS + 31) / 32;
+  static_assert(BOX_COLS >= 32, "");
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8, to += 8 * ldc, box += 8 * ROW_BYTES) {
+    O v[8][EACH];
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const uint32_t c = (uint32_t)(lane + 32 * e), key = ROW_BYTES == 128 ? (uint32_t)r : (uint32_t)(r >> 1) & 3u;
+        const uint32_t at = box + (uint32_t)r * ROW_BYTES + (((c / PER ^ key) & (PIECES - 1)) << 4) + (c % PER) * (uint32_t)sizeof(O);
+        if constexpr (sizeof(O) == 4) {
+          uint32_t w;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+          memcpy(&v[r][e], &w, 4);
+        } else {
+          uint16_t w;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
+          memcpy(&v[r][e], &w, 2);
+        }
+      }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (r0 + r < rows && lane + 32 * e < cols) to[r * ldc + lane + 32 * e] = v[r][e];
+  }
+}
+
 // Finished values of this warp's 32 rows and COLS columns (their biases in shared memory) -> C, a box of 32 rows x 128 bytes at a time (64 bytes where the
 // columns are no more): by a TMA store, or by coalesced stores where C's rows are not whole 16-byte pieces.
 template <typename O, int COLS>
@@ -359,24 +393,7 @@ __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tma
       }
     } else {
       __syncwarp();
-#pragma unroll 4
-      for (int i = lane; i < 32 * BOX_COLS; i += 32) {
-        const uint32_t r = (uint32_t)i / BOX_COLS, c = (uint32_t)i % BOX_COLS;
-        const uint32_t key = ROW_BYTES == 128 ? (r & 7u) : ((r >> 1) & 3u);
-        const uint32_t at = box + r * ROW_BYTES + (((c / PER ^ key) & (PIECES - 1)) << 4) + (c % PER) * (uint32_t)sizeof(O);
-        if (row0 + r < g.m && first + (int)c < g.n) {
-          O* to = (O*)g.c + (row0 + r) * g.ldc + first + c;
-          if (sizeof(O) == 4) {
-            uint32_t w;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
-            *reinterpret_cast<uint32_t*>(to) = w;
-          } else {
-            uint16_t w;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(w) : "r"(at) : "memory");
-            *reinterpret_cast<uint16_t*>(to) = w;
-          }
-        }
-      }
+      f8_write_rows<O, BOX_COLS>((O*)g.c + row0 * g.ldc + first, g.ldc, (int)min(32LL, g.m - row0), g.n - first, box, lane);
       __syncwarp();
     }
   }

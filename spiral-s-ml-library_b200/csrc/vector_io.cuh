@@ -61,6 +61,23 @@ __device__ __forceinline__ void sb_load_words(SbWords<2>& w, const void* from, b
   asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.L1::no_allocate.b16 %0, [%1];\n\t}"
                : "+h"(w.v) : "l"(from), "r"((uint32_t)issue));
 }
+// The same, kept in L1 and L2 as an ordinary load is: rows that are read again.
+__device__ __forceinline__ void sb_load_kept(SbWords<16>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(w.v.x), "+r"(w.v.y), "+r"(w.v.z), "+r"(w.v.w) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_kept(SbWords<8>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t@q ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
+               : "+r"(w.v.x), "+r"(w.v.y) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_kept(SbWords<4>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.b32 %0, [%1];\n\t}"
+               : "+r"(w.v) : "l"(from), "r"((uint32_t)issue));
+}
+__device__ __forceinline__ void sb_load_kept(SbWords<2>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q ld.global.nc.b16 %0, [%1];\n\t}"
+               : "+h"(w.v) : "l"(from), "r"((uint32_t)issue));
+}
 template <typename T, int V>
 __device__ __forceinline__ void sb_unpack_words(const SbWords<sizeof(T) * V>& w, float* x) {
   SbPack<T, V> p;
