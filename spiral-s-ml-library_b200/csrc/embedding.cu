@@ -15,7 +15,8 @@ namespace {
 
 // ------------------------------- lookup -----------------------------------------
 // `lanes` threads per row (a power of two), PACKS packs of V neighbouring elements each at a time, all loads before the first
-// store; the next row's token is on its way meanwhile.
+// store; the next row's token is on its way meanwhile.  Bound by memory: 65537 x 1000 from 50001 fp32 rows to bf16 56 us, 5.9 TB/s
+// (62 with one pack at a time); single elements, 999 columns 67 us (92 with four at a time), 177 with an index and a division for every element.
 template <typename I, typename T, typename O, int V, int PACKS>
 __global__ void __launch_bounds__(256)
 embedding_kernel(const I* __restrict__ tokens, const T* __restrict__ table, O* __restrict__ out, long long n, int vocab, int dim,
@@ -424,18 +425,19 @@ __device__ __forceinline__ int walk_split(const int* __restrict__ keys, int n, i
 }
 
 // The rows that a block adds up and finishes: groups x run_len steps of the walk, whose tokens and positions it brings to
-// shared memory; a group of threads per run, V neighbouring columns per thread, the next UNROLL rows of dout on their way
-// while the ones before are added.  (Every group searching the sorted tokens for itself, 17 dependent loads twice, and
+// shared memory; a group of threads per run, PACKS times V neighbouring columns per thread, the next UNROLL rows of dout on their way
+// while the ones before are added.  Rows that only single elements fit have four of those per thread: 60000 x 333 of 5000 57 us,
+// 88 with one; 336 columns 38.  (Every group searching the sorted tokens for itself, 17 dependent loads twice, and
 // reading token and position from global memory in the loop: 50001 x 1000 fp32 213 us.)
-template <typename T, int V>
+template <typename T, int V, int PACKS>
 __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
-  constexpr int UNROLL = 8;
+  constexpr int UNROLL = 8, W = V * PACKS;
   extern __shared__ __align__(16) int s_walk[];
   __shared__ int ends[2];
   const int groups = blockDim.x / a.group;
   const int steps = groups * a.run_len;
-  float* s_carry = reinterpret_cast<float*>(s_walk);         // [256][V]: what each run leaves behind
-  int* s_end = s_walk + 256 * V;                             // [groups]: the row that the run ends in
+  float* s_carry = reinterpret_cast<float*>(s_walk);         // [256][W]: what each run leaves behind
+  int* s_end = s_walk + 256 * W;                             // [groups]: the row that the run ends in
   int* s_key = s_end + groups;
   int* s_pos = s_key + steps;
   const long long first = (long long)blockIdx.x * steps, all = (long long)a.n + a.vocab;
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
   }
   __syncthreads();
   const int in_group = threadIdx.x % a.group, g = threadIdx.x / a.group;
-  const int col = (blockIdx.y * a.group + in_group) * V;
+  const int stride = a.group * V, col = blockIdx.y * PACKS * stride + in_group * V;   // of the first pack
   // The run's own part, by halves.
   auto split = [&](long long d) {
     int lo = (int)max(0LL, d - a.vocab - k_first), hi = (int)min((long long)count, d - k_first);
@@ -476,47 +478,59 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
   const int k_end = split(d1);
   const int row0 = (int)(d0 - (k_first + k)), row_end = (int)(d1 - (k_first + k_end));
   const bool active = col < a.dim;
+  bool has[PACKS];
+#pragma unroll
+  for (int p = 0; p < PACKS; ++p) has[p] = col + p * stride < a.dim;
   int row = row0;
   const T* dout = (const T*)a.dout + (active ? col : 0);
   float* to = a.dtable + (long long)row * a.ld_dtable + col;
-  float acc[V];
+  float acc[W];
 #pragma unroll
-  for (int t = 0; t < V; ++t) acc[t] = 0.f;
+  for (int t = 0; t < W; ++t) acc[t] = 0.f;
   auto finish = [&]() {
-    float out[V];
 #pragma unroll
-    for (int t = 0; t < V; ++t) out[t] = acc[t] * a.scale;
-    if (a.accumulate) {
+    for (int p = 0; p < PACKS; ++p) {
+      float out[V];
 #pragma unroll
-      for (int t = 0; t < V; ++t) out[t] += to[t];
+      for (int t = 0; t < V; ++t) out[t] = acc[p * V + t] * a.scale;
+      if (has[p]) {
+        float* at = to + p * stride;
+        if (a.accumulate) {
+#pragma unroll
+          for (int t = 0; t < V; ++t) out[t] += at[t];
+        }
+#pragma unroll
+        for (int t = 0; t < V; t += 4) {
+          if constexpr (V >= 4) sb_store_f32<float, 4>(at + t, out + t);
+          else sb_store_f32<float, V>(at, out);
+        }
+      }
     }
 #pragma unroll
-    for (int t = 0; t < V; t += 4) {
-      if constexpr (V >= 4) sb_store_f32<float, 4>(to + t, out + t);
-      else sb_store_f32<float, V>(to, out);
-    }
-#pragma unroll
-    for (int t = 0; t < V; ++t) acc[t] = 0.f;
+    for (int t = 0; t < W; ++t) acc[t] = 0.f;
     to += a.ld_dtable;
     ++row;
   };
   if (active) {
     while (k < k_end) {
-      SbWords<sizeof(T) * V> in[UNROLL] = {};
+      SbWords<sizeof(T) * V> in[UNROLL][PACKS] = {};
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         const bool issue = k + u < k_end && s_key[k + u] < a.vocab;
-        sb_load_words(in[u], dout + (long long)(issue ? s_pos[k + u] : 0) * a.ld_dout, issue);
+        const T* from = dout + (long long)(issue ? s_pos[k + u] : 0) * a.ld_dout;
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) sb_load_words(in[u][p], from + p * stride, issue && has[p]);
       }
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         const int key = k + u < k_end ? s_key[k + u] : a.vocab;
         if (key < a.vocab) {
           while (row < key) finish();
-          float v[V];
-          sb_unpack_words<T, V>(in[u], v);
+          float v[W];
 #pragma unroll
-          for (int t = 0; t < V; ++t) acc[t] += v[t];
+          for (int p = 0; p < PACKS; ++p) sb_unpack_words<T, V>(in[u][p], v + p * V);
+#pragma unroll
+          for (int t = 0; t < W; ++t) acc[t] += v[t];
         }
       }
       k += UNROLL;
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
   // What is left belongs to the row that the next run begins in.  Where a run finishes the row that it begins in, it adds
   // what the block's runs before it left for that row, in their order; the block's last leftover goes to the workspace.
 #pragma unroll
-  for (int t = 0; t < V; ++t) s_carry[threadIdx.x * V + t] = acc[t];
+  for (int t = 0; t < W; ++t) s_carry[threadIdx.x * W + t] = acc[t];
   if (in_group == 0) s_end[g] = row_end;
   __syncthreads();
   if (!active) return;
@@ -534,27 +548,29 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
     int from = last;
     while (from > 0 && s_end[from - 1] == r) --from;
 #pragma unroll
-    for (int t = 0; t < V; ++t) sum[t] = 0.f;
+    for (int t = 0; t < W; ++t) sum[t] = 0.f;
     for (int h = from; h <= last; ++h)
 #pragma unroll
-      for (int t = 0; t < V; ++t) sum[t] += s_carry[(h * a.group + in_group) * V + t];
+      for (int t = 0; t < W; ++t) sum[t] += s_carry[(h * a.group + in_group) * W + t];
   };
-  float sum[V];
+  float sum[W];
   if (g > 0 && row_end > row0) {
     leftover(g - 1, row0, sum);
     float* at = a.dtable + (long long)row0 * a.ld_dtable + col;
 #pragma unroll
-    for (int t = 0; t < V; ++t) at[t] += sum[t] * a.scale;
+    for (int t = 0; t < W; ++t)
+      if (has[t / V]) at[t / V * stride + t % V] += sum[t] * a.scale;
   }
   if (g == groups - 1) {
     leftover(g, row_end, sum);
 #pragma unroll
-    for (int t = 0; t < V; ++t) a.carry[(long long)blockIdx.x * a.dim + col + t] = sum[t];
+    for (int t = 0; t < W; ++t)
+      if (has[t / V]) a.carry[(long long)blockIdx.x * a.dim + col + t / V * stride + t % V] = sum[t];
   }
 }
 
 // A table of few rows needs no sort: every warp (or part of one) adds its share of the positions, in their order, to a table of
-// its own in shared memory, V columns per thread and G x V per block; the block adds its tables up, and the blocks' sums are
+// its own in shared memory, one or two columns per thread; the block adds its tables up, and the blocks' sums are
 // added in their order by a second launch.  Bound by reading dout: 524288 x 64 bf16 over 53 tokens 28 us (floor 11).
 constexpr int EF_THREADS = 512;
 constexpr int EF_SMEM = 200 * 1024;
@@ -571,17 +587,17 @@ struct FewArgs {
   int accumulate;
 };
 
-template <typename T, int V>
+template <typename T, int V, int PACKS>
 __global__ void __launch_bounds__(EF_THREADS) embedding_few_kernel(FewArgs a) {
   constexpr int UNROLL = 16;                                 // at most `lanes`: as many tokens as one load of the group brings
-  extern __shared__ __align__(16) float s_tables[];          // [copies][vocab + 1][lanes * V]; the last row is for no token
-  const int width = a.lanes * V, table = (a.vocab + 1) * width;
+  extern __shared__ __align__(16) float s_tables[];          // [copies][vocab + 1][lanes * V * PACKS]; the last row is for no token
+  const int stride = a.lanes * V, width = stride * PACKS, table = (a.vocab + 1) * width;
   const int copy = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes;
   for (int i = threadIdx.x; i < a.copies * table / 4; i += EF_THREADS) reinterpret_cast<float4*>(s_tables)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   __syncthreads();
-  const int col = (blockIdx.y * a.lanes + lane) * V;
+  const int col = blockIdx.y * width + lane * V;             // of the first pack
   const long long first = ((long long)blockIdx.x * a.copies + copy) * a.per;
   const int count = (int)max(0LL, min((long long)a.per, a.n - first));
   // Rows do not wait for their tokens, and the next UNROLL of both are on their way while these are added.
@@ -589,26 +605,33 @@ __global__ void __launch_bounds__(EF_THREADS) embedding_few_kernel(FewArgs a) {
   const bool active = col < a.dim;
   const T* dout = (const T*)a.dout + (active ? first * a.ld_dout + col : 0);
   struct Ahead {
-    SbWords<sizeof(T) * V> row[UNROLL];
+    SbWords<sizeof(T) * V> row[UNROLL][PACKS];
     TokenWords token;            // lane u holds row u's, as it was read: looking at it would wait for it
   };
   auto fetch = [&](Ahead& x, int i) {
     load_token(x.token, a.tokens, first + i + lane, a.index64 != 0, lane < UNROLL && i + lane < count);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      sb_load_words(x.row[u], dout + (active ? (long long)(i + u) * a.ld_dout : 0), active && i + u < count);
+#pragma unroll
+      for (int p = 0; p < PACKS; ++p) {
+        const bool in = col + p * stride < a.dim;
+        sb_load_words(x.row[u][p], dout + (in ? (long long)(i + u) * a.ld_dout + p * stride : 0), in && i + u < count);
+      }
   };
   auto add = [&](const Ahead& x, int i) {
     const int token = i + lane < count ? token_of(x.token, a.index64 != 0, a.vocab, a.vocab) : a.vocab;
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      float v[V], t[V];
-      sb_unpack_words<T, V>(x.row[u], v);
       float* to = mine + __shfl_sync(0xffffffffu, token, u, a.lanes) * width;
-      sb_unpack<float, V>(sb_load_pack<float, V>(to), t);
 #pragma unroll
-      for (int k = 0; k < V; ++k) t[k] += v[k];
-      sb_store_f32<float, V>(to, t);
+      for (int p = 0; p < PACKS; ++p) {
+        float v[V], t[V];
+        sb_unpack_words<T, V>(x.row[u][p], v);
+        sb_unpack<float, V>(sb_load_pack<float, V>(to + p * stride), t);
+#pragma unroll
+        for (int k = 0; k < V; ++k) t[k] += v[k];
+        sb_store_f32<float, V>(to + p * stride, t);
+      }
     }
   };
   if (copy < a.copies) {         // whole warps; the others help before and after
@@ -745,8 +768,8 @@ struct FewPlan {
 // Copies of 64 columns of the table (two per thread; 32 or 16, one per thread, of shorter rows and where dout does not allow
 // pairs) in a block's shared memory: nine or more of them, up to 85 rows or so.  524288 tokens, 64 columns bf16, 53 / 120 rows: 28 /
 // 56 us (14 / 6 copies), sorted 42.  256 tokens of 53 / 256: 6 / 19 us (14 / 3 copies), sorted 17.
-bool few_plan(long long n, int vocab, int dim, int v, FewPlan* p) {
-  p->v = dim >= 64 ? v : 1;
+bool few_plan(long long n, int vocab, int dim, FewPlan* p) {
+  p->v = dim >= 64 ? 2 : 1;
   p->lanes = 32;
   if (p->v == 1)
     while (p->lanes > 16 && p->lanes / 2 >= dim) p->lanes /= 2;
@@ -775,11 +798,11 @@ struct GradPlan {
   size_t keys, pos, counts, totals, part_key, carry, bytes;   // byte offsets
 };
 
-GradPlan grad_plan(long long n, int vocab, int dim, int v) {
+GradPlan grad_plan(long long n, int vocab, int dim, int w) {   // w columns per thread
   GradPlan p;
   p.sort = sort_plan(n, vocab);
   p.group = 1;
-  while (p.group < (dim + v - 1) / v && p.group < 256) p.group *= 2;
+  while (p.group < (dim + w - 1) / w && p.group < 256) p.group *= 2;
   // Runs of 8 to 512 steps: one wave of 768 threads per SM, whose blocks share the search for their part; two and a half where a
   // run has most of a block (524288 tokens of 2000, 64 columns 50 us against 63; 65537 of 50001, 1000 columns 132 against 123).
   const long long steps = n + vocab, waves = (long long)sb_sm_count() * (p.group >= 128 ? 2048 : 768) / p.group;
@@ -819,12 +842,12 @@ int launch_sort_pass(const SortArgs& a, const SortPlan& p, cudaStream_t s) {
   return SB_OK;
 }
 
-template <typename T, int V>
+template <typename T, int V, int PACKS>
 int launch_grad(GradArgs& a, cudaStream_t s) {
-  const int threads = (a.dim + V - 1) / V, groups = 256 / a.group;
+  const int threads = (a.dim + V * PACKS - 1) / (V * PACKS), groups = 256 / a.group;
   const dim3 grid(a.parts, (threads + a.group - 1) / a.group);
-  const size_t smem = sizeof(int) * (size_t)(256 * V + groups + 2 * a.part_len);   // at most 41 KB
-  SB_CUDA(sb_launch(embedding_grad_kernel<T, V>, grid, dim3(256), smem, s, 1, a));
+  const size_t smem = sizeof(int) * (size_t)(256 * V * PACKS + groups + 2 * a.part_len);   // at most 41 KB
+  SB_CUDA(sb_launch(embedding_grad_kernel<T, V, PACKS>, grid, dim3(256), smem, s, 1, a));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
@@ -839,26 +862,28 @@ int grad_width(const void* dout, long long ld_dout, const float* dtable, long lo
 template <typename T>
 int launch_grad_type(GradArgs& a, int v, cudaStream_t s) {
   constexpr int MOST = 16 / sizeof(T);
-  if (v == 8) return launch_grad<T, MOST>(a, s);
-  if (v == 4) return launch_grad<T, 4>(a, s);
-  if (v == 2) return launch_grad<T, 2>(a, s);
-  return launch_grad<T, 1>(a, s);
+  if (v == 8) return launch_grad<T, MOST, 1>(a, s);
+  if (v == 4) return launch_grad<T, 4, 1>(a, s);
+  if (v == 2) return launch_grad<T, 2, 2>(a, s);
+  return launch_grad<T, 1, 4>(a, s);
 }
 
 template <typename T>
-int launch_few(const FewArgs& a, const FewPlan& p, cudaStream_t s) {
+int launch_few(const FewArgs& a, const FewPlan& p, bool pairs, cudaStream_t s) {
   const size_t smem = sizeof(float) * (size_t)p.copies * (size_t)(a.vocab + 1) * p.lanes * p.v;
   static std::atomic<bool> ready[64];
   int dev = 0;
   SB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {   // setting it twice is harmless
-    SB_CUDA(cudaFuncSetAttribute(embedding_few_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, EF_SMEM));
-    SB_CUDA(cudaFuncSetAttribute(embedding_few_kernel<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, EF_SMEM));
+    SB_CUDA(cudaFuncSetAttribute(embedding_few_kernel<T, 1, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, EF_SMEM));
+    SB_CUDA(cudaFuncSetAttribute(embedding_few_kernel<T, 1, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, EF_SMEM));
+    SB_CUDA(cudaFuncSetAttribute(embedding_few_kernel<T, 2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, EF_SMEM));
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
   const dim3 grid(p.blocks, p.slabs);
-  if (p.v == 2) SB_CUDA(sb_launch(embedding_few_kernel<T, 2>, grid, dim3(EF_THREADS), smem, s, 1, a));
-  else SB_CUDA(sb_launch(embedding_few_kernel<T, 1>, grid, dim3(EF_THREADS), smem, s, 1, a));
+  if (p.v == 1) SB_CUDA(sb_launch(embedding_few_kernel<T, 1, 1>, grid, dim3(EF_THREADS), smem, s, 1, a));
+  else if (pairs) SB_CUDA(sb_launch(embedding_few_kernel<T, 2, 1>, grid, dim3(EF_THREADS), smem, s, 1, a));
+  else SB_CUDA(sb_launch(embedding_few_kernel<T, 1, 2>, grid, dim3(EF_THREADS), smem, s, 1, a));
   SB_COUNT_LAUNCH();
   if (p.blocks > 1) {
     const long long size = (long long)a.vocab * a.dim;
@@ -886,10 +911,10 @@ cudaError_t launch_lookup_width(const void* tokens, const void* table, void* out
   constexpr int MOST = SMALL == 4 ? 4 : (sizeof(T) == sizeof(O) ? 8 : 4);
   int v = sb_vector_width(table, ld_table, dim, sizeof(T), MOST);
   v = sb_vector_width(out, ld_out, dim, sizeof(O), v);
-  if (v == 8) return launch_lookup<I, T, O, MOST, 1>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  if (v == 4) return launch_lookup<I, T, O, 4, 1>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  if (v == 2) return launch_lookup<I, T, O, 2, 2>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
-  return launch_lookup<I, T, O, 1, 4>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 8) return launch_lookup<I, T, O, MOST, 2>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 4) return launch_lookup<I, T, O, 4, 2>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  if (v == 2) return launch_lookup<I, T, O, 2, 4>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
+  return launch_lookup<I, T, O, 1, 8>(tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
 }
 
 template <typename I, typename T>
@@ -940,18 +965,21 @@ int sb_embedding_grad_workspace_bytes(long long n, int vocab, int dim, size_t* b
   if (!bytes) return sb_fail(SB_ERR_BAD_ARG, "sb_embedding_grad_workspace_bytes: null output");
   if (n < 0 || vocab < 0 || dim < 0) return sb_fail(SB_ERR_BAD_ARG, "sb_embedding_grad_workspace_bytes: negative size");
   if (n > 0x40000000LL || vocab > 0x40000000) return sb_fail(SB_ERR_TOO_LARGE, "sb_embedding_grad: at most 2^30 tokens and a vocabulary of 2^30");
-  // For whichever width the call's pointers and pitches allow.
+  // For whichever number of columns per thread the call's pointers and pitches allow.
   size_t most = 16;
   if (n == 0 || vocab == 0 || dim == 0) {
     *bytes = most;
     return SB_OK;
   }
-  for (int v = 1; v <= 8; v *= 2) {
-    const size_t need = grad_plan(n, vocab, dim, v).bytes;
+  FewPlan few;
+  if (few_plan(n, vocab, dim, &few)) {
+    const size_t need = sizeof(float) * (size_t)few.blocks * (size_t)vocab * (size_t)dim;
     if (need > most) most = need;
-    FewPlan few;
-    if (v <= 2 && few_plan(n, vocab, dim, v, &few) && sizeof(float) * (size_t)few.blocks * (size_t)vocab * (size_t)dim > most)
-      most = sizeof(float) * (size_t)few.blocks * (size_t)vocab * (size_t)dim;
+  } else {
+    for (int w = 4; w <= 8; w *= 2) {
+      const size_t need = grad_plan(n, vocab, dim, w).bytes;
+      if (need > most) most = need;
+    }
   }
   *bytes = most;
   return SB_OK;
@@ -984,16 +1012,17 @@ int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const vo
   const int item = sb_dtype_size(dout_dtype);
   const int v = grad_width(dout, ld_dout, dtable, ld_dtable, dim, item);
   FewPlan few;
-  if (few_plan(n, vocab, dim, sb_vector_width(dout, ld_dout, dim, item, 2), &few)) {
+  if (few_plan(n, vocab, dim, &few)) {
     FewArgs f;
     memset(&f, 0, sizeof(f));
     f.tokens = tokens; f.dout = dout; f.dtable = dtable; f.partial = (float*)workspace; f.ld_dout = ld_dout; f.ld_dtable = ld_dtable;
     f.n = (int)n; f.vocab = vocab; f.dim = dim; f.index64 = index_dtype == SB_I64; f.lanes = few.lanes; f.copies = few.copies;
     f.per = few.per; f.scale = scale; f.accumulate = accumulate;
-    return dout_dtype == SB_F32 ? launch_few<float>(f, few, s)
-           : dout_dtype == SB_BF16 ? launch_few<__nv_bfloat16>(f, few, s) : launch_few<__half>(f, few, s);
+    const bool pairs = sb_vector_width(dout, ld_dout, dim, item, 2) == 2;
+    return dout_dtype == SB_F32 ? launch_few<float>(f, few, pairs, s)
+           : dout_dtype == SB_BF16 ? launch_few<__nv_bfloat16>(f, few, pairs, s) : launch_few<__half>(f, few, pairs, s);
   }
-  const GradPlan p = grad_plan(n, vocab, dim, v);
+  const GradPlan p = grad_plan(n, vocab, dim, v < 4 ? 4 : v);
   char* ws = (char*)workspace;
   SortArgs a;
   memset(&a, 0, sizeof(a));
