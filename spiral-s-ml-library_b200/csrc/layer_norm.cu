@@ -29,12 +29,40 @@ struct NormArgs {
 // Rows that fit into registers.  LANES threads share a row (a part of a warp, a warp, or W warps), each with NV packs of V
 // elements, R rows at a time.  In the backward pass the running column sums stay in registers over all rows of a thread.
 // The arithmetic is packed, two fp32 operations per instruction: with 12 operations per element and 16 warps per SM the
-// scalar form was bound by issue (65536 x 1024 bf16: 97 us forward, 107 backward).
+// scalar form was bound by issue (65536 x 1024 bf16: 97 us forward, 107 backward; now 65 and 79, fp32 91 and 127, 6 TB/s).  What bounds
+// the 16-bit types is still issue (62 % backward) and, forward, the weights' way from L1.
 constexpr int LN_THREADS = 512;                              // of a block at most
 struct NormShape {
   int warps;                     // per row; 1: `lanes` threads of a warp
   int lanes;                     // threads per row
   int groups;                    // of threads with rows of their own, per block
+  int span;                      // packs of a warp, a multiple of 32, where warps have packs of their own
+};
+// Which packs of a row a thread has.  APART: warps have neighbouring packs of their own, and a thread's are 32 apart: a number
+// that the compiler knows, so that all of a thread's addresses are one register and a constant (20000 x 1501 forward, single
+// elements: fp32 84 -> 67 us, bf16 83 -> 60, against the row's number of threads as the distance, which took 53 instructions per
+// element).  Else the row's `lanes` threads take turns.
+template <int V, int NV, bool APART>
+struct LnPlace {
+  int first, count, apart;       // packs `first` + i * `apart`, i < `count`
+  bool full;                     // all threads of the warp have NV
+  __device__ __forceinline__ LnPlace(const NormShape& s, int lane, int cols) {
+    const int packs = (cols + V - 1) / V;
+    int end = packs, begin = 0;
+    if constexpr (APART) {
+      apart = 32;
+      begin = (lane >> 5) * s.span;
+      end = min(packs, begin + s.span);
+      first = begin + (lane & 31);
+    } else {
+      apart = s.lanes;
+      first = lane;
+    }
+    const int left = end - first + apart - 1;
+    count = left <= 0 ? 0 : APART ? left >> 5 : left / apart;
+    full = end - begin == NV * apart;
+  }
+  __device__ __forceinline__ int stride() const { return (APART ? 32 : apart) * V; }   // elements
 };
 typedef unsigned long long Pair; // two fp32 values
 __device__ __forceinline__ Pair ln_pair(float v) { return pack_f32x2(v, v); }
@@ -86,26 +114,34 @@ struct LnAhead {
     stride = blockDim.x * PACK;
     mine = smem + threadIdx.x * PACK;
     slot = 0;
+    if constexpr (RING)                                      // places behind a row's end stay zero
+      for (uint32_t k = 0; k < DEPTH * TURN; ++k)
+#pragma unroll
+        for (uint32_t w = 0; w < PACK; w += 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(mine + k * stride + w), "r"(0) : "memory");
   }
   // Rows `row` .. `row` + R - 1; `from` points at this thread's first element of the first.
-  __device__ __forceinline__ void fetch(int matrix, const T* from, long long row, long long ld, const NormArgs& a, int lane, int lanes, int to) {
+  template <typename Place>
+  __device__ __forceinline__ void fetch(int matrix, const T* from, long long row, long long ld, const NormArgs& a, const Place& place, int to) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      const int count = row + r < a.rows ? place.count : 0;
+      const T* at = from + (row + r < a.rows ? r * ld : 0);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const bool in = row + r < a.rows && (lane + i * lanes) * V < a.cols;
-        const T* at = in ? from + r * ld + i * lanes * V : from;
         const int k = (matrix * R + r) * NV + i;
         if constexpr (RING) {
           const uint32_t dst = mine + (uint32_t)(to * (int)TURN + k) * stride;
           if constexpr (PACK == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? at : (const T*)a.x), "r"(in ? 16u : 0u) : "memory");
+            asm volatile("{\n\t.reg .pred q;\n\tsetp.lt.s32 q, %2, %3;\n\t@q cp.async.cg.shared.global [%0], [%1], 16;\n\t}"
+                         ::"r"(dst), "l"(at + i * place.stride()), "r"(i), "r"(count) : "memory");
           else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(in ? at : (const T*)a.x), "r"(in ? 4u : 0u) : "memory");
+            asm volatile("{\n\t.reg .pred q;\n\tsetp.lt.s32 q, %2, %3;\n\t@q cp.async.ca.shared.global [%0], [%1], 4;\n\t}"
+                         ::"r"(dst), "l"(at + i * place.stride()), "r"(i), "r"(count) : "memory");
         } else {
-          held[k] = in ? sb_load_pack<T, V>(at) : sb_zero_pack<T, V>();
+          held[k] = i < count ? sb_load_pack<T, V>(at + i * place.stride()) : sb_zero_pack<T, V>();
         }
       }
+    }
   }
   __device__ __forceinline__ void read(int matrix, int r, int i, float* x) const {
     static_assert(!RING || PACK == 4 || PACK == 16, "");
@@ -132,10 +168,10 @@ struct LnAhead {
   }
 };
 
-// V weights from column `col` on (16-byte loads where V allows them); `other` where there are none or the row has ended.
+// V weights (16-byte loads where V allows them); `other` where there are none (`have`: the row goes that far).
 template <int V>
-__device__ __forceinline__ void ln_weights(const float* w, int col, int cols, float other, float* to) {
-  if (!w || col >= cols) {
+__device__ __forceinline__ void ln_weights(const float* w, int col, bool have, float other, float* to) {
+  if (!w || !have) {
 #pragma unroll
     for (int k = 0; k < V; ++k) to[k] = other;
   } else if constexpr (V >= 4) {
@@ -174,12 +210,14 @@ __device__ __forceinline__ void ln_store(T* to, const Pair* x, int i) {
 constexpr int LN_DEPTH = 3;
 
 // Weights are read for every row, from L1: in registers they would cost half of the warps.
-template <typename T, int V, int NV, int R>
+template <typename T, int V, int NV, int R, bool APART>
 __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, NormShape s) {
   constexpr int E = NV * V;
   __shared__ float4 slots[2][LN_THREADS / 32];
   extern __shared__ __align__(16) uint8_t ln_smem[];
   const int group = threadIdx.x / s.lanes, lane = threadIdx.x % s.lanes;
+  const LnPlace<V, NV, APART> place(s, lane, a.cols);
+  const int stride = place.stride();
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const long long step = (long long)R * gridDim.x * s.groups;
@@ -189,18 +227,17 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
   LnAhead<T, V, NV, R, 1, LN_DEPTH> rows;
   constexpr bool RING = decltype(rows)::RING;
   rows.start(smem_u32(ln_smem));
-  const T* x_at = (const T*)a.x + row * a.ldx + lane * V;
-  T* y_at = (T*)a.out + row * a.ldout + lane * V;
+  const T* x_at = (const T*)a.x + row * a.ldx + place.first * V;
+  T* y_at = (T*)a.out + row * a.ldout + place.first * V;
   constexpr int FIRST = RING ? LN_DEPTH - 1 : 1;
 #pragma unroll
   for (int d = 0; d < FIRST; ++d) {
-    rows.fetch(0, x_at + d * step * a.ldx, row + d * step, a.ldx, a, lane, s.lanes, d);
+    rows.fetch(0, x_at + d * step * a.ldx, row + d * step, a.ldx, a, place, d);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  const bool full = a.cols == s.lanes * E;
   for (long long at = last; at < a.rows; at += step, row += step, x_at += step * a.ldx, y_at += step * a.ldout) {
     if (RING) {
-      rows.fetch(0, x_at + (LN_DEPTH - 1) * step * a.ldx, row + (LN_DEPTH - 1) * step, a.ldx, a, lane, s.lanes,
+      rows.fetch(0, x_at + (LN_DEPTH - 1) * step * a.ldx, row + (LN_DEPTH - 1) * step, a.ldx, a, place,
                  rows.slot == 0 ? LN_DEPTH - 1 : rows.slot - 1);
       asm volatile("cp.async.commit_group;" ::: "memory");
       asm volatile("cp.async.wait_group %0;" ::"n"(LN_DEPTH - 1) : "memory");
@@ -215,7 +252,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
       for (int j = 1; j < E / 2; ++j) t = add_f32x2(t, x[r][j]);
       v[r] = ln_both(t);
     }
-    if (!RING) rows.fetch(0, x_at + step * a.ldx, row + step, a.ldx, a, lane, s.lanes, 0);
+    if (!RING) rows.fetch(0, x_at + step * a.ldx, row + step, a.ldx, a, place, 0);
     rows.next();
     ln_row_sums<R>(v, s, group, slots[0]);
     float mean[R];
@@ -226,13 +263,13 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
       Pair t = 0ull;
 #pragma unroll
       for (int j = 0; j < E / 2; ++j) x[r][j] = sub_f32x2(x[r][j], m);
-      if (!full) {                                           // what lies behind the row's end deviates by nothing
+      if (!place.full) {                                           // what lies behind the row's end deviates by nothing
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
           float lo, hi;
           unpack_f32x2(x[r][j], lo, hi);
-          if ((lane + 2 * j / V * s.lanes) * V >= a.cols) lo = 0.f;
-          if ((lane + (2 * j + 1) / V * s.lanes) * V >= a.cols) hi = 0.f;
+          if (2 * j / V >= place.count) lo = 0.f;
+          if ((2 * j + 1) / V >= place.count) hi = 0.f;
           x[r][j] = pack_f32x2(lo, hi);
         }
       }
@@ -255,8 +292,8 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
       float w[P * V], b[P * V];
 #pragma unroll
       for (int q = 0; q < P; ++q) {
-        ln_weights<V>(a.weight, (lane + (i + q) * s.lanes) * V, a.cols, 1.f, w + q * V);
-        ln_weights<V>(a.bias, (lane + (i + q) * s.lanes) * V, a.cols, 0.f, b + q * V);
+        ln_weights<V>(a.weight, place.first * V + (i + q) * stride, i + q < place.count, 1.f, w + q * V);
+        ln_weights<V>(a.bias, place.first * V + (i + q) * stride, i + q < place.count, 0.f, b + q * V);
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -268,8 +305,8 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
         }
 #pragma unroll
         for (int q = 0; q < P; ++q)
-          if (row + r < a.rows && (lane + (i + q) * s.lanes) * V < a.cols)
-            ln_store<T, V>(y_at + r * a.ldout + (i + q) * s.lanes * V, x[r], i + q);
+          if (row + r < a.rows && i + q < place.count)
+            ln_store<T, V>(y_at + r * a.ldout + (i + q) * stride, x[r], i + q);
       }
     }
     if (lane == 0) {
@@ -285,7 +322,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_kernel(NormArgs a, Norm
 }
 
 // The backward pass: x and dy are read once for dx and the column sums together.
-template <typename T, int V, int NV, int R>
+template <typename T, int V, int NV, int R, bool APART>
 __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a, NormShape s) {
   constexpr int E = NV * V;
   __shared__ float4 slots[2][LN_THREADS / 32];
@@ -293,7 +330,9 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
   extern __shared__ __align__(16) uint8_t ln_smem[];
   float* columns = reinterpret_cast<float*>(ln_smem);        // [2][cols], where several groups of a block add up at the end
   const int group = threadIdx.x / s.lanes, lane = threadIdx.x % s.lanes;
-  const int unit = s.warps > 1 ? threadIdx.x >> 5 : group, place = s.warps > 1 ? threadIdx.x & 31 : lane;
+  const int unit = s.warps > 1 ? threadIdx.x >> 5 : group, member = s.warps > 1 ? threadIdx.x & 31 : lane;
+  const LnPlace<V, NV, APART> place(s, lane, a.cols);
+  const int stride = place.stride();
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const long long step = (long long)R * gridDim.x * s.groups;
@@ -302,17 +341,17 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
   LnAhead<T, V, NV, R, 2, LN_DEPTH> rows;
   constexpr bool RING = decltype(rows)::RING;
   rows.start(smem_u32(ln_smem));
-  const T* x_at = (const T*)a.x + row * a.ldx + lane * V;
-  const T* dy_at = (const T*)a.dy + row * a.lddy + lane * V;
-  T* dx_at = (T*)a.out + row * a.ldout + lane * V;
+  const T* x_at = (const T*)a.x + row * a.ldx + place.first * V;
+  const T* dy_at = (const T*)a.dy + row * a.lddy + place.first * V;
+  T* dx_at = (T*)a.out + row * a.ldout + place.first * V;
   auto fetch = [&](int turns, int to) {
     const long long at = row + turns * step;
-    rows.fetch(0, x_at + turns * step * a.ldx, at, a.ldx, a, lane, s.lanes, RING ? to : 0);
-    rows.fetch(1, dy_at + turns * step * a.lddy, at, a.lddy, a, lane, s.lanes, RING ? to : 0);
-    if (place < 2 * R) {
-      const bool in = at + place % R < a.rows;
-      const float* from = (place < R ? a.mean : a.rstd) + (in ? at + place % R : 0);
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&stats[to][unit][place])), "l"(from), "r"(in ? 4u : 0u) : "memory");
+    rows.fetch(0, x_at + turns * step * a.ldx, at, a.ldx, a, place, RING ? to : 0);
+    rows.fetch(1, dy_at + turns * step * a.lddy, at, a.lddy, a, place, RING ? to : 0);
+    if (member < 2 * R) {
+      const bool in = at + member % R < a.rows;
+      const float* from = (member < R ? a.mean : a.rstd) + (in ? at + member % R : 0);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(&stats[to][unit][member])), "l"(from), "r"(in ? 4u : 0u) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -323,7 +362,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
   {
     float f[E];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) ln_weights<V>(a.weight, (lane + i * s.lanes) * V, a.cols, 1.f, f + i * V);
+    for (int i = 0; i < NV; ++i) ln_weights<V>(a.weight, place.first * V + i * stride, i < place.count, 1.f, f + i * V);
 #pragma unroll
     for (int j = 0; j < E / 2; ++j) {
       w[j] = pack_f32x2(f[2 * j], f[2 * j + 1]);
@@ -346,8 +385,13 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
       const float mean = *(volatile float*)&stats[rows.slot][unit][r];
       rstd[r] = *(volatile float*)&stats[rows.slot][unit][R + r];
       const Pair m = ln_pair(mean), f = ln_pair(rstd[r]);
-      ln_read<decltype(rows), V, NV>(rows, 0, r, h[r]);
-      ln_read<decltype(rows), V, NV>(rows, 1, r, g[r]);
+      if (row + r < a.rows) {                                // else the places hold an earlier row
+        ln_read<decltype(rows), V, NV>(rows, 0, r, h[r]);
+        ln_read<decltype(rows), V, NV>(rows, 1, r, g[r]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) h[r][j] = g[r][j] = 0ull;
+      }
       Pair s1 = 0ull, s2 = 0ull;
 #pragma unroll
       for (int j = 0; j < E / 2; ++j) {
@@ -377,7 +421,7 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-          if (row + r < a.rows && (lane + i * s.lanes) * V < a.cols) ln_store<T, V>(dx_at + r * a.ldout + i * s.lanes * V, g[r], i);
+          if (row + r < a.rows && i < place.count) ln_store<T, V>(dx_at + r * a.ldout + i * stride, g[r], i);
       }
     }
     row += step;
@@ -397,8 +441,8 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
   if (s.groups == 1) {
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const int col = (lane + j / V * s.lanes) * V + j % V;
-      if (col < a.cols) {
+      const int col = place.first * V + j / V * stride + j % V;
+      if (j / V < place.count) {
         part[col] = sums[0][j];
         part[a.cols + col] = sums[1][j];
       }
@@ -419,8 +463,8 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_grad_kernel(NormArgs a,
     if (t == my_turn && mine) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const int col = (lane + j / V * s.lanes) * V + j % V;
-        if (col < a.cols) {
+        const int col = place.first * V + j / V * stride + j % V;
+        if (j / V < place.count) {
           columns[col] = (t ? columns[col] : 0.f) + sums[0][j];
           columns[a.cols + col] = (t ? columns[a.cols + col] : 0.f) + sums[1][j];
         }
@@ -573,17 +617,19 @@ int norm_element_aligned(const char* who, const void* p, int dtype) {
   return SB_OK;
 }
 
-// How many threads share a row, for packs of v elements and nv of them per thread; false: the row does not fit.
-bool norm_shape(int cols, int v, int nv, NormShape* s) {
+// How many threads share a row, for packs of v elements and nv of them per thread (whole warps where these have packs of their
+// own); false: the row does not fit.
+bool norm_shape(int cols, int v, int nv, bool apart, NormShape* s) {
   const int packs = (cols + v - 1) / v, most = LN_THREADS * nv;
   if (packs > most) return false;
   s->warps = (packs + 32 * nv - 1) / (32 * nv);
   s->lanes = 32 * s->warps;
-  if (s->warps == 1) {
+  if (s->warps == 1 && !apart) {
     s->lanes = 4;
     while (s->lanes * nv < packs) s->lanes *= 2;
   }
   s->groups = s->lanes < 256 ? 256 / s->lanes : 1;
+  s->span = ((packs + s->warps - 1) / s->warps + 31) / 32 * 32;
   return true;
 }
 
@@ -607,20 +653,37 @@ cudaError_t norm_resident(int threads, size_t smem, int* blocks) {
   return cudaSuccess;
 }
 
+// The groups of a block, and the blocks: as many threads as fit at a time.  Numbers of threads per row that do not divide 256
+// may do better in blocks of up to 512 (96 threads per row at 128 registers: one block of five rows, two of two).
+template <auto KERNEL, typename Smem>
+cudaError_t norm_groups(NormShape* s, const Smem& smem, int* blocks) {
+  cudaError_t e = norm_resident<KERNEL>(s->lanes * s->groups, smem(*s), blocks);
+  if (e != cudaSuccess || 256 % s->lanes == 0 || LN_THREADS / s->lanes <= s->groups) return e;
+  NormShape other = *s;
+  other.groups = LN_THREADS / s->lanes;
+  int more = 0;
+  if ((e = norm_resident<KERNEL>(other.lanes * other.groups, smem(other), &more)) != cudaSuccess) return e;
+  if (more * other.groups > *blocks * s->groups) {
+    *s = other;
+    *blocks = more;
+  }
+  return e;
+}
+
 int norm_grid(const NormArgs& a, const NormShape& s, int r, int most) {
   const long long at_once = (long long)r * s.groups, want = (a.rows + at_once - 1) / at_once;
   return (int)(want < most ? want : most);
 }
 
-template <typename T, int V, int NV, int R>
+template <typename T, int V, int NV, int R, bool APART>
 bool try_norm(const NormArgs& a, cudaStream_t s, cudaError_t* e) {
   NormShape shape;
-  if (!norm_shape(a.cols, V, NV, &shape)) return false;
-  const int threads = shape.lanes * shape.groups;
-  const size_t smem = LnAhead<T, V, NV, R, 1, LN_DEPTH>::bytes(threads);
+  if (!norm_shape(a.cols, V, NV, APART, &shape)) return false;
+  const auto smem = [](const NormShape& s) { return LnAhead<T, V, NV, R, 1, LN_DEPTH>::bytes(s.lanes * s.groups); };
   int blocks = 0;
-  if ((*e = norm_resident<layer_norm_kernel<T, V, NV, R>>(threads, smem, &blocks)) == cudaSuccess)
-    *e = sb_launch(layer_norm_kernel<T, V, NV, R>, dim3(norm_grid(a, shape, R, blocks)), dim3(threads), smem, s, 1, a, shape);
+  if ((*e = norm_groups<layer_norm_kernel<T, V, NV, R, APART>>(&shape, smem, &blocks)) == cudaSuccess)
+    *e = sb_launch(layer_norm_kernel<T, V, NV, R, APART>, dim3(norm_grid(a, shape, R, blocks)), dim3(shape.lanes * shape.groups), smem(shape), s,
+                   1, a, shape);
   return true;
 }
 
@@ -637,16 +700,18 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
   v = norm_width(sb_vector_width(a.out, a.ldout, a.cols, sizeof(T), v), sizeof(T), a);
   cudaError_t e = cudaSuccess;
   if (v == MOST) {
-    // Two rows share a load of their weights: 16384 x 4096 bf16 71 us, 79 with twice the columns of one row.
-    if (a.cols <= 32 * MOST && try_norm<T, MOST, 1, 2>(a, s, &e)) return e;
-    if (try_norm<T, MOST, 2, 2>(a, s, &e)) return e;
-    if (try_norm<T, MOST, 4, 1>(a, s, &e)) return e;
+    // Two rows share a load of their weights: 16384 x 4096 bf16 72 us, 79 with twice the columns of one row.
+    if (a.cols <= 32 * MOST && try_norm<T, MOST, 1, 2, false>(a, s, &e)) return e;
+    if (try_norm<T, MOST, 2, 2, true>(a, s, &e)) return e;
+    if (try_norm<T, MOST, 4, 1, true>(a, s, &e)) return e;
   } else if (v == WORD && WORD > 1) {
-    if (a.cols <= 128 * WORD && try_norm<T, WORD, 4, 2>(a, s, &e)) return e;
-    if (try_norm<T, WORD, 16, 1>(a, s, &e)) return e;
+    if (a.cols <= 128 * WORD && try_norm<T, WORD, 4, 2, false>(a, s, &e)) return e;
+    if (try_norm<T, WORD, 8, 2, true>(a, s, &e)) return e;
+    if (try_norm<T, WORD, 16, 1, true>(a, s, &e)) return e;
   } else {
-    if (a.cols <= 128 && try_norm<T, 1, 4, 2>(a, s, &e)) return e;
-    if (try_norm<T, 1, 16, 1>(a, s, &e)) return e;
+    if (a.cols <= 128 && try_norm<T, 1, 4, 2, false>(a, s, &e)) return e;
+    if (try_norm<T, 1, 8, 2, true>(a, s, &e)) return e;
+    if (try_norm<T, 1, 16, 1, true>(a, s, &e)) return e;
   }
   const int threads = a.cols >= 1024 ? 1024 : (a.cols + 31) / 32 * 32;
   const long long most = 16LL * sb_sm_count();
@@ -654,18 +719,19 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t s) {
 }
 
 // Writes the partial sums' number to *parts where the row fits into registers.
-template <typename T, int V, int NV, int R>
+template <typename T, int V, int NV, int R, bool APART>
 bool try_norm_grad(const NormArgs& a, cudaStream_t s, cudaError_t* e, int* parts) {
   NormShape shape;
-  if (!norm_shape(a.cols, V, NV, &shape)) return false;
-  const int threads = shape.lanes * shape.groups;
-  const size_t ahead = LnAhead<T, V, NV, R, 2, LN_DEPTH>::bytes(threads);
-  const size_t sums = shape.groups > 1 ? 2 * sizeof(float) * (size_t)a.cols : 0;   // at most 16 KB: two groups share 256 threads
-  const size_t smem = ahead > sums ? ahead : sums;
+  if (!norm_shape(a.cols, V, NV, APART, &shape)) return false;
+  const auto smem = [&a](const NormShape& s) {
+    const size_t ahead = LnAhead<T, V, NV, R, 2, LN_DEPTH>::bytes(s.lanes * s.groups);
+    const size_t sums = s.groups > 1 ? 2 * sizeof(float) * (size_t)a.cols : 0;     // at most 32 KB: two groups share 512 threads
+    return ahead > sums ? ahead : sums;
+  };
   int blocks = 0;
-  if ((*e = norm_resident<layer_norm_grad_kernel<T, V, NV, R>>(threads, smem, &blocks)) != cudaSuccess) return true;
+  if ((*e = norm_groups<layer_norm_grad_kernel<T, V, NV, R, APART>>(&shape, smem, &blocks)) != cudaSuccess) return true;
   *parts = norm_grid(a, shape, R, blocks);
-  *e = sb_launch(layer_norm_grad_kernel<T, V, NV, R>, dim3(*parts), dim3(threads), smem, s, 1, a, shape);
+  *e = sb_launch(layer_norm_grad_kernel<T, V, NV, R, APART>, dim3(*parts), dim3(shape.lanes * shape.groups), smem(shape), s, 1, a, shape);
   return true;
 }
 
@@ -679,14 +745,16 @@ cudaError_t launch_norm_grad(const NormArgs& a, cudaStream_t s, int* parts) {
   cudaError_t e = cudaSuccess;
   // Short rows two at a time (65536 x 1024 fp32 147 -> 127 us, bf16 82 -> 80, against one pack per thread and more warps per row).
   if (v == MOST) {
-    if (a.cols <= 64 * MOST && try_norm_grad<T, MOST, 1, 2>(a, s, &e, parts)) return e;
-    if (try_norm_grad<T, MOST, 2, 1>(a, s, &e, parts)) return e;
+    if (a.cols <= 64 * MOST && try_norm_grad<T, MOST, 1, 2, false>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, MOST, 2, 1, true>(a, s, &e, parts)) return e;
   } else if (v == WORD && WORD > 1) {
-    if (try_norm_grad<T, WORD, 4, 1>(a, s, &e, parts)) return e;
-    if (try_norm_grad<T, WORD, 8, 1>(a, s, &e, parts)) return e;
+    if (a.cols <= 128 * WORD && try_norm_grad<T, WORD, 4, 1, false>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, WORD, 4, 1, true>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, WORD, 8, 1, true>(a, s, &e, parts)) return e;
   } else {
-    if (try_norm_grad<T, 1, 8, 1>(a, s, &e, parts)) return e;
-    if (try_norm_grad<T, 1, 16, 1>(a, s, &e, parts)) return e;
+    if (a.cols <= 256 && try_norm_grad<T, 1, 8, 1, false>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, 1, 8, 1, true>(a, s, &e, parts)) return e;
+    if (try_norm_grad<T, 1, 16, 1, true>(a, s, &e, parts)) return e;
   }
   *parts = 0;
   if (!a.out) return cudaSuccess;
