@@ -11,6 +11,8 @@
 #include "common.cuh"
 #include "vector_io.cuh"
 
+#include <limits.h>
+
 namespace {
 
 // ------------------------------- lookup -----------------------------------------
@@ -569,6 +571,105 @@ __global__ void __launch_bounds__(256, 3) embedding_grad_kernel(GradArgs a) {
   }
 }
 
+// Few tokens in one launch: a block has neighbouring rows of the table to itself, picks the tokens that are theirs out of all,
+// sorts them by counting the ones before each, and goes through its rows; nothing crosses blocks.  Bound by latency and by writing
+// the table.  Against the sort, walk and join in three launches: 1 token of 2439, 369 columns 3.2 us (13.4), 256 of 5611, 37 columns
+// 7.0 (15.9), 256 of 70000, 64 columns 8.5 (19.5); 256 positions of one token 28 (15.6), 128 of them 19 (19).  A call's host time
+// falls from 13 to 8 us.
+constexpr int GRAD_FEW_TOKENS = 256;
+template <typename T, int V, int PACKS>
+__global__ void __launch_bounds__(GRAD_FEW_TOKENS, 4) embedding_scan_kernel(GradArgs a, const void* tokens, int index64, int rows) {
+  __shared__ __align__(16) int s_raw[GRAD_FEW_TOKENS];
+  __shared__ int s_key[GRAD_FEW_TOKENS], s_pos[GRAD_FEW_TOKENS], s_count;
+  const int first = blockIdx.x * rows, last = (int)min((long long)first + rows, (long long)a.vocab);
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  long long token = -1;
+  if ((int)threadIdx.x < a.n) token = index64 ? ((const long long*)tokens)[threadIdx.x] : (long long)((const int*)tokens)[threadIdx.x];
+  const bool mine = token >= first && token < last;
+  s_raw[threadIdx.x] = mine ? (int)token : INT_MAX;          // last in the order, and no key is as large
+  const unsigned with = __ballot_sync(0xffffffffu, mine);
+  if ((threadIdx.x & 31) == 0 && with) atomicAdd(&s_count, __popc(with));
+  __syncthreads();
+  const int count = s_count;
+  if (mine) {
+    int before = 0;
+#pragma unroll 4
+    for (int i = 0; i < a.n; i += 4) {
+      const int4 w = *reinterpret_cast<const int4*>(&s_raw[i]);
+      const int t = (int)token, at = (int)threadIdx.x - i;   // equal ones count where they come first
+      before += (w.x < t + (at > 0)) + (w.y < t + (at > 1)) + (w.z < t + (at > 2)) + (w.w < t + (at > 3));
+    }
+    s_key[before] = (int)token;
+    s_pos[before] = threadIdx.x;
+  }
+  __syncthreads();
+  const int in_group = threadIdx.x % a.group, g = threadIdx.x / a.group, groups = blockDim.x / a.group;
+  const int col = blockIdx.y * PACKS * a.group * V + in_group * V;
+  const int each = (last - first + groups - 1) / groups, row0 = min(first + g * each, last), row_end = min(row0 + each, last);
+  if (col >= a.dim || row0 >= row_end) return;
+  auto lower = [&](int row) {                                // the first entry of `row` or behind
+    int lo = 0, hi = count;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_key[mid] < row) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo;
+  };
+  // A row at a time; few have any token.
+  constexpr int UNROLL = 8;
+  const int stride = a.group * V;
+  const T* dout = (const T*)a.dout + col;
+  float* to = a.dtable + (long long)row0 * a.ld_dtable + col;
+  int k = lower(row0);
+  int next = k < count ? s_key[k] : INT_MAX;
+  for (int row = row0; row < row_end; ++row, to += a.ld_dtable) {
+    float acc[PACKS * V];
+#pragma unroll
+    for (int t = 0; t < PACKS * V; ++t) acc[t] = 0.f;
+    if (next == row) {
+      int end = k + 1;
+      while (end < count && s_key[end] == row) ++end;
+      for (; k < end; k += UNROLL) {
+        SbWords<sizeof(T) * V> in[UNROLL][PACKS] = {};       // zeros where there is no row
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          const bool issue = k + u < end;
+          const T* from = dout + (long long)(issue ? s_pos[k + u] : 0) * a.ld_dout;
+#pragma unroll
+          for (int p = 0; p < PACKS; ++p) sb_load_words(in[u][p], from + p * stride, issue && col + p * stride < a.dim);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+          for (int p = 0; p < PACKS; ++p) {
+            float v[V];
+            sb_unpack_words<T, V>(in[u][p], v);
+#pragma unroll
+            for (int t = 0; t < V; ++t) acc[p * V + t] += v[t];
+          }
+      }
+      k = end;
+      next = k < count ? s_key[k] : INT_MAX;
+    }
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p) {
+      if (col + p * stride >= a.dim) continue;
+      float* at = to + p * stride;
+#pragma unroll
+      for (int t = 0; t < V; ++t) acc[p * V + t] = a.accumulate ? at[t] + acc[p * V + t] * a.scale : acc[p * V + t] * a.scale;
+#pragma unroll
+      for (int t = 0; t < V; t += 4) {
+        if constexpr (V >= 4) sb_store_f32<float, 4>(at + t, acc + p * V + t);
+        else sb_store_f32<float, V>(at, acc + p * V);
+      }
+    }
+  }
+}
+
 // A table of few rows needs no sort: every warp (or part of one) adds its share of the positions, in their order, to a table of
 // its own in shared memory, one or two columns per thread; the block adds its tables up, and the blocks' sums are
 // added in their order by a second launch.  Bound by reading dout: 524288 x 64 bf16 over 53 tokens 28 us (floor 11).
@@ -859,6 +960,30 @@ int grad_width(const void* dout, long long ld_dout, const float* dtable, long lo
   return w < most ? w : v;
 }
 
+template <typename T, int V, int PACKS>
+int launch_scan(GradArgs& a, const void* tokens, int index64, cudaStream_t s) {
+  a.group = 1;
+  while (a.group < (a.dim + V * PACKS - 1) / (V * PACKS) && a.group < 256) a.group *= 2;
+  // Sixteen blocks per SM (200 tokens of 50001, 1000 columns 37 us, 54 with four), or a row per group.
+  const int groups = GRAD_FEW_TOKENS / a.group, most = 16 * sb_sm_count();
+  const int threads = (a.dim + V * PACKS - 1) / (V * PACKS), slabs = (threads + a.group - 1) / a.group;
+  int rows = (int)(((long long)a.vocab * slabs + most - 1) / most);
+  if (rows < groups) rows = groups;
+  SB_CUDA(sb_launch(embedding_scan_kernel<T, V, PACKS>, dim3((unsigned)((a.vocab + (long long)rows - 1) / rows), slabs), dim3(GRAD_FEW_TOKENS), 0, s, 1, a,
+                    tokens, index64, rows));
+  SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+template <typename T>
+int launch_scan_type(GradArgs& a, int v, const void* tokens, int index64, cudaStream_t s) {
+  constexpr int MOST = 16 / sizeof(T);
+  if (v == 8) return launch_scan<T, MOST, 1>(a, tokens, index64, s);
+  if (v == 4) return launch_scan<T, 4, 1>(a, tokens, index64, s);
+  if (v == 2) return launch_scan<T, 2, 2>(a, tokens, index64, s);
+  return launch_scan<T, 1, 4>(a, tokens, index64, s);
+}
+
 template <typename T>
 int launch_grad_type(GradArgs& a, int v, cudaStream_t s) {
   constexpr int MOST = 16 / sizeof(T);
@@ -1021,6 +1146,15 @@ int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const vo
     const bool pairs = sb_vector_width(dout, ld_dout, dim, item, 2) == 2;
     return dout_dtype == SB_F32 ? launch_few<float>(f, few, pairs, s)
            : dout_dtype == SB_BF16 ? launch_few<__nv_bfloat16>(f, few, pairs, s) : launch_few<__half>(f, few, pairs, s);
+  }
+  if (n <= GRAD_FEW_TOKENS) {
+    GradArgs g;
+    memset(&g, 0, sizeof(g));
+    g.dout = dout; g.dtable = dtable; g.ld_dout = ld_dout; g.ld_dtable = ld_dtable; g.n = (int)n; g.vocab = vocab; g.dim = dim;
+    g.scale = scale; g.accumulate = accumulate;
+    const int index64 = index_dtype == SB_I64;
+    return dout_dtype == SB_F32 ? launch_scan_type<float>(g, v, tokens, index64, s)
+           : dout_dtype == SB_BF16 ? launch_scan_type<__nv_bfloat16>(g, v, tokens, index64, s) : launch_scan_type<__half>(g, v, tokens, index64, s);
   }
   const GradPlan p = grad_plan(n, vocab, dim, v < 4 ? 4 : v);
   char* ws = (char*)workspace;
