@@ -672,7 +672,8 @@ __global__ void __launch_bounds__(GRAD_FEW_TOKENS, 4) embedding_scan_kernel(Grad
 
 // A table of few rows needs no sort: every warp (or part of one) adds its share of the positions, in their order, to a table of
 // its own in shared memory, one or two columns per thread; the block adds its tables up, and the blocks' sums are
-// added in their order by a second launch.  Bound by reading dout: 524288 x 64 bf16 over 53 tokens 28 us (floor 11).
+// added in their order by a second launch.  524288 x 64 bf16 over 53 tokens
+// 28 us (floor 11): bound by the tables' turns of load, add and store in shared memory.
 constexpr int EF_THREADS = 512;
 constexpr int EF_SMEM = 200 * 1024;
 struct FewArgs {
@@ -866,9 +867,9 @@ struct FewPlan {
   int v, lanes, copies, per, blocks, slabs;
 };
 
-// Copies of 64 columns of the table (two per thread; 32 or 16, one per thread, of shorter rows and where dout does not allow
-// pairs) in a block's shared memory: nine or more of them, up to 85 rows or so.  524288 tokens, 64 columns bf16, 53 / 120 rows: 28 /
-// 56 us (14 / 6 copies), sorted 42.  256 tokens of 53 / 256: 6 / 19 us (14 / 3 copies), sorted 17.
+// Copies of 64 columns of the table (two per thread, neighbours where dout allows pairs; 32 or 16, one per thread, of shorter
+// rows) in a block's shared memory: nine or more of them, up to 85 rows or so.  524288 tokens, 64 columns bf16, 53 / 120 rows: 28 /
+// 56 us (14 / 6 copies), sorted 42.  24116 x 1347 f16 of 16: 42 us with pairs 32 columns apart, 73 with one column per thread.
 bool few_plan(long long n, int vocab, int dim, FewPlan* p) {
   p->v = dim >= 64 ? 2 : 1;
   p->lanes = 32;

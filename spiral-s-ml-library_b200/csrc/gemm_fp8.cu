@@ -69,6 +69,8 @@ __device__ __forceinline__ uint32_t f8_largest_bits(uint32_t largest) {
 
 // A block of 256 threads per ROWS x 128 tile of x, which stays in registers between the search for its largest magnitude
 // and the rounding; L lanes share a row, V neighbouring elements each.  SQUARE: one scale for the tile, else one per row.
+// Bound by issue (products, roundings and packing: three quarters of the slots) more than by memory: 16384 x 4096 bf16 40 us,
+// 5.0 TB/s, 65536 x 1024 f16 39.5 (42 with the magnitudes one at a time).
 template <typename T, int V, int ROWS, bool SQUARE>
 __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
   constexpr int L = F8_BLOCK / V < 32 ? F8_BLOCK / V : 32;   // lanes per row
@@ -262,6 +264,8 @@ constexpr int F8_FIRST = 4;                                  // the first of the
 constexpr int F8_THREADS = 32 * (F8_FIRST + F8_WARPS);
 constexpr int F8_SMEM = 225 * 1024;
 constexpr uint32_t F8_BOX = 4096;                            // a warp's staging box: 32 rows x 128 bytes
+// Boxes of a warp: where it fills several per tile, one is read by its store while the next is filled.
+__host__ __device__ constexpr int f8_boxes(int bn) { return bn == 256 ? 2 : 1; }
 constexpr int F8_AHEAD = 4;                                  // blocks whose scales are on their way or in use
 constexpr uint32_t F8_SCALES = F8_WARPS * 32 * 8;            // bytes of one block's: a pair per adding thread
 
@@ -316,8 +320,9 @@ __device__ __forceinline__ void f8_add(unsigned long long* sum, const uint32_t* 
     fma_f32x2(sum[j], pack_f32x2(__uint_as_float(part[2 * j]), __uint_as_float(part[2 * j + 1])), scale);
 }
 
-// A box of 32 rows -> C with plain stores.  Lane l has columns l, l + 32, ... of a row; the places of 8 rows (4 where a row is
-// 64 bytes: two rows share a 128-byte line) repeat with the swizzle, so the loop over rows knows them as constants.
+// A box of 32 rows -> C with plain stores.  Lane l has columns l, l + 32, ... of a row; the places of 8 rows repeat with the
+// swizzle, so the loop over rows knows them as constants.  9653 x 1114 x 1008 bf16 27 us (24 for the 1120 columns that TMA stores),
+// 42 with an element's row and place worked out one by one; 3778 x 2006 x 2496 fp32 35.5 and 44.
 template <typename O, int BOX_COLS>
 __device__ __forceinline__ void f8_write_rows(O* to, long long ldc, int rows, int cols, uint32_t box, int lane) {
   constexpr int PER = 16 / sizeof(O), ROW_BYTES = BOX_COLS * sizeof(O), PIECES = ROW_BYTES / 16;
@@ -352,17 +357,21 @@ __device__ __forceinline__ void f8_write_rows(O* to, long long ldc, int rows, in
 
 // Finished values of this warp's 32 rows and COLS columns (their biases in shared memory) -> C, a box of 32 rows x 128 bytes at a time (64 bytes where the
 // columns are no more): by a TMA store, or by coalesced stores where C's rows are not whole 16-byte pieces.
-template <typename O, int COLS>
+template <typename O, int COLS, int BOXES>
 __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tmap_c, bool tma, const unsigned long long* sum,
-                                         long long row0, int col0, uint32_t box, uint32_t bias, int lane) {
+                                         long long row0, int col0, uint32_t boxes, uint32_t bias, int lane) {
   constexpr int BOX_COLS = COLS * sizeof(O) >= 128 ? 128 / sizeof(O) : COLS;
   constexpr int ROW_BYTES = BOX_COLS * sizeof(O), PIECES = ROW_BYTES / 16, PER = 16 / sizeof(O);
 #pragma unroll
   for (int b = 0; b < COLS / BOX_COLS; ++b) {
     const int first = col0 + b * BOX_COLS;
     if (first >= g.n) return;
-    if (tma) {
-      if (lane == 0) bulk_wait_group_read<0>();
+    const uint32_t box = boxes + (uint32_t)(b % BOXES) * F8_BOX;
+    if (tma) {                                               // what this box held has been read: all of the tile before, or all but the last
+      if (lane == 0) {
+        if (b == 0) bulk_wait_group_read<0>();
+        else bulk_wait_group_read<BOXES - 1>();
+      }
       __syncwarp();
     }
 #pragma unroll
@@ -407,6 +416,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   constexpr int PART_N = BN / PARTS;
   constexpr int DEPTH = 4 / PARTS;                           // accumulators of each
   constexpr int COLS = BN / 2;                               // of a thread
+  constexpr int BOXES = f8_boxes(BN);
   constexpr uint32_t TMEM_COLS = PARTS * DEPTH * PART_N;
   constexpr uint32_t A_BYTES = 128 * F8_BLOCK, W_BYTES = BN * F8_BLOCK, STAGE = A_BYTES + W_BYTES;
   extern __shared__ uint8_t f8_smem_raw[];
@@ -506,9 +516,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   } else if (warp >= F8_FIRST) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     const int quad = warp & 3, half = (warp - F8_FIRST) >> 2;   // a warp reads the TMEM lanes of its number modulo 4
-    const uint32_t boxes = stage0 + (uint32_t)p.stages * STAGE, box = boxes + (uint32_t)(warp - F8_FIRST) * F8_BOX;
-    const uint32_t scales = boxes + F8_WARPS * F8_BOX + (uint32_t)(threadIdx.x - 32 * F8_FIRST) * 4u;
-    const uint32_t bias = boxes + F8_WARPS * F8_BOX + F8_AHEAD * F8_SCALES + (uint32_t)(warp - F8_FIRST) * 512u;
+    const uint32_t boxes = stage0 + (uint32_t)p.stages * STAGE, box = boxes + (uint32_t)(warp - F8_FIRST) * F8_BOX * BOXES;
+    const uint32_t scales = boxes + F8_WARPS * BOXES * F8_BOX + (uint32_t)(threadIdx.x - 32 * F8_FIRST) * 4u;
+    const uint32_t bias = boxes + F8_WARPS * BOXES * F8_BOX + F8_AHEAD * F8_SCALES + (uint32_t)(warp - F8_FIRST) * 512u;
     const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -577,9 +587,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
       if (row0 < g.m) {
-        if (g.out_dtype == SB_F32) f8_write<float, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
-        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
-        else f8_write<__half, COLS>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+        if (g.out_dtype == SB_F32) f8_write<float, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+        else f8_write<__half, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
       }
       __syncwarp();                                          // the biases have been read
     }
@@ -824,7 +834,7 @@ int f8_allow_smem(K* kernel, int bytes, std::atomic<bool>* ready) {
 
 template <int BN>
 int launch_fp8(const F8Args& g, cudaStream_t s) {
-  constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * (F8_BOX + 512) + F8_AHEAD * F8_SCALES;
+  constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * (f8_boxes(BN) * F8_BOX + 512) + F8_AHEAD * F8_SCALES;
   F8Plan p;
   memset(&p, 0, sizeof(p));
   p.tiles_m = (g.m + 127) / 128;

@@ -257,6 +257,10 @@ def values_ptr(x, n, what):
     """Address of n contiguous fp32 values (None -> NULL)."""
     if x is None:
         return None
+    if type(x) is not DeviceArray:
+        numel = getattr(x, "numel", None)
+        if numel is not None and numel() == n and x.is_contiguous() and _TAG_OF.get(x.dtype) == "f32":
+            return x.data_ptr()
     if dtype_tag(x) != "f32" or flat_size(x, what) != n:
         raise ValueError("%s must be %d contiguous fp32 values" % (what, n))
     return device_ptr(x)

@@ -224,3 +224,42 @@ def test_device_arrays(gpu):
     ws = gpu.DeviceArray((gpu.primitives.embedding_grad_workspace(77, 13, 6),), "u8")
     gpu.primitives.embedding_grad(gpu.DeviceArray.from_numpy(tokens), gpu.DeviceArray.from_numpy(dout), dtable, workspace=ws)
     check_grad(dtable.numpy().astype(np.float64), tokens, dout.astype(np.float64), 13, 1.0)
+
+
+@pytest.mark.parametrize("kind", ["random", "one", "none", "last", "descending"])
+@pytest.mark.parametrize("n,vocab,dim,dtype,index,offset", [
+    (1, 2439, 369, "f32", "int32", 0), (31, 86, 64, "bf16", "int64", 0), (256, 5611, 37, "f16", "int64", 0), (257, 5611, 37, "f16", "int64", 0),
+    (255, 300, 1100, "f32", "int32", 0), (130, 300, 2050, "bf16", "int32", 0), (200, 70001, 6, "f32", "int32", 1), (64, 3000, 66, "bf16", "int32", 1)])
+def test_grad_of_few_tokens(gpu, kind, n, vocab, dim, dtype, index, offset):
+    """Up to 256 tokens and a table of many rows; a column offset and a pitch on both sides; added to old values."""
+    torch = _torch()
+    rng = np.random.default_rng(n + vocab)
+    tokens = {"random": make_tokens(rng, n, vocab), "one": np.full(n, vocab // 2), "none": np.full(n, -1), "last": np.full(n, vocab - 1),
+              "descending": (np.arange(n)[::-1] * 3) % vocab}[kind].astype(np.int64)
+    dout = torch.randn((n, dim + 2 * offset), device="cuda").to(dtype_of(dtype))[:, offset:offset + dim]
+    whole = torch.full((vocab, dim + 2 * offset), float("nan"), device="cuda")
+    dtable = whole[:, offset:offset + dim]
+    dev = torch.from_numpy(tokens).to(getattr(torch, index)).cuda()
+    gpu.primitives.embedding_grad(dev, dout, dtable, scale=1.25)
+    first = dtable.clone()
+    check_grad(host(dtable), tokens, host(dout), vocab, 1.25)
+    gpu.primitives.embedding_grad(dev, dout, dtable, scale=1.25, accumulate=True)
+    check_grad(host(dtable), tokens, host(dout), vocab, 1.25, host(first))
+    if offset:
+        assert torch.isnan(whole[:, :offset]).all() and torch.isnan(whole[:, offset + dim:]).all()
+
+
+@pytest.mark.parametrize("table_type,out_type", [("f32", "bf16"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("dim", [1, 31, 999, 1002, 1004, 5001])
+def test_lookup_of_odd_widths(gpu, table_type, out_type, dim):
+    """Single elements, pairs and packs, several turns of a row's threads."""
+    torch = _torch()
+    rng = np.random.default_rng(dim)
+    n, vocab = 300, 77
+    tokens = torch.from_numpy(make_tokens(rng, n, vocab)).cuda()
+    table = torch.randn((vocab, dim), device="cuda").to(dtype_of(table_type))
+    out = torch.full((n, dim), float("nan"), device="cuda").to(dtype_of(out_type))
+    gpu.primitives.embedding(tokens, table, out, scale=2.0)
+    known = ((tokens >= 0) & (tokens < vocab))[:, None]
+    want = torch.where(known, table.float()[tokens.clamp(0, vocab - 1)] * 2.0, torch.zeros((), device="cuda")).to(dtype_of(out_type))
+    assert torch.equal(out, want)
