@@ -523,14 +523,38 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+    // Each thread copies its own scales some blocks ahead, past the registers that the sums need; a tile's first ones before the
+    // tile before is written (after it: 16384 x 4096 x 4096 292 us, now 275; 4096^3 88 and 80).
+    long long row0 = 0;
+    int col0 = 0, ahead = 0;
+    bool inside = false;
+    const float *sa = g.sa, *sw = g.sw;
+    auto fetch = [&]() {
+      if (ahead < g.k_blocks) {
+        const uint32_t to = scales + (uint32_t)(ahead & (F8_AHEAD - 1)) * F8_SCALES;
+        f8_copy4(to, sa, inside ? 4u : 0u);
+        f8_copy4(to + F8_SCALES / 2, sw, inside ? 4u : 0u);
+        sa += g.m;
+        ++sw;
+        ++ahead;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto begin = [&](int tile) {
+      if (tile >= p.tiles) return;
       int m_blk, n_blk;
       f8_tile(p, tile, m_blk, n_blk);
-      const long long row0 = (long long)m_blk * 128 + quad * 32;
-      const int col0 = n_blk * BN + half * COLS;
-      const bool inside = row0 + lane < g.m && col0 < g.n;
-      const float* sa = g.sa + (inside ? row0 + lane : 0);
-      const float* sw = g.sw + (inside ? (long long)(col0 / F8_BLOCK) * g.k_blocks : 0);
+      row0 = (long long)m_blk * 128 + quad * 32;
+      col0 = n_blk * BN + half * COLS;
+      inside = row0 + lane < g.m && col0 < g.n;
+      sa = g.sa + (inside ? row0 + lane : 0);
+      sw = g.sw + (inside ? (long long)(col0 / F8_BLOCK) * g.k_blocks : 0);
+      ahead = 0;
+#pragma unroll
+      for (int i = 0; i < F8_AHEAD - 1; ++i) fetch();
+    };
+    begin(blockIdx.x);
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
       unsigned long long sum[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
@@ -538,21 +562,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       if (g.bias)
 #pragma unroll
         for (int j = lane; j < COLS; j += 32) f8_copy4(bias + 4u * (uint32_t)j, g.bias + (col0 + j < g.n ? col0 + j : 0), col0 + j < g.n ? 4u : 0u);
-      // Each thread copies its own scales some blocks ahead, past the registers that the sums need.
-      int ahead = 0;
-      auto fetch = [&]() {
-        if (ahead < g.k_blocks) {
-          const uint32_t to = scales + (uint32_t)(ahead & (F8_AHEAD - 1)) * F8_SCALES;
-          f8_copy4(to, sa, inside ? 4u : 0u);
-          f8_copy4(to + F8_SCALES / 2, sw, inside ? 4u : 0u);
-          sa += g.m;
-          ++sw;
-          ++ahead;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-#pragma unroll
-      for (int i = 0; i < F8_AHEAD - 1; ++i) fetch();
       for (int kb = 0; kb < g.k_blocks; ++kb) {
         const uint32_t at = (uint32_t)(PARTS == 2 ? 2 * acc + half : acc);
         fetch();
@@ -586,10 +595,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       if (!ok) break;
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
-      if (row0 < g.m) {
-        if (g.out_dtype == SB_F32) f8_write<float, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
-        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
-        else f8_write<__half, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row0, col0, box, bias, lane);
+      const long long row = row0;
+      const int col = col0;
+      begin(tile + gridDim.x);
+      if (row < g.m) {
+        if (g.out_dtype == SB_F32) f8_write<float, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row, col, box, bias, lane);
+        else if (g.out_dtype == SB_BF16) f8_write<__nv_bfloat16, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row, col, box, bias, lane);
+        else f8_write<__half, COLS, BOXES>(g, &tmap_c, p.tma_store != 0, sum, row, col, box, bias, lane);
       }
       __syncwarp();                                          // the biases have been read
     }
