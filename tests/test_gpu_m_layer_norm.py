@@ -244,3 +244,18 @@ def test_stream_and_device_arrays(gpu):
     got = yd.numpy(stream=s)
     check_forward(x.astype(np.float64), np.ones(48), np.zeros(48), got.astype(np.float64), mean.numpy().astype(np.float64),
                   rstd.numpy().astype(np.float64), "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(3, 258), (13, 330), (101, 513), (4003, 1002), (2501, 1001), (9, 2050), (7, 4098), (5, 4097), (3, 8194), (1, 16382)])
+def test_rows_of_pairs_and_single_elements(gpu, rows, cols, dtype):
+    """Widths whose packs do not fill a warp's share, odd numbers of rows, more rows than are on the chip at a time."""
+    torch = _torch()
+    x, dy, w, b = inputs(rows, cols, dtype, 3)
+    y, dx = torch.full_like(x, float("nan")), torch.full_like(x, float("nan"))
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    dw, db = torch.full((cols,), float("nan"), device="cuda"), torch.full((cols,), float("nan"), device="cuda")
+    gpu.primitives.layer_norm(x, y, w, b, eps=EPS, mean=mean, rstd=rstd)
+    check_forward(host(x), host(w), host(b), host(y), host(mean), host(rstd), dtype)
+    gpu.primitives.layer_norm_grad(dy, x, mean, rstd, dx, w, dw, db)
+    check_backward(host(dy), host(x), host(mean), host(rstd), host(w), host(dx), host(dw), host(db), dtype)
