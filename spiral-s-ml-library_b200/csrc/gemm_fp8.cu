@@ -253,8 +253,8 @@ __global__ void __launch_bounds__(256) gemm_fp8_simple_kernel(F8Args g) {
 // of N: the product of the scales is one number per thread and block.  At BN = 256 the two halves of the columns are
 // products of their own with two accumulators each, so that the adding warps of a half wait for their own MMAs only.
 //
-// Bound by the operands' way from L2 into shared memory: at BN = 256 a block is 48 KB in 0.6 us per SM, 12 TB/s over the chip
-// (8192^3: 529 us, 2077 TFLOP/s, the same without the multiply-adds).  Pairs of CTAs (cta_group::2, 256 x 256) load a third
+// Bound by the operands' way from L2 into shared memory: at BN = 256 a block is 48 KB in 0.55 us per SM, 13 TB/s over the chip
+// (8192^3: 530 us, 2070 TFLOP/s, the same without the multiply-adds).  Pairs of CTAs (cta_group::2, 256 x 256) load a third
 // less and were slower, 320 us against 271 for 16384 x 4096 x 4096: the round trip from the MMAs over both CTAs' adding warps
 // back to the issuer is longer than two accumulators cover.  Four stages instead of three: 288 us; sixteen adding warps, whose
 // 112 registers spill: 327 us (in pairs).
@@ -916,7 +916,7 @@ int launch_fp8_few(const F8Args& g, int splits, cudaStream_t s) {
 }
 
 // Which form a product takes: the least of rounds over the SMs x (time of a tile + blocks of K x time of a block), in us as
-// measured.  Times of back-to-back launches on operands beyond L2, tiles of 256 / 128 / 64 columns: 16384 x 4096 x 4096 296 / 342 /
+// measured.  Times of back-to-back launches on operands beyond L2, tiles of 256 / 128 / 64 columns: 16384 x 4096 x 4096 275 / 342 /
 // 580, 4000 x 3000 x 1008 25.5 / 27.0 / 39.5, 1024^3 9.3 / 6.2 / 5.6.  Few rows, 16 x 4096 x 4096 with K over 1 / 2 / 4 / 8 CTAs: 11.4 /
 // 8.1 / 6.4 / 5.7, and 13.6 as 64-column tiles; 64 x 4096 x 4096 20.2 / 12.6 / 9.9 / 21.0 (two rounds), 12.9; 512 x 512 x 4096 18.2 / 11.3 /
 // 8.9 / 20.0, 12.3.

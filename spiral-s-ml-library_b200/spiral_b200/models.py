@@ -476,7 +476,8 @@ class TokenPolicy:
         return self
 
     def forward_8bit(self, tokens, mask=None, stream=None):
-        """``forward`` with the dense layers in 8 bits: activations quantised per row and 128 columns, products of codes."""
+        """``forward`` with the dense layers in 8 bits: activations quantised per row and 128 columns, products of codes (on the
+        tensor cores where a layer's input width is a multiple of 16)."""
         if self._codes is None:
             raise ValueError("quantize() the weights first")
         self._input(tokens, stream)
