@@ -101,6 +101,7 @@ const char* sb_last_error_string(void);
 int sb_version(void);
 int sb_device_count(int* count);
 int sb_set_device(int device);
+int sb_get_device(int* device);                 /* the calling thread's */
 int sb_device_sm_count(int* sms);
 /* cupy.empty / cp.cuda memory calls of corecuda/cupy.spi:20-58 are replaced by
  * the caller's own allocator; these exist so that hosts without one (tests,

@@ -120,6 +120,12 @@ int sb_set_device(int device) {
   return SB_OK;
 }
 
+int sb_get_device(int* device) {
+  if (!device) return sb_fail(SB_ERR_BAD_ARG, "sb_get_device: null output");
+  SB_CUDA(cudaGetDevice(device));
+  return SB_OK;
+}
+
 int sb_device_sm_count(int* sms) {
   if (!sms) return sb_fail(SB_ERR_BAD_ARG, "sb_device_sm_count: null output");
   int dev = 0;

@@ -82,6 +82,7 @@ SIGNATURES = {
     "sb_last_error_string": (c_char_p, []),
     "sb_version": (_I, []),
     "sb_device_count": (_I, [_IP]),
+    "sb_get_device": (_I, [_IP]),
     "sb_set_device": (_I, [_I]),
     "sb_device_sm_count": (_I, [_IP]),
     "sb_malloc": (_I, [_PP, _Z]),

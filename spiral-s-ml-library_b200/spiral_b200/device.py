@@ -8,6 +8,7 @@ integer -- and passes the raw pointer through the C ABI.
 """
 import ctypes
 import math
+import threading
 
 import numpy as np
 
@@ -266,18 +267,29 @@ def values_ptr(x, n, what):
     return device_ptr(x)
 
 
-_WORKSPACES = {}
+class _Workspaces(threading.local):
+    """A host thread's workspaces by (device, stream)."""
+
+    def __init__(self):
+        self.held = {}
+        self.device = ctypes.c_int(0)
+
+
+_WORKSPACES = _Workspaces()
 
 
 def stream_workspace(nbytes, stream):
-    """Device memory for one call's intermediate results: kept per stream, grown on demand (the C ABI itself allocates
-    nothing), so calls on one stream share it in their order and calls on different streams never do."""
-    key = stream_ptr(stream) or 0
-    ws = _WORKSPACES.get(key)
+    """Device memory for one call's intermediate results: kept per device, stream and host thread, grown on demand (the C ABI
+    itself allocates nothing).  A thread's calls on one stream share it in their order.  Calls of other threads, whose launches
+    may come between those of one call, on other streams or on other devices (whose default streams share a handle) never do."""
+    mine = _WORKSPACES
+    _lib.call("sb_get_device", ctypes.byref(mine.device))
+    key = mine.device.value, stream_ptr(stream) or 0
+    ws = mine.held.get(key)
     if ws is None or ws.nbytes < nbytes:
         if ws is not None:
             _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
-        ws = _WORKSPACES[key] = DeviceArray((max(int(nbytes), 1 << 16),), "u8")
+        ws = mine.held[key] = DeviceArray((max(int(nbytes), 1 << 16),), "u8")
     return ws
 
 

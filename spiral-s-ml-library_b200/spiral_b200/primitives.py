@@ -160,7 +160,7 @@ def embedding(tokens, table, out, scale=1.0, stream=None):
 def embedding_grad(tokens, dout, dtable, scale=1.0, accumulate=False, workspace=None, stream=None):
     """Gradient of ``embedding``: ``dtable[v, :] = scale * sum of dout[i, :] over tokens[i] == v``, fp32 [vocab, dim]
     (``accumulate``: added to it).  Sums in the order of the positions, the same bits on every call.  ``workspace``: device
-    memory of ``embedding_grad_workspace`` bytes; by default one is kept per stream."""
+    memory of ``embedding_grad_workspace`` bytes; by default one is kept per device, stream and host thread."""
     n = flat_size(tokens, "tokens")
     rows, cols, ld_dout = matrix_of(dout, "dout")
     vocab, dim, ld_dtable = matrix_of(dtable, "dtable")
@@ -209,7 +209,7 @@ def layer_norm_grad(dy, x, mean, rstd, dx=None, weight=None, dweight=None, dbias
                     stream=None):
     """Gradient of ``layer_norm``: ``dx`` (like ``x``), ``dweight`` and ``dbias`` (fp32 [cols]), each where given;
     ``accumulate`` adds to the old ``dweight`` and ``dbias``.  Sums in a fixed order, the same bits on every call.
-    ``workspace``: device memory of ``layer_norm_grad_workspace`` bytes; by default one is kept per stream."""
+    ``workspace``: device memory of ``layer_norm_grad_workspace`` bytes; by default one is kept per device, stream and thread."""
     rows, cols, ldx = matrix_of(x, "x")
     code = _code(x, "x")
     dy_rows, dy_cols, lddy = matrix_of(dy, "dy")

@@ -1,0 +1,73 @@
+"""Whose device memory a call works in: one workspace per device, stream and host thread (CPU only, a library that is not there)."""
+import threading
+
+import pytest
+
+
+class Library:
+    """The few entry points that a workspace takes, of a process with several devices."""
+
+    def __init__(self):
+        self.current = threading.local()
+        self.lies_on = {}
+        self.synced = []
+        self.lock = threading.Lock()
+
+    def device(self):
+        return getattr(self.current, "index", 0)
+
+    def call(self, name, *args):
+        if name == "sb_set_device":
+            self.current.index = args[0]
+        elif name == "sb_get_device":
+            args[0]._obj.value = self.device()
+        elif name == "sb_malloc":
+            with self.lock:
+                at = 0x100000 * (len(self.lies_on) + 1)
+                self.lies_on[at] = self.device()
+            args[0]._obj.value = at
+        elif name == "sb_stream_sync":
+            self.synced.append(args[0])
+        else:
+            assert name == "sb_free", name
+
+
+@pytest.fixture
+def library(sb, monkeypatch):
+    lib = Library()
+    from spiral_b200 import _lib, device
+    monkeypatch.setattr(_lib, "call", lib.call)
+    monkeypatch.setattr(device, "_WORKSPACES", type(device._WORKSPACES)())    # none of other tests, and none left to them
+    return lib
+
+
+def test_of_a_device(sb, library):
+    """The default stream has one handle on all devices; its workspaces lie where the kernels run."""
+    from spiral_b200.device import stream_workspace
+    held = []
+    for device in (0, 1, 0, 1):
+        sb.set_device(device)
+        held.append(stream_workspace(100000, None))
+        assert library.lies_on[held[-1].ptr] == device
+    assert held[0] is held[2] and held[1] is held[3]
+
+
+def test_of_a_stream(sb, library):
+    from spiral_b200.device import stream_workspace
+    sb.set_device(2)
+    a, b = stream_workspace(100000, 0x71), stream_workspace(100000, 0x72)
+    assert a.ptr != b.ptr and stream_workspace(5, 0x71) is a and not library.synced
+    grown = stream_workspace(200000, 0x71)                             # the old one may be in use: a wait for its stream
+    assert grown.nbytes >= 200000 and library.synced == [0x71] and stream_workspace(5, 0x72) is b
+
+
+def test_of_a_host_thread(sb, library):
+    """The launches of one call may have those of another thread between them."""
+    from spiral_b200.device import stream_workspace
+    mine, others = stream_workspace(100000, None), []
+    threads = [threading.Thread(target=lambda: others.append(stream_workspace(100000, None))) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len({w.ptr for w in others} | {mine.ptr}) == 4 and stream_workspace(100000, None) is mine
