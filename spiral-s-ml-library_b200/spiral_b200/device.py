@@ -267,30 +267,42 @@ def values_ptr(x, n, what):
     return device_ptr(x)
 
 
-class _Workspaces(threading.local):
-    """A host thread's workspaces by (device, stream)."""
+class Workspaces:
+    """Device memory for one call's intermediate results: kept per device, host thread and stream, grown on demand (the C ABI
+    itself allocates nothing).  A thread's calls on one stream share it in their order.  Calls of other threads, whose launches
+    may come between those of one call, on other streams or on other devices (whose default streams share a handle) never do.
+    A thread that ends leaves its own to the next one of its number: its launches, or a graph that holds them, may yet run."""
 
     def __init__(self):
         self.held = {}
-        self.device = ctypes.c_int(0)
+
+    @staticmethod
+    def _key(stream):
+        device = ctypes.c_int(0)
+        _lib.call("sb_get_device", ctypes.byref(device))
+        return device.value, threading.get_ident(), stream_ptr(stream) or 0
+
+    def of(self, stream):
+        """What is kept for `stream` on the current device, or None."""
+        return self.held.get(self._key(stream))
+
+    def grown(self, nbytes, stream):
+        """The same with at least `nbytes`."""
+        key = self._key(stream)
+        ws = self.held.get(key)
+        if ws is None or ws.nbytes < nbytes:
+            if ws is not None:
+                _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
+            ws = self.held[key] = DeviceArray((int(nbytes),), "u8")
+        return ws
 
 
-_WORKSPACES = _Workspaces()
+_WORKSPACES = Workspaces()
 
 
 def stream_workspace(nbytes, stream):
-    """Device memory for one call's intermediate results: kept per device, stream and host thread, grown on demand (the C ABI
-    itself allocates nothing).  A thread's calls on one stream share it in their order.  Calls of other threads, whose launches
-    may come between those of one call, on other streams or on other devices (whose default streams share a handle) never do."""
-    mine = _WORKSPACES
-    _lib.call("sb_get_device", ctypes.byref(mine.device))
-    key = mine.device.value, stream_ptr(stream) or 0
-    ws = mine.held.get(key)
-    if ws is None or ws.nbytes < nbytes:
-        if ws is not None:
-            _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
-        ws = mine.held[key] = DeviceArray((max(int(nbytes), 1 << 16),), "u8")
-    return ws
+    """The token operators' workspace for a call on `stream` (see ``Workspaces``)."""
+    return _WORKSPACES.grown(max(nbytes, 1 << 16), stream)
 
 
 def stream_ptr(stream):

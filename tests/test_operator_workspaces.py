@@ -11,6 +11,7 @@ class Library:
         self.current = threading.local()
         self.lies_on = {}
         self.synced = []
+        self.freed = []
         self.lock = threading.Lock()
 
     def device(self):
@@ -30,6 +31,7 @@ class Library:
             self.synced.append(args[0])
         else:
             assert name == "sb_free", name
+            self.freed.append(args[0])
 
 
 @pytest.fixture
@@ -65,9 +67,25 @@ def test_of_a_host_thread(sb, library):
     """The launches of one call may have those of another thread between them."""
     from spiral_b200.device import stream_workspace
     mine, others = stream_workspace(100000, None), []
-    threads = [threading.Thread(target=lambda: others.append(stream_workspace(100000, None))) for _ in range(3)]
+    meet = threading.Barrier(3)                                        # alive together: numbers of threads come again
+
+    def work():
+        others.append(stream_workspace(100000, None))
+        meet.wait()
+    threads = [threading.Thread(target=work) for _ in range(3)]
     for t in threads:
         t.start()
     for t in threads:
         t.join()
-    assert len({w.ptr for w in others} | {mine.ptr}) == 4 and stream_workspace(100000, None) is mine
+    assert len({w.ptr for w in others}) == 3
+    assert mine.ptr not in {w.ptr for w in others} and stream_workspace(100000, None) is mine
+
+
+def test_outlives_its_thread(sb, library):
+    """What a thread launched, or captured in a graph, may run after it has ended."""
+    from spiral_b200.device import stream_workspace
+    at = []
+    thread = threading.Thread(target=lambda: at.append(stream_workspace(100000, 0x71).ptr))
+    thread.start()
+    thread.join()
+    assert not library.freed and at[0] in library.lies_on
