@@ -7,7 +7,7 @@ updated in place: ``c <- alpha * op(a) @ op(b) + beta * c``.
 import ctypes
 
 from . import _lib
-from .device import DeviceArray, device_ptr, dtype_tag, matrix_of, stream_ptr, values_ptr
+from .device import Workspaces, device_ptr, dtype_tag, matrix_of, stream_ptr, values_ptr
 
 EPILOGUE_FLAGS = {
     "bias": _lib.EPI_BIAS, "relu": _lib.EPI_RELU, "relu_grad": _lib.EPI_RELU_GRAD,
@@ -35,7 +35,7 @@ def _dims(a_trans, b_trans, a, b, c):
     return m, n, k
 
 
-_F32X3_WORKSPACES = {}
+_F32X3_WORKSPACES = Workspaces()
 
 
 def _f32x3_aligned(a_trans, b_trans, m, n, k):
@@ -44,18 +44,12 @@ def _f32x3_aligned(a_trans, b_trans, m, n, k):
 
 
 def _f32x3_workspace(m, n, k, stream):
-    key = stream_ptr(stream) or 0
-    ws = _F32X3_WORKSPACES.get(key)
+    ws = _F32X3_WORKSPACES.of(stream)
     if ws is not None and ws.nbytes >= 8 * (m + n) * k + 1024:      # no more than this is ever asked for
         return ws
     need = ctypes.c_size_t(0)
     _lib.call("sb_matmul_f32_workspace_bytes", m, n, k, ctypes.byref(need))
-    if ws is None or ws.nbytes < need.value:
-        if ws is not None:
-            _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
-        ws = DeviceArray((need.value,), "u8")
-        _F32X3_WORKSPACES[key] = ws
-    return ws
+    return _F32X3_WORKSPACES.grown(need.value, stream)
 
 
 def matmul(a_trans, b_trans, alpha, a, b, beta, c, in_dtype=None, epilogue=(), bias=None, mask=None,
@@ -84,7 +78,7 @@ def matmul(a_trans, b_trans, alpha, a, b, beta, c, in_dtype=None, epilogue=(), b
     if in_dtype == "f32" and out_dtype == "f32" and not (epi & ~(_lib.EPI_BIAS | _lib.EPI_RELU)) and k > 0 \
             and _f32x3_aligned(bool(a_trans), bool(b_trans), m, n, k) and device_ptr(c) % 16 == 0:
         # fp32 class on the tensor cores (3 x TF32); the split operands live in a workspace this host
-        # keeps per stream and grows on demand (the C ABI itself allocates nothing).
+        # keeps per device, stream and thread and grows on demand (the C ABI itself allocates nothing).
         ws = _f32x3_workspace(m, n, k, stream)
         _lib.call("sb_matmul_f32x3", int(bool(a_trans)), int(bool(b_trans)), ctypes.c_float(alpha), device_ptr(a),
                   device_ptr(b), ctypes.c_float(beta), device_ptr(c), m, n, k, epi, device_ptr(bias), ws.ptr,

@@ -1,4 +1,5 @@
 """Whose device memory a call works in: one workspace per device, stream and host thread (CPU only, a library that is not there)."""
+import importlib
 import threading
 
 import pytest
@@ -89,3 +90,28 @@ def test_outlives_its_thread(sb, library):
     thread.start()
     thread.join()
     assert not library.freed and at[0] in library.lies_on
+
+
+def test_split_operands_of_the_fp32_class(sb, library, monkeypatch):
+    """matmul in the fp32 class keeps its split operands under the same rule."""
+    matmul = importlib.import_module("spiral_b200.matmul")             # the module, not the function of its name
+
+    def call(name, *args):
+        if name == "sb_matmul_f32_workspace_bytes":
+            args[3]._obj.value = 8 * (args[0] + args[1]) * args[2] + 1024
+        else:
+            library.call(name, *args)
+    monkeypatch.setattr(matmul._lib, "call", call)
+    monkeypatch.setattr(matmul, "_F32X3_WORKSPACES", type(matmul._F32X3_WORKSPACES)())
+    held, others = [], []
+    for device in (0, 1, 0):
+        sb.set_device(device)
+        held.append(matmul._f32x3_workspace(64, 64, 64, None))
+        assert library.lies_on[held[-1].ptr] == device
+    assert held[0] is held[2] and matmul._f32x3_workspace(8, 8, 8, None) is held[0]
+    grown = matmul._f32x3_workspace(64, 64, 128, None)
+    assert grown.nbytes >= 8 * 128 * 128 and library.synced == [None]
+    thread = threading.Thread(target=lambda: others.append(matmul._f32x3_workspace(64, 64, 64, None)))
+    thread.start()
+    thread.join()
+    assert others[0].ptr not in {w.ptr for w in held} | {grown.ptr}
