@@ -534,6 +534,9 @@ int sb_quantize_fp8(const void* x, long long ldx, int dtype, long long rows, int
 int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const uint8_t* w, long long ldw,
                   const float* w_scales, void* c, long long ldc, int m, int n, int k, int out_dtype, int epilogue,
                   const float* bias, void* stream);
+/* The tiles that sb_matmul_fp8 takes for rows of codes that start on 16 bytes: plan = {rows of A, rows of W, CTAs that share
+ * K}; fewer than 128 rows of A are the form for few rows. */
+int sb_matmul_fp8_plan(int m, int n, int k, int* plan);
 
 /* ---- data-parallel update over peer memory ---------------------------------
  * No reference counterpart (the reference is single-device, corecuda/base.spi:7);

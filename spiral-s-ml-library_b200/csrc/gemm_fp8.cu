@@ -961,6 +961,10 @@ F8Choice f8_choose(int m, int n, int k_blocks) {
 }
 
 bool f8_aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// TMA takes rows that begin on 16-byte boundaries.
+bool f8_tma_rows(const void* a, long long lda, const void* w, long long ldw) {
+  return f8_aligned(a, 16) && f8_aligned(w, 16) && lda % 16 == 0 && ldw % 16 == 0;
+}
 
 }  // namespace
 
@@ -1009,15 +1013,24 @@ int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const 
   g.lda = lda; g.ldw = ldw; g.ldc = ldc; g.m = m; g.n = n; g.k = k; g.k_blocks = (k + F8_BLOCK - 1) / F8_BLOCK;
   g.relu = (epilogue & SB_EPI_RELU) ? 1 : 0; g.out_dtype = out_dtype;
   cudaStream_t s = (cudaStream_t)stream;
-  // TMA takes rows that begin on 16-byte boundaries.
-  if (k > 0 && f8_aligned(a, 16) && f8_aligned(w, 16) && lda % 16 == 0 && ldw % 16 == 0) {
-    const F8Choice c = f8_choose(m, n, g.k_blocks);
-    if (c.few) return c.tile == 16 ? launch_fp8_few<16>(g, c.splits, s) : c.tile == 32 ? launch_fp8_few<32>(g, c.splits, s) : launch_fp8_few<64>(g, c.splits, s);
-    return c.tile == 256 ? launch_fp8<256>(g, s) : c.tile == 128 ? launch_fp8<128>(g, s) : launch_fp8<64>(g, s);
+  if (k > 0 && f8_tma_rows(a, lda, w, ldw)) {
+    const F8Choice f = f8_choose(m, n, g.k_blocks);
+    if (f.few) return f.tile == 16 ? launch_fp8_few<16>(g, f.splits, s) : f.tile == 32 ? launch_fp8_few<32>(g, f.splits, s) : launch_fp8_few<64>(g, f.splits, s);
+    return f.tile == 256 ? launch_fp8<256>(g, s) : f.tile == 128 ? launch_fp8<128>(g, s) : launch_fp8<64>(g, s);
   }
   const dim3 grid((unsigned)((m + 63) / 64), (unsigned)((n + 63) / 64));
   SB_CUDA(sb_launch(gemm_fp8_simple_kernel, grid, dim3(256), 0, s, 1, g));
   SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+int sb_matmul_fp8_plan(int m, int n, int k, int* plan) {
+  if (!plan) return sb_fail(SB_ERR_BAD_ARG, "sb_matmul_fp8_plan: null output");
+  if (m < 1 || n < 1 || k < 1) return sb_fail(SB_ERR_BAD_ARG, "sb_matmul_fp8_plan: sizes must be positive");
+  const F8Choice c = f8_choose(m, n, (k + F8_BLOCK - 1) / F8_BLOCK);
+  plan[0] = c.few ? c.tile : 128;
+  plan[1] = c.few ? 128 : c.tile;
+  plan[2] = c.splits;
   return SB_OK;
 }
 

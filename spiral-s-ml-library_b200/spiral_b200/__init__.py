@@ -7,7 +7,7 @@ library every operation raises.
 from ._lib import SpiralError, LIB_PATH  # noqa: F401
 from .device import (DeviceArray, Event, Stream, wait_event, GemmProfile, launch_count, device_count, device_ptr, device_status, check_device, mem_info, set_device, sm_count,  # noqa: F401
                      synchronize)
-from .matmul import head_spec, matmul, matmul_fp8, matmul_head, matmul_plan, matmul_tf32, quantize_fp8  # noqa: F401
+from .matmul import head_spec, matmul, matmul_fp8, matmul_fp8_plan, matmul_head, matmul_plan, matmul_tf32, quantize_fp8  # noqa: F401
 from . import primitives  # noqa: F401
 from .models import EnsemblePolicyMLP, PolicyMLP, TokenPolicy, param_offsets, to_storage  # noqa: F401
 from . import layers  # noqa: F401

@@ -164,6 +164,7 @@ SIGNATURES = {
     "sb_adamw_step": (_I, [_I, POINTER(AdamwTensor), _I, _I, _I, POINTER(AdamwHyper), _P]),
     "sb_quantize_fp8": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _P]),
     "sb_matmul_fp8": (_I, [_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P]),
+    "sb_matmul_fp8_plan": (_I, [_I, _I, _I, _IP]),
     "sb_sgd_update": (_I, [_P, _P, _P, ctypes.c_longlong, _F, _I, _P]),
     "sb_mlp_train_step": (_I, [_I, _IP, _I, _I, _P, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _F, _P, _Z, _P, _P]),
 }

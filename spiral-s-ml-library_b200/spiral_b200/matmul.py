@@ -207,3 +207,11 @@ def matmul_fp8(a, a_scales, b, b_scales, c, epilogue=(), bias=None, stream=None)
               values_ptr(b_scales, -(-n // 128) * across, "b_scales"), device_ptr(c), ldc, m, n, k, _FP8_FLOATS[tag], epi,
               values_ptr(bias, n, "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
     return c
+
+
+def matmul_fp8_plan(m, n, k):
+    """Tile plan of ``matmul_fp8`` on the tensor cores: dict(block_m, block_n, splits).  ``block_m`` below 128 is the form
+    for few rows, ``splits`` the CTAs of a cluster that share k."""
+    plan = (ctypes.c_int * 3)()
+    _lib.call("sb_matmul_fp8_plan", int(m), int(n), int(k), plan)
+    return dict(zip(("block_m", "block_n", "splits"), list(plan)))
