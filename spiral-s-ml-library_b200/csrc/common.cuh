@@ -526,9 +526,11 @@ __device__ __forceinline__ uint32_t cluster_cta_rank() {
   return r;
 }
 // Cluster-wide barrier: every thread of every CTA of the cluster arrives, then waits.
+__device__ __forceinline__ void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive_all();
+  cluster_wait_all();
 }
 // Address, in the shared::cluster window, of the same shared-memory location in CTA `rank`.
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t rank) {

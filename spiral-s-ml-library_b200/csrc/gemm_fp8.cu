@@ -688,6 +688,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  // Another CTA's shared memory may be written once that CTA has started: all arrive here, and wait before the first such write.
+  if (SPLITS > 1) cluster_arrive_all();
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &g_f8_abort;
   const bool one = elect_one_lane();
@@ -782,6 +784,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       for (int j = 0; j < TN; ++j)
         if (n < g.n && m0 + j < g.m) f8_store(g, m0 + j, n, sum[j]);
     } else {
+      __syncwarp();
+      cluster_wait_all();
 #pragma unroll
       for (int to = 0; to < SPLITS; ++to)
         f8_send<PER>(map_to_cta(meet + (uint32_t)(rank * 128 + (int)threadIdx.x) * PITCH, (uint32_t)to), sum + to * PER);
@@ -790,6 +794,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   tc_fence_before_sync();
   if (SPLITS > 1) {
     __syncwarp();
+    if (warp >= 4) cluster_wait_all();                       // the start's, which the adding warps have waited for
     cluster_sync_all();
     const int n = n0 + threadIdx.x;
     if (warp < 4) {

@@ -216,3 +216,28 @@ def test_layer_in_eight_bits(gpu):
     ref = x.astype(np.float64) @ w.T.astype(np.float64)
     # Each operand is off by at most 1/16 of each value (nearest of 3 bits behind the leading one), with signs at random.
     assert np.linalg.norm(got - ref) / np.linalg.norm(ref) < 0.06
+
+
+# Few rows: every width of a tile with every number of CTAs that share K, ragged at all ends; where the text says so, more blocks of K per
+# CTA than stages of its ring.
+FEW = [(13, 4000, 4080, 16, 8), (16, 500, 1000, 16, 4), (1, 100, 500, 16, 2), (115, 2170, 512, 32, 2), (30, 4300, 1000, 32, 4), (31, 2100, 2048, 32, 8),
+       (1850, 1270, 300, 64, 1), (397, 2430, 512, 64, 2), (45, 4300, 1024, 64, 4), (48, 1500, 4000, 64, 8)]
+FEW_LONG = [(3, 200, 20000, 16, 8), (40, 1500, 14000, 64, 8)]        # 20 and 14 blocks, 8 stages at most
+
+
+@pytest.mark.parametrize("m,n,k,rows,splits", FEW + FEW_LONG)
+def test_forms_for_few_rows(gpu, m, n, k, rows, splits):
+    torch = _torch()
+    plan = gpu.matmul_fp8_plan(m, n, k)
+    assert (plan["block_m"], plan["splits"]) == (rows, splits)         # 148 SMs
+    (a, sa), (w, sw) = operands(m, n, k, m + n)
+    pitch = -(-k // 16) * 16
+    da, dsa, dw, dsw = device_operands(np.pad(a, ((0, 0), (0, pitch - k)), constant_values=0x7f), sa, np.pad(w, ((0, 0), (0, pitch - k)), constant_values=0x7f), sw)
+    bias = np.random.default_rng(k).standard_normal(n).astype(f32)
+    c = torch.full((m, n), 7.0, device="cuda")
+    gpu.matmul_fp8(da[:, :k], dsa, dw[:, :k], dsw, c, epilogue=("bias",), bias=torch.from_numpy(bias).cuda())
+    check_product(c, a, sa, w, sw, "f32", bias.astype(np.float64))
+    first = c.clone()
+    for _ in range(3):
+        gpu.matmul_fp8(da[:, :k], dsa, dw[:, :k], dsw, c, epilogue=("bias",), bias=torch.from_numpy(bias).cuda())
+        assert torch.equal(first, c)
