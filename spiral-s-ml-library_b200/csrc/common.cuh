@@ -527,6 +527,7 @@ __device__ __forceinline__ uint32_t cluster_cta_rank() {
 }
 // Cluster-wide barrier: every thread of every CTA of the cluster arrives, then waits.
 __device__ __forceinline__ void cluster_arrive_all() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed_all() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }   // orders no memory
 __device__ __forceinline__ void cluster_wait_all() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
   cluster_arrive_all();

@@ -689,7 +689,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   __syncthreads();
   tc_fence_after_sync();
   // Another CTA's shared memory may be written once that CTA has started: all arrive here, and wait before the first such write.
-  if (SPLITS > 1) cluster_arrive_all();
+  if (SPLITS > 1) cluster_arrive_relaxed_all();
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &g_f8_abort;
   const bool one = elect_one_lane();
@@ -778,25 +778,38 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         acc_phase ^= 1u;
       }
     }
-    const int n = n0 + threadIdx.x;
-    if (SPLITS == 1) {
+  }
+  // Tensor memory goes back as soon as it has been read, whatever the other CTAs do: they may be waiting for tensor memory
+  // themselves, and beside a product of CTA pairs on another stream all could else wait for one another.
+  tc_fence_before_sync();
+  if (warp < 4) {
+    asm volatile("bar.arrive 2, 160;" ::: "memory");
+  } else if (warp == 5) {
+    asm volatile("bar.sync 2, 160;" ::: "memory");
+    tc_fence_after_sync();
+    if (*abortp != 0) {                                      // as in gemm_fp8_kernel
+      const unsigned long long t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 200000ull) { }
+    }
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+  const int n = n0 + threadIdx.x;
+  if constexpr (SPLITS == 1) {
+    if (warp < 4) {
 #pragma unroll
       for (int j = 0; j < TN; ++j)
         if (n < g.n && m0 + j < g.m) f8_store(g, m0 + j, n, sum[j]);
-    } else {
-      __syncwarp();
-      cluster_wait_all();
+    }
+  } else {
+    __syncwarp();
+    cluster_wait_all();                                      // for the others' start
+    if (warp < 4) {
 #pragma unroll
       for (int to = 0; to < SPLITS; ++to)
         f8_send<PER>(map_to_cta(meet + (uint32_t)(rank * 128 + (int)threadIdx.x) * PITCH, (uint32_t)to), sum + to * PER);
     }
-  }
-  tc_fence_before_sync();
-  if (SPLITS > 1) {
     __syncwarp();
-    if (warp >= 4) cluster_wait_all();                       // the start's, which the adding warps have waited for
     cluster_sync_all();
-    const int n = n0 + threadIdx.x;
     if (warp < 4) {
       float total[PER];
 #pragma unroll
@@ -809,17 +822,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       for (int j = 0; j < PER; ++j)
         if (n < g.n && m0 + rank * PER + j < g.m) f8_store(g, m0 + rank * PER + j, n, total[j]);
     }
-  }
-  // As in gemm_fp8_kernel.
-  __syncthreads();
-  if (*abortp != 0) {
-    const unsigned long long t0 = global_timer_ns();
-    while (global_timer_ns() - t0 < 200000ull) { }
-  }
-  __syncthreads();
-  if (warp == 5) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, TMEM_COLS);
   }
 }
 
