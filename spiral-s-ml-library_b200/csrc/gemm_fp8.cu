@@ -914,8 +914,9 @@ int launch_fp8_few(const F8Args& g, cudaStream_t s) {
 
 template <int TN>
 int launch_fp8_few(const F8Args& g, int splits, cudaStream_t s) {
+  if constexpr (TN == 64)
+    if (splits == 1) return launch_fp8_few<TN, 1>(g, s);
   switch (splits) {
-    case 1: return launch_fp8_few<TN, 1>(g, s);
     case 2: return launch_fp8_few<TN, 2>(g, s);
     case 4: return launch_fp8_few<TN, 4>(g, s);
     default: return launch_fp8_few<TN, 8>(g, s);
@@ -948,7 +949,8 @@ F8Choice f8_choose(int m, int n, int k_blocks) {
     if (across > 65535 || down > 65535) continue;
     const double block = tn == 16 ? 0.28 : tn == 32 ? 0.36 : 0.50;
     const double weights = 128e-6 * 128.0 * across * k_blocks / 5.0;           // on their way from DRAM
-    for (int splits = 1; splits <= 8; splits *= 2) {
+    // All of K in one CTA pays for many short products only, 64 rows at a time (1856 x 1280 x 384); narrower tiles never won there.
+    for (int splits = tn == 64 ? 1 : 2; splits <= 8; splits *= 2) {
       const int blocks = (k_blocks + splits - 1) / splits;
       if (blocks > F8_FEW_BLOCKS || (splits > 1 && k_blocks < 2 * splits)) continue;
       const F8FewSize size = f8_few_size(tn, splits, k_blocks);

@@ -20,3 +20,14 @@ def test_plans_refuse_sizes_of_nothing(sb):
     for args in ((0, 8, 8, plan), (8, 0, 8, plan), (8, 8, 0, plan), (8, 8, 8, None)):
         with pytest.raises(sb.SpiralError):
             _lib.call("sb_matmul_fp8_plan", *args)
+
+
+def test_narrow_tiles_of_an_8_bit_product_share_k(sb):
+    """All of K in one CTA is for 64 rows; narrower tiles have no kernel of that kind."""
+    seen = set()
+    for k in (128, 384, 1024, 8192):
+        for m in list(range(1, 200, 13)) + [400, 1856]:
+            for n in list(range(16, 40000, 1240)) + [1280]:
+                plan = sb.matmul_fp8_plan(m, n, k)
+                seen.add((plan["block_m"], plan["splits"]))
+    assert (16, 1) not in seen and (32, 1) not in seen and (64, 1) in seen and (128, 1) in seen
