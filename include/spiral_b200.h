@@ -530,7 +530,9 @@ int sb_quantize_fp8(const void* x, long long ldx, int dtype, long long rows, int
                     long long ldc, float* scales, void* stream);
 /* C[m, n] = sum over blocks b of K of a_scales[b, m] * w_scales[n / 128, b] * (A[m, k in b] . W[n, k in b]): a dense layer in
  * 8 bits, A [M, K] and W [N, K] codes with the scales that sb_quantize_fp8 leaves for block_rows 1 and 128.  fp32
- * accumulation; C in SB_F32, SB_BF16 or SB_F16; epilogue: SB_EPI_BIAS (fp32 [N]), SB_EPI_RELU. */
+ * accumulation; C in SB_F32, SB_BF16 or SB_F16; epilogue: SB_EPI_BIAS (fp32 [N]), SB_EPI_RELU (a NaN gives 0, as in the other products).
+ * Scales are not negative.  Where the product of two is outside fp32's normal numbers they are multiplied by one after the other, more
+ * slowly; with a scale of at most 2^-100 / 448 (a block of zeros, or of magnitudes of at most 2^-100) such a block may count as zero. */
 int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const uint8_t* w, long long ldw,
                   const float* w_scales, void* c, long long ldc, int m, int n, int k, int out_dtype, int epilogue,
                   const float* bias, void* stream);

@@ -186,6 +186,25 @@ struct F8Args {
   int relu, out_dtype;
 };
 
+// The product of a block's two scales, or, where that is no normal number although both are (1e-20 each are enough), two factors that
+// are taken one after the other: values beside which neither step leaves the range unless the result does.  A scale of at most
+// 2^-100 / 448 is that of a block of zeros, or of magnitudes of at most 2^-100: what it gives below the normal range may be lost.
+struct F8Scale {
+  float first, second;
+};
+__device__ __forceinline__ bool f8_unsafe(float sa, float sw) {
+  const float product = sa * sw;
+  return (product < 1.17549435e-38f || product == INFINITY) && fminf(sa, sw) > F8_FLOOR / F8_TOP && fmaxf(sa, sw) < INFINITY;
+}
+// Two instructions and one register of a product of scales: F8_OUTSIDE and more where it is no normal number.
+constexpr uint32_t F8_OUTSIDE = 0x7f000000u;
+__device__ __forceinline__ uint32_t f8_outside(float product) { return __float_as_uint(product) - 0x00800000u; }
+__device__ __forceinline__ F8Scale f8_scale(float sa, float sw) {
+  const float product = sa * sw;
+  if (!f8_unsafe(sa, sw)) return {1.f, product};
+  return (sa >= sw) == (product < 1.f) ? F8Scale{sa, sw} : F8Scale{sw, sa};   // the larger one first where they shrink
+}
+
 __device__ __forceinline__ void f8_store(const F8Args& g, long long row, int col, float v) {
   if (g.bias) v += g.bias[col];
   if (g.relu) v = fmaxf(v, 0.f);
@@ -193,6 +212,40 @@ __device__ __forceinline__ void f8_store(const F8Args& g, long long row, int col
   if (g.out_dtype == SB_F32) ((float*)g.c)[at] = v;
   else if (g.out_dtype == SB_BF16) ((__nv_bfloat16*)g.c)[at] = __float2bfloat16_rn(v);
   else ((__half*)g.c)[at] = __float2half_rn(v);
+}
+
+// Whether a row and a block of columns have such scales in blocks `begin` .. `end` - 1 of K; LOADS of each on their way at a time.
+template <int LOADS>
+__device__ __forceinline__ bool f8_row_unsafe(const F8Args& g, long long row, int n_block, int begin, int end) {
+  bool unsafe = false;
+#pragma unroll LOADS
+  for (int b = begin; b < end; ++b) unsafe |= f8_unsafe(g.sa[(long long)b * g.m + row], g.sw[(long long)n_block * g.k_blocks + b]);
+  return unsafe;
+}
+// Such a row's product with a row of W over these blocks, by one thread and as slow as it is rare.  The rows of codes start on 16 bytes.
+__device__ __forceinline__ float f8_dot(const F8Args& g, long long row, int col, int begin, int end) {
+  const uint8_t *a = g.a + row * g.lda, *w = g.w + (long long)col * g.ldw;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int b = begin; b < end; ++b) {
+    float part = 0.f;
+    const int last = min(g.k, (b + 1) * F8_BLOCK);
+    int k = b * F8_BLOCK;
+#pragma unroll 1
+    for (; k + 16 <= last; k += 16) {
+      const SbPack<uint16_t, 8> pa = *reinterpret_cast<const SbPack<uint16_t, 8>*>(a + k), pw = *reinterpret_cast<const SbPack<uint16_t, 8>*>(w + k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 va = f8_unpack2(pa.v[i]), vw = f8_unpack2(pw.v[i]);
+        part = fmaf(va.y, vw.y, fmaf(va.x, vw.x, part));
+      }
+    }
+#pragma unroll 1
+    for (; k < last; ++k) part = fmaf(f8_to_f32(a[k]), f8_to_f32(w[k]), part);
+    const F8Scale f = f8_scale(g.sa[(long long)b * g.m + row], g.sw[(long long)(col / F8_BLOCK) * g.k_blocks + b]);
+    sum = fmaf(part * f.first, f.second, sum);
+  }
+  return sum;
 }
 
 // Any sizes, pitches and alignment: 64 x 64 tiles on the CUDA cores, 4 x 4 values per thread, 16 elements of K at a time.
@@ -231,7 +284,8 @@ __global__ void __launch_bounds__(256) gemm_fp8_simple_kernel(F8Args g) {
       for (int j = 0; j < 4; ++j) {
         const int col = col0 + tx + 16 * j;
         const float sw = col < g.n ? g.sw[(long long)(col / F8_BLOCK) * g.k_blocks + b] : 0.f;
-        acc[i][j] += part[i][j] * (sa * sw);
+        const F8Scale s = f8_scale(sa, sw);
+        acc[i][j] = fmaf(part[i][j] * s.first, s.second, acc[i][j]);
       }
     }
   }
@@ -408,6 +462,24 @@ __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tma
   }
 }
 
+// An adding thread's rows with scales that f8_scale takes apart, written once more behind the last tile; the loop only notes that there
+// may be some.  16384 x 4096 x 4096 308 us, 304 without; two steps in the loop 351, the whole look at a block's scales in the loop 331,
+// by the two idle warps beside it 360 (their loads are in the way of the scales').
+template <int BN>
+__device__ __noinline__ void f8_again(const F8Args g, const F8Plan p) {
+  const int t = threadIdx.x;
+#pragma unroll 1
+  for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+    int m_blk, n_blk;
+    f8_tile(p, tile, m_blk, n_blk);
+    const long long row = (long long)m_blk * 128 + (t & 127);  // of warp t / 32 modulo 4
+    const int col = n_blk * BN + (t / 128 - F8_FIRST / 4) * (BN / 2);
+    if (row >= g.m || col >= g.n || !f8_row_unsafe<16>(g, row, col / F8_BLOCK, 0, g.k_blocks)) continue;
+#pragma unroll 1
+    for (int j = col; j < min(g.n, col + BN / 2); ++j) f8_store(g, row, j, f8_dot(g, row, j, 0, g.k_blocks));
+  }
+}
+
 template <int BN>
 __global__ void __launch_bounds__(F8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
@@ -422,6 +494,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   extern __shared__ uint8_t f8_smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[F8_STAGES_MAX], bar_empty[F8_STAGES_MAX], bar_acc_full[4], bar_acc_empty[4];
   __shared__ uint32_t tmem_slot;
+  __shared__ int unsafe_scales;                              // noted by an adding warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t stage0 = (smem_u32(f8_smem_raw) + 1023u) & ~1023u;
   if (threadIdx.x == 0) {
@@ -434,6 +507,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       mbar_init(smem_u32(&bar_acc_empty[i]), F8_WARPS / PARTS);
     }
     g_f8_abort = 0;
+    unsafe_scales = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_w);
@@ -558,6 +632,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       unsigned long long sum[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
+      uint32_t noted = 0u;
       // The columns' biases, for when the sums are done.  (Read there one by one they took 33 of 374 us at 16384 x 4096 x 4096.)
       if (g.bias)
 #pragma unroll
@@ -570,6 +645,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         asm volatile("cp.async.wait_group %0;" ::"n"(F8_AHEAD - 1) : "memory");
         const uint32_t from = scales + (uint32_t)(kb & (F8_AHEAD - 1)) * F8_SCALES;
         const float scale = f8_lds(from) * f8_lds(from + F8_SCALES / 2);
+        noted = max(noted, f8_outside(scale));
         const unsigned long long scale2 = pack_f32x2(scale, scale);
         tc_fence_after_sync();
         const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + at * PART_N + (PARTS == 2 ? 0u : (uint32_t)(half * COLS));
@@ -595,6 +671,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       if (!ok) break;
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
+      if (noted >= F8_OUTSIDE && inside) unsafe_scales = 1;
       const long long row = row0;
       const int col = col0;
       begin(tile + gridDim.x);
@@ -607,6 +684,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     if (lane == 0) bulk_wait_group<0>();
     __syncwarp();
+    if (ok && *(volatile int*)&unsafe_scales != 0) f8_again<BN>(g, p);
   }
   // After an expired wait copies and MMAs in flight get time to land before shared and tensor memory are released.
   tc_fence_before_sync();
@@ -659,6 +737,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   __shared__ __align__(8) uint64_t bar_full[F8_FEW_STAGES], bar_empty[F8_FEW_STAGES], bar_acc_full[DEPTH], bar_acc_empty[DEPTH];
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float scales[F8_FEW_BLOCKS][TN];  // of A times of W
+  __shared__ int unsafe_scales;                              // some of these products are no normal numbers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int PER = TN / SPLITS;                           // columns that a CTA finishes
   constexpr uint32_t PITCH = 4u * PER + (PER > 4 ? 16u : 0u);   // of a row's sums: 16-byte accesses without bank conflicts
@@ -677,6 +756,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       mbar_init(smem_u32(&bar_acc_empty[i]), 4);
     }
     g_f8_abort = 0;
+    unsafe_scales = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_w);
@@ -700,6 +780,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   float sum[TN];
+  bool again = false;                                        // some rows have scales that f8_scale takes apart
   if (warp == 4) {
     int stage = 0;
     uint32_t phase = 0;
@@ -743,9 +824,12 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   } else {
     for (int i = threadIdx.x; i < (kb1 - kb0) * TN; i += 128) {
       const int kb = i / TN, j = i % TN;
-      scales[kb][j] = m0 + j < g.m ? g.sa[(long long)(kb0 + kb) * g.m + m0 + j] * g.sw[(long long)blockIdx.y * g.k_blocks + kb0 + kb] : 0.f;
+      const float va = m0 + j < g.m ? g.sa[(long long)(kb0 + kb) * g.m + m0 + j] : 0.f, vw = g.sw[(long long)blockIdx.y * g.k_blocks + kb0 + kb];
+      scales[kb][j] = va * vw;
+      if (f8_unsafe(va, vw)) unsafe_scales = 1;
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
+    again = unsafe_scales != 0;
     const uint32_t acc_full0 = smem_u32(&bar_acc_full[0]), acc_empty0 = smem_u32(&bar_acc_empty[0]);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -778,6 +862,18 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         acc_phase ^= 1u;
       }
     }
+  }
+  if (again) {
+    const int n = n0 + threadIdx.x;
+    float total[TN];                                         // by way of local memory: unrolled it would cost everybody registers
+#pragma unroll
+    for (int j = 0; j < TN; ++j) total[j] = sum[j];
+#pragma unroll 1
+    for (int j = 0; j < min(TN, g.m - m0) && n < g.n; ++j)
+      if (f8_row_unsafe<2>(g, m0 + j, blockIdx.y, kb0, kb1)) total[j] = f8_dot(g, m0 + j, n, kb0, kb1);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) sum[j] = total[j];
+    __syncwarp();
   }
   // Tensor memory goes back as soon as it has been read, whatever the other CTAs do: they may be waiting for tensor memory
   // themselves, and beside a product of CTA pairs on another stream all could else wait for one another.

@@ -187,7 +187,7 @@ def matmul_fp8(a, a_scales, b, b_scales, c, epilogue=(), bias=None, stream=None)
 
     ``a`` [m, k] with ``a_scales`` [ceil(k / 128), m] (``quantize_fp8`` with block_rows 1), ``b`` [n, k] with ``b_scales``
     [ceil(n / 128), ceil(k / 128)] (block_rows 128), ``c`` [m, n] in fp32, bf16 or f16; ``epilogue``: "bias" (fp32 [n]),
-    "relu".  Rows may have a pitch.  Rows of codes that start on 16 bytes (a pitch of a multiple of 16, whatever k is) run
+    "relu" (a NaN gives 0, as in ``matmul``).  Rows may have a pitch.  Rows of codes that start on 16 bytes (a pitch of a multiple of 16, whatever k is) run
     on the tensor cores, others on the CUDA cores at about 1 % of their rate."""
     m, k, lda = matrix_of(a, "a")
     n, kb, ldb = matrix_of(b, "b")

@@ -241,3 +241,37 @@ def test_forms_for_few_rows(gpu, m, n, k, rows, splits):
     for _ in range(3):
         gpu.matmul_fp8(da[:, :k], dsa, dw[:, :k], dsw, c, epilogue=("bias",), bias=torch.from_numpy(bias).cuda())
         assert torch.equal(first, c)
+
+
+@pytest.mark.parametrize("grow", [0, 1])
+@pytest.mark.parametrize("m,n,k,shift", [(13, 200, 4080, 0), (48, 1500, 4000, 0), (150, 270, 256, 0), (1000, 2049, 272, 0), (4000, 3000, 400, 0), (40, 200, 300, 1)])
+def test_scales_whose_product_leaves_the_range(gpu, m, n, k, shift, grow):
+    """Two scales of 1e-20, or of 1e20 beside small codes: the values are ordinary numbers, though the scales' product is none.  Rows with
+    ordinary scales keep their bits beside such rows."""
+    torch = _torch()
+    (a, sa), (w, sw) = operands(m, n, k, m)
+    rows, blocks = np.arange(m), (np.arange(n) // 128 + grow) % 2
+    small, large = rows % 5 == 1, rows % 5 == 2
+    a[large] = a[large] % 3                                            # up to 2 steps of 2^-9
+    w[blocks == 1] = w[blocks == 1] % 2
+    plain = (sa * f32(1e-3)).astype(f32)
+    odd = plain.copy()
+    odd[small] *= f32(1e-20)
+    odd[large] *= f32(1e20)
+    sw = (sw * np.where((np.arange(-(-n // 128)) + grow) % 2, f32(1e20), f32(1e-20))[:, None]).astype(f32)
+    da, _, dw, dsw = device_operands(np.pad(a, ((0, 0), (shift, 0))), odd, np.pad(w, ((0, 0), (shift, 0))), sw)
+
+    def product(scales):
+        c = torch.full((m, n), 7.0, device="cuda")
+        gpu.matmul_fp8(da[:, shift:], torch.from_numpy(np.ascontiguousarray(scales.T)).cuda(), dw[:, shift:], dsw, c)
+        return c
+    c = product(odd)
+    av, wv = dequantized(a, odd, 1), dequantized(w, sw, 128)
+    want, mags = av @ wv.T, np.abs(av) @ np.abs(wv).T
+    assert np.abs(want).max() < 1e38
+    # As check_product, one more product per block, and what sums below the normal range lose.
+    bound = (128 + k / 128 + 7) * 2 * U * mags + U * np.abs(want) + (k / 128 + 2) * 2.0 ** -149
+    err = np.abs(c.double().cpu().numpy() - want)
+    assert np.all(err <= bound), "off by up to %g of the bound" % np.max(err / bound)
+    others = torch.from_numpy(~(small | large)).cuda()
+    assert torch.equal(c[others], product(plain)[others])
