@@ -12,6 +12,7 @@
 #include "vector_io.cuh"
 
 #include <limits.h>
+#include <stdlib.h>
 
 namespace {
 
@@ -284,6 +285,7 @@ constexpr int ES_ROUNDS = 6;
 constexpr int ES_CLUSTER_THREADS = 1024;
 constexpr int ES_CLUSTER_BITS = 10;                          // of a digit, at most: a bin per thread
 constexpr int ES_CLUSTER = ES_BLOCKS * ES_ROUNDS * ES_CLUSTER_THREADS;
+constexpr int ES_SMEM = 112 * 1024;                          // at most: the pairs, and every warp's counts
 __global__ void __launch_bounds__(ES_CLUSTER_THREADS) token_sort_kernel(SortArgs a, int* keys, int* pos, int bits, int rounds) {
   constexpr int WARPS = ES_CLUSTER_THREADS / 32;
   __shared__ int totals[ES_CLUSTER_THREADS], base[ES_CLUSTER_THREADS], here[ES_CLUSTER_THREADS], warp_total[2][WARPS];
@@ -1060,6 +1062,40 @@ cudaError_t launch_lookup_table(int table_dtype, int out_dtype, const void* toke
   return launch_lookup_out<I, __half>(out_dtype, tokens, table, out, n, vocab, dim, ld_table, ld_out, scale, s);
 }
 
+// Whether n tokens are sorted in one launch: by one block, or by a cluster of ES_BLOCKS where the device has room for one, which
+// it is asked once (a part of it, or one with fewer SMs side by side, need not have).  SB_SORT_CLUSTER=0 in the environment: never a cluster.
+int token_sort_fits(long long n, bool* fits) {
+  static std::atomic<int> known[64];                         // 1: one block only, 2: a cluster too
+  int dev = 0;
+  SB_CUDA(cudaGetDevice(&dev));
+  const bool keep = dev >= 0 && dev < 64;
+  int state = keep ? known[dev].load(std::memory_order_acquire) : 0;
+  if (state == 0) {                                          // asking twice is harmless
+    SB_CUDA(cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ES_SMEM));
+    state = 1;
+    const char* e = getenv("SB_SORT_CLUSTER");
+    if (!(e && e[0] == '0') && cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cfg.gridDim = dim3(ES_BLOCKS);
+      cfg.blockDim = dim3(ES_CLUSTER_THREADS);
+      cfg.dynamicSmemBytes = ES_SMEM;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = ES_BLOCKS;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, token_sort_kernel, &cfg) == cudaSuccess && clusters > 0) state = 2;
+    }
+    if (state == 1) cudaGetLastError();                      // an answer of "no" is none of the caller's errors
+    if (keep) known[dev].store(state, std::memory_order_release);
+  }
+  *fits = n <= ES_SMALL || (n <= ES_CLUSTER && state == 2);
+  return SB_OK;
+}
+
 bool embed_dtype_ok(int dt) { return dt == SB_F32 || dt == SB_BF16 || dt == SB_F16; }
 bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
@@ -1167,22 +1203,15 @@ int sb_embedding_grad(const void* tokens, int index_dtype, long long n, const vo
   int* keys = (int*)(ws + p.keys);
   int* pos = (int*)(ws + p.pos);
   a.keys_out = keys; a.pos_out = pos;
-  if (n <= ES_CLUSTER) {
+  bool one_launch = false;
+  if ((rc = token_sort_fits(n, &one_launch)) != SB_OK) return rc;
+  if (one_launch) {
     int bits = 1;
     while (bits < 31 && (1LL << bits) <= vocab) ++bits;
     const int passes = (bits + ES_CLUSTER_BITS - 1) / ES_CLUSTER_BITS;
     a.bits = (bits + passes - 1) / passes;
     const int blocks = n <= ES_SMALL ? 1 : ES_BLOCKS;
     const int rounds = (int)((n + (long long)blocks * ES_CLUSTER_THREADS - 1) / ((long long)blocks * ES_CLUSTER_THREADS));
-    static std::atomic<bool> ready[64];
-    int dev = 0;
-    SB_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {   // setting it twice is harmless
-      SB_CUDA(cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
-      SB_CUDA(cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
-    }
-    // At most 112 KB: the pairs, and every warp's counts.
     const size_t smem = 2 * sizeof(int) * (size_t)(ES_CLUSTER_THREADS * rounds) + (sizeof(short) * ES_CLUSTER_THREADS / 32 << a.bits);
     SB_CUDA(sb_launch(token_sort_kernel, dim3(blocks), dim3(ES_CLUSTER_THREADS), smem, s, blocks, a, keys, pos, bits, rounds));
     SB_COUNT_LAUNCH();
