@@ -43,3 +43,42 @@ def test_without_a_cluster(gpu, tmp_path, n, vocab, index, digits):
     assert [int(r["launches"]) for r in results] == [3 * digits + 2, 3]    # the walk and the join besides
     assert np.array_equal(results[0]["grad"], results[1]["grad"])
     check_grad(results[0]["grad"].astype(np.float64), tokens.astype(np.int64), dout.astype(np.float64), vocab, 1.0)
+
+
+@pytest.mark.parametrize("index", ["int32", "int64"])
+@pytest.mark.parametrize("n,vocab,dim,dtype,digits", [
+    (98305, 2000, 20, "bf16", 1), (131072, 2047, 8, "f32", 1), (300001, 2048, 33, "f16", 2), (100003, 50001, 24, "f32", 2),
+    (524288, 90, 64, "bf16", 1), (300000, 5000000, 4, "bf16", 3)])
+def test_more_tokens_than_a_cluster_takes(gpu, n, vocab, dim, dtype, digits, index):
+    """Three launches per digit of up to eleven bits, walk and join; chunks of 4096 tokens that end inside one, one digit and several."""
+    import torch
+    rng = np.random.default_rng(n)
+    tokens = make_tokens(rng, n, vocab)
+    tokens[[0, -1]] = vocab - 1
+    dout = torch.randn((n, dim), device="cuda").to(dtype_of(dtype))
+    dtable = torch.full((vocab, dim), float("nan"), device="cuda")
+    dev = torch.from_numpy(tokens).to(getattr(torch, index)).cuda()
+    before = gpu.launch_count()
+    gpu.primitives.embedding_grad(dev, dout, dtable, scale=1.5)
+    assert gpu.launch_count() - before == 3 * digits + 2
+    first = dtable.clone()
+    check_grad(host(dtable), tokens, host(dout), vocab, 1.5)
+    gpu.primitives.embedding_grad(dev, dout, dtable, scale=1.5, accumulate=True)
+    check_grad(host(dtable), tokens, host(dout), vocab, 1.5, host(first))
+
+
+@pytest.mark.parametrize("kind", ["one", "none", "last", "descending", "two"])
+def test_skewed_tokens_of_a_large_batch(gpu, kind):
+    import torch
+    n, vocab = 150000, 3000
+    tokens = {"one": np.zeros(n), "none": np.full(n, -1), "last": np.full(n, vocab - 1), "descending": np.arange(n)[::-1] % vocab,
+              "two": np.where(np.arange(n) % 3 == 0, 7, 2999)}[kind].astype(np.int64)
+    # Whole numbers: every sum is exact, whatever its order.
+    dout = torch.randint(-4, 5, (n, 12), device="cuda").float()
+    dtable = torch.full((vocab, 12), float("nan"), device="cuda")
+    before = gpu.launch_count()
+    gpu.primitives.embedding_grad(torch.from_numpy(tokens).cuda(), dout, dtable)
+    assert gpu.launch_count() - before == 3 * 2 + 2                    # twelve bits
+    ok = tokens >= 0
+    want = torch.zeros((vocab, 12), device="cuda").index_add_(0, torch.from_numpy(tokens[ok]).cuda(), dout[torch.from_numpy(ok).cuda()])
+    assert torch.equal(dtable, want)
