@@ -275,3 +275,28 @@ def test_scales_whose_product_leaves_the_range(gpu, m, n, k, shift, grow):
     assert np.all(err <= bound), "off by up to %g of the bound" % np.max(err / bound)
     others = torch.from_numpy(~(small | large)).cuda()
     assert torch.equal(c[others], product(plain)[others])
+
+
+# Tiles of 256, 128 and 64 columns, more of them than SMs: a CTA's second tile and later ones, rings that wrap, C by TMA and by hand.
+TILES = [(4000, 3000, 1008, 256, "f16"), (2500, 4100, 272, 256, "f32"), (2500, 4099, 270, 256, "bf16"), (20000, 500, 900, 256, "bf16"),
+         (9700, 300, 1200, 128, "f32"), (9700, 299, 300, 128, "bf16"), (40000, 100, 300, 128, "f16"),
+         (40000, 64, 2000, 64, "f32"), (20000, 51, 1000, 64, "bf16"), (19200, 48, 128, 64, "f16")]
+
+
+@pytest.mark.parametrize("m,n,k,columns,dtype", TILES)
+def test_tiles_behind_one_another(gpu, m, n, k, columns, dtype):
+    torch = _torch()
+    plan = gpu.matmul_fp8_plan(m, n, k)
+    assert (plan["block_m"], plan["block_n"]) == (128, columns) and -(-m // 128) * -(-n // columns) > 148
+    (a, sa), (w, sw) = operands(m, n, k, m + n)
+    pitch = -(-k // 16) * 16
+    da, dsa, dw, dsw = device_operands(np.pad(a, ((0, 0), (0, pitch - k)), constant_values=0x7f), sa, np.pad(w, ((0, 0), (0, pitch - k)), constant_values=0x7f), sw)
+    bias = np.random.default_rng(k).standard_normal(n).astype(f32)
+    for epilogue in ((), ("bias", "relu")):
+        hold = torch.full((m + 1, n), 7.0, device="cuda").to(dtype_of(dtype))
+        gpu.matmul_fp8(da[:, :k], dsa, dw[:, :k], dsw, hold[:m], epilogue=epilogue, bias=torch.from_numpy(bias).cuda())
+        check_product(hold[:m], a, sa, w, sw, dtype, bias.astype(np.float64) if epilogue else None, bool(epilogue))
+        assert (hold[m] == 7.0).all()
+        first = hold.clone()
+        gpu.matmul_fp8(da[:, :k], dsa, dw[:, :k], dsw, hold[:m], epilogue=epilogue, bias=torch.from_numpy(bias).cuda())
+        assert torch.equal(first, hold)
