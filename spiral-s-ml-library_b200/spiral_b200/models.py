@@ -51,6 +51,7 @@ class PolicyMLP:
         self._sizes_c = (ctypes.c_int * len(self.sizes))(*self.sizes)
         self.params = DeviceArray.zeros((self.n_params,), "f32")
         self.w_compute = DeviceArray.zeros((self.n_params,), self.storage)
+        self.weight_changes = 0          # calls that changed the weights, for what is made from them
         self.activations = [DeviceArray((self.batch, self.sizes[i + 1]), self.storage)
                             for i in range(self.n_layers - 1)]
         self._acts_c = (ctypes.c_void_p * max(1, self.n_layers - 1))(*[a.ptr for a in self.activations])
@@ -92,6 +93,7 @@ class PolicyMLP:
                 flat[ob:ob + b.size] = b
         self.params.upload(flat)
         self.w_compute.upload(flat)       # the upload rounds to the storage type
+        self.weight_changes += 1
         return self
 
     def get_weights(self):
@@ -119,6 +121,7 @@ class PolicyMLP:
             raise ValueError("checkpoint holds %d parameters, the model %d" % (flat.size, self.n_params))
         self.params.upload(flat)
         self.w_compute.upload(flat)
+        self.weight_changes += 1
         return self
 
     def split_flat(self, flat):
@@ -232,12 +235,14 @@ class PolicyMLP:
         return self.offsets[2 * layer], end
 
     def sgd(self, lr, stream=None):
+        self.weight_changes += 1
         _lib.call("sb_sgd_update", self.params.ptr, device_ptr(self.grads), self.w_compute.ptr,
                   ctypes.c_longlong(self.n_params), ctypes.c_float(lr), _lib.DTYPE_CODES[self.storage],
                   stream_ptr(stream))
 
     def train_step(self, x, mask, target, lr, stream=None):
         """Forward + backward + SGD on one GPU (no gradient exchange)."""
+        self.weight_changes += 1
         _lib.call("sb_mlp_train_step", self.n_layers, self._sizes_c, self.batch, _lib.DTYPE_CODES[self.in_dtype],
                   device_ptr(x), self.params.ptr, self.w_compute.ptr, self._acts_c, self._bits_c, device_ptr(mask),
                   device_ptr(target), self.probs.ptr, device_ptr(self.grads), int(self.with_bias),
@@ -394,7 +399,8 @@ class TokenPolicy:
     """A policy net whose states are sequences of ``n_tokens`` small integers (cards, actions, history; anything outside the
     vocabulary means "none"): embedding -> layer normalisation over the whole state -> a ``PolicyMLP`` with a masked-softmax
     head.  ``train_step`` is one AdamW step on the mean cross-entropy; ``forward_8bit`` answers with the dense layers in
-    8-bit floating point (``quantize`` first, and after every change of the weights).
+    8-bit floating point: ``quantize`` first.  After a step, an upload or a checkpoint the next answer quantises them anew; a
+    caller who writes ``mlp.params`` in another way calls ``quantize`` again.
 
     Buffers: ``table`` fp32 [vocab, dim], ``norm_weight`` and ``norm_bias`` fp32 [n_tokens * dim], ``mlp.params``; all are
     stepped by one ``AdamW`` (``optimizer``, states in fp32 or 'e4m3')."""
@@ -414,7 +420,7 @@ class TokenPolicy:
         self.x = DeviceArray((self.batch, self.width), in_dtype)
         self.mean, self.rstd = DeviceArray((self.batch,), "f32"), DeviceArray((self.batch,), "f32")
         self.optimizer = None
-        self._codes = None
+        self._codes = self._codes_of = None
         if training:
             self.dx = DeviceArray((self.batch, self.width), in_dtype)
             self.dembedded = DeviceArray((self.batch, self.width), in_dtype)
@@ -473,13 +479,19 @@ class TokenPolicy:
         for layer, (codes, scales, _, _) in enumerate(self._codes):
             w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
             quantize_fp8(w, codes, scales, block_rows=128, stream=stream)
+        self._codes_of = self._weight_changes()
         return self
+
+    def _weight_changes(self):
+        return self.mlp.weight_changes, self.optimizer.calls if self.optimizer else 0
 
     def forward_8bit(self, tokens, mask=None, stream=None):
         """``forward`` with the dense layers in 8 bits: activations quantised per row and 128 columns, products of codes (on the
         tensor cores where a layer's input width is a multiple of 16)."""
         if self._codes is None:
             raise ValueError("quantize() the weights first")
+        if self._codes_of != self._weight_changes():
+            self.quantize(stream=stream)
         self._input(tokens, stream)
         x = self.x
         for layer, (codes, scales, x_codes, x_scales) in enumerate(self._codes):

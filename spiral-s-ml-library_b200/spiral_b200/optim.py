@@ -67,7 +67,7 @@ class AdamW:
         if coded:
             self.exp_avg_scale, self.exp_avg_sq_scale = (self._made(x, blocks, "f32")
                                                          for x in (self.exp_avg_scale, self.exp_avg_sq_scale))
-        self.steps = 0
+        self.steps = self.calls = 0
         self._codes = (_lib.E4M3 if coded else _lib.F32, _GRADS[grad_tag], _lib.DTYPE_CODES[copy_tag])
         self._table = (_lib.AdamwTensor * max(1, len(self.params)))()
         for i, n in enumerate(self.sizes):
@@ -84,6 +84,7 @@ class AdamW:
         """One step over all tensors.  ``step`` counts from 1 (default: the calls so far and this one); ``seed`` is that of
         the 8-bit rounding (default: ``step``); gradients are multiplied by ``grad_scale`` first."""
         self.steps = self.steps + 1 if step is None else int(step)
+        self.calls += 1
         h = self._hyper
         h.lr, h.eps, h.weight_decay, h.grad_scale = lr, eps, weight_decay, grad_scale
         h.beta1, h.beta2 = betas

@@ -158,6 +158,7 @@ class PeerUpdate:
                   ctypes.c_float(lr), _lib.DTYPE_CODES[net.storage], mode, self._ranges, self._n_ranges,
                   int(max_blocks), self.timeout_ms, 1, stream_ptr(stream))
         self._epochs[block] += 2
+        net.weight_changes = getattr(net, "weight_changes", 0) + 1
 
     @property
     def epoch(self):
