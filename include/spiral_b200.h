@@ -244,7 +244,7 @@ int sb_philox_uniform(float* out, long long n, unsigned long long seed, unsigned
 int sb_row_binarize(const float* x, uint32_t* out, int rows, int cols, uint32_t modulo, void* stream);
 /* Rounds fp32 to the storage type of a tensor-core input class (SB_BF16,
  * SB_F16 -> 16-bit; SB_TF32 -> fp32 with the low 13 mantissa bits cleared,
- * round-to-nearest-even). */
+ * round-to-nearest-even).  `out` may be x for the types of four bytes. */
 int sb_convert(const float* x, void* out, size_t n, int out_dtype, void* stream);
 /* Game-state encoder: compact records -> the dense network input x [rows,
  * sum(widths) + n_dense] in storage type `dtype`.  Replaces the device-side

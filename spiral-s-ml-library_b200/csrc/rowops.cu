@@ -162,7 +162,8 @@ __device__ __forceinline__ float round_to_tf32(float v) {
   return __uint_as_float(u);
 }
 
-__global__ void convert_kernel(const float* __restrict__ x, void* __restrict__ out, size_t n, int dt) {
+// `out` may be x for the types of four bytes.
+__global__ void convert_kernel(const float* x, void* out, size_t n, int dt) {
   const size_t step = (size_t)gridDim.x * blockDim.x;
   for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
     const float v = x[i];

@@ -267,6 +267,13 @@ def values_ptr(x, n, what):
     return device_ptr(x)
 
 
+def keep_tf32(x, stream):
+    """An output that has just been written in fp32: one that is tagged 'tf32' is rounded to it, as the other operations leave it."""
+    if type(x) is DeviceArray and x.dtype == "tf32":
+        _lib.call("sb_convert", x.ptr, x.ptr, x.size, _lib.TF32, stream_ptr(stream))
+    return x
+
+
 class Workspaces:
     """Device memory for one call's intermediate results: kept per device, host thread and stream, grown on demand (the C ABI
     itself allocates nothing).  A thread's calls on one stream share it in their order.  Calls of other threads, whose launches

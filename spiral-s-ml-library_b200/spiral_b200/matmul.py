@@ -7,7 +7,7 @@ updated in place: ``c <- alpha * op(a) @ op(b) + beta * c``.
 import ctypes
 
 from . import _lib
-from .device import Workspaces, device_ptr, dtype_tag, matrix_of, stream_ptr, values_ptr
+from .device import Workspaces, device_ptr, dtype_tag, keep_tf32, matrix_of, stream_ptr, values_ptr
 
 EPILOGUE_FLAGS = {
     "bias": _lib.EPI_BIAS, "relu": _lib.EPI_RELU, "relu_grad": _lib.EPI_RELU_GRAD,
@@ -206,7 +206,7 @@ def matmul_fp8(a, a_scales, b, b_scales, c, epilogue=(), bias=None, stream=None)
     _lib.call("sb_matmul_fp8", _fp8_codes(a, "a"), lda, values_ptr(a_scales, across * m, "a_scales"), _fp8_codes(b, "b"), ldb,
               values_ptr(b_scales, -(-n // 128) * across, "b_scales"), device_ptr(c), ldc, m, n, k, _FP8_FLOATS[tag], epi,
               values_ptr(bias, n, "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
-    return c
+    return keep_tf32(c, stream)
 
 
 def matmul_fp8_plan(m, n, k):

@@ -3,7 +3,7 @@ operators in front of the dense layers of a net that reads tokens (embedding, la
 import ctypes
 
 from . import _lib
-from .device import device_ptr, dtype_tag, flat_size, matrix_of, stream_ptr, stream_workspace, values_ptr
+from .device import device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, stream_ptr, stream_workspace, values_ptr
 
 
 def _rows_cols(x):
@@ -154,7 +154,7 @@ def embedding(tokens, table, out, scale=1.0, stream=None):
         raise ValueError("embedding: out is %dx%d for %d tokens and rows of %d" % (rows, cols, n, dim))
     _lib.call("sb_embedding", device_ptr(tokens), _code(tokens, "tokens", _INDICES), n, device_ptr(table), ld_table,
               _code(table, "table"), vocab, dim, scale, device_ptr(out), ld_out, _code(out, "out"), stream_ptr(stream))
-    return out
+    return keep_tf32(out, stream)
 
 
 def embedding_grad(tokens, dout, dtable, scale=1.0, accumulate=False, workspace=None, stream=None):
@@ -202,7 +202,7 @@ def layer_norm(x, out=None, weight=None, bias=None, eps=1e-5, mean=None, rstd=No
     _lib.call("sb_layer_norm", device_ptr(x), ldx, device_ptr(out), ldy, values_ptr(weight, cols, "weight"),
               values_ptr(bias, cols, "bias"), eps, values_ptr(mean, rows, "mean"), values_ptr(rstd, rows, "rstd"), rows, cols, code,
               stream_ptr(stream))
-    return out
+    return keep_tf32(out, stream)
 
 
 def layer_norm_grad(dy, x, mean, rstd, dx=None, weight=None, dweight=None, dbias=None, accumulate=False, workspace=None,
@@ -230,7 +230,7 @@ def layer_norm_grad(dy, x, mean, rstd, dx=None, weight=None, dweight=None, dbias
               values_ptr(rstd, rows, "rstd"), values_ptr(weight, cols, "weight"), device_ptr(dx), lddx,
               values_ptr(dweight, cols, "dweight"), values_ptr(dbias, cols, "dbias"), int(bool(accumulate)), rows, cols, code,
               device_ptr(workspace), nbytes, stream_ptr(stream))
-    return dx
+    return keep_tf32(dx, stream)
 
 
 def layer_norm_grad_workspace(rows, cols):
