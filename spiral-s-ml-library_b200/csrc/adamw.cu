@@ -257,7 +257,8 @@ __device__ __forceinline__ void adamw_coded(const AdamwTensor& t, const AdamwHyp
 
 // 32-bit states: bound by memory, 100 M parameters 448 us, 6.7 TB/s.  8-bit states: by issue (73 % of the slots), 96 instructions
 // per element, a third of them the square root and the division, a quarter the noise: 40 M parameters with bf16 gradients 146 us,
-// 3.9 TB/s (174 without packed products and the finite path; 165 with the 80 registers that leave 24 warps per SM instead of 32).
+// 3.9 TB/s (174 without packed products and the finite path; 165 with the 80 registers that leave 24 warps per SM instead of 32).  At its 64
+// registers the 8-bit form spills 20 (fp32 gradients) to 36 bytes (bf16).
 template <typename G, bool CODED, int MOST>
 __global__ void __launch_bounds__(256, 4) adamw_kernel(const __grid_constant__ AdamwTable<MOST> a) {
   sb_grid_dependency_wait();

@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t f8_largest_bits(uint32_t largest) {
 // A block of 256 threads per ROWS x 128 tile of x, which stays in registers between the search for its largest magnitude
 // and the rounding; L lanes share a row, V neighbouring elements each.  SQUARE: one scale for the tile, else one per row.
 // Bound by issue (products, roundings and packing: three quarters of the slots) more than by memory: 16384 x 4096 bf16 40 us,
-// 5.0 TB/s, 65536 x 1024 f16 39.5 (42 with the magnitudes one at a time).
+// 5.0 TB/s, 65536 x 1024 f16 39.5 (42 with the magnitudes one at a time).  One scale per tile, whose rows all wait for the largest
+// magnitude: 16384 x 4096 bf16 54 us, 3.7 TB/s; 4096 x 4096 fp32 22, 3.7 TB/s.
 template <typename T, int V, int ROWS, bool SQUARE>
 __global__ void __launch_bounds__(256) quantize_fp8_kernel(QuantArgs a) {
   constexpr int L = F8_BLOCK / V < 32 ? F8_BLOCK / V : 32;   // lanes per row
@@ -309,9 +310,10 @@ __global__ void __launch_bounds__(256) gemm_fp8_simple_kernel(F8Args g) {
 //
 // Bound by the operands' way from L2 into shared memory: at BN = 256 a block is 48 KB in 0.55 us per SM, 13 TB/s over the chip
 // (8192^3: 530 us, 2070 TFLOP/s, the same without the multiply-adds).  Pairs of CTAs (cta_group::2, 256 x 256) load a third
-// less and were slower, 320 us against 271 for 16384 x 4096 x 4096: the round trip from the MMAs over both CTAs' adding warps
-// back to the issuer is longer than two accumulators cover.  Four stages instead of three: 288 us; sixteen adding warps, whose
-// 112 registers spill: 327 us (in pairs).
+// less and were slower, 16384 x 4096 x 4096 in short bursts 320 us against 271: the round trip from the MMAs over both CTAs' adding
+// warps back to the issuer is longer than two accumulators cover.  Four stages instead of three 288 us, sixteen adding warps, whose
+// 112 registers spill, 327 (in pairs), measured alike.  Back to back, that is under the power cap, this form takes 275 us on codes of
+// normal values and 308 on codes of random bits.
 constexpr int F8_STAGES_MAX = 12;
 constexpr int F8_WARPS = 8;                                  // that add
 constexpr int F8_FIRST = 4;                                  // the first of them: warp 0 loads, warp 1 issues
@@ -463,7 +465,7 @@ __device__ __forceinline__ void f8_write(const F8Args& g, const CUtensorMap* tma
 }
 
 // An adding thread's rows with scales that f8_scale takes apart, written once more behind the last tile; the loop only notes that there
-// may be some.  16384 x 4096 x 4096 308 us, 304 without; two steps in the loop 351, the whole look at a block's scales in the loop 331,
+// may be some.  16384 x 4096 x 4096 308 us, 304 without, 8192^3 629 and 616; two steps in the loop 351, the whole look at a block's scales in the loop 331,
 // by the two idle warps beside it 360 (their loads are in the way of the scales').
 template <int BN>
 __device__ __noinline__ void f8_again(const F8Args g, const F8Plan p) {

@@ -543,7 +543,10 @@ __device__ __forceinline__ float ln_block_sum(float v, float* slot) {
   return ln_warp_sum(w);
 }
 
-// Any row length and alignment: a block per row, the row read three times (the second and third time from L2).
+// Any row length and alignment: a block per row, the row read three times (the second and third time from L2), element by element.
+// Rows that no register form takes: past 8192 columns (16384 of 16 bits in 16-byte packs), backward past 4096 in fp32 and 8192 in 16 bits
+// (or 8192 single elements).  4096 x 16384 forward fp32 249 us (floor 82), backward fp32 446 and bf16 434 (123 and 62); 8192 x 8192 fp32
+// backward 411, where rows of 4096 take 144 for twice as many.
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_wide_kernel(NormArgs a) {
   __shared__ float slots[2][32];
@@ -807,6 +810,7 @@ cudaError_t launch_norm_grad(const NormArgs& a, cudaStream_t s, int* parts) {
   } else {
     if (a.cols <= 256 && try_norm_grad<T, 1, 8, 1, false>(a, s, &e, parts)) return e;
     if (try_norm_grad<T, 1, 8, 1, true>(a, s, &e, parts)) return e;
+    // Sixteen single 16-bit elements spill 168 bytes at 128 registers; more warps per row do not fit.
     if (try_norm_grad<T, 1, 16, 1, true>(a, s, &e, parts)) return e;
   }
   *parts = 0;
