@@ -540,6 +540,63 @@ int sb_matmul_fp8(const uint8_t* a, long long lda, const float* a_scales, const 
  * K}; fewer than 128 rows of A are the form for few rows. */
 int sb_matmul_fp8_plan(int m, int n, int k, int* plan);
 
+/* Log probabilities of given tokens (or actions) under the rows of logits [rows, cols] (SB_F32, SB_BF16, SB_F16), for a policy
+ * gradient or a token loss.  Legal columns: j < prefix when prefix >= 0, else those with a non-zero byte in mask (uint8 [rows,
+ * cols], NULL: all).  With M the largest legal logit of a row and S the sum of exp(scale (x_j - M)), log p_j = scale (x_j - M) - log S:
+ *   out [rows]            log p of tokens[row] (index_dtype SB_I32 or SB_I64); 0 for a token outside [0, cols) (no token), -inf for one
+ *                         that is not legal
+ *   entropy [rows]        -sum p_j log p_j, natural logarithms
+ *   stats [rows, 2]       M and log S, which sb_log_probs_grad reads
+ *   top_values, top_tokens [rows, top]   the log p and columns of the `top` (at most 64) largest logits, equal ones in the order of
+ *                         their columns; places beyond the legal logits above -inf hold -inf and -1
+ * each fp32 (columns int32) and NULL where it is not wanted.  A row without a legal logit above -inf has entropy 0, stats (0,
+ * +inf), and -inf for its token.  What masked columns hold does not matter; a NaN or +inf among the legal ones makes the
+ * row's values NaN.  scale > 0 is one over the temperature. */
+int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
+                 const void* tokens, int index_dtype, float* out, float* entropy, float* stats, int top, float* top_values,
+                 int32_t* top_tokens, void* stream);
+/* Its gradient: with dout and dentropy the gradients of `out` and `entropy` (fp32 [rows], NULL: none),
+ *   dlogits_j = scale (dout ([j = token] - p_j) - dentropy p_j (log p_j + entropy))
+ * in the type of the logits; 0 in columns that are not legal and in rows without a legal logit, and no dout where there is no token.
+ * The token of a row that is not legal is a constant -inf: its dout reaches the logits through -p_j only.  stats and entropy are
+ * those that sb_log_probs left.  dlogits may be the logits. */
+int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
+                      const void* tokens, int index_dtype, const float* stats, const float* dout, const float* entropy,
+                      const float* dentropy, void* dlogits, long long ldd, void* stream);
+
+/* A gated layer, both projections, the activation and their product in one kernel:
+ *   g = x w[0 .. f)^T   u = x w[f .. 2 f)^T   h = act(g) * u
+ * x [m, k], w [2 f, k] (the gate's rows, then the other projection's), h [m, f] and, where not NULL, saved [m, 2 f] = (g, u) for the
+ * gradient; SB_BF16 or SB_F16, the same for all, fp32 sums, each output rounded once.  Rows of x and w that start on
+ * 16 bytes run on the tensor cores, others on the CUDA cores at about 1 % of their rate.  f and k of at most 2^21. */
+enum { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* g (1 + erf(g / sqrt 2)) / 2 */, SB_ACT_RELU = 2 };
+int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h, long long ldh, void* saved, long long lds, int m, int f,
+             int k, int dtype, int activation, void* stream);
+/* Its gradient from dh [m, f] and what was saved:
+ *   dg = dh u act'(g)   du = dh act(g)   dx = [dg du] w   dw = [dg du]^T x
+ * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
+ * the old dw.  dg and du are rounded to the storage type for the products, whose sums are fp32 in a fixed order.  workspace:
+ * 256-byte aligned, at least sb_gated_grad_workspace_bytes. */
+int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
+int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,
+                  void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, int accumulate, int m, int f, int k, int dtype,
+                  int activation, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Weights in 4 bits with a scale per group of 32, 64 or 128 along a row: w[n, k] = scales[k / group, n] * (q - 8).  codes: uint8 [n,
+ * ceil(k / 2)], two in a byte, the even column in the low half (the high half behind an odd k holds 8); scales [ceil(k / group), n] in SB_F32, SB_BF16 or
+ * SB_F16.  Quantising: scale = largest magnitude / 7, rounded to its type, q = x / scale rounded to nearest even, kept in 0 .. 15.  A
+ * group that holds a NaN or an infinity has no meaning; one whose scale rounds to zero is zero. */
+int sb_quantize_int4(const void* x, long long ldx, int dtype, long long n, int k, int group, uint8_t* codes, long long ldc, void* scales,
+                     int scale_dtype, void* stream);
+/* The values that codes stand for, rounded to out_dtype. */
+int sb_dequantize_int4(const uint8_t* codes, long long ldw, const void* scales, int scale_dtype, void* out, long long ldo, int out_dtype,
+                       long long n, int k, int group, void* stream);
+/* c [m, n] = a w^T (+ bias) (relu) for few rows of a [m, k] (SB_BF16 or SB_F16); c in SB_F32, SB_BF16 or SB_F16, fp32 sums; epilogue:
+ * SB_EPI_BIAS (fp32 [n]), SB_EPI_RELU (a NaN gives 0, as in the other products).  Made for up to 64 rows, which read the weights once;
+ * more rows are right, and with many of them sb_dequantize_int4 and sb_matmul_ex are faster. */
+int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes, long long ldw, const void* scales, int scale_dtype, void* c,
+                   long long ldc, int m, int n, int k, int group, int out_dtype, int epilogue, const float* bias, void* stream);
+
 /* ---- data-parallel update over peer memory ---------------------------------
  * No reference counterpart (the reference is single-device, corecuda/base.spi:7);
  * follows the benchmark's data-parallel training configurations.  One process

@@ -13,4 +13,7 @@
 #include "layer_norm.cu"
 #include "adamw.cu"
 #include "gemm_fp8.cu"
+#include "log_probs.cu"
+#include "gated.cu"
+#include "gemm_int4.cu"
 #include "selftest.cu"

@@ -26,6 +26,9 @@ EPI_MASKED_SOFTMAX, EPI_REGRET_MATCHING, EPI_ARGMAX = 8, 16, 32
 EPI_RELU_MASK_OUT, EPI_RELU_GRAD_MASK, EPI_COLSUM_OUT = 64, 128, 256
 EPI_SAMPLE, EPI_BINARIZE, EPI_LN_L2 = 512, 1024, 2048
 
+# activations of a gated layer
+ACT_SILU, ACT_GELU, ACT_RELU = 0, 1, 2
+
 
 class HeadSpec(ctypes.Structure):
     """sb_head_spec of include/spiral_b200.h."""
@@ -165,6 +168,14 @@ SIGNATURES = {
     "sb_quantize_fp8": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _P]),
     "sb_matmul_fp8": (_I, [_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P]),
     "sb_matmul_fp8_plan": (_I, [_I, _I, _I, _IP]),
+    "sb_log_probs": (_I, [_P, _L, _I, _L, _I, _P, _I, _F, _P, _I, _P, _P, _P, _I, _P, _P, _P]),
+    "sb_log_probs_grad": (_I, [_P, _L, _I, _L, _I, _P, _I, _F, _P, _I, _P, _P, _P, _P, _P, _L, _P]),
+    "sb_gated": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P]),
+    "sb_gated_grad_workspace_bytes": (_I, [_I, _I, _I, POINTER(c_size_t)]),
+    "sb_gated_grad": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
+    "sb_quantize_int4": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _I, _P]),
+    "sb_dequantize_int4": (_I, [_P, _L, _P, _I, _P, _L, _I, _L, _I, _I, _P]),
+    "sb_matmul_int4": (_I, [_P, _L, _I, _P, _L, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P]),
     "sb_sgd_update": (_I, [_P, _P, _P, ctypes.c_longlong, _F, _I, _P]),
     "sb_mlp_train_step": (_I, [_I, _IP, _I, _I, _P, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _F, _P, _Z, _P, _P]),
 }

@@ -254,6 +254,12 @@ def flat_size(x, what):
     return rows * cols
 
 
+def nbytes_of(x):
+    """Bytes of a device array."""
+    n = getattr(x, "nbytes", None)
+    return int(n) if n is not None else int(x.numel()) * int(x.element_size())
+
+
 def values_ptr(x, n, what):
     """Address of n contiguous fp32 values (None -> NULL)."""
     if x is None:

@@ -1,9 +1,10 @@
 """Stand-alone row / elementwise operations (reference: ml/primitives.spi:701-780, ml/layers.spi:353-420), and the
-operators in front of the dense layers of a net that reads tokens (embedding, layer normalisation)."""
+operators around the dense layers of a net that reads tokens (embedding and layer normalisation in front of them, the log
+probabilities of its answers behind them)."""
 import ctypes
 
 from . import _lib
-from .device import device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, stream_ptr, stream_workspace, values_ptr
+from .device import device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, nbytes_of, stream_ptr, stream_workspace, values_ptr
 
 
 def _rows_cols(x):
@@ -168,7 +169,7 @@ def embedding_grad(tokens, dout, dtable, scale=1.0, accumulate=False, workspace=
         raise ValueError("embedding_grad: dout is %dx%d for %d tokens and rows of %d" % (rows, cols, n, dim))
     if dtype_tag(dtable) != "f32":
         raise TypeError("dtable must hold f32, not %s" % dtype_tag(dtable))
-    nbytes = embedding_grad_workspace(n, vocab, dim) if workspace is None else _nbytes(workspace)
+    nbytes = embedding_grad_workspace(n, vocab, dim) if workspace is None else nbytes_of(workspace)
     if workspace is None:
         workspace = stream_workspace(nbytes, stream)
     _lib.call("sb_embedding_grad", device_ptr(tokens), _code(tokens, "tokens", _INDICES), n, device_ptr(dout), ld_dout,
@@ -182,11 +183,6 @@ def embedding_grad_workspace(n, vocab, dim):
     nbytes = ctypes.c_size_t(0)
     _lib.call("sb_embedding_grad_workspace_bytes", n, vocab, dim, ctypes.byref(nbytes))
     return nbytes.value
-
-
-def _nbytes(x):
-    n = getattr(x, "nbytes", None)
-    return int(n) if n is not None else int(x.numel()) * int(x.element_size())
 
 
 def layer_norm(x, out=None, weight=None, bias=None, eps=1e-5, mean=None, rstd=None, stream=None):
@@ -222,7 +218,7 @@ def layer_norm_grad(dy, x, mean, rstd, dx=None, weight=None, dweight=None, dbias
             raise ValueError("layer_norm_grad: dx must be like x, %dx%d" % (rows, cols))
     nbytes = 0
     if workspace is not None:
-        nbytes = _nbytes(workspace)
+        nbytes = nbytes_of(workspace)
     elif dweight is not None or dbias is not None:
         nbytes = layer_norm_grad_workspace(rows, cols)
         workspace = stream_workspace(nbytes, stream)
@@ -238,3 +234,62 @@ def layer_norm_grad_workspace(rows, cols):
     nbytes = ctypes.c_size_t(0)
     _lib.call("sb_layer_norm_grad_workspace_bytes", rows, cols, ctypes.byref(nbytes))
     return nbytes.value
+
+
+def _row_args(who, logits, tokens, mask, prefix):
+    """What ``log_probs`` and its gradient share: (rows, cols, pitch, type, mask, prefix, tokens, their type)."""
+    rows, cols, ld = matrix_of(logits, "logits")
+    code = _code(logits, "logits")
+    if mask is not None:
+        if dtype_tag(mask) != "u8" or flat_size(mask, "mask") != rows * cols:
+            raise ValueError("%s: mask must be %dx%d contiguous bytes" % (who, rows, cols))
+    index = _lib.I32
+    if tokens is not None:
+        index = _code(tokens, "tokens", _INDICES)
+        if flat_size(tokens, "tokens") != rows:
+            raise ValueError("%s: %d tokens for %d rows" % (who, flat_size(tokens, "tokens"), rows))
+    return rows, cols, ld, code, device_ptr(mask), int(prefix), device_ptr(tokens), index
+
+
+def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None, top_tokens=None, mask=None, prefix=-1, scale=1.0,
+              stream=None):
+    """Log probabilities of the given tokens (or actions) under ``softmax(scale * logits)`` of each row, for a policy gradient
+    or a token loss, with the rows' entropy and likeliest alternatives.
+
+    ``logits`` [rows, cols] in fp32, bf16 or f16 (rows may have a pitch); ``tokens`` int32 or int64 [rows]; ``mask`` (uint8, same
+    shape) or ``prefix`` (legal iff j < prefix) restricts the columns as in ``softmax``.  Filled where given: ``out`` fp32 [rows] (0 where
+    the token is outside [0, cols), -inf where it is not legal), ``entropy`` fp32 [rows], ``stats`` fp32 [rows, 2] (the largest logit and the
+    logarithm of the sum over it, for ``log_probs_grad``), ``top`` fp32 and ``top_tokens`` int32 [rows, n], n at most 64: the log
+    probabilities and columns of the largest logits, equal ones in the order of their columns, -inf and -1 beyond the legal
+    ones.  ``scale`` is one over the temperature.  Returns ``out``."""
+    rows, cols, ld, code, mask, prefix, tokens, index = _row_args("log_probs", logits, tokens, mask, prefix)
+    n = 0
+    if top is not None or top_tokens is not None:
+        for x, tag, what in ((top, "f32", "top"), (top_tokens, "i32", "top_tokens")):
+            if x is None:
+                continue
+            if dtype_tag(x) != tag or len(x.shape) != 2 or int(x.shape[0]) != rows:
+                raise ValueError("log_probs: %s must be %s [%d, n]" % (what, tag, rows))
+            if rows > 0 and flat_size(x, what) != rows * int(x.shape[1]) or (n and int(x.shape[1]) != n):
+                raise ValueError("log_probs: top and top_tokens must be of one shape")
+            n = int(x.shape[1])
+    if n == 0:
+        top = top_tokens = None
+    _lib.call("sb_log_probs", device_ptr(logits), ld, code, rows, cols, mask, prefix, scale, tokens, index, values_ptr(out, rows, "out"),
+              values_ptr(entropy, rows, "entropy"), values_ptr(stats, 2 * rows, "stats"), n, device_ptr(top), device_ptr(top_tokens),
+              stream_ptr(stream))
+    return out
+
+
+def log_probs_grad(logits, tokens, stats, dlogits, dout=None, dentropy=None, entropy=None, mask=None, prefix=-1, scale=1.0, stream=None):
+    """Gradient of ``log_probs``: ``dlogits`` (like ``logits``, and may be them) from ``dout`` and ``dentropy``, the gradients of
+    ``out`` and ``entropy`` (fp32 [rows], None: none), with the ``stats`` and, for ``dentropy``, the ``entropy`` that the forward call
+    left.  Zero in columns that are not legal; a row without a token gets no ``dout``.  None flows through the alternatives."""
+    rows, cols, ld, code, mask, prefix, tokens, index = _row_args("log_probs_grad", logits, tokens, mask, prefix)
+    drows, dcols, ldd = matrix_of(dlogits, "dlogits")
+    if drows != rows or dcols != cols or _code(dlogits, "dlogits") != code:
+        raise ValueError("log_probs_grad: dlogits must be like logits, %dx%d" % (rows, cols))
+    _lib.call("sb_log_probs_grad", device_ptr(logits), ld, code, rows, cols, mask, prefix, scale, tokens, index, values_ptr(stats, 2 * rows, "stats"),
+              values_ptr(dout, rows, "dout"), values_ptr(entropy, rows, "entropy"), values_ptr(dentropy, rows, "dentropy"),
+              device_ptr(dlogits), ldd, stream_ptr(stream))
+    return keep_tf32(dlogits, stream)
