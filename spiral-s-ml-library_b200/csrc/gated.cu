@@ -5,7 +5,10 @@
 //   silu: a = g s(g), a' = s (1 + g (1 - s)) with s = 1 / (1 + exp(-g));  gelu: a = g P(g), a' = P(g) + g exp(-g^2 / 2) / sqrt(2 pi)
 //   with the normal distribution P(g) = (1 + erf(g / sqrt 2)) / 2;  relu: a = max(0, g), a' = [g > 0].
 #include "common.cuh"
+#include "few_rows.cuh"
 #include "vector_io.cuh"
+
+#include <type_traits>
 
 namespace {
 
@@ -132,6 +135,350 @@ __global__ void __launch_bounds__(256) gated_product_simple_kernel(Strided a, St
     }
 }
 
+// ---- tensor cores ----------------------------------------------------------------------------------------------
+// One persistent kernel: tiles of 128 rows (256 for a pair of CTAs) and `bf` columns of h.  A tile's accumulator has 2 bf columns, the
+// gate's and beside them the other projection's, from one sequence of MMAs with N = 2 bf whose B operand is bf rows of each half of w: in
+// a pair the leader brings the gate's and its peer the other's.  The epilogue finds both values of an output in one TMEM lane.
+//   warp 0: TMA of x      warp 10: TMA of w      warp 1: MMAs      warps 2 .. 9: epilogue, two per lane quadrant on alternate 32-column chunks
+// Two accumulators let the epilogue of a tile run beside the MMAs of the next.
+constexpr int GU_EPI_WARPS = 8;
+constexpr int GU_THREADS = 96 + 32 * GU_EPI_WARPS;
+constexpr int GU_MAX_STAGES = 8;
+constexpr int GU_BOX = 32 * 64;                 // 32 rows of 32 16-bit columns on their way to memory
+constexpr int GU_BOXES = 3;                     // per epilogue warp: h, g, u of a chunk
+constexpr int GU_STAGING = GU_EPI_WARPS * GU_BOXES * GU_BOX;
+constexpr int GU_SMEM = 225 * 1024;
+
+struct GatedMaps {
+  CUtensorMap x, gate, up, h, g, u;
+};
+struct GatedPlan {
+  int bf, tiles_m, tiles_f, tiles, k_blocks, stages, acc_stride, tmem_cols;
+  uint32_t idesc, b_bytes;                      // of w per stage and CTA
+  int boxes_out;                                // 1: outputs leave as TMA boxes
+};
+
+__device__ __forceinline__ void gated_tile(const GatedPlan& q, int tile, int& mb, int& fb) {
+  // Eight row blocks at a time: the CTAs that run together share rows of w and of x in L2.
+  const int per_group = 8 * q.tiles_f, group = tile / per_group, first = 8 * group;
+  const int rows = min(8, q.tiles_m - first), r = tile - group * per_group;
+  mb = first + r % rows;
+  fb = r / rows;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t gated_pack(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t gated_pack<__nv_bfloat16>(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+template <>
+__device__ __forceinline__ uint32_t gated_pack<__half>(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// A lane's row of 32 values into its row of a swizzled box.
+template <typename T>
+__device__ __forceinline__ void gated_to_box(uint32_t box, int lane, const float* v) {
+  const uint32_t row = box + 64u * (uint32_t)lane, key = ((uint32_t)lane >> 1) & 3u;
+#pragma unroll
+  for (uint32_t q = 0; q < 4; ++q)
+    st_shared_v4(row + ((q ^ key) << 4), make_uint4(gated_pack<T>(v[8 * q], v[8 * q + 1]), gated_pack<T>(v[8 * q + 2], v[8 * q + 3]),
+                                                    gated_pack<T>(v[8 * q + 4], v[8 * q + 5]), gated_pack<T>(v[8 * q + 6], v[8 * q + 7])));
+}
+
+template <bool PAIR, typename T, int ACT>
+__global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs p, const GatedPlan q) {
+  extern __shared__ uint8_t gu_smem[];
+  __shared__ __align__(8) uint64_t bar_full[GU_MAX_STAGES], bar_empty[GU_MAX_STAGES], bar_acc_full[2], bar_acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  constexpr uint32_t A_BYTES = 128 * 128;
+  constexpr int TILE_M = PAIR ? 256 : 128;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+  const int worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const uint32_t base = (smem_u32(gu_smem) + 1023u) & ~1023u;
+  const uint32_t stage_bytes = A_BYTES + q.b_bytes;
+  if (tid == 0) {
+    for (int i = 0; i < q.stages; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 1);
+      mbar_init(smem_u32(&bar_acc_empty[i]), (PAIR ? 2 : 1) * GU_EPI_WARPS);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&maps.x);
+    tma_prefetch_desc(&maps.gate);
+    tma_prefetch_desc(&maps.up);
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(&tmem_slot), (uint32_t)q.tmem_cols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(&tmem_slot), (uint32_t)q.tmem_cols);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before_sync();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &abort_flag;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+
+  const bool one = elect_one_lane();
+  if (warp == 0 || warp == 2 + GU_EPI_WARPS) {
+    const bool do_x = warp == 0;
+    const uint32_t full_local = smem_u32(&bar_full[0]), full0 = PAIR ? map_to_cta(full_local, 0u) : full_local, empty0 = smem_u32(&bar_empty[0]);
+    const uint32_t tx = (PAIR ? 2u : 1u) * stage_bytes;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = worker; ok && tile < q.tiles; tile += workers) {
+      int mb, fb;
+      gated_tile(q, tile, mb, fb);
+      const int m0 = mb * TILE_M + (int)rank * 128, f0 = fb * q.bf;
+      for (int kb = 0; kb < q.k_blocks; ++kb) {
+        if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = full0 + 8u * (uint32_t)stage, dst = base + (uint32_t)stage * stage_bytes;
+        if (do_x) {
+          // In a pair the leader arms its barrier with the bytes of both CTAs.
+          if (one && rank == 0u) mbar_arrive_expect_tx(full_local + 8u * (uint32_t)stage, tx);
+          if (PAIR) tma_load_2d_pair(dst, &maps.x, kb * 64, m0, full, one);
+          else tma_load_2d(dst, &maps.x, kb * 64, m0, full, one);
+        } else if (PAIR) {
+          tma_load_2d_pair(dst + A_BYTES, rank == 0u ? &maps.gate : &maps.up, kb * 64, f0, full, one);
+        } else {
+          tma_load_2d(dst + A_BYTES, &maps.gate, kb * 64, f0, full, one);
+          tma_load_2d(dst + A_BYTES + (uint32_t)q.bf * 128u, &maps.up, kb * 64, f0, full, one);
+        }
+        if (++stage == q.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0u) {
+      const uint64_t a_desc = umma_smem_desc(base, 16u, 1024u, 2u), b_desc = umma_smem_desc(base + A_BYTES, 16u, 1024u, 2u);
+      const uint32_t a_hi = (uint32_t)(a_desc >> 32), b_hi = (uint32_t)(b_desc >> 32), a_lo0 = (uint32_t)a_desc, b_lo0 = (uint32_t)b_desc;
+      const uint32_t step = stage_bytes >> 4, full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+      uint32_t a_lo = a_lo0, b_lo = b_lo0, phase = 0, acc_phase = 0;
+      int stage = 0, acc = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < q.tiles; tile += workers) {
+        if (!mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY)) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem + (uint32_t)(acc * q.acc_stride);
+        for (int kb = 0; kb < q.k_blocks; ++kb) {
+          if (!mbar_wait_warp(full0 + 8u * (uint32_t)stage, phase, abortp, SB_SITE_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) umma_issue<PAIR, false>(d, a_lo + 2u * i, a_hi, b_lo + 2u * i, b_hi, q.idesc, kb > 0 || i > 0 ? 1u : 0u, one);
+          if (PAIR) tc_commit_pair(empty0 + 8u * (uint32_t)stage, (uint16_t)3, one);
+          else tc_commit(empty0 + 8u * (uint32_t)stage, one);
+          a_lo += step;
+          b_lo += step;
+          if (++stage == q.stages) {
+            stage = 0;
+            phase ^= 1u;
+            a_lo = a_lo0;
+            b_lo = b_lo0;
+          }
+        }
+        if (!ok) break;
+        if (PAIR) tc_commit_pair(smem_u32(&bar_acc_full[acc]), (uint16_t)3, one);
+        else tc_commit(smem_u32(&bar_acc_full[acc]), one);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else if (warp < 2 + GU_EPI_WARPS) {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t boxes = base + (uint32_t)q.stages * stage_bytes + (uint32_t)(warp - 2) * (GU_BOXES * GU_BOX);
+    const bool keep = p.saved != nullptr;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = worker; tile < q.tiles; tile += workers) {
+      int mb, fb;
+      gated_tile(q, tile, mb, fb);
+      const int row0 = mb * TILE_M + (int)rank * 128 + quad * 32, f0 = fb * q.bf;
+      const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * q.acc_stride);
+      if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abortp, SB_SITE_EPI_TMEM_FULL)) break;
+      tc_fence_after_sync();
+      bool released = false;
+      for (int c = 32 * half; c < q.bf; c += 64) {
+        uint32_t raw_g[32], raw_u[32];
+        tmem_ld32(t_row + (uint32_t)c, raw_g);
+        tmem_ld32(t_row + (uint32_t)(q.bf + c), raw_u);
+        tmem_ld_wait();
+        if (c + 64 >= q.bf) {                     // this warp's last: the accumulator is free
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0u));
+            else mbar_arrive(smem_u32(&bar_acc_empty[acc]));
+          }
+          released = true;
+        }
+        const int col0 = f0 + c;
+        if (row0 >= p.m || col0 >= p.f) continue;
+        float* g = reinterpret_cast<float*>(raw_g);
+        float* u = reinterpret_cast<float*>(raw_u);
+        if (q.boxes_out) {
+          if (lane == 0) bulk_wait_group_read<0>();            // the boxes of the chunk before have been read
+          __syncwarp();
+          if (keep) {
+            gated_to_box<T>(boxes + GU_BOX, lane, g);
+            gated_to_box<T>(boxes + 2 * GU_BOX, lane, u);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) g[j] = gated_act<ACT>(g[j]) * u[j];
+          gated_to_box<T>(boxes, lane, g);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.h, boxes, col0, row0);
+            if (keep) {
+              tma_store_2d(&maps.g, boxes + GU_BOX, col0, row0);
+              tma_store_2d(&maps.u, boxes + 2 * GU_BOX, col0, row0);
+            }
+            bulk_commit_group();
+          }
+        } else if (row0 + lane < p.m) {
+          T* h = reinterpret_cast<T*>(p.h) + (long long)(row0 + lane) * p.ldh + col0;
+          T* saved = keep ? reinterpret_cast<T*>(p.saved) + (long long)(row0 + lane) * p.lds + col0 : nullptr;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col0 + j < p.f) {
+              h[j] = sb_from_f32<T>(gated_act<ACT>(g[j]) * u[j]);
+              if (saved) {
+                saved[j] = sb_from_f32<T>(g[j]);
+                saved[p.f + j] = sb_from_f32<T>(u[j]);
+              }
+            }
+        }
+      }
+      if (!released) {                            // a tile of 32 columns is one warp's
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0u));
+          else mbar_arrive(smem_u32(&bar_acc_empty[acc]));
+        }
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
+  }
+  // After an expired wait, copies and MMAs in flight get time to land before shared and tensor memory go back; in a pair neither CTA
+  // leaves while its peer can still touch its memory.
+  tc_fence_before_sync();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  if (*abortp != 0) {
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) { }
+  }
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    if (PAIR) tmem_dealloc_pair(tmem, (uint32_t)q.tmem_cols);
+    else tmem_dealloc(tmem, (uint32_t)q.tmem_cols);
+  }
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------
+// Up to 8 NT rows: a block has 16 columns of h, 16 rows of each half of w, and its eight warps share K, UNROLL blocks of 32 on their way at a
+// time.  Their sums are joined in the order of the warps.
+constexpr int GF_ROWS = 16, GF_WARPS = 8;
+
+template <typename T, int ACT, int NT>
+__global__ void __launch_bounds__(32 * GF_WARPS) gated_few_kernel(GatedArgs p) {
+  constexpr int UNROLL = 4;
+  __shared__ float part[GF_WARPS][2][NT][GF_ROWS][9];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int f0 = blockIdx.x * GF_ROWS, n0 = blockIdx.y * 8 * NT;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const T* w = reinterpret_cast<const T*>(p.w);
+  const T* x = reinterpret_cast<const T*>(p.x);
+  // Rows of w that are not there give outputs that are not written: they read row 0 of their half.
+  const T* rows[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int f = f0 + g + 8 * (i & 1);
+    rows[i] = w + (long long)((i >> 1) * (long long)p.f + (f < p.f ? f : 0)) * p.ldw;
+  }
+  float acc[2][NT][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
+  for (int k0 = warp * 32 * UNROLL; k0 < p.k; k0 += GF_WARPS * 32 * UNROLL) {
+    uint4 a[UNROLL][4], b[UNROLL][NT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[u][i] = load_eight<false>(rows[i], k0 + 32 * u + 8 * t, p.k, true);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) b[u][n] = load_eight<true>(x + (long long)(n0 + 8 * n + g) * p.ldx, k0 + 32 * u + 8 * t, p.k, n0 + 8 * n + g < p.m);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mma_16x8x16<T>(acc[i][n], a[u][2 * i].x, a[u][2 * i + 1].x, a[u][2 * i].y, a[u][2 * i + 1].y, b[u][n].x, b[u][n].y);
+          mma_16x8x16<T>(acc[i][n], a[u][2 * i].z, a[u][2 * i + 1].z, a[u][2 * i].w, a[u][2 * i + 1].w, b[u][n].z, b[u][n].w);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][i][n][g + 8 * (j >> 1)][2 * t + (j & 1)] = acc[i][n][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < GF_ROWS * 8 * NT; e += 32 * GF_WARPS) {
+    const int f = e % GF_ROWS, c = e / GF_ROWS, row = n0 + c;
+    if (f0 + f >= p.f || row >= p.m) continue;
+    float gate = 0.f, up = 0.f;
+#pragma unroll
+    for (int v = 0; v < GF_WARPS; ++v) {
+      gate += part[v][0][c / 8][f][c % 8];
+      up += part[v][1][c / 8][f][c % 8];
+    }
+    reinterpret_cast<T*>(p.h)[(long long)row * p.ldh + f0 + f] = sb_from_f32<T>(gated_act<ACT>(gate) * up);
+    if (p.saved) {
+      T* saved = reinterpret_cast<T*>(p.saved) + (long long)row * p.lds + f0 + f;
+      saved[0] = sb_from_f32<T>(gate);
+      saved[p.f] = sb_from_f32<T>(up);
+    }
+  }
+}
+
 struct GatedGradArgs {
   const void* dh;
   const void* saved;
@@ -140,19 +487,48 @@ struct GatedGradArgs {
   int m, f;
 };
 
-template <typename T, int ACT>
+// V columns per thread, every access as wide as they are.
+template <typename T, int ACT, int V>
 __global__ void __launch_bounds__(256) gated_act_grad_kernel(GatedGradArgs p) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const long long total = (long long)p.m * p.f;
+  const int across = p.f / V;
+  const long long total = (long long)p.m * across;
   for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-    const long long r = e / p.f, c = e - r * p.f;
+    const long long r = e / across, c = (e - r * across) * V;
     const T* saved = reinterpret_cast<const T*>(p.saved) + r * p.lds + c;
-    const float dh = sb_to_f32<T>(reinterpret_cast<const T*>(p.dh)[r * p.lddh + c]);
-    const float2 a = gated_act_grad<ACT>(sb_to_f32<T>(saved[0]));
+    SbWords<sizeof(T) * V> dh_w, g_w, u_w;
+    sb_load_words(dh_w, reinterpret_cast<const T*>(p.dh) + r * p.lddh + c, true);
+    sb_load_words(g_w, saved, true);
+    sb_load_words(u_w, saved + p.f, true);
+    float dh[V], g[V], u[V];
+    sb_unpack_words<T, V>(dh_w, dh);
+    sb_unpack_words<T, V>(g_w, g);
+    sb_unpack_words<T, V>(u_w, u);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 a = gated_act_grad<ACT>(g[i]);
+      g[i] = dh[i] * u[i] * a.y;
+      u[i] = dh[i] * a.x;
+    }
     T* d = reinterpret_cast<T*>(p.d) + r * p.ldd + c;
-    d[0] = sb_from_f32<T>(dh * sb_to_f32<T>(saved[p.f]) * a.y);
-    d[p.f] = sb_from_f32<T>(dh * a.x);
+    sb_store_f32<T, V>(d, g);
+    sb_store_f32<T, V>(d + p.f, u);
+  }
+}
+
+// out (+)= the sum of `splits` packed [rows, cols] matrices, in their order.
+template <typename Out>
+__global__ void __launch_bounds__(256) gated_join_kernel(const float* partial, Out* out, long long ld, long long rows, int cols, int splits, int accumulate) {
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const long long total = rows * cols;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+    float sum = 0.f;
+    for (int i = 0; i < splits; ++i) sum += partial[i * total + e];
+    const long long r = e / cols;
+    Out* o = out + r * ld + (e - r * cols);
+    *o = sb_from_f32<Out>(accumulate ? sum + sb_to_f32<Out>(*o) : sum);
   }
 }
 
@@ -165,24 +541,135 @@ int gated_args_ok(const char* who, int m, int f, int k, int dtype, int activatio
   if (activation != SB_ACT_SILU && activation != SB_ACT_GELU && activation != SB_ACT_RELU)
     return sb_fail(SB_ERR_UNSUPPORTED, "%s: unknown activation %d", who, activation);
   if (f > (1 << 21) || k > (1 << 21)) return sb_fail(SB_ERR_TOO_LARGE, "%s: layers of at most 2^21 columns and inputs", who);
+  if (m > (1 << 30)) return sb_fail(SB_ERR_TOO_LARGE, "%s: at most 2^30 rows", who);
+  return SB_OK;
+}
+
+template <typename T>
+constexpr int gated_code() { return std::is_same<T, __half>::value ? SB_F16 : SB_BF16; }
+
+template <bool PAIR, typename T, int ACT>
+int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
+  const CUtensorMapDataType type = gated_code<T>() == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  GatedPlan q;
+  memset(&q, 0, sizeof(q));
+  const int tile_m = PAIR ? 256 : 128;
+  q.bf = bf;
+  q.tiles_m = (p.m + tile_m - 1) / tile_m;
+  q.tiles_f = (p.f + bf - 1) / bf;
+  if ((long long)q.tiles_m * q.tiles_f > 0x3fffffff) return sb_fail(SB_ERR_TOO_LARGE, "sb_gated: too many outputs");
+  q.tiles = q.tiles_m * q.tiles_f;
+  q.k_blocks = (p.k + 63) / 64;
+  q.acc_stride = bf > 64 ? 256 : 2 * bf;
+  q.tmem_cols = 2 * q.acc_stride;
+  q.b_bytes = (uint32_t)bf * 128u * (PAIR ? 1u : 2u);
+  q.idesc = sb_umma_idesc(gated_code<T>(), 0, 0, tile_m, 2 * bf);
+  q.stages = (GU_SMEM - 1024 - GU_STAGING) / (int)(128 * 128 + q.b_bytes);
+  if (q.stages > GU_MAX_STAGES) q.stages = GU_MAX_STAGES;
+  const T* w = reinterpret_cast<const T*>(p.w);
+  T* saved = reinterpret_cast<T*>(p.saved);
+  GatedMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  int rc = sb_tensor_map(&maps.x, type, 2, p.x, p.m, p.k, p.ldx, 128, 64);
+  if (rc == SB_OK) rc = sb_tensor_map(&maps.gate, type, 2, w, p.f, p.k, p.ldw, bf, 64);
+  if (rc == SB_OK) rc = sb_tensor_map(&maps.up, type, 2, w + (long long)p.f * p.ldw, p.f, p.k, p.ldw, bf, 64);
+  q.boxes_out = gated_rows16(p.h, p.ldh, gated_code<T>()) && (!saved || (gated_rows16(saved, p.lds, gated_code<T>()) && p.f % 8 == 0)) ? 1 : 0;
+  if (q.boxes_out) {
+    if (rc == SB_OK) rc = sb_tensor_map(&maps.h, type, 2, p.h, p.m, p.f, p.ldh, 32, 32);
+    if (rc == SB_OK && saved) rc = sb_tensor_map(&maps.g, type, 2, saved, p.m, p.f, p.lds, 32, 32);
+    if (rc == SB_OK && saved) rc = sb_tensor_map(&maps.u, type, 2, saved + p.f, p.m, p.f, p.lds, 32, 32);
+  }
+  static std::atomic<bool> ready[64];
+  if (rc == SB_OK) rc = sb_allow_smem(gated_umma_kernel<PAIR, T, ACT>, GU_SMEM, ready);
+  if (rc != SB_OK) return rc;
+  const int most = PAIR ? sb_sm_count() / 2 : sb_sm_count(), workers = q.tiles < most ? q.tiles : most;
+  const size_t smem = 1024 + (size_t)q.stages * (128 * 128 + q.b_bytes) + GU_STAGING;
+  SB_CUDA(sb_launch(gated_umma_kernel<PAIR, T, ACT>, dim3((unsigned)(PAIR ? 2 * workers : workers)), dim3(GU_THREADS), smem, s, PAIR ? 2 : 1, maps, p, q));
+  SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+template <typename T, int ACT, int NT>
+int launch_gated_few(const GatedArgs& p, cudaStream_t s) {
+  const dim3 grid((unsigned)((p.f + GF_ROWS - 1) / GF_ROWS), (unsigned)((p.m + 8 * NT - 1) / (8 * NT)));
+  SB_CUDA(sb_launch(gated_few_kernel<T, ACT, NT>, grid, dim3(32 * GF_WARPS), 0, s, 1, p));
+  SB_COUNT_LAUNCH();
   return SB_OK;
 }
 
 template <typename T, int ACT>
 int launch_gated(const GatedArgs& p, cudaStream_t s) {
+  if (p.k > 0 && gated_rows16(p.x, p.m == 1 ? 8 : p.ldx, gated_code<T>()) && gated_rows16(p.w, p.ldw, gated_code<T>())) {
+    if (p.m <= 8) return launch_gated_few<T, ACT, 1>(p, s);
+    if (p.m <= 16) return launch_gated_few<T, ACT, 2>(p, s);
+    const int sms = sb_sm_count();
+    // Tiles as wide as still fill the chip.
+    if (p.m > 128 && (long long)((p.m + 255) / 256) * ((p.f + 127) / 128) >= sms / 4) return launch_gated_umma<true, T, ACT>(p, 128, s);
+    for (int bf = 128; bf > 32; bf /= 2)
+      if ((long long)((p.m + 127) / 128) * ((p.f + bf - 1) / bf) >= sms / 2) return launch_gated_umma<false, T, ACT>(p, bf, s);
+    return launch_gated_umma<false, T, ACT>(p, 32, s);
+  }
   const dim3 grid((unsigned)((p.m + GS_TILE - 1) / GS_TILE), (unsigned)((p.f + GS_TILE - 1) / GS_TILE));
   SB_CUDA(sb_launch(gated_simple_kernel<T, ACT>, grid, dim3(256), 0, s, 1, p));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
 
-template <typename T, int ACT>
+template <typename T, int ACT, int V>
 int launch_gated_act_grad(const GatedGradArgs& p, cudaStream_t s) {
-  long long blocks = ((long long)p.m * p.f + 255) / 256;
-  const long long most = 16LL * sb_sm_count();
-  SB_CUDA(sb_launch(gated_act_grad_kernel<T, ACT>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, p));
+  const long long blocks = ((long long)p.m * (p.f / V) + 255) / 256, most = 32LL * sb_sm_count();
+  SB_CUDA(sb_launch(gated_act_grad_kernel<T, ACT, V>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, p));
   SB_COUNT_LAUNCH();
   return SB_OK;
+}
+template <typename T, int ACT>
+int launch_gated_act_grad(const GatedGradArgs& p, cudaStream_t s) {
+  constexpr int CODE = gated_code<T>();
+  const bool wide = p.f % 8 == 0 && gated_rows16(p.dh, p.lddh, CODE) && gated_rows16(p.saved, p.lds, CODE);
+  return wide ? launch_gated_act_grad<T, ACT, 8>(p, s) : launch_gated_act_grad<T, ACT, 1>(p, s);
+}
+
+// How many parts K is cut into for a product of tiles of 256 x 256, in us as measured: a tile takes 0.4 per 64 of K and 4 besides; parts are
+// written in fp32 and joined by a launch of its own.
+int gated_splits(long long rows, long long cols, long long k) {
+  const long long tiles = ((rows + 255) / 256) * ((cols + 255) / 256), blocks = (k + 63) / 64, workers = sb_sm_count() / 2;
+  int best = 1;
+  double least = 1e30;
+  for (int i = 1; i <= 32 && 8 * (i - 1) < blocks; ++i) {
+    const double parts = i == 1 ? 0.0 : 3.0 + 8e-6 * (double)rows * cols * i / 4.0;
+    const double t = (double)((tiles * i + workers - 1) / workers) * (0.4 * ((blocks + i - 1) / i) + 4.0) + parts;
+    if (t < least) {
+      least = t;
+      best = i;
+    }
+  }
+  return best;
+}
+
+template <typename Out>
+int launch_gated_join(const float* partial, void* out, long long ld, long long rows, int cols, int splits, int accumulate, cudaStream_t s) {
+  const long long blocks = (rows * cols + 255) / 256, most = 16LL * sb_sm_count();
+  SB_CUDA(sb_launch(gated_join_kernel<Out>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, partial, reinterpret_cast<Out*>(out), ld,
+                    rows, cols, splits, accumulate));
+  SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+// out [rows, cols] (+)= op(a) b on the tensor cores, in parts of K where that is faster.
+template <typename T>
+int gated_product(bool a_trans, const void* a, const void* b, void* out, int rows, int cols, int k, const SbPitches& ld, int out_dtype, int accumulate,
+                  float* partial, cudaStream_t s) {
+  const int splits = gated_splits(rows, cols, k);
+  if (splits == 1)
+    return sb_umma_gemm_launch(a_trans ? 1 : 0, 0, 1.f, a, b, accumulate ? 1.f : 0.f, out, rows, cols, k, gated_code<T>(), out_dtype, 0, nullptr, nullptr,
+                               nullptr, nullptr, s, 1, nullptr, nullptr, nullptr, nullptr, false, &ld);
+  int used = splits;
+  const SbPitches packed = {ld.a, ld.b, cols};
+  int rc = sb_umma_gemm_launch(a_trans ? 1 : 0, 0, 1.f, a, b, 0.f, partial, rows, cols, k, gated_code<T>(), SB_F32, 0, nullptr, nullptr, nullptr, nullptr, s,
+                               splits, &used, nullptr, nullptr, nullptr, false, &packed);
+  if (rc != SB_OK) return rc;
+  return out_dtype == SB_F32 ? launch_gated_join<float>(partial, out, ld.c, rows, cols, used, accumulate, s)
+                             : launch_gated_join<T>(partial, out, ld.c, rows, cols, used, accumulate, s);
 }
 
 template <typename T, typename Out>
@@ -193,19 +680,38 @@ int launch_product_simple(const Strided& a, const Strided& b, void* c, long long
   return SB_OK;
 }
 
+struct GatedGradOut {
+  const void* x;
+  const void* w;
+  void* dx;
+  void* dw;
+  long long ldx, ldw, lddx, lddw;
+  int dw_dtype, accumulate, k;
+  float* partial;
+};
+
 template <typename T>
-int gated_grad_simple(const GatedGradArgs& g, const void* x, long long ldx, const void* w, long long ldw, void* dx, long long lddx, void* dw,
-                      long long lddw, int dw_dtype, int accumulate, int k, cudaStream_t s) {
+int gated_grad_products(const GatedGradArgs& g, const GatedGradOut& o, cudaStream_t s) {
+  constexpr int CODE = gated_code<T>();
+  const int f2 = 2 * g.f;
   int rc = SB_OK;
-  const long long f2 = 2LL * g.f;
-  if (dx && g.m > 0 && k > 0) rc = launch_product_simple<T, T>({g.d, g.ldd, 1}, {w, 1, ldw}, dx, lddx, g.m, k, f2, 0, s);
-  if (rc == SB_OK && dw && f2 > 0 && k > 0) {
-    const Strided a = {g.d, 1, g.ldd}, b = {x, 1, ldx};
-    rc = dw_dtype == SB_F32 ? launch_product_simple<T, float>(a, b, dw, lddw, f2, k, g.m, accumulate, s)
-                            : launch_product_simple<T, T>(a, b, dw, lddw, f2, k, g.m, accumulate, s);
+  if (o.k == 0) return rc;
+  if (o.dx && g.m > 0) {
+    if (f2 > 0 && gated_rows16(o.w, o.ldw, CODE))
+      rc = gated_product<T>(false, g.d, o.w, o.dx, g.m, o.k, f2, {g.ldd, o.ldw, o.lddx}, CODE, 0, o.partial, s);
+    else rc = launch_product_simple<T, T>({g.d, g.ldd, 1}, {o.w, 1, o.ldw}, o.dx, o.lddx, g.m, o.k, f2, 0, s);
   }
-  return rc;
+  if (rc != SB_OK || !o.dw || f2 == 0) return rc;
+  if (g.m > 0 && gated_rows16(o.x, g.m == 1 ? 8 : o.ldx, CODE))
+    return gated_product<T>(true, g.d, o.x, o.dw, f2, o.k, g.m, {g.ldd, g.m == 1 ? (o.ldx + 7) / 8 * 8 : o.ldx, o.lddw}, o.dw_dtype, o.accumulate, o.partial, s);
+  const Strided a = {g.d, 1, g.ldd}, b = {o.x, 1, o.ldx};
+  return o.dw_dtype == SB_F32 ? launch_product_simple<T, float>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s)
+                              : launch_product_simple<T, T>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s);
 }
+
+// The workspace: dg and du [m, 2 f] with rows on 16 bytes, and behind them the parts of a product.
+long long gated_grad_pitch(int f) { return (2LL * f + 7) / 8 * 8; }
+size_t gated_grad_first(int m, int f) { return ((size_t)m * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -232,7 +738,9 @@ int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes) {
   const char* who = "sb_gated_grad_workspace_bytes";
   if (!bytes) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
   if (m < 0 || f < 0 || k < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
-  *bytes = (size_t)m * 2 * (size_t)f * 2;
+  const int a = gated_splits(m, k, 2LL * f), b = gated_splits(2LL * f, k, m);
+  const size_t dx = a > 1 ? (size_t)a * m * k * 4 : 0, dw = b > 1 ? (size_t)b * 2 * f * k * 4 : 0;
+  *bytes = gated_grad_first(m, f) + (dx > dw ? dx : dw);
   return SB_OK;
 }
 
@@ -255,14 +763,14 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
   if ((rc = sb_gated_grad_workspace_bytes(m, f, k, &need)) != SB_OK) return rc;
   if (any && workspace_bytes < need) return sb_fail(SB_ERR_BAD_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
   if (!dx && !dw) return SB_OK;
-  const GatedGradArgs g = {dh, saved, workspace, lddh, lds, 2LL * f, m, f};
+  const GatedGradArgs g = {dh, saved, workspace, lddh, lds, gated_grad_pitch(f), m, f};
+  const GatedGradOut o = {x, w, dx, dw, ldx, ldw, lddx, lddw, dw_dtype, accumulate, k, reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + gated_grad_first(m, f))};
   cudaStream_t s = (cudaStream_t)stream;
 #define SB_GATED_CALL(ACT) (dtype == SB_BF16 ? launch_gated_act_grad<__nv_bfloat16, ACT>(g, s) : launch_gated_act_grad<__half, ACT>(g, s))
   if (any) rc = activation == SB_ACT_SILU ? SB_GATED_CALL(ACT_SILU) : activation == SB_ACT_GELU ? SB_GATED_CALL(ACT_GELU) : SB_GATED_CALL(ACT_RELU);
 #undef SB_GATED_CALL
   if (rc != SB_OK) return rc;
-  return dtype == SB_BF16 ? gated_grad_simple<__nv_bfloat16>(g, x, ldx, w, ldw, dx, lddx, dw, lddw, dw_dtype, accumulate, k, s)
-                          : gated_grad_simple<__half>(g, x, ldx, w, ldw, dx, lddx, dw, lddw, dw_dtype, accumulate, k, s);
+  return dtype == SB_BF16 ? gated_grad_products<__nv_bfloat16>(g, o, s) : gated_grad_products<__half>(g, o, s);
 }
 
 }  // extern "C"

@@ -923,32 +923,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   }
 }
 
-// Row-major matrix -> tensor map with boxes of box_rows x box_cols, swizzled by 128 bytes (64 where the box is no wider).
-int f8_tensor_map(CUtensorMap* map, CUtensorMapDataType type, int item, const void* base, long long rows, long long cols, long long pitch,
-                  int box_rows, int box_cols) {
-  EncodeTiledFn enc = get_encode_tiled();
-  if (!enc) return sb_fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dim[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)(pitch * item)};
-  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, step[2] = {1, 1};
-  CUresult r = enc(map, type, 2, const_cast<void*>(base), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   box_cols * item == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return sb_fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return SB_OK;
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory on the current device, once per device (again is harmless).
-template <typename K>
-int f8_allow_smem(K* kernel, int bytes, std::atomic<bool>* ready) {
-  int dev = 0;
-  SB_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
-    SB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
-  }
-  return SB_OK;
-}
-
 template <int BN>
 int launch_fp8(const F8Args& g, cudaStream_t s) {
   constexpr int STAGE = (128 + BN) * F8_BLOCK, REST = 1024 + F8_WARPS * (f8_boxes(BN) * F8_BOX + 512) + F8_AHEAD * F8_SCALES;
@@ -964,16 +938,16 @@ int launch_fp8(const F8Args& g, cudaStream_t s) {
   p.tma_store = reinterpret_cast<uintptr_t>(g.c) % 16 == 0 && (g.ldc * es) % 16 == 0 && ((long long)g.n * es) % 16 == 0;
   CUtensorMap ta, tw, tc;
   memset(&tc, 0, sizeof(tc));
-  int rc = f8_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, 128, F8_BLOCK);
-  if (rc == SB_OK) rc = f8_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, BN, F8_BLOCK);
+  int rc = sb_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, 128, F8_BLOCK);
+  if (rc == SB_OK) rc = sb_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, BN, F8_BLOCK);
   if (rc == SB_OK && p.tma_store) {
     const int cols = (BN / 2) * es >= 128 ? 128 / es : BN / 2;
-    rc = f8_tensor_map(&tc, g.out_dtype == SB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+    rc = sb_tensor_map(&tc, g.out_dtype == SB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                             : g.out_dtype == SB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                        es, g.c, g.m, g.n, g.ldc, 32, cols);
   }
   static std::atomic<bool> ready[64];
-  if (rc == SB_OK) rc = f8_allow_smem(gemm_fp8_kernel<BN>, F8_SMEM, ready);
+  if (rc == SB_OK) rc = sb_allow_smem(gemm_fp8_kernel<BN>, F8_SMEM, ready);
   if (rc != SB_OK) return rc;
   const int workers = p.tiles < sb_sm_count() ? p.tiles : sb_sm_count();
   SB_CUDA(sb_launch(gemm_fp8_kernel<BN>, dim3(workers), dim3(F8_THREADS), (size_t)(REST + p.stages * STAGE), s, 1, ta, tw, tc, g, p));
@@ -999,10 +973,10 @@ template <int TN, int SPLITS>
 int launch_fp8_few(const F8Args& g, cudaStream_t s) {
   const F8FewSize size = f8_few_size(TN, SPLITS, g.k_blocks);
   CUtensorMap ta, tw;
-  int rc = f8_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, TN, F8_BLOCK);
-  if (rc == SB_OK) rc = f8_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, 128, F8_BLOCK);
+  int rc = sb_tensor_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.a, g.m, g.k, g.lda, TN, F8_BLOCK);
+  if (rc == SB_OK) rc = sb_tensor_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.w, g.n, g.k, g.ldw, 128, F8_BLOCK);
   static std::atomic<bool> ready[64];
-  if (rc == SB_OK) rc = f8_allow_smem(gemm_fp8_few_kernel<TN, SPLITS>, F8_FEW_SMEM, ready);
+  if (rc == SB_OK) rc = sb_allow_smem(gemm_fp8_few_kernel<TN, SPLITS>, F8_FEW_SMEM, ready);
   if (rc != SB_OK) return rc;
   const dim3 grid(SPLITS, (g.n + 127) / 128, (g.m + TN - 1) / TN);
   SB_CUDA(sb_launch(gemm_fp8_few_kernel<TN, SPLITS>, grid, dim3(F8_FEW_THREADS), (size_t)size.bytes, s, SPLITS, ta, tw, g, size.stages));
