@@ -7,9 +7,12 @@
 #include "common.cuh"
 #include "vector_io.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int LP_MAX_TOP = 64;
+constexpr float LP_LOG2E = 1.4426950408889634f;
 
 struct LogProbArgs {
   const void* logits;
@@ -19,6 +22,7 @@ struct LogProbArgs {
   const uint8_t* mask;
   float scale;
   const void* tokens;
+  int wide_tokens;               // 64-bit tokens
   float* out;
   float* entropy;
   float* stats;
@@ -32,92 +36,512 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
 constexpr float LP_LOWEST = -3.402823466e38f;
 // What a distance from the largest logit counts as at least where it is multiplied by its own probability: 0, not NaN, for -inf.
 constexpr float LP_FAR = -1e30f;
 
-template <typename T>
-__device__ __forceinline__ float lp_logit(const LogProbArgs& g, long long row, int j) {
-  const float x = sb_to_f32<T>(reinterpret_cast<const T*>(g.logits)[row * g.ld + j]);
-  return g.mask && g.mask[row * g.mask_cols + j] == 0 ? -INFINITY : x;
+__device__ __forceinline__ long long lp_token(const void* tokens, int wide, long long row) {
+  return wide ? reinterpret_cast<const long long*>(tokens)[row] : (long long)reinterpret_cast<const int*>(tokens)[row];
 }
 
-template <typename I>
-__device__ __forceinline__ long long lp_token(const void* tokens, long long row) { return (long long)reinterpret_cast<const I*>(tokens)[row]; }
+// Largest logit so far (NaN left out: it shows in the sum), sum = S and dist = sum exp(s (x - top)) (x - top).  Of nothing: the lowest
+// number, which no -inf reaches, and zeros.
+struct RowSums {
+  float top, sum, dist;
+};
+// The same, seen from `top`, which is not below its own.
+__device__ __forceinline__ void lp_raise(RowSums& r, float top, float c) {
+  const float d = fmaxf(r.top - top, LP_FAR), f = exp2_approx(d * c);
+  r.dist = fmaf(r.sum, d, r.dist) * f;
+  r.sum *= f;
+  r.top = top;
+}
+// In N values, whose largest is not above r.top.
+template <int N>
+__device__ __forceinline__ void lp_take(RowSums& r, const float* x, float c) {
+  if constexpr (N % 2 == 0) {
+    const unsigned long long top2 = pack_f32x2(r.top, r.top), c2 = pack_f32x2(c, c);
+    unsigned long long sum2 = 0ull, dist2 = 0ull;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float d0, d1, a0, a1;
+      unpack_f32x2(sub_f32x2(pack_f32x2(x[i], x[i + 1]), top2), d0, d1);
+      const unsigned long long d2 = pack_f32x2(max_nan(d0, LP_FAR), max_nan(d1, LP_FAR));
+      unpack_f32x2(mul_f32x2(d2, c2), a0, a1);
+      const unsigned long long e2 = pack_f32x2(exp2_approx(a0), exp2_approx(a1));
+      sum2 = add_f32x2(sum2, e2);
+      fma_f32x2(dist2, e2, d2);
+    }
+    float s0, s1, d0, d1;
+    unpack_f32x2(sum2, s0, s1);
+    unpack_f32x2(dist2, d0, d1);
+    r.sum += s0 + s1;
+    r.dist += d0 + d1;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = max_nan(x[i] - r.top, LP_FAR), e = exp2_approx(d * c);
+      r.sum += e;
+      r.dist = fmaf(e, d, r.dist);
+    }
+  }
+}
 
-// One block per row, the row read three times and once more per alternative.
-template <typename T, typename I>
-__global__ void __launch_bounds__(256) log_probs_kernel(LogProbArgs g) {
-  __shared__ float part[8];
-  __shared__ float part2[8];
-  __shared__ int place[8];
+// What a row's sums give: the logarithm of S and the entropy; a row of nothing has the sum 0.
+__device__ __forceinline__ void lp_finish(const LogProbArgs& g, long long row, const RowSums& r, float log_sum, float token_logit, long long token) {
+  const bool empty = r.sum == 0.f;
+  if (g.out)
+    g.out[row] = token < 0 || token >= g.mask_cols ? 0.f : token >= g.cols || empty ? -INFINITY : g.scale * (token_logit - r.top) - log_sum;
+  if (g.entropy) g.entropy[row] = empty ? 0.f : log_sum - g.scale * (r.dist / r.sum);
+  if (g.stats) {
+    g.stats[2 * row] = empty ? 0.f : r.top;
+    g.stats[2 * row + 1] = log_sum;
+  }
+}
+__device__ __forceinline__ void lp_alternative(const LogProbArgs& g, long long row, int place, float x, int column, float top, float log_sum) {
+  const bool none = column < 0;
+  if (g.top_values) g.top_values[row * g.top + place] = none ? -INFINITY : g.scale * (x - top) - log_sum;
+  if (g.top_tokens) g.top_tokens[row * g.top + place] = none ? -1 : column;
+}
+
+// A logit by itself; -inf where the mask forbids it.
+template <typename T>
+__device__ __forceinline__ float lp_logit(const T* x, const uint8_t* mask, int j) {
+  const float v = sb_to_f32<T>(x[j]);
+  return mask && mask[j] == 0 ? -INFINITY : v;
+}
+
+// Rows of up to G E columns: G lanes per row, E columns each, in registers.  Alternatives by rounds: every lane offers its best.
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(128) log_probs_short_kernel(LogProbArgs g) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long row = blockIdx.x; row < g.rows; row += gridDim.x) {
-    float top = LP_LOWEST;
-    for (int j = threadIdx.x; j < g.cols; j += 256) top = max_nan(top, lp_logit<T>(g, row, j));
-    for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __syncthreads();
-    if (lane == 0) part[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) top = max_nan(top, part[w]);
-    float sum = 0.f, dist = 0.f;
-    for (int j = threadIdx.x; j < g.cols; j += 256) {
-      const float d = max_nan(lp_logit<T>(g, row, j) - top, LP_FAR);
-      const float e = __expf(d * g.scale);
-      sum += e;
-      dist += e * d;
+  const int lane = threadIdx.x % G;
+  const float c = g.scale * LP_LOG2E;
+  const long long groups = (long long)gridDim.x * (128 / G);
+  // Whole warps go round together.
+  const long long first = (long long)blockIdx.x * (128 / G) + threadIdx.x / G, warp_first = first - (threadIdx.x % 32) / G;
+  for (long long at = 0; warp_first + at < g.rows; at += groups) {
+    const long long row = first + at;
+    const bool there = row < g.rows;
+    const T* logits = reinterpret_cast<const T*>(g.logits) + (there ? row : 0) * g.ld;
+    const uint8_t* mask = g.mask ? g.mask + (there ? row : 0) * g.mask_cols : nullptr;
+    const long long token = there && g.out ? lp_token(g.tokens, g.wide_tokens, row) : -1;
+    float x[E];
+    RowSums r = {LP_LOWEST, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = lane + G * e;
+      x[e] = there && j < g.cols ? sb_to_f32<T>(logits[j]) : -INFINITY;
     }
-    for (int o = 16; o; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      dist += __shfl_xor_sync(0xffffffffu, dist, o);
-    }
-    __syncthreads();
-    if (lane == 0) { part[warp] = sum; part2[warp] = dist; }
-    __syncthreads();
-    sum = dist = 0.f;
-    for (int w = 0; w < 8; ++w) { sum += part[w]; dist += part2[w]; }
-    const bool empty = sum == 0.f;
-    const float log_sum = empty ? INFINITY : logf(sum);
-    if (threadIdx.x == 0) {
-      if (g.out) {
-        const long long t = lp_token<I>(g.tokens, row);
-        g.out[row] = t < 0 || t >= g.mask_cols ? 0.f : t >= g.cols || empty ? -INFINITY : g.scale * (lp_logit<T>(g, row, (int)t) - top) - log_sum;
-      }
-      if (g.entropy) g.entropy[row] = empty ? 0.f : log_sum - g.scale * (dist / sum);
-      if (g.stats) {
-        g.stats[2 * row] = empty ? 0.f : top;
-        g.stats[2 * row + 1] = log_sum;
+    if (mask) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int j = lane + G * e;
+        if (there && j < g.cols && mask[j] == 0) x[e] = -INFINITY;
       }
     }
-    float last = INFINITY;
-    int last_at = -1;
-    for (int i = 0; i < g.top; ++i) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) r.top = fmaxf(r.top, x[e]);
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) r.top = fmaxf(r.top, __shfl_xor_sync(0xffffffffu, r.top, o));
+    lp_take<E>(r, x, c);
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) {
+      r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+      r.dist += __shfl_xor_sync(0xffffffffu, r.dist, o);
+    }
+    const float log_sum = r.sum == 0.f ? INFINITY : logf(r.sum);
+    if (there && lane == 0) {
+      const bool legal = token >= 0 && token < g.cols;
+      lp_finish(g, row, r, log_sum, legal ? lp_logit<T>(logits, mask, (int)token) : 0.f, token);
+    }
+    if (g.top > 0) {
       float best = -INFINITY;
-      int at = 0x7fffffff;
-      for (int j = threadIdx.x; j < g.cols; j += 256) {
-        const float x = lp_logit<T>(g, row, j);
-        if ((x < last || (x == last && j > last_at)) && x > best) { best = x; at = j; }
+      int column = 0x7fffffff;
+      auto offer = [&]() {
+        best = -INFINITY;
+        column = 0x7fffffff;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (x[e] > best) {
+            best = x[e];
+            column = lane + G * e;
+          }
+      };
+      offer();
+      for (int i = 0; i < g.top; ++i) {
+        float v = best;
+        int j = column;
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) {
+          const float w = __shfl_xor_sync(0xffffffffu, v, o);
+          const int k = __shfl_xor_sync(0xffffffffu, j, o);
+          if (w > v || (w == v && k < j)) {
+            v = w;
+            j = k;
+          }
+        }
+        if (there && lane == i % G) lp_alternative(g, row, i, v, j == 0x7fffffff ? -1 : j, r.top, log_sum);
+        if (j == column && j != 0x7fffffff) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (lane + G * e == j) x[e] = -INFINITY;
+          offer();
+        }
       }
+    }
+  }
+}
+
+// A row's place in memory: single elements up to the first 16-byte boundary, packs of 16 bytes, single elements behind them.
+template <typename T>
+struct RowShape {
+  static constexpr int V = 16 / sizeof(T);
+  int head, packs, tail;
+  __device__ __forceinline__ RowShape(const T* x, int cols) {
+    head = (int)((16u - (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / (int)sizeof(T);
+    head = head < cols ? head : cols;
+    packs = (cols - head) / V;
+    tail = cols - head - packs * V;
+  }
+  __device__ __forceinline__ int column(int pack) const { return head + pack * V; }
+  // The i-th of the head + tail single elements.
+  __device__ __forceinline__ int single(int i) const { return i < head ? i : packs * V + i; }
+};
+
+template <typename T>
+__device__ __forceinline__ float lp_largest(const SbWords<16>& w);
+template <>
+__device__ __forceinline__ float lp_largest<float>(const SbWords<16>& w) {
+  return fmaxf(fmaxf(__uint_as_float(w.v.x), __uint_as_float(w.v.y)), fmaxf(__uint_as_float(w.v.z), __uint_as_float(w.v.w)));
+}
+template <>
+__device__ __forceinline__ float lp_largest<__nv_bfloat16>(const SbWords<16>& w) {
+  __nv_bfloat162 v[4];
+  memcpy(v, &w, 16);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+  return fmaxf(m.x, m.y);
+}
+template <>
+__device__ __forceinline__ float lp_largest<__half>(const SbWords<16>& w) {
+  __half2 v[4];
+  memcpy(v, &w, 16);
+  const float2 m = __half22float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+  return fmaxf(m.x, m.y);
+}
+
+template <typename T>
+__device__ __forceinline__ void lp_mask_pack(float* x, const uint8_t* mask) {
+#pragma unroll
+  for (int i = 0; i < RowShape<T>::V; ++i)
+    if (mask[i] == 0) x[i] = -INFINITY;
+}
+
+// An order of floats as unsigned numbers.
+__device__ __forceinline__ uint32_t lp_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int LP_CANDIDATES = 512;
+
+// Longer rows: a block per row, or a cluster of blocks that share one, in one pass over memory.  Each thread keeps its own
+// sums and raises their reference when a batch of packs brings a larger logit.
+//
+// Alternatives: the top-th largest of the threads' own largest logits is a bound that `top` logits at least reach and few others do.  Only
+// the threads that reach it hold alternatives; the block reads their share of the row once more, from L2, and ranks what reaches
+// the bound.  Rows with more of those than there is room for (long runs of equal logits) find them one after the other.
+template <typename T, int NT, bool MASKED, bool CLUSTER>
+__global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
+  constexpr int V = RowShape<T>::V, WARPS = NT / 32, UNROLL = 4;
+  __shared__ RowSums part[WARPS];
+  __shared__ RowSums whole;                      // of this block's share
+  __shared__ float largest[NT];
+  __shared__ int hot[NT];
+  __shared__ float value[LP_CANDIDATES];
+  __shared__ int column[LP_CANDIDATES];
+  __shared__ float best_value[LP_MAX_TOP];
+  __shared__ int best_column[LP_MAX_TOP];
+  __shared__ int hot_count, candidate_count;
+  __shared__ float bound;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int blocks = CLUSTER ? (int)gridDim.x : 1, rank = CLUSTER ? (int)blockIdx.x : 0;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const float c = g.scale * LP_LOG2E;
+  for (long long row = blockIdx.y; row < g.rows; row += gridDim.y) {
+    const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
+    const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
+    const RowShape<T> shape(x, g.cols);
+    const int stride = NT * blocks, first = rank * NT + tid;
+    const int singles = shape.head + shape.tail;               // fewer than 2 V: the first threads of the first block have one each
+    RowSums r = {LP_LOWEST, 0.f, 0.f};
+    if (first < singles) {
+      const float v = lp_logit<T>(x, mask, shape.single(first));
+      r.top = fmaxf(r.top, v);
+      lp_take<1>(r, &v, c);
+    }
+    for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
+      SbWords<16> w[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        // Packs that are not there hold -inf.
+        w[u].v = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
+                 : std::is_same<T, __half>::value ? make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u)
+                                                  : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+        sb_load_words(w[u], x + shape.column(p0 + u * stride < shape.packs ? p0 + u * stride : 0), p0 + u * stride < shape.packs);
+      }
+      float top = r.top;
+      if constexpr (!MASKED) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) top = fmaxf(top, lp_largest<T>(w[u]));
+        lp_raise(r, top, c);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          float v[V];
+          sb_unpack_words<T, V>(w[u], v);
+          lp_take<V>(r, v, c);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          float v[V];
+          sb_unpack_words<T, V>(w[u], v);
+          if (p0 + u * stride < shape.packs) lp_mask_pack<T>(v, mask + shape.column(p0 + u * stride));
+          float most = r.top;
+#pragma unroll
+          for (int i = 0; i < V; ++i) most = fmaxf(most, v[i]);
+          lp_raise(r, most, c);
+          lp_take<V>(r, v, c);
+        }
+      }
+    }
+    const float mine = r.top;
+    float top = r.top;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    lp_raise(r, top, c);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+      r.dist += __shfl_xor_sync(0xffffffffu, r.dist, o);
+    }
+    __syncthreads();                             // what the row before left has been read
+    if (lane == 0) part[warp] = r;
+    if (g.top > 0) largest[tid] = mine;
+    if (tid == 0) hot_count = candidate_count = 0;
+    __syncthreads();
+    if (warp == 0) {
+      RowSums all = lane < WARPS ? part[lane] : RowSums{LP_LOWEST, 0.f, 0.f};
+      float most = all.top;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      lp_raise(all, most, c);
+#pragma unroll
       for (int o = 16; o; o >>= 1) {
-        const float b = __shfl_xor_sync(0xffffffffu, best, o);
-        const int a = __shfl_xor_sync(0xffffffffu, at, o);
-        if (b > best || (b == best && a < at)) { best = b; at = a; }
+        all.sum += __shfl_xor_sync(0xffffffffu, all.sum, o);
+        all.dist += __shfl_xor_sync(0xffffffffu, all.dist, o);
+      }
+      if (lane == 0) whole = all;
+    }
+    if (g.top > 0) {
+      if (warp == WARPS - 1) {
+        // Bit by bit the largest key that `top` of the threads reach; near it is near enough.
+        uint32_t keys[NT / 32], key = 0u;
+#pragma unroll
+        for (int i = 0; i < NT / 32; ++i) keys[i] = lp_key(largest[lane + 32 * i]);
+        for (int bit = 31; bit >= 0; --bit) {
+          const uint32_t tried = key | 1u << bit;
+          int reach = 0;
+#pragma unroll
+          for (int i = 0; i < NT / 32; ++i) reach += keys[i] >= tried ? 1 : 0;
+          reach = (int)__reduce_add_sync(0xffffffffu, (unsigned)reach);
+          if (reach >= g.top) {
+            key = tried;
+            if (reach <= g.top + 4) break;
+          }
+        }
+        // The key as a number; below the lowest number's (fewer threads than alternatives have a logit) everything counts.
+        const float b = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+        if (lane == 0) bound = key <= lp_key(LP_LOWEST) ? LP_LOWEST : b;
       }
       __syncthreads();
-      if (lane == 0) { part[warp] = best; place[warp] = at; }
+      const float least = bound;
+      if (mine >= least) hot[atomicAdd(&hot_count, 1)] = tid;
       __syncthreads();
-      for (int w = 0; w < 8; ++w)
-        if (part[w] > best || (part[w] == best && place[w] < at)) { best = part[w]; at = place[w]; }
-      const bool none = at == 0x7fffffff;
-      if (threadIdx.x == 0) {
-        if (g.top_values) g.top_values[row * g.top + i] = none ? -INFINITY : g.scale * (best - top) - log_sum;
-        if (g.top_tokens) g.top_tokens[row * g.top + i] = none ? -1 : at;
+      // A thread's share: its packs, then its single element.
+      const int each = (shape.packs + stride - 1) / stride + 1, items = hot_count * each;
+      for (int item = tid; item < items; item += NT) {
+        const int who = hot[item / each], k = item % each;
+        const int pack = rank * NT + who + k * stride;
+        auto candidate = [&](float v, int j) {
+          if (v >= least && v > -INFINITY) {
+            const int at = atomicAdd(&candidate_count, 1);
+            if (at < LP_CANDIDATES) {
+              value[at] = v;
+              column[at] = j;
+            }
+          }
+        };
+        if (k == each - 1) {
+          if (rank * NT + who < singles) {
+            const int j = shape.single(rank * NT + who);
+            candidate(lp_logit<T>(x, mask, j), j);
+          }
+        } else if (pack < shape.packs) {
+          SbWords<16> w;
+          sb_load_words(w, x + shape.column(pack), true);
+          if (MASKED || lp_largest<T>(w) >= least) {
+            float v[V];
+            sb_unpack_words<T, V>(w, v);
+            if (MASKED) lp_mask_pack<T>(v, mask + shape.column(pack));
+#pragma unroll
+            for (int i = 0; i < V; ++i) candidate(v[i], shape.column(pack) + i);
+          }
+        }
       }
-      last = best;
-      last_at = at;
+      if (tid < LP_MAX_TOP) best_column[tid] = -1;
+      __syncthreads();
+      const int n = candidate_count;
+      if (n <= LP_CANDIDATES) {
+        for (int i = tid; i < n; i += NT) {
+          const float v = value[i];
+          const int j = column[i];
+          int before = 0;
+          for (int k = 0; k < n; ++k) before += value[k] > v || (value[k] == v && column[k] < j) ? 1 : 0;
+          if (before < g.top) {
+            best_value[before] = v;
+            best_column[before] = j;
+          }
+        }
+        __syncthreads();
+      } else {
+        float last = INFINITY;
+        int last_at = -1;
+        for (int i = 0; i < g.top; ++i) {
+          float v = -INFINITY;
+          int j = 0x7fffffff;
+          auto look = [&](float a, int at) {
+            if ((a < last || (a == last && at > last_at)) && (a > v || (a == v && at < j)) && a > -INFINITY) {
+              v = a;
+              j = at;
+            }
+          };
+          if (first < singles) look(lp_logit<T>(x, mask, shape.single(first)), shape.single(first));
+          for (int p = first; p < shape.packs; p += stride) {
+            SbWords<16> w;
+            sb_load_words(w, x + shape.column(p), true);
+            float a[V];
+            sb_unpack_words<T, V>(w, a);
+            if (MASKED) lp_mask_pack<T>(a, mask + shape.column(p));
+#pragma unroll
+            for (int e = 0; e < V; ++e) look(a[e], shape.column(p) + e);
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            const float w = __shfl_xor_sync(0xffffffffu, v, o);
+            const int k = __shfl_xor_sync(0xffffffffu, j, o);
+            if (w > v || (w == v && k < j)) {
+              v = w;
+              j = k;
+            }
+          }
+          __syncthreads();
+          if (lane == 0) {
+            value[warp] = v;
+            column[warp] = j;
+          }
+          __syncthreads();
+          for (int w = 0; w < WARPS; ++w)
+            if (value[w] > v || (value[w] == v && column[w] < j)) {
+              v = value[w];
+              j = column[w];
+            }
+          if (tid == 0 && j != 0x7fffffff) {
+            best_value[i] = v;
+            best_column[i] = j;
+          }
+          last = v;
+          last_at = j;
+        }
+        __syncthreads();
+      }
+    } else {
+      __syncthreads();
+    }
+    RowSums all = whole;
+    if constexpr (CLUSTER) {
+      // The first block joins the others' sums and alternatives, in their order.
+      cluster_sync_all();
+      if (rank == 0) {
+        if (tid == 0) candidate_count = 0;
+        __syncthreads();
+        RowSums parts[8];
+        float most = LP_LOWEST;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          parts[b] = {LP_LOWEST, 0.f, 0.f};
+          if (b < blocks) {
+            const uint32_t at = map_to_cta(smem_u32(&whole), (uint32_t)b);
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(parts[b].top) : "r"(at) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(parts[b].sum) : "r"(at + 4u) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(parts[b].dist) : "r"(at + 8u) : "memory");
+          }
+          most = fmaxf(most, parts[b].top);
+        }
+        all = {most, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          lp_raise(parts[b], most, c);
+          all.sum += parts[b].sum;
+          all.dist += parts[b].dist;
+        }
+        for (int i = tid; i < blocks * g.top; i += NT) {
+          const uint32_t b = (uint32_t)(i / g.top), k = (uint32_t)(i % g.top);
+          float v = 0.f;
+          int j;
+          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(j) : "r"(map_to_cta(smem_u32(&best_column[k]), b)) : "memory");
+          if (j >= 0) {
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(&best_value[k]), b)) : "memory");
+            const int at = atomicAdd(&candidate_count, 1);
+            value[at] = v;
+            column[at] = j;
+          }
+        }
+        __syncwarp();
+      }
+      cluster_sync_all();                        // the others may go on
+      if (rank == 0 && g.top > 0) {
+        const int n = candidate_count;
+        if (tid < LP_MAX_TOP) best_column[tid] = -1;
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+          const float v = value[i];
+          const int j = column[i];
+          int before = 0;
+          for (int k = 0; k < n; ++k) before += value[k] > v || (value[k] == v && column[k] < j) ? 1 : 0;
+          if (before < g.top) {
+            best_value[before] = v;
+            best_column[before] = j;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (rank == 0) {
+      const float log_sum = all.sum == 0.f ? INFINITY : logf(all.sum);
+      if (tid == 0) {
+        const long long token = g.out ? lp_token(g.tokens, g.wide_tokens, row) : -1;
+        lp_finish(g, row, all, log_sum, token >= 0 && token < g.cols ? lp_logit<T>(x, mask, (int)token) : 0.f, token);
+      }
+      if (tid < g.top) lp_alternative(g, row, tid, best_value[tid], best_column[tid], all.top, log_sum);
     }
   }
 }
@@ -130,31 +554,132 @@ struct LogProbGradArgs {
   const uint8_t* mask;
   float scale;
   const void* tokens;
+  int wide_tokens;
   const float* stats;
   const float* dout;
   const float* entropy;
   const float* dentropy;
 };
 
-template <typename T, typename I>
-__global__ void __launch_bounds__(256) log_probs_grad_kernel(LogProbGradArgs g) {
+// What a row's gradient is made of: p_j = exp(s (x_j - top) - log_sum), d_j = -s p_j (c + h log p_j), and `a` more at the token.
+struct RowGrad {
+  float scale, top, log_sum, c, h, a;
+  int token;
+};
+__device__ __forceinline__ RowGrad lp_row_grad(const LogProbGradArgs& g, long long row) {
+  RowGrad r;
+  r.scale = g.scale;
+  r.top = g.stats[2 * row];
+  r.log_sum = g.stats[2 * row + 1];
+  const long long t = g.dout ? lp_token(g.tokens, g.wide_tokens, row) : -1;
+  const float a = t >= 0 && t < g.mask_cols ? g.dout[row] : 0.f;
+  r.h = g.dentropy ? g.dentropy[row] : 0.f;
+  r.c = g.dentropy ? fmaf(r.h, g.entropy[row], a) : a;
+  r.a = g.scale * a;
+  r.token = t >= 0 && t < g.cols && r.log_sum != INFINITY ? (int)t : -1;
+  return r;
+}
+// Logarithms of probabilities at least this far from 1, whose probabilities are 0 in fp32.
+constexpr float LP_NOTHING = -1e4f;
+__device__ __forceinline__ float lp_grad(const RowGrad& r, float x) {
+  const float lp = max_nan(fmaf(r.scale, x - r.top, -r.log_sum), LP_NOTHING);
+  return exp2_approx(lp * LP_LOG2E) * fmaf(r.h, lp, r.c) * -r.scale;
+}
+// A pack of logits whose place the gradient may take: not by the path for data that stays as it is.
+__device__ __forceinline__ void lp_load_once(SbWords<16>& w, const void* from, bool issue) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t@q ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(w.v.x), "+r"(w.v.y), "+r"(w.v.z), "+r"(w.v.w) : "l"(from), "r"((uint32_t)issue) : "memory");
+}
+// Of a single column.
+template <typename T>
+__device__ __forceinline__ void lp_grad_one(const RowGrad& r, const T* x, const uint8_t* mask, T* d, int j, int cols) {
+  float v = 0.f;
+  if (j < cols && !(mask && mask[j] == 0)) {
+    v = lp_grad(r, sb_to_f32<T>(x[j]));
+    if (j == r.token) v += r.a;
+  }
+  d[j] = sb_from_f32<T>(v);
+}
+
+// Short rows: G lanes per row.
+template <typename T, int G>
+__global__ void __launch_bounds__(256) log_probs_grad_short_kernel(LogProbGradArgs g) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  for (long long row = blockIdx.x; row < g.rows; row += gridDim.x) {
-    const float top = g.stats[2 * row], log_sum = g.stats[2 * row + 1];
-    long long t = g.dout ? lp_token<I>(g.tokens, row) : -1;
-    const float a = t >= 0 && t < g.mask_cols ? g.dout[row] : 0.f;
-    const float h = g.dentropy ? g.dentropy[row] : 0.f, entropy = g.dentropy ? g.entropy[row] : 0.f;
-    if (log_sum == INFINITY) t = -1;
-    for (int j = threadIdx.x; j < g.mask_cols; j += 256) {
-      float d = 0.f;
-      if (j < g.cols && !(g.mask && g.mask[row * g.mask_cols + j] == 0)) {
-        const float x = sb_to_f32<T>(reinterpret_cast<const T*>(g.logits)[row * g.ld + j]);
-        const float lp = max_nan(g.scale * (x - top) - log_sum, LP_FAR);
-        const float p = __expf(lp);
-        d = g.scale * ((j == t ? a : 0.f) - p * (a + h * (lp + entropy)));
+  const int lane = threadIdx.x % G;
+  const long long groups = (long long)gridDim.x * (256 / G);
+  for (long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; row < g.rows; row += groups) {
+    const RowGrad r = lp_row_grad(g, row);
+    const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
+    const uint8_t* mask = g.mask ? g.mask + row * g.mask_cols : nullptr;
+    T* d = reinterpret_cast<T*>(g.dlogits) + row * g.ldd;
+    for (int j = lane; j < g.mask_cols; j += G) lp_grad_one<T>(r, x, mask, d, j, g.cols);
+  }
+}
+
+// Long rows: packs of 16 bytes, several on their way; the blocks of a column of the grid share the rows.
+template <typename T, bool MASKED>
+__global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArgs g) {
+  constexpr int V = RowShape<T>::V, UNROLL = 4;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const int first = blockIdx.x * 256 + threadIdx.x, stride = gridDim.x * 256;
+  for (long long row = blockIdx.y; row < g.rows; row += gridDim.y) {
+    const RowGrad r = lp_row_grad(g, row);
+    const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
+    const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
+    T* d = reinterpret_cast<T*>(g.dlogits) + row * g.ldd;
+    const RowShape<T> shape(x, g.cols);
+    const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
+    if (first < shape.head + shape.tail) lp_grad_one<T>(r, x, mask, d, shape.single(first), g.cols);
+    for (int j = g.cols + first; j < g.mask_cols; j += stride) d[j] = sb_from_f32<T>(0.f);
+    for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
+      SbWords<16> w[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        w[u].v = make_uint4(0u, 0u, 0u, 0u);
+        const bool there = p0 + u * stride < shape.packs;
+        lp_load_once(w[u], x + shape.column(there ? p0 + u * stride : 0), there);
       }
-      reinterpret_cast<T*>(g.dlogits)[row * g.ldd + j] = sb_from_f32<T>(d);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (p0 + u * stride >= shape.packs) break;
+        const int j = shape.column(p0 + u * stride);
+        float v[V];
+        sb_unpack_words<T, V>(w[u], v);
+        const unsigned long long top2 = pack_f32x2(r.top, r.top), scale2 = pack_f32x2(r.scale, r.scale), sum2 = pack_f32x2(-r.log_sum, -r.log_sum),
+                                 log2 = pack_f32x2(LP_LOG2E, LP_LOG2E), h2 = pack_f32x2(r.h, r.h), c2 = pack_f32x2(r.c, r.c),
+                                 minus2 = pack_f32x2(-r.scale, -r.scale);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          unsigned long long lp2 = sum2;
+          fma_f32x2(lp2, scale2, sub_f32x2(pack_f32x2(v[i], v[i + 1]), top2));
+          float l0, l1;
+          unpack_f32x2(lp2, l0, l1);
+          lp2 = pack_f32x2(max_nan(l0, LP_NOTHING), max_nan(l1, LP_NOTHING));
+          unpack_f32x2(mul_f32x2(lp2, log2), l0, l1);
+          unsigned long long q2 = c2;
+          fma_f32x2(q2, h2, lp2);
+          q2 = mul_f32x2(mul_f32x2(pack_f32x2(exp2_approx(l0), exp2_approx(l1)), q2), minus2);
+          unpack_f32x2(q2, v[i], v[i + 1]);
+        }
+        if ((unsigned)(r.token - j) < (unsigned)V) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (j + i == r.token) v[i] += r.a;
+        }
+        if (MASKED) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (mask[j + i] == 0) v[i] = 0.f;
+        }
+        if (alike) {
+          sb_store_f32<T, V>(d + j, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) d[j + i] = sb_from_f32<T>(v[i]);
+        }
+      }
     }
   }
 }
@@ -181,20 +706,55 @@ int lp_args_ok(const char* who, const void* logits, long long ld, int dtype, lon
 
 bool lp_words(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
-template <typename T>
-int launch_log_probs(const LogProbArgs& g, int index_dtype, cudaStream_t s) {
-  const int grid = (int)(g.rows < 65536 ? g.rows : 65536);
-  if (index_dtype == SB_I64) SB_CUDA(sb_launch(log_probs_kernel<T, long long>, dim3(grid), dim3(256), 0, s, 1, g));
-  else SB_CUDA(sb_launch(log_probs_kernel<T, int>, dim3(grid), dim3(256), 0, s, 1, g));
+template <typename T, int G, int E>
+int launch_log_probs_short(const LogProbArgs& g, cudaStream_t s) {
+  const long long blocks = (g.rows + 128 / G - 1) / (128 / G), most = 64LL * sb_sm_count();
+  SB_CUDA(sb_launch(log_probs_short_kernel<T, G, E>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(128), 0, s, 1, g));
+  SB_COUNT_LAUNCH();
+  return SB_OK;
+}
+
+template <typename T, int NT, bool CLUSTER>
+int launch_log_probs_long(const LogProbArgs& g, int blocks, cudaStream_t s) {
+  const dim3 grid((unsigned)blocks, (unsigned)(g.rows < 65535 ? g.rows : 65535));
+  if (g.mask) SB_CUDA(sb_launch(log_probs_long_kernel<T, NT, true, CLUSTER>, grid, dim3(NT), 0, s, blocks, g));
+  else SB_CUDA(sb_launch(log_probs_long_kernel<T, NT, false, CLUSTER>, grid, dim3(NT), 0, s, blocks, g));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
 
 template <typename T>
-int launch_log_probs_grad(const LogProbGradArgs& g, int index_dtype, cudaStream_t s) {
-  const int grid = (int)(g.rows < 65536 ? g.rows : 65536);
-  if (index_dtype == SB_I64) SB_CUDA(sb_launch(log_probs_grad_kernel<T, long long>, dim3(grid), dim3(256), 0, s, 1, g));
-  else SB_CUDA(sb_launch(log_probs_grad_kernel<T, int>, dim3(grid), dim3(256), 0, s, 1, g));
+int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
+  if (g.cols <= 16) return launch_log_probs_short<T, 4, 4>(g, s);
+  if (g.cols <= 64) return launch_log_probs_short<T, 8, 8>(g, s);
+  if (g.cols <= 256) return launch_log_probs_short<T, 32, 8>(g, s);
+  if (g.cols <= 1024) return launch_log_probs_short<T, 32, 32>(g, s);
+  int blocks = 1;
+  while (blocks < 8 && g.rows * blocks * 2 <= 2LL * sb_sm_count() && g.cols / (2 * blocks) >= 4096) blocks *= 2;
+  if (blocks > 1) return launch_log_probs_long<T, 512, true>(g, blocks, s);
+  if (g.cols <= 4096) return launch_log_probs_long<T, 128, false>(g, 1, s);
+  return launch_log_probs_long<T, 256, false>(g, 1, s);
+}
+
+template <typename T>
+int launch_log_probs_grad(const LogProbGradArgs& g, cudaStream_t s) {
+  if (g.mask_cols <= 256) {
+    const int lanes = g.mask_cols <= 16 ? 4 : g.mask_cols <= 64 ? 8 : 32;
+    const long long blocks = (g.rows * lanes + 255) / 256, most = 32LL * sb_sm_count();
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    if (lanes == 4) SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 4>, grid, dim3(256), 0, s, 1, g));
+    else if (lanes == 8) SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 8>, grid, dim3(256), 0, s, 1, g));
+    else SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 32>, grid, dim3(256), 0, s, 1, g));
+    SB_COUNT_LAUNCH();
+    return SB_OK;
+  }
+  // Enough blocks for the chip where rows are few, each with a batch of packs per thread at least.
+  const int batch = 256 * 4 * (16 / (int)sizeof(T));
+  long long across = (8LL * sb_sm_count() + g.rows - 1) / g.rows;
+  if (across > (g.mask_cols + batch - 1) / batch) across = (g.mask_cols + batch - 1) / batch;
+  const dim3 grid((unsigned)across, (unsigned)(g.rows < 65535 ? g.rows : 65535));
+  if (g.mask) SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, true>, grid, dim3(256), 0, s, 1, g));
+  else SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, false>, grid, dim3(256), 0, s, 1, g));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
@@ -219,11 +779,11 @@ int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, in
   LogProbArgs g;
   memset(&g, 0, sizeof(g));
   g.logits = logits; g.ld = ld; g.rows = rows; g.cols = prefix >= 0 ? prefix : cols; g.mask_cols = cols;
-  g.mask = prefix >= 0 ? nullptr : mask; g.scale = scale; g.tokens = tokens; g.out = out; g.entropy = entropy; g.stats = stats;
+  g.mask = prefix >= 0 ? nullptr : mask; g.scale = scale; g.tokens = tokens; g.wide_tokens = index_dtype == SB_I64; g.out = out; g.entropy = entropy; g.stats = stats;
   g.top = top; g.top_values = top_values; g.top_tokens = top_tokens;
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == SB_F32 ? launch_log_probs<float>(g, index_dtype, s)
-         : dtype == SB_BF16 ? launch_log_probs<__nv_bfloat16>(g, index_dtype, s) : launch_log_probs<__half>(g, index_dtype, s);
+  return dtype == SB_F32 ? launch_log_probs<float>(g, s)
+         : dtype == SB_BF16 ? launch_log_probs<__nv_bfloat16>(g, s) : launch_log_probs<__half>(g, s);
 }
 
 int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
@@ -243,11 +803,11 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
   LogProbGradArgs g;
   memset(&g, 0, sizeof(g));
   g.logits = logits; g.ld = ld; g.rows = rows; g.cols = prefix >= 0 ? prefix : cols; g.mask_cols = cols;
-  g.mask = prefix >= 0 ? nullptr : mask; g.scale = scale; g.tokens = tokens; g.stats = stats; g.dout = dout; g.entropy = entropy;
+  g.mask = prefix >= 0 ? nullptr : mask; g.scale = scale; g.tokens = tokens; g.wide_tokens = index_dtype == SB_I64; g.stats = stats; g.dout = dout; g.entropy = entropy;
   g.dentropy = dentropy; g.dlogits = dlogits; g.ldd = ldd;
   cudaStream_t s = (cudaStream_t)stream;
-  return dtype == SB_F32 ? launch_log_probs_grad<float>(g, index_dtype, s)
-         : dtype == SB_BF16 ? launch_log_probs_grad<__nv_bfloat16>(g, index_dtype, s) : launch_log_probs_grad<__half>(g, index_dtype, s);
+  return dtype == SB_F32 ? launch_log_probs_grad<float>(g, s)
+         : dtype == SB_BF16 ? launch_log_probs_grad<__nv_bfloat16>(g, s) : launch_log_probs_grad<__half>(g, s);
 }
 
 }  // extern "C"
