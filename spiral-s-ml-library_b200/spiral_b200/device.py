@@ -273,6 +273,32 @@ def values_ptr(x, n, what):
     return device_ptr(x)
 
 
+def array_ptr(x, n, tag, what):
+    """Address of n contiguous values of the storage type ``tag`` (None -> NULL)."""
+    if x is None:
+        return None
+    if type(x) is not DeviceArray:
+        numel = getattr(x, "numel", None)
+        if numel is not None and numel() == n and _TAG_OF.get(x.dtype) == tag and x.is_contiguous():
+            return x.data_ptr()
+    if dtype_tag(x) != tag or flat_size(x, what) != n:
+        raise ValueError("%s must be %d contiguous %s values" % (what, n, tag))
+    return device_ptr(x)
+
+
+def typed_matrix(x, what):
+    """(rows, cols, pitch, address, storage type) of a row-major device matrix (see ``matrix_of``)."""
+    if type(x) is not DeviceArray:
+        try:                                       # torch, two dimensions
+            rows, cols = x.shape
+            pitch, step = x.stride()
+            if step == 1 and pitch >= cols:
+                return rows, cols, pitch, x.data_ptr(), _TAG_OF[x.dtype]
+        except (AttributeError, KeyError, TypeError, ValueError):
+            pass
+    return matrix_of(x, what) + (device_ptr(x), dtype_tag(x))
+
+
 def keep_tf32(x, stream):
     """An output that has just been written in fp32: one that is tagged 'tf32' is rounded to it, as the other operations leave it."""
     if type(x) is DeviceArray and x.dtype == "tf32":

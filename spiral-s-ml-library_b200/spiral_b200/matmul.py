@@ -7,7 +7,8 @@ updated in place: ``c <- alpha * op(a) @ op(b) + beta * c``.
 import ctypes
 
 from . import _lib
-from .device import Workspaces, device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, nbytes_of, stream_ptr, stream_workspace, values_ptr
+from .device import (Workspaces, array_ptr, device_ptr, dtype_tag, keep_tf32, matrix_of, nbytes_of, stream_ptr, stream_workspace, typed_matrix,
+                     values_ptr)
 
 EPILOGUE_FLAGS = {
     "bias": _lib.EPI_BIAS, "relu": _lib.EPI_RELU, "relu_grad": _lib.EPI_RELU_GRAD,
@@ -222,24 +223,23 @@ _GATED = {"bf16": _lib.BF16, "f16": _lib.F16}
 
 
 def _gated_matrix(who, x, what, tag, rows, cols):
-    """Pitch of a matrix of the layer's storage type and the given shape."""
-    r, c, ld = matrix_of(x, what)
-    if (r, c) != (rows, cols) or dtype_tag(x) != tag:
+    """Address and pitch of a matrix of the layer's storage type and the given shape."""
+    r, c, ld, ptr, own = typed_matrix(x, what)
+    if r != rows or c != cols or own != tag:
         raise ValueError("%s: %s must be %s, %dx%d" % (who, what, tag, rows, cols))
-    return ld
+    return ptr, ld
 
 
 def _gated_sizes(who, x, w, activation):
-    m, k, ldx = matrix_of(x, "x")
-    f2, kw, ldw = matrix_of(w, "w")
-    tag = dtype_tag(x)
+    m, k, ldx, x, tag = typed_matrix(x, "x")
+    f2, kw, ldw, w, w_tag = typed_matrix(w, "w")
     if tag not in _GATED:
         raise TypeError("%s: x must hold bf16 or f16, not %s" % (who, tag))
-    if f2 % 2 or kw != k or dtype_tag(w) != tag:
+    if f2 % 2 or kw != k or w_tag != tag:
         raise ValueError("%s: w must be %s, an even number of rows of %d" % (who, tag, k))
     if activation not in ACTIVATIONS:
         raise ValueError("%s: the activation is one of %s, got %r" % (who, ", ".join(sorted(ACTIVATIONS)), activation))
-    return m, f2 // 2, k, ldx, ldw, tag, ACTIVATIONS[activation]
+    return m, f2 // 2, k, x, ldx, w, ldw, tag, ACTIVATIONS[activation]
 
 
 def gated(x, w, out, activation="silu", saved=None, stream=None):
@@ -248,11 +248,12 @@ def gated(x, w, out, activation="silu", saved=None, stream=None):
     ``x`` [m, k], ``w`` [2 f, k] (the gate's rows, then the other projection's), ``out`` [m, f] in bf16 or f16, one type; rows may have a
     pitch.  ``activation``: "silu", "gelu" (of the normal distribution) or "relu".  ``saved`` [m, 2 f]: where given, both projections are left there for
     ``gated_grad``.  Rows of x and w that start on 16 bytes run on the tensor cores, others on the CUDA cores at about 1 % of their rate."""
-    m, f, k, ldx, ldw, tag, act = _gated_sizes("gated", x, w, activation)
-    ldo = _gated_matrix("gated", out, "out", tag, m, f)
-    lds = _gated_matrix("gated", saved, "saved", tag, m, 2 * f) if saved is not None else 2 * f
-    _lib.call("sb_gated", device_ptr(x), ldx, device_ptr(w), ldw, device_ptr(out), ldo, device_ptr(saved), lds, m, f, k, _GATED[tag], act,
-              stream_ptr(stream))
+    m, f, k, x, ldx, w, ldw, tag, act = _gated_sizes("gated", x, w, activation)
+    h, ldh = _gated_matrix("gated", out, "out", tag, m, f)
+    lds = 2 * f
+    if saved is not None:
+        saved, lds = _gated_matrix("gated", saved, "saved", tag, m, 2 * f)
+    _lib.call("sb_gated", x, ldx, w, ldw, h, ldh, saved, lds, m, f, k, _GATED[tag], act, stream_ptr(stream))
     return out
 
 
@@ -260,20 +261,23 @@ def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulat
     """Gradient of ``gated`` from ``dout`` [m, f] and what it ``saved``: ``dx`` (like ``x``) and ``dw`` (like ``w``, or fp32), each where given;
     ``accumulate`` adds to the old ``dw``.  ``workspace``: device memory of ``gated_grad_workspace`` bytes; by default one is kept per device,
     stream and host thread.  Returns (dx, dw)."""
-    m, f, k, ldx, ldw, tag, act = _gated_sizes("gated_grad", x, w, activation)
-    lddo = _gated_matrix("gated_grad", dout, "dout", tag, m, f)
-    lds = _gated_matrix("gated_grad", saved, "saved", tag, m, 2 * f)
-    lddx = _gated_matrix("gated_grad", dx, "dx", tag, m, k) if dx is not None else k
-    dw_tag = tag if dw is None else dtype_tag(dw)
-    if dw_tag not in (tag, "f32", "tf32"):
-        raise TypeError("gated_grad: dw must hold %s or f32, not %s" % (tag, dw_tag))
-    lddw = _gated_matrix("gated_grad", dw, "dw", dw_tag, 2 * f, k) if dw is not None else k
+    m, f, k, x, ldx, w, ldw, tag, act = _gated_sizes("gated_grad", x, w, activation)
+    dh, lddh = _gated_matrix("gated_grad", dout, "dout", tag, m, f)
+    saved, lds = _gated_matrix("gated_grad", saved, "saved", tag, m, 2 * f)
+    dx_ptr, lddx, dw_ptr, lddw, dw_tag = None, k, None, k, tag
+    if dx is not None:
+        dx_ptr, lddx = _gated_matrix("gated_grad", dx, "dx", tag, m, k)
+    if dw is not None:
+        rows, cols, lddw, dw_ptr, dw_tag = typed_matrix(dw, "dw")
+        if dw_tag not in (tag, "f32", "tf32"):
+            raise TypeError("gated_grad: dw must hold %s or f32, not %s" % (tag, dw_tag))
+        if rows != 2 * f or cols != k:
+            raise ValueError("gated_grad: dw must be like w, %dx%d" % (2 * f, k))
     nbytes = gated_grad_workspace(m, f, k) if workspace is None else nbytes_of(workspace)
     if workspace is None:
         workspace = stream_workspace(nbytes, stream)
-    _lib.call("sb_gated_grad", device_ptr(dout), lddo, device_ptr(x), ldx, device_ptr(w), ldw, device_ptr(saved), lds, device_ptr(dx), lddx,
-              device_ptr(dw), lddw, _GATED.get(dw_tag, _lib.F32), int(bool(accumulate)), m, f, k, _GATED[tag], act, device_ptr(workspace), nbytes,
-              stream_ptr(stream))
+    _lib.call("sb_gated_grad", dh, lddh, x, ldx, w, ldw, saved, lds, dx_ptr, lddx, dw_ptr, lddw, _GATED.get(dw_tag, _lib.F32),
+              int(bool(accumulate)), m, f, k, _GATED[tag], act, device_ptr(workspace), nbytes, stream_ptr(stream))
     return dx, keep_tf32(dw, stream)
 
 
@@ -284,48 +288,44 @@ def gated_grad_workspace(m, f, k):
     return nbytes.value
 
 
-def _int4_sizes(who, codes, scales, k, group):
-    """Rows, pitch and the scales' type of 4-bit weights of k columns."""
-    if dtype_tag(codes) != "u8":
-        raise TypeError("%s: codes must be bytes, not %s" % (who, dtype_tag(codes)))
-    n, nbytes, ldw = matrix_of(codes, "codes")
+def _int4_weights(who, codes, scales, k, group):
+    """Rows, address and pitch of 4-bit weights of k columns, address and type of their scales."""
+    n, nbytes, ldw, codes, tag = typed_matrix(codes, "codes")
+    if tag != "u8":
+        raise TypeError("%s: codes must be bytes, not %s" % (who, tag))
     if group not in (32, 64, 128):
         raise ValueError("%s: groups are of 32, 64 or 128" % who)
     if nbytes != (k + 1) // 2:
         raise ValueError("%s: codes of %d columns are %d bytes a row, got %d" % (who, k, (k + 1) // 2, nbytes))
     tag = dtype_tag(scales)
-    if tag not in _FP8_FLOATS or flat_size(scales, "scales") != -(-k // group) * n:
-        raise ValueError("%s: scales must be %d x %d contiguous f32, bf16 or f16 values" % (who, -(-k // group), n))
-    return n, ldw, _FP8_FLOATS[tag]
+    if tag not in _FP8_FLOATS:
+        raise TypeError("%s: scales must hold f32, bf16 or f16, not %s" % (who, tag))
+    return n, codes, ldw, array_ptr(scales, -(-k // group) * n, tag, "scales"), _FP8_FLOATS[tag]
 
 
 def quantize_int4(x, codes, scales, group=128, stream=None):
     """4-bit ``codes`` (uint8 [n, ceil(k / 2)], two in a byte, the even column in the low half) of the weights ``x`` [n, k] (fp32, bf16,
     f16) with a scale per ``group`` (32, 64, 128) columns of a row: ``scales`` [ceil(k / group), n] in fp32, bf16 or f16, the largest
     magnitude / 7.  A weight is ``scale * (code - 8)``.  Returns (codes, scales)."""
-    rows, k, ldx = matrix_of(x, "x")
-    n, ldc, scale_code = _int4_sizes("quantize_int4", codes, scales, k, group)
-    tag = dtype_tag(x)
+    rows, k, ldx, x, tag = typed_matrix(x, "x")
+    n, codes_ptr, ldc, scales_ptr, scale_code = _int4_weights("quantize_int4", codes, scales, k, group)
     if tag not in _FP8_FLOATS:
         raise TypeError("quantize_int4: x must hold f32, bf16 or f16, not %s" % tag)
     if n != rows:
         raise ValueError("quantize_int4: codes have %d rows, x has %d" % (n, rows))
-    _lib.call("sb_quantize_int4", device_ptr(x), ldx, _FP8_FLOATS[tag], n, k, group, device_ptr(codes), ldc, device_ptr(scales), scale_code,
-              stream_ptr(stream))
+    _lib.call("sb_quantize_int4", x, ldx, _FP8_FLOATS[tag], n, k, group, codes_ptr, ldc, scales_ptr, scale_code, stream_ptr(stream))
     return codes, scales
 
 
 def dequantize_int4(codes, scales, out, group=128, stream=None):
     """The weights [n, k] that 4-bit ``codes`` and ``scales`` stand for, in fp32, bf16 or f16: for products of many rows."""
-    rows, k, ldo = matrix_of(out, "out")
-    n, ldw, scale_code = _int4_sizes("dequantize_int4", codes, scales, k, group)
-    tag = dtype_tag(out)
+    rows, k, ldo, out_ptr, tag = typed_matrix(out, "out")
+    n, codes, ldw, scales, scale_code = _int4_weights("dequantize_int4", codes, scales, k, group)
     if tag not in _FP8_FLOATS:
         raise TypeError("dequantize_int4: out must hold f32, bf16 or f16, not %s" % tag)
     if n != rows:
         raise ValueError("dequantize_int4: codes have %d rows, out has %d" % (n, rows))
-    _lib.call("sb_dequantize_int4", device_ptr(codes), ldw, device_ptr(scales), scale_code, device_ptr(out), ldo, _FP8_FLOATS[tag], n, k, group,
-              stream_ptr(stream))
+    _lib.call("sb_dequantize_int4", codes, ldw, scales, scale_code, out_ptr, ldo, _FP8_FLOATS[tag], n, k, group, stream_ptr(stream))
     return keep_tf32(out, stream)
 
 
@@ -334,14 +334,13 @@ def matmul_int4(a, codes, scales, c, group=128, epilogue=(), bias=None, stream=N
 
     ``a`` [m, k] in bf16 or f16, ``c`` [m, n] in fp32, bf16 or f16, fp32 accumulation; ``epilogue``: "bias" (fp32 [n]), "relu" (a NaN gives 0, as in
     ``matmul``).  Rows may have a pitch.  Made for up to 64 rows; for many, ``dequantize_int4`` and ``matmul`` are faster."""
-    m, k, lda = matrix_of(a, "a")
-    n, ldw, scale_code = _int4_sizes("matmul_int4", codes, scales, k, group)
-    cm, cn, ldc = matrix_of(c, "c")
+    m, k, lda, a, a_tag = typed_matrix(a, "a")
+    n, codes, ldw, scales, scale_code = _int4_weights("matmul_int4", codes, scales, k, group)
+    cm, cn, ldc, c_ptr, tag = typed_matrix(c, "c")
     if cm != m or cn != n:
         raise ValueError("shape mismatch: a is %dx%d, w^T is %dx%d, c is %dx%d" % (m, k, k, n, cm, cn))
-    if dtype_tag(a) not in _GATED:
-        raise TypeError("matmul_int4: a must hold bf16 or f16, not %s" % dtype_tag(a))
-    tag = dtype_tag(c)
+    if a_tag not in _GATED:
+        raise TypeError("matmul_int4: a must hold bf16 or f16, not %s" % a_tag)
     if tag not in _FP8_FLOATS:
         raise TypeError("matmul_int4: c must hold f32, bf16 or f16, not %s" % tag)
     epi = _FP8_EPILOGUES.get(tuple(epilogue))
@@ -349,6 +348,6 @@ def matmul_int4(a, codes, scales, c, group=128, epilogue=(), bias=None, stream=N
         raise ValueError("matmul_int4: the epilogue is made of bias and relu, got %r" % (epilogue,))
     if epi & _lib.EPI_BIAS and bias is None:
         raise ValueError("matmul_int4: bias must be %d fp32 values" % n)
-    _lib.call("sb_matmul_int4", device_ptr(a), lda, _GATED[dtype_tag(a)], device_ptr(codes), ldw, device_ptr(scales), scale_code, device_ptr(c), ldc,
-              m, n, k, group, _FP8_FLOATS[tag], epi, values_ptr(bias, n, "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
+    _lib.call("sb_matmul_int4", a, lda, _GATED[a_tag], codes, ldw, scales, scale_code, c_ptr, ldc, m, n, k, group, _FP8_FLOATS[tag], epi,
+              array_ptr(bias, n, "f32", "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
     return keep_tf32(c, stream)

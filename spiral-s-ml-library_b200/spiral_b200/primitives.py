@@ -4,7 +4,8 @@ probabilities of its answers behind them)."""
 import ctypes
 
 from . import _lib
-from .device import device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, nbytes_of, stream_ptr, stream_workspace, values_ptr
+from .device import (array_ptr, device_ptr, dtype_tag, flat_size, keep_tf32, matrix_of, nbytes_of, stream_ptr, stream_workspace,
+                     typed_matrix, values_ptr)
 
 
 def _rows_cols(x):
@@ -236,19 +237,30 @@ def layer_norm_grad_workspace(rows, cols):
     return nbytes.value
 
 
-def _row_args(who, logits, tokens, mask, prefix):
-    """What ``log_probs`` and its gradient share: (rows, cols, pitch, type, mask, prefix, tokens, their type)."""
-    rows, cols, ld = matrix_of(logits, "logits")
-    code = _code(logits, "logits")
+def _row_args(who, logits, tokens, mask):
+    """What ``log_probs`` and its gradient share: (address, rows, cols, pitch, type), the mask, the tokens and their type."""
+    rows, cols, ld, ptr, tag = typed_matrix(logits, "logits")
+    code = _FLOATS.get(tag)
+    if code is None:
+        raise TypeError("logits must hold %s, not %s" % (" / ".join(_FLOATS), tag))
     if mask is not None:
-        if dtype_tag(mask) != "u8" or flat_size(mask, "mask") != rows * cols:
-            raise ValueError("%s: mask must be %dx%d contiguous bytes" % (who, rows, cols))
+        mask = array_ptr(mask, rows * cols, "u8", "mask")
     index = _lib.I32
     if tokens is not None:
-        index = _code(tokens, "tokens", _INDICES)
-        if flat_size(tokens, "tokens") != rows:
-            raise ValueError("%s: %d tokens for %d rows" % (who, flat_size(tokens, "tokens"), rows))
-    return rows, cols, ld, code, device_ptr(mask), int(prefix), device_ptr(tokens), index
+        tag = dtype_tag(tokens)
+        index = _INDICES.get(tag)
+        if index is None:
+            raise TypeError("tokens must hold %s, not %s" % (" / ".join(_INDICES), tag))
+        tokens = array_ptr(tokens, rows, tag, "tokens")
+    return ptr, rows, cols, ld, code, mask, tokens, index
+
+
+def _places(who, x, rows, n, tag, what):
+    """Alternatives per row of a matrix that takes them; `n` is that of the other one, if there is one."""
+    shape = x.shape
+    if len(shape) != 2 or shape[0] != rows or (n is not None and shape[1] != n):
+        raise ValueError("%s: %s must be [%d, %s], got %s" % (who, what, rows, "n" if n is None else n, tuple(shape)))
+    return int(shape[1]), array_ptr(x, rows * shape[1], tag, what)
 
 
 def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None, top_tokens=None, mask=None, prefix=-1, scale=1.0,
@@ -262,21 +274,16 @@ def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None,
     logarithm of the sum over it, for ``log_probs_grad``), ``top`` fp32 and ``top_tokens`` int32 [rows, n], n at most 64: the log
     probabilities and columns of the largest logits, equal ones in the order of their columns, -inf and -1 beyond the legal
     ones.  ``scale`` is one over the temperature.  Returns ``out``."""
-    rows, cols, ld, code, mask, prefix, tokens, index = _row_args("log_probs", logits, tokens, mask, prefix)
-    n = 0
-    if top is not None or top_tokens is not None:
-        for x, tag, what in ((top, "f32", "top"), (top_tokens, "i32", "top_tokens")):
-            if x is None:
-                continue
-            if dtype_tag(x) != tag or len(x.shape) != 2 or int(x.shape[0]) != rows:
-                raise ValueError("log_probs: %s must be %s [%d, n]" % (what, tag, rows))
-            if rows > 0 and flat_size(x, what) != rows * int(x.shape[1]) or (n and int(x.shape[1]) != n):
-                raise ValueError("log_probs: top and top_tokens must be of one shape")
-            n = int(x.shape[1])
-    if n == 0:
-        top = top_tokens = None
-    _lib.call("sb_log_probs", device_ptr(logits), ld, code, rows, cols, mask, prefix, scale, tokens, index, values_ptr(out, rows, "out"),
-              values_ptr(entropy, rows, "entropy"), values_ptr(stats, 2 * rows, "stats"), n, device_ptr(top), device_ptr(top_tokens),
+    ptr, rows, cols, ld, code, mask, tokens, index = _row_args("log_probs", logits, tokens, mask)
+    n = None
+    if top is not None:
+        n, top = _places("log_probs", top, rows, n, "f32", "top")
+    if top_tokens is not None:
+        n, top_tokens = _places("log_probs", top_tokens, rows, n, "i32", "top_tokens")
+    if not n:
+        n, top, top_tokens = 0, None, None
+    _lib.call("sb_log_probs", ptr, ld, code, rows, cols, mask, prefix, scale, tokens, index, array_ptr(out, rows, "f32", "out"),
+              array_ptr(entropy, rows, "f32", "entropy"), array_ptr(stats, 2 * rows, "f32", "stats"), n, top, top_tokens,
               stream_ptr(stream))
     return out
 
@@ -285,11 +292,11 @@ def log_probs_grad(logits, tokens, stats, dlogits, dout=None, dentropy=None, ent
     """Gradient of ``log_probs``: ``dlogits`` (like ``logits``, and may be them) from ``dout`` and ``dentropy``, the gradients of
     ``out`` and ``entropy`` (fp32 [rows], None: none), with the ``stats`` and, for ``dentropy``, the ``entropy`` that the forward call
     left.  Zero in columns that are not legal; a row without a token gets no ``dout``.  None flows through the alternatives."""
-    rows, cols, ld, code, mask, prefix, tokens, index = _row_args("log_probs_grad", logits, tokens, mask, prefix)
-    drows, dcols, ldd = matrix_of(dlogits, "dlogits")
-    if drows != rows or dcols != cols or _code(dlogits, "dlogits") != code:
+    ptr, rows, cols, ld, code, mask, tokens, index = _row_args("log_probs_grad", logits, tokens, mask)
+    drows, dcols, ldd, dptr, dtag = typed_matrix(dlogits, "dlogits")
+    if drows != rows or dcols != cols or _FLOATS.get(dtag) != code:
         raise ValueError("log_probs_grad: dlogits must be like logits, %dx%d" % (rows, cols))
-    _lib.call("sb_log_probs_grad", device_ptr(logits), ld, code, rows, cols, mask, prefix, scale, tokens, index, values_ptr(stats, 2 * rows, "stats"),
-              values_ptr(dout, rows, "dout"), values_ptr(entropy, rows, "entropy"), values_ptr(dentropy, rows, "dentropy"),
-              device_ptr(dlogits), ldd, stream_ptr(stream))
+    _lib.call("sb_log_probs_grad", ptr, ld, code, rows, cols, mask, prefix, scale, tokens, index, array_ptr(stats, 2 * rows, "f32", "stats"),
+              array_ptr(dout, rows, "f32", "dout"), array_ptr(entropy, rows, "f32", "entropy"), array_ptr(dentropy, rows, "f32", "dentropy"),
+              dptr, ldd, stream_ptr(stream))
     return keep_tf32(dlogits, stream)
