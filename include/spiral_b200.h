@@ -583,8 +583,8 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
                   int activation, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Weights in 4 bits with a scale per group of 32, 64 or 128 along a row: w[n, k] = scales[k / group, n] * (q - 8).  codes: uint8 [n,
- * ceil(k / 2)], two in a byte, the even column in the low half (the high half behind an odd k holds 8); scales [ceil(k / group), n] in SB_F32, SB_BF16 or
- * SB_F16.  Quantising: scale = largest magnitude / 7, rounded to its type, q = x / scale rounded to nearest even, kept in 0 .. 15.  A
+ * ceil(k / 2)], two in a byte, the even column in the low half (the high half behind an odd k holds 8); scales [ceil(k / group), n] in SB_BF16 or SB_F16.
+ * Quantising: scale = largest magnitude / 7, rounded to its type, q = x / scale rounded to nearest even, kept in 0 .. 15.  A
  * group that holds a NaN or an infinity has no meaning; one whose scale rounds to zero is zero. */
 int sb_quantize_int4(const void* x, long long ldx, int dtype, long long n, int k, int group, uint8_t* codes, long long ldc, void* scales,
                      int scale_dtype, void* stream);

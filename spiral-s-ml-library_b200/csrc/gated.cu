@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
 // Up to 8 NT rows: a block has 16 columns of h, 16 rows of each half of w, and its eight warps share K, UNROLL blocks of 32 on their way at a
 // time.  Their sums are joined in the order of the warps.
 constexpr int GF_ROWS = 16, GF_WARPS = 8;
+constexpr long long GF_NO_END = 1LL << 60;
 
 template <typename T, int ACT, int NT>
 __global__ void __launch_bounds__(32 * GF_WARPS) gated_few_kernel(GatedArgs p) {
@@ -436,14 +437,25 @@ __global__ void __launch_bounds__(32 * GF_WARPS) gated_few_kernel(GatedArgs p) {
       for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.f;
   for (int k0 = warp * 32 * UNROLL; k0 < p.k; k0 += GF_WARPS * 32 * UNROLL) {
     uint4 a[UNROLL][4], b[UNROLL][NT];
+    if (k0 + 32 * UNROLL <= p.k) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+      for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[u][i] = load_eight<false>(rows[i], k0 + 32 * u + 8 * t, p.k, true);
+        for (int i = 0; i < 4; ++i) a[u][i] = load_eight<false>(rows[i], k0 + 32 * u + 8 * t, GF_NO_END, true);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
+      for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) b[u][n] = load_eight<true>(x + (long long)(n0 + 8 * n + g) * p.ldx, k0 + 32 * u + 8 * t, p.k, n0 + 8 * n + g < p.m);
+        for (int n = 0; n < NT; ++n) b[u][n] = load_eight<true>(x + (long long)(n0 + 8 * n + g) * p.ldx, k0 + 32 * u + 8 * t, GF_NO_END, n0 + 8 * n + g < p.m);
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[u][i] = load_eight<false>(rows[i], k0 + 32 * u + 8 * t, p.k, true);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) b[u][n] = load_eight<true>(x + (long long)(n0 + 8 * n + g) * p.ldx, k0 + 32 * u + 8 * t, p.k, n0 + 8 * n + g < p.m);
+    }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll

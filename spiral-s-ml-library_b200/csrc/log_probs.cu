@@ -250,7 +250,33 @@ __device__ __forceinline__ uint32_t lp_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// An order of alternatives: by their logits (zeros of both signs are equal), the lower column first.
+__device__ __forceinline__ unsigned long long lp_place(float x, int column) {
+  return (unsigned long long)lp_key(x + 0.f) << 32 | (uint32_t)~column;
+}
+__device__ __forceinline__ float lp_place_logit(unsigned long long place) {
+  const uint32_t key = (uint32_t)(place >> 32);
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ int lp_place_column(unsigned long long place) { return (int)~(uint32_t)place; }
+
 constexpr int LP_CANDIDATES = 512;
+// The `top` best of n candidates in their order: each counts those before it. 
+__device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, unsigned long long* best, int top, int threads) {
+  for (int i = threadIdx.x; i < n; i += threads) {
+    const unsigned long long mine = candidates[i];
+    int before = 0, k = 0;
+    for (; k + 8 <= n; k += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; u += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(candidates + k + u);
+        before += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+      }
+    }
+    for (; k < n; ++k) before += candidates[k] > mine ? 1 : 0;
+    if (before < top) best[before] = mine;
+  }
+}
 
 // Longer rows: a block per row, or a cluster of blocks that share one, in one pass over memory.  Each thread keeps its own
 // sums and raises their reference when a batch of packs brings a larger logit.
@@ -265,10 +291,8 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
   __shared__ RowSums whole;                      // of this block's share
   __shared__ float largest[NT];
   __shared__ int hot[NT];
-  __shared__ float value[LP_CANDIDATES];
-  __shared__ int column[LP_CANDIDATES];
-  __shared__ float best_value[LP_MAX_TOP];
-  __shared__ int best_column[LP_MAX_TOP];
+  __shared__ __align__(16) unsigned long long candidates[LP_CANDIDATES];
+  __shared__ unsigned long long best[LP_MAX_TOP];      // 0: none
   __shared__ int hot_count, candidate_count;
   __shared__ float bound;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -354,10 +378,18 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
     if (g.top > 0) {
       if (warp == WARPS - 1) {
         // Bit by bit the largest key that `top` of the threads reach; near it is near enough.
-        uint32_t keys[NT / 32], key = 0u;
+        uint32_t keys[NT / 32], low = 0xffffffffu, high = 0u;
 #pragma unroll
-        for (int i = 0; i < NT / 32; ++i) keys[i] = lp_key(largest[lane + 32 * i]);
-        for (int bit = 31; bit >= 0; --bit) {
+        for (int i = 0; i < NT / 32; ++i) {
+          keys[i] = lp_key(largest[lane + 32 * i]);
+          low = min(low, keys[i]);
+          high = max(high, keys[i]);
+        }
+        low = __reduce_min_sync(0xffffffffu, low);
+        high = __reduce_max_sync(0xffffffffu, high);
+        const int alike = __clz((int)(low ^ high));    // leading bits that all keys share: 32 where they are equal
+        uint32_t key = alike == 32 ? low : low & ~(0xffffffffu >> alike);
+        for (int bit = 31 - alike; bit >= 0; --bit) {
           const uint32_t tried = key | 1u << bit;
           int reach = 0;
 #pragma unroll
@@ -384,10 +416,7 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
         auto candidate = [&](float v, int j) {
           if (v >= least && v > -INFINITY) {
             const int at = atomicAdd(&candidate_count, 1);
-            if (at < LP_CANDIDATES) {
-              value[at] = v;
-              column[at] = j;
-            }
+            if (at < LP_CANDIDATES) candidates[at] = lp_place(v, j);
           }
         };
         if (k == each - 1) {
@@ -407,69 +436,41 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
           }
         }
       }
-      if (tid < LP_MAX_TOP) best_column[tid] = -1;
+      if (tid < LP_MAX_TOP) best[tid] = 0ull;
       __syncthreads();
       const int n = candidate_count;
       if (n <= LP_CANDIDATES) {
-        for (int i = tid; i < n; i += NT) {
-          const float v = value[i];
-          const int j = column[i];
-          int before = 0;
-          for (int k = 0; k < n; ++k) before += value[k] > v || (value[k] == v && column[k] < j) ? 1 : 0;
-          if (before < g.top) {
-            best_value[before] = v;
-            best_column[before] = j;
-          }
-        }
+        lp_rank(candidates, n, best, g.top, NT);
         __syncthreads();
       } else {
-        float last = INFINITY;
-        int last_at = -1;
+        unsigned long long last = ~0ull;
         for (int i = 0; i < g.top; ++i) {
-          float v = -INFINITY;
-          int j = 0x7fffffff;
-          auto look = [&](float a, int at) {
-            if ((a < last || (a == last && at > last_at)) && (a > v || (a == v && at < j)) && a > -INFINITY) {
-              v = a;
-              j = at;
-            }
+          unsigned long long next = 0ull;
+          auto look = [&](float v, int j) {
+            const unsigned long long place = lp_place(v, j);
+            if (v > -INFINITY && place < last && place > next) next = place;
           };
           if (first < singles) look(lp_logit<T>(x, mask, shape.single(first)), shape.single(first));
           for (int p = first; p < shape.packs; p += stride) {
             SbWords<16> w;
             sb_load_words(w, x + shape.column(p), true);
-            float a[V];
-            sb_unpack_words<T, V>(w, a);
-            if (MASKED) lp_mask_pack<T>(a, mask + shape.column(p));
+            float v[V];
+            sb_unpack_words<T, V>(w, v);
+            if (MASKED) lp_mask_pack<T>(v, mask + shape.column(p));
 #pragma unroll
-            for (int e = 0; e < V; ++e) look(a[e], shape.column(p) + e);
+            for (int e = 0; e < V; ++e) look(v[e], shape.column(p) + e);
           }
 #pragma unroll
           for (int o = 16; o; o >>= 1) {
-            const float w = __shfl_xor_sync(0xffffffffu, v, o);
-            const int k = __shfl_xor_sync(0xffffffffu, j, o);
-            if (w > v || (w == v && k < j)) {
-              v = w;
-              j = k;
-            }
+            const unsigned long long other = __shfl_xor_sync(0xffffffffu, next, o);
+            next = other > next ? other : next;
           }
           __syncthreads();
-          if (lane == 0) {
-            value[warp] = v;
-            column[warp] = j;
-          }
+          if (lane == 0) candidates[warp] = next;
           __syncthreads();
-          for (int w = 0; w < WARPS; ++w)
-            if (value[w] > v || (value[w] == v && column[w] < j)) {
-              v = value[w];
-              j = column[w];
-            }
-          if (tid == 0 && j != 0x7fffffff) {
-            best_value[i] = v;
-            best_column[i] = j;
-          }
-          last = v;
-          last_at = j;
+          for (int w = 0; w < WARPS; ++w) next = candidates[w] > next ? candidates[w] : next;
+          if (tid == 0) best[i] = next;
+          last = next;
         }
         __syncthreads();
       }
@@ -504,34 +505,18 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
           all.dist += parts[b].dist;
         }
         for (int i = tid; i < blocks * g.top; i += NT) {
-          const uint32_t b = (uint32_t)(i / g.top), k = (uint32_t)(i % g.top);
-          float v = 0.f;
-          int j;
-          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(j) : "r"(map_to_cta(smem_u32(&best_column[k]), b)) : "memory");
-          if (j >= 0) {
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(smem_u32(&best_value[k]), b)) : "memory");
-            const int at = atomicAdd(&candidate_count, 1);
-            value[at] = v;
-            column[at] = j;
-          }
+          unsigned long long place;
+          asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(place) : "r"(map_to_cta(smem_u32(&best[i % g.top]), (uint32_t)(i / g.top))) : "memory");
+          if (place != 0ull) candidates[atomicAdd(&candidate_count, 1)] = place;
         }
         __syncwarp();
       }
       cluster_sync_all();                        // the others may go on
       if (rank == 0 && g.top > 0) {
         const int n = candidate_count;
-        if (tid < LP_MAX_TOP) best_column[tid] = -1;
+        if (tid < LP_MAX_TOP) best[tid] = 0ull;
         __syncthreads();
-        for (int i = tid; i < n; i += NT) {
-          const float v = value[i];
-          const int j = column[i];
-          int before = 0;
-          for (int k = 0; k < n; ++k) before += value[k] > v || (value[k] == v && column[k] < j) ? 1 : 0;
-          if (before < g.top) {
-            best_value[before] = v;
-            best_column[before] = j;
-          }
-        }
+        lp_rank(candidates, n, best, g.top, NT);
         __syncthreads();
       }
     }
@@ -541,7 +526,7 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
         const long long token = g.out ? lp_token(g.tokens, g.wide_tokens, row) : -1;
         lp_finish(g, row, all, log_sum, token >= 0 && token < g.cols ? lp_logit<T>(x, mask, (int)token) : 0.f, token);
       }
-      if (tid < g.top) lp_alternative(g, row, tid, best_value[tid], best_column[tid], all.top, log_sum);
+      if (tid < g.top) lp_alternative(g, row, tid, lp_place_logit(best[tid]), best[tid] == 0ull ? -1 : lp_place_column(best[tid]), all.top, log_sum);
     }
   }
 }

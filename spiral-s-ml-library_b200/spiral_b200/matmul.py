@@ -298,14 +298,14 @@ def _int4_weights(who, codes, scales, k, group):
     if nbytes != (k + 1) // 2:
         raise ValueError("%s: codes of %d columns are %d bytes a row, got %d" % (who, k, (k + 1) // 2, nbytes))
     tag = dtype_tag(scales)
-    if tag not in _FP8_FLOATS:
-        raise TypeError("%s: scales must hold f32, bf16 or f16, not %s" % (who, tag))
-    return n, codes, ldw, array_ptr(scales, -(-k // group) * n, tag, "scales"), _FP8_FLOATS[tag]
+    if tag not in _GATED:
+        raise TypeError("%s: scales must hold bf16 or f16, not %s" % (who, tag))
+    return n, codes, ldw, array_ptr(scales, -(-k // group) * n, tag, "scales"), _GATED[tag]
 
 
 def quantize_int4(x, codes, scales, group=128, stream=None):
     """4-bit ``codes`` (uint8 [n, ceil(k / 2)], two in a byte, the even column in the low half) of the weights ``x`` [n, k] (fp32, bf16,
-    f16) with a scale per ``group`` (32, 64, 128) columns of a row: ``scales`` [ceil(k / group), n] in fp32, bf16 or f16, the largest
+    f16) with a scale per ``group`` (32, 64, 128) columns of a row: ``scales`` [ceil(k / group), n] in bf16 or f16, the largest
     magnitude / 7.  A weight is ``scale * (code - 8)``.  Returns (codes, scales)."""
     rows, k, ldx, x, tag = typed_matrix(x, "x")
     n, codes_ptr, ldc, scales_ptr, scale_code = _int4_weights("quantize_int4", codes, scales, k, group)

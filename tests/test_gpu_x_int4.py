@@ -49,6 +49,13 @@ def check(gpu, a, codes, scales, group, out_type, epilogue=(), bias=None, c=None
     torch.cuda.synchronize()
     assert gpu.matmul_int4(a, codes, scales, c, group=group, epilogue=epilogue, bias=bias, stream=stream) is c
     torch.cuda.synchronize()
+    return compare(c, a, codes, scales, group, out_type, epilogue, bias)
+
+
+def compare(c, a, codes, scales, group, out_type, epilogue=(), bias=None):
+    """A product against the definition."""
+    torch = _torch()
+    k = a.shape[1]
     w = values(codes, scales, k, group)
     y, mag = a.double() @ w.t(), a.double().abs() @ w.abs().t()
     if "bias" in epilogue:
@@ -67,7 +74,7 @@ def rows(m, k, dtype, seed=1):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("scale_type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale_type", ["bf16", "f16"])
 @pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 33, 32), (5, 64, 64), (130, 200, 64), (64, 257, 128), (100, 1024, 128)])
 def test_quantize_and_back(gpu, n, k, group, scale_type, dtype):
     torch = _torch()
@@ -107,7 +114,7 @@ def test_product(gpu, m, n, k, group, dtype):
     check(gpu, a, codes, scales, group, "f32", ("bias", "relu"), bias)
 
 
-@pytest.mark.parametrize("scale_type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale_type", ["bf16", "f16"])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_types(gpu, dtype, scale_type):
     torch = _torch()
@@ -157,7 +164,7 @@ def test_nothing(gpu, m, n, k):
 def test_values_far_apart(gpu):
     """f16 rows near the type's ends: code differences times values stay finite in the products."""
     torch = _torch()
-    codes, scales = weights(64, 256, 64, "f32")
+    codes, scales = weights(64, 256, 64, "f16")
     a = rows(4, 256, "f16") * 1000
     a[0] = 65504.0
     a[1] = 2.0 ** -24
@@ -190,8 +197,8 @@ def test_places_beyond_32_bits(gpu):
     c = torch.zeros((2, n), device="cuda")
     gpu.matmul_int4(a, codes, scales, c, group=group)
     torch.cuda.synchronize()
-    last = check(gpu, a, codes[-64:], scales[:, -64:].contiguous(), group, "f32")
-    assert torch.equal(c[:, -64:], last)
+    compare(c[:, :64], a, codes[:64], scales[:, :64], group, "f32")
+    compare(c[:, -64:], a, codes[-64:], scales[:, -64:], group, "f32")
 
 
 def test_streams_graphs_and_bits(gpu):

@@ -136,7 +136,7 @@ def test_gated_arrays(sb):
 
 
 def test_int4(sb):
-    def quantize(x=0x1000, ldx=64, dt=0, n=4, k=64, group=32, codes=0x2000, ldc=32, scales=0x3000, st=0):
+    def quantize(x=0x1000, ldx=64, dt=0, n=4, k=64, group=32, codes=0x2000, ldc=32, scales=0x3000, st=2):
         return ("sb_quantize_int4", x, ldx, dt, n, k, group, codes, ldc, scales, st, None)
     refused(sb, BAD, *quantize(x=None))
     refused(sb, BAD, *quantize(n=-1))
@@ -144,8 +144,8 @@ def test_int4(sb):
     refused(sb, BAD, *quantize(ldx=63))
     refused(sb, UNSUPPORTED, *quantize(group=16))
     refused(sb, UNSUPPORTED, *quantize(dt=7))
-    refused(sb, UNSUPPORTED, *quantize(st=4))
-    refused(sb, MISALIGNED, *quantize(scales=0x3002))
+    refused(sb, UNSUPPORTED, *quantize(st=0))
+    refused(sb, MISALIGNED, *quantize(scales=0x3001))
     refused(sb, LARGE, *quantize(n=1 << 31))
 
     def dequantize(codes=0x1000, ldw=32, scales=0x2000, st=2, out=0x3000, ldo=64, ot=2, n=4, k=64, group=64):
