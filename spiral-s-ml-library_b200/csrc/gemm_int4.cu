@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint8_t* cod
   }
 }
 
-__device__ __forceinline__ void int4_store(const Int4Args& p, long long row, int col, float v) {
-  if (p.bias) v += p.bias[col];
+__device__ __forceinline__ void int4_store(const Int4Args& p, long long row, int col, float v, float bias) {
+  v += bias;
   if (p.relu) v = fmaxf(v, 0.f);
   const long long at = row * p.ldc + col;
   if (p.out_dtype == SB_F32) reinterpret_cast<float*>(p.c)[at] = v;
@@ -87,217 +87,286 @@ __device__ __forceinline__ void int4_store(const Int4Args& p, long long row, int
   else reinterpret_cast<__half*>(p.c)[at] = __float2half_rn(v);
 }
 
+// (w & mask) | bits as one instruction.
+__device__ __forceinline__ uint32_t int4_pick(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
 // Eight codes as four pairs of 16-bit numbers q - 8, (0, 4), (1, 5), (2, 6), (3, 7): with the bits of 1024 (f16) or 128 (bf16) above them a
-// code is the number 1024 + q or 128 + q, from which 1032 or 136 is taken without rounding.
+// code is the number 1024 + q or 128 + q, from which 1032 or 136 is taken without rounding.  Four bits further up, where f16 has room for
+// them, it is 1024 + 16 q.
 template <typename T>
 __device__ __forceinline__ void int4_pairs(uint32_t w, uint32_t* out) {
-  constexpr bool HALF = std::is_same<T, __half>::value;
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 up = __floats2half2_rn(0.0625f, 0.0625f), low = __floats2half2_rn(-1032.f, -1032.f), high = __floats2half2_rn(-72.f, -72.f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | (HALF ? 0x64006400u : 0x43004300u);
-    if (HALF) {
-      const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __floats2half2_rn(1032.f, 1032.f));
-      memcpy(&out[i], &r, 4);
-    } else {
-      const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
-      memcpy(&out[i], &r, 4);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t a = int4_pick(w, 0x000f000fu, 0x64006400u), b = int4_pick(w, 0x00f000f0u, 0x64006400u);
+      const __half2 c = __hadd2(*reinterpret_cast<const __half2*>(&a), low), d = __hfma2(*reinterpret_cast<const __half2*>(&b), up, high);
+      memcpy(&out[2 * i], &c, 4);
+      memcpy(&out[2 * i + 1], &d, 4);
+      w >>= 8;
+    }
+  } else {
+    const __nv_bfloat162 low = __floats2bfloat162_rn(-136.f, -136.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = int4_pick(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const __nv_bfloat162 c = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), low);
+      memcpy(&out[i], &c, 4);
     }
   }
 }
 
-constexpr int I4_WARPS = 8;
 struct Int4Few {
-  int whole_words;               // codes can be read by the words of a lane
+  int code_piece;                // bytes of a row of codes that are copied at a time: 16, 8, 4, or 1 where rows start anywhere
   int whole_rows;                // rows of a start on 16 bytes
   int scale_dtype;
   int blocks;                    // of a cluster
+  int range;                     // columns of a block, whole steps
+  int chunk;                     // of them, those that shared memory holds of a at a time
+  int sums_at;                   // where in shared memory the other blocks' sums go
 };
 
 // A scale from its 16 bits.
-__device__ __forceinline__ float int4_scale(SbWords<2> s, int dtype) {
-  const float half = __half2float(__ushort_as_half(s.v));
-  return dtype == SB_BF16 ? __uint_as_float((uint32_t)s.v << 16) : half;
+__device__ __forceinline__ float int4_scale(uint32_t bits, int dtype) {
+  const float half = __half2float(__ushort_as_half((unsigned short)bits));
+  return dtype == SB_BF16 ? __uint_as_float(bits << 16) : half;
 }
 
-// V words (8 codes each) from column k0 on, byte by byte; what lies beyond k holds anything, since the rows of a are zero there.
-template <int V>
-__device__ __forceinline__ void int4_bytes(uint32_t* out, const uint8_t* row, int k0, int k) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    uint32_t word = 0u;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int at = k0 + 8 * v + 2 * b;
-      if (at < k) word |= (uint32_t)row[at / 2] << (8 * b);
-    }
-    out[v] = word;
-  }
+// N bytes, of which `there` are read and the others zero.
+template <int N>
+__device__ __forceinline__ void int4_copy(uint32_t to, const void* from, int there) {
+  if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(there) : "memory");
 }
-// Eight elements of a row of a one by one, zeros beyond k.
-template <typename T>
-__device__ __forceinline__ uint4 int4_eight(const T* row, int k0, int k) {
+// Eight elements of a row one by one, `there` of them.
+__device__ __noinline__ uint4 int4_elements(const uint16_t* from, int there) {
   uint32_t v[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (k0 + i < k) v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[k0 + i] << (16 * (i % 2));
+    if (i < there) v[i / 2] |= (uint32_t)from[i] << (16 * (i % 2));
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// A block has 16 RT rows of w and up to 8 NT rows of a; its warps take groups in turn, UNROLL of them on their way at a time, and the blocks
-// of a cluster share K.  The codes of a lane (32 / 4 = 8 per word) are of one group in all four lanes of a row, so the products of a word
-// are summed as whole numbers times elements of a and scaled as sums.  All partial sums are joined in a fixed order.
-template <typename T, int G, int NT, int RT>
-__global__ void __launch_bounds__(32 * I4_WARPS, NT <= 4 ? 2 : 1) gemm_int4_kernel(Int4Args p, Int4Few q) {
-  constexpr int V = G / 32, UNROLL = RT == 1 ? (V == 1 ? 8 : 4) : V == 1 ? 2 : 1, ROWS = 16 * RT, COLS = 8 * NT, PITCH = COLS + 1;
-  extern __shared__ float i4_smem[];
-  float* part = i4_smem;                               // [warps][16][PITCH]
-  float* sums = i4_smem + I4_WARPS * 16 * PITCH;       // [ROWS][PITCH], this block's
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int blocks = q.blocks, rank = blockIdx.x % blocks;
-  const int r0 = blockIdx.x / blocks * ROWS, n0 = blockIdx.y * COLS;
-  sb_grid_dependency_wait();
-  sb_grid_dependents_launch();
-  const T* a = reinterpret_cast<const T*>(p.a);
-  const bool whole_words = q.whole_words != 0, whole_rows = q.whole_rows != 0;
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[r][n][j] = 0.f;
-  const int groups = (p.k + G - 1) / G;
-  for (int b0 = rank + blocks * warp; b0 < groups; b0 += blocks * I4_WARPS * UNROLL) {
-    SbWords<4 * V> words[UNROLL][RT][2];
-    SbWords<2> raw[UNROLL][RT][2];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int b = b0 + u * blocks * I4_WARPS;
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = r0 + 16 * r + g + 8 * h;
-          const bool there = b < groups && row < p.n;
-          memset(&words[u][r][h], 0, 4 * V);
-          sb_load_words(words[u][r][h], p.codes + (long long)(there ? row : 0) * p.ldw + (b * G + 8 * V * t) / 2, there && whole_words && (b + 1) * G <= p.k);
-          raw[u][r][h].v = 0;
-          sb_load_kept(raw[u][r][h], reinterpret_cast<const uint16_t*>(p.scales) + (there ? (long long)b * p.n + row : 0), there);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int b = b0 + u * blocks * I4_WARPS;
-      if (b >= groups) break;
-      const bool whole = (b + 1) * G <= p.k;
-      if (!whole_words || !whole) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = r0 + 16 * r + g + 8 * h;
-            uint32_t w[V];
-            if (row < p.n) {
-              int4_bytes<V>(w, p.codes + (long long)row * p.ldw, b * G + 8 * V * t, p.k);
-              memcpy(&words[u][r][h], w, 4 * V);
-            }
-          }
-      }
-      float scale[RT][2];
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) scale[r][h] = int4_scale(raw[u][r][h], q.scale_dtype);
-      // Words of a at a time: all of a group's where there is room for them.
-      constexpr int AHEAD = NT * V <= 4 ? V : 1;
-#pragma unroll
-      for (int v0 = 0; v0 < V; v0 += AHEAD) {
-        SbWords<16> x[AHEAD][NT];
-        if (whole_rows && whole) {
-#pragma unroll
-          for (int v = 0; v < AHEAD; ++v)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int row = n0 + 8 * n + g;
-              x[v][n].v = make_uint4(0u, 0u, 0u, 0u);
-              sb_load_kept(x[v][n], a + (long long)row * p.lda + b * G + 8 * (V * t + v0 + v), row < p.m);
-            }
-        } else {
-#pragma unroll
-          for (int v = 0; v < AHEAD; ++v)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int row = n0 + 8 * n + g;
-              x[v][n].v = row < p.m ? int4_eight<T>(a + (long long)row * p.lda, b * G + 8 * (V * t + v0 + v), p.k) : make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < AHEAD; ++v) {
-          uint32_t w[RT][2][4];
-#pragma unroll
-          for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t codes[V];
-              memcpy(codes, &words[u][r][h], 4 * V);
-              int4_pairs<T>(codes[v0 + v], w[r][h]);
-            }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 e = x[v][n].v;
-            const uint32_t x04 = __byte_perm(e.x, e.z, 0x5410), x15 = __byte_perm(e.x, e.z, 0x7632), x26 = __byte_perm(e.y, e.w, 0x5410),
-                           x37 = __byte_perm(e.y, e.w, 0x7632);
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_16x8x16<T>(c, w[r][0][0], w[r][1][0], w[r][0][1], w[r][1][1], x04, x15);
-              mma_16x8x16<T>(c, w[r][0][2], w[r][1][2], w[r][0][3], w[r][1][3], x26, x37);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[r][n][j] = fmaf(scale[r][j >> 1], c[j], acc[r][n][j]);
-            }
-          }
-        }
-      }
+template <int NT>
+constexpr int int4_chunk = NT <= 2 ? 1024 : 2048 / NT;          // columns of a that shared memory holds at most
+constexpr int I4_STEP = 256;                            // columns of a stage: 128 bytes of codes a row
+constexpr int I4_STAGE = 16 * I4_STEP / 2;
+// Where 16 bytes of a row of codes lie in a stage.  The lanes that read together are of two rows and four pieces (groups of 128), of four rows
+// and two or of eight and one: with the row's bits in reverse order they meet different banks.
+__device__ __forceinline__ uint32_t int4_code_at(int row, int piece) {
+  return (uint32_t)(row * 128 + (piece ^ ((row & 1) << 2 | (row & 2) | (row >> 2 & 1))) * 16);
+}
+// Where eight elements of a row of a (a piece) lie: those of eight rows side by side, turned so that the lanes which read together, of two
+// rows and four pieces V apart, meet different banks.
+template <int NT, int V>
+__device__ __forceinline__ uint32_t int4_at(int piece, int row) {
+  return (uint32_t)(((piece * NT + (row >> 3)) * 8 + ((row & 7) ^ (2 * ((piece / V) & 3)))) * 16);
+}
+
+// Asks for a stage of a warp's 16 rows, of which `rows` are there with `bytes` bytes, in pieces of PIECE bytes.
+template <int PIECE>
+__device__ __noinline__ void int4_ask_pieces(uint32_t to, const uint8_t* from, long long pitch, int rows, int bytes) {
+  constexpr int ACROSS = 128 / PIECE;
+#pragma unroll 4
+  for (int e = threadIdx.x & 31; e < 16 * ACROSS; e += 32) {
+    const int row = e / ACROSS, b = e % ACROSS * PIECE;
+    const int there = row < rows ? min(max(bytes - b, 0), PIECE) : 0;
+    const uint32_t at = to + int4_code_at(row, b / 16) + b % 16;
+    const uint8_t* source = there > 0 ? from + row * pitch + b : from;
+    if constexpr (PIECE >= 4) {
+      int4_copy<PIECE>(at, source, there);
+    } else {
+      const uint16_t v = there > 0 ? *source : (uint16_t)0;
+      asm volatile("st.shared.b8 [%0], %1;" ::"r"(at), "h"(v) : "memory");
     }
   }
-  for (int r = 0; r < RT; ++r) {
+}
+
+// A warp has 16 rows of w, whose codes come to it through a ring of STAGES steps in shared memory; a block's warps share up to 8 NT
+// rows of a there, and the blocks of a cluster share K.  The V = G / 32 words of a lane (8 codes each) are of one group in all four lanes
+// of a row, so the products of a group are summed as whole numbers times elements of a, and the sums are scaled.  The blocks' sums are
+// joined in their order.
+template <typename T, int G, int NT, int WARPS, int STAGES>
+__global__ void __launch_bounds__(32 * WARPS) gemm_int4_kernel(Int4Args p, Int4Few q) {
+  constexpr int V = G / 32, PER = I4_STEP / G, COLS = 8 * NT, PITCH = COLS + 2, ROWS = 16 * WARPS;
+  extern __shared__ __align__(16) uint8_t i4_smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int blocks = q.blocks, rank = blockIdx.x % blocks;
+  const int tile0 = blockIdx.x / blocks * ROWS, r0 = tile0 + 16 * warp, n0 = blockIdx.y * COLS;
+  const int begin = min(p.k, rank * q.range), end = min(p.k, begin + q.range);
+  uint8_t* ring = i4_smem + warp * (STAGES * I4_STAGE);
+  const uint32_t ring_at = smem_u32(ring);
+  uint8_t* xs = i4_smem + WARPS * STAGES * I4_STAGE;
+  float* scales = reinterpret_cast<float*>(xs + q.chunk * COLS * 2);      // [groups of a chunk][ROWS]
+  if (blocks > 1) cluster_arrive_relaxed_all();
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const int steps = (end - begin + I4_STEP - 1) / I4_STEP, groups = (p.k + G - 1) / G, rows = min(16, p.n - r0);
+  const uint8_t* lane_codes = p.codes + (long long)(r0 + (lane >> 3)) * p.ldw + begin / 2 + 16 * (lane & 7);
+  // Asks for the codes of a step.
+  auto ask = [&](int step, int slot) {
+    if (step < steps && rows > 0) {
+      const int k0 = begin + step * I4_STEP;
+      const uint32_t at = ring_at + (uint32_t)(slot * I4_STAGE);
+      if (q.code_piece == 16 && rows == 16 && k0 + I4_STEP <= p.k) {
+        const uint8_t* from = lane_codes + step * (I4_STEP / 2);
 #pragma unroll
-    for (int s = 0; s < RT; ++s)
-      if (s == r) {
+        for (int i = 0; i < 4; ++i) int4_copy<16>(at + int4_code_at((lane >> 3) + 4 * i, lane & 7), from + i * (4 * p.ldw), 16);
+      } else {
+        // What lies beyond k meets zeros of a; rows that are not there are zero.
+        const uint8_t* from = p.codes + (long long)r0 * p.ldw + k0 / 2;
+        const int bytes = (p.k - k0 + 1) / 2;
+        if (q.code_piece == 16) int4_ask_pieces<16>(at, from, p.ldw, rows, bytes);
+        else if (q.code_piece == 8) int4_ask_pieces<8>(at, from, p.ldw, rows, bytes);
+        else if (q.code_piece == 4) int4_ask_pieces<4>(at, from, p.ldw, rows, bytes);
+        else int4_ask_pieces<1>(at, from, p.ldw, rows, bytes);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // What a chunk needs of a and of the scales is read into registers a chunk ahead: rows of a in the order of the codes' pairs, zeros
+  // beyond k and for rows that are not there, of which a thread has one row and every (4 WARPS / NT)-th piece; and the scales of a row of w.
+  constexpr int MOST = int4_chunk<NT>, X = MOST / 8 * COLS / (32 * WARPS), SCALES = MOST / G * ROWS / (32 * WARPS);
+  const uint16_t* a = reinterpret_cast<const uint16_t*>(p.a);
+  const int x_row = threadIdx.x % 8 + threadIdx.x / 32 % NT * 8, x_first = threadIdx.x / 8 % 4 + threadIdx.x / (32 * NT) * 4;
+  const int s_row = threadIdx.x % ROWS, s_first = threadIdx.x / ROWS;
+  SbWords<16> x_held[X];
+  SbWords<2> s_held[SCALES];
+  auto load_chunk = [&](int chunk0) {
+    const bool there = n0 + x_row < p.m && q.whole_rows;
+    const uint16_t* from = a + (long long)(n0 + x_row) * p.lda + chunk0;
+#pragma unroll
+    for (int i = 0; i < X; ++i) {
+      const int at = 8 * (x_first + i * (4 * WARPS / NT));
+      x_held[i].v = make_uint4(0u, 0u, 0u, 0u);
+      sb_load_kept(x_held[i], from + at, there && at < q.chunk && chunk0 + at + 8 <= p.k);
+    }
+    const uint16_t* scales_from = reinterpret_cast<const uint16_t*>(p.scales) + (long long)(chunk0 / G) * p.n + tile0 + s_row;
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) {
+      const int b = s_first + i * (32 * WARPS / ROWS);
+      s_held[i].v = 0;
+      sb_load_kept(s_held[i], scales_from + (long long)b * p.n, b * G < q.chunk && chunk0 / G + b < groups && tile0 + s_row < p.n);
+    }
+  };
+  auto store_chunk = [&](int chunk0) {
+    const uint16_t* from = a + (long long)(n0 + x_row) * p.lda + chunk0;
+#pragma unroll
+    for (int i = 0; i < X; ++i) {
+      const int piece = x_first + i * (4 * WARPS / NT), left = p.k - chunk0 - 8 * piece;
+      if (8 * piece >= q.chunk) break;
+      uint4 v = x_held[i].v;
+      if (n0 + x_row < p.m && left > 0 && (left < 8 || !q.whole_rows)) v = int4_elements(from + 8 * piece, left);
+      *reinterpret_cast<uint4*>(xs + int4_at<NT, V>(piece, x_row)) = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                                                                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+    }
+#pragma unroll
+    for (int i = 0; i < SCALES; ++i) {
+      const int b = s_first + i * (32 * WARPS / ROWS);
+      if (b * G < q.chunk) scales[b * ROWS + s_row] = int4_scale(s_held[i].v, q.scale_dtype);
+    }
+  };
+  // Before the codes, which are many times more: what everything waits for.
+  if (begin < end) load_chunk(begin);
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) ask(s, s);
+  // This thread's row of those that this block will finish.
+  const int share = ROWS / blocks, out_row = share * rank + threadIdx.x % share;
+  const float out_bias = blocks > 1 && p.bias && tile0 + out_row < p.n ? p.bias[tile0 + out_row] : 0.f;
+
+  float acc[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
+  // Where this lane's words lie in a stage (of the group b: with bits of b turned over, eight rows on: 1024 bytes on), and its elements of
+  // a in a chunk.
+  const uint32_t lane_word = int4_code_at(g, V * t / 4) + 4 * V * t % 16;
+  const uint8_t* lane_xs = xs + int4_at<NT, V>(V * t, g);
+  int slot = 0, step = 0;
+  for (int chunk0 = begin; chunk0 < end; chunk0 += q.chunk) {
+    const int chunk1 = min(begin + steps * I4_STEP, chunk0 + q.chunk);
+    if (chunk0 != begin) __syncthreads();
+    store_chunk(chunk0);
+    if (chunk0 + q.chunk < end) load_chunk(chunk0 + q.chunk);
+    __syncthreads();
+    for (int k0 = chunk0; k0 < chunk1; k0 += I4_STEP, ++step) {
+      __syncwarp();                                     // all lanes have read the slot that is filled now
+      ask(step + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const uint8_t* stage = ring + slot * I4_STAGE;
+      const float* step_scales = scales + (k0 - chunk0) / G * ROWS + 16 * warp + g;
+      const uint8_t* step_xs = lane_xs + (k0 - chunk0) / 8 * (NT * 128);
+#pragma unroll
+      for (int b = 0; b < PER; ++b) {
+        SbWords<4 * V> words[2];
+        float scale[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          words[h] = *reinterpret_cast<const SbWords<4 * V>*>(stage + (lane_word ^ (uint32_t)(b * (G / 2))) + 1024 * h);
+          scale[h] = step_scales[b * ROWS + 8 * h];
+        }
+        float sum[NT][4];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          uint32_t codes[V], w[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            memcpy(codes, &words[h], 4 * V);
+            int4_pairs<T>(codes[v], w[h]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 x = *reinterpret_cast<const uint4*>(step_xs + ((b * (G / 8) + v) * NT + n) * 128);
+            if (v == 0) mma_16x8x16_first<T>(sum[n], w[0][0], w[1][0], w[0][1], w[1][1], x.x, x.y);
+            else mma_16x8x16<T>(sum[n], w[0][0], w[1][0], w[0][1], w[1][1], x.x, x.y);
+            mma_16x8x16<T>(sum[n], w[0][2], w[1][2], w[0][3], w[1][3], x.z, x.w);
+          }
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part[(warp * 16 + g + 8 * (j >> 1)) * PITCH + 8 * n + 2 * t + (j & 1)] = acc[s][n][j];
+          for (int j = 0; j < 4; ++j) acc[n][j] = fmaf(scale[j >> 1], sum[n][j], acc[n][j]);
       }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 16 * COLS; e += 32 * I4_WARPS) {
-      const int row = e % 16, col = e / 16;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < I4_WARPS; ++w) sum += part[(w * 16 + row) * PITCH + col];
-      sums[(16 * r + row) * PITCH + col] = sum;
+      slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
-    __syncthreads();
   }
-  if (blocks > 1) cluster_sync_all();
-  for (int e = threadIdx.x + 32 * I4_WARPS * rank; e < ROWS * COLS; e += 32 * I4_WARPS * blocks) {
-    const int row = e % ROWS, col = e / ROWS;
-    if (r0 + row >= p.n || n0 + col >= p.m) continue;
-    float sum = 0.f;
-    if (blocks == 1) {
-      sum = sums[row * PITCH + col];
-    } else {
-      const uint32_t at = smem_u32(&sums[row * PITCH + col]);
-      for (int b = 0; b < blocks; ++b) {
-        float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_cta(at, (uint32_t)b)) : "memory");
-        sum += v;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (blocks == 1) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = r0 + g + 8 * (j >> 1), col = n0 + 8 * n + 2 * t + (j & 1);
+        if (row < p.n && col < p.m) int4_store(p, col, row, acc[n][j], p.bias ? p.bias[row] : 0.f);
       }
-    }
-    int4_store(p, n0 + col, r0 + row, sum);
+    return;
+  }
+  // Each block finishes `share` of the rows: the others lay their sums of these into its shared memory, [blocks][share][PITCH].  All blocks of
+  // the cluster have started.
+  cluster_wait_all();
+  float* sums = reinterpret_cast<float*>(i4_smem + q.sums_at);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = 16 * warp + g + 8 * h;
+    const uint32_t at = map_to_cta(smem_u32(sums + (rank * share + row % share) * PITCH + 2 * t), (uint32_t)(row / share));
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at + 32u * n), "f"(acc[n][2 * h]), "f"(acc[n][2 * h + 1]) : "memory");
   }
   __syncwarp();
-  if (blocks > 1) cluster_sync_all();                  // no block leaves while another reads its sums
+  cluster_sync_all();
+  for (int e = threadIdx.x; e < share * COLS; e += 32 * WARPS) {
+    const int col = e / share;
+    if (tile0 + out_row >= p.n || n0 + col >= p.m) continue;
+    float sum = 0.f;
+    for (int b = 0; b < blocks; ++b) sum += sums[(b * share + threadIdx.x % share) * PITCH + col];
+    int4_store(p, n0 + col, tile0 + out_row, sum, out_bias);
+  }
 }
 
 int int4_args_ok(const char* who, long long n, int k, int group, int scale_dtype) {
@@ -310,39 +379,48 @@ int int4_args_ok(const char* who, long long n, int k, int group, int scale_dtype
 
 bool int4_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (size_t)sb_dtype_size(dtype) == 0; }
 
-template <typename T, int G, int NT, int RT>
+template <typename T, int G, int NT, int WARPS, int STAGES>
 int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
-  constexpr int PITCH = 8 * NT + 1, BYTES = (I4_WARPS * 16 + 16 * RT) * PITCH * 4;
-  const long long tiles = ((long long)p.n + 16 * RT - 1) / (16 * RT), down = ((long long)p.m + 8 * NT - 1) / (8 * NT);
-  // Blocks that share K until there are three for every two SMs, each warp with a group of its own.
+  constexpr int ROWS = 16 * WARPS, COLS = 8 * NT, MOST = int4_chunk<NT>, RING = WARPS * STAGES * I4_STAGE, SUMS = ROWS * (COLS + 2) * 4, LIMIT = RING + MOST * COLS * 2 + MOST / G * ROWS * 4 + SUMS;
+  static_assert(LIMIT <= 227 * 1024, "more shared memory than an SM has");
+  const long long tiles = ((long long)p.n + ROWS - 1) / ROWS, down = ((long long)p.m + COLS - 1) / COLS;
+  // Blocks that share K until every SM has the warps it can hold, each with 512 columns at least.
   int blocks = 1;
-  while (blocks < 8 && 2 * tiles * down * blocks < 3LL * sb_sm_count() && (p.k + G - 1) / G >= 2 * blocks * I4_WARPS) blocks *= 2;
-  static std::atomic<bool> ready[64];
-  if (BYTES > 48 * 1024) {
-    const int rc = sb_allow_smem(gemm_int4_kernel<T, G, NT, RT>, BYTES, ready);
-    if (rc != SB_OK) return rc;
-  }
+  while (blocks < 8 && tiles * down * blocks * (WARPS / 8) <= sb_sm_count() && p.k >= 1024 * blocks) blocks *= 2;
   q.blocks = blocks;
-  SB_CUDA(sb_launch(gemm_int4_kernel<T, G, NT, RT>, dim3((unsigned)(tiles * blocks), (unsigned)down), dim3(32 * I4_WARPS), (size_t)BYTES, s, blocks, p, q));
+  q.range = ((p.k + blocks - 1) / blocks + I4_STEP - 1) / I4_STEP * I4_STEP;
+  q.chunk = q.range < MOST ? q.range : MOST;
+  q.sums_at = RING + q.chunk * COLS * 2 + q.chunk / G * ROWS * 4;
+  const int bytes = q.sums_at + (blocks > 1 ? SUMS : 0);
+  static std::atomic<bool> ready[64];
+  const int rc = sb_allow_smem(gemm_int4_kernel<T, G, NT, WARPS, STAGES>, LIMIT, ready);
+  if (rc != SB_OK) return rc;
+  SB_CUDA(sb_launch(gemm_int4_kernel<T, G, NT, WARPS, STAGES>, dim3((unsigned)(tiles * blocks), (unsigned)down), dim3(32 * WARPS), (size_t)bytes, s, blocks, p, q));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }
 
 template <typename T, int G>
 int launch_int4(const Int4Args& p, const Int4Few& q, cudaStream_t s) {
-  if (p.m <= 2) return launch_int4<T, G, 1, 1>(p, q, s);
-  if (p.m <= 8) return launch_int4<T, G, 1, 4>(p, q, s);
-  if (p.m <= 16) return launch_int4<T, G, 2, 4>(p, q, s);
-  if (p.m <= 32) return launch_int4<T, G, 4, 2>(p, q, s);
-  return launch_int4<T, G, 8, 2>(p, q, s);
+  if (p.m <= 8) return launch_int4<T, G, 1, 8, 4>(p, q, s);
+  if (p.m <= 16) return launch_int4<T, G, 2, 16, 4>(p, q, s);
+  if (p.m <= 32) return launch_int4<T, G, 4, 16, 4>(p, q, s);
+  return launch_int4<T, G, 8, 16, 3>(p, q, s);
+}
+
+// The widest pieces in which rows can be copied.
+int int4_piece(const void* p, long long pitch, int least) {
+  for (int piece = 16; piece >= 4; piece /= 2)
+    if (reinterpret_cast<uintptr_t>(p) % piece == 0 && pitch % piece == 0) return piece;
+  return least;
 }
 
 template <typename T>
 int launch_int4(const Int4Args& p, int scale_dtype, cudaStream_t s) {
   Int4Few q;
-  const int lane_bytes = p.group / 8;
-  q.whole_words = (reinterpret_cast<uintptr_t>(p.codes) % lane_bytes == 0 && p.ldw % lane_bytes == 0) ? 1 : 0;
-  q.whole_rows = (reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && (p.m == 1 || p.lda % 8 == 0)) ? 1 : 0;
+  memset(&q, 0, sizeof(q));
+  q.code_piece = int4_piece(p.codes, p.n == 1 ? 16 : p.ldw, 1);
+  q.whole_rows = int4_piece(p.a, p.m == 1 ? 16 : 2 * p.lda, 2) == 16 ? 1 : 0;
   q.scale_dtype = scale_dtype;
   return p.group == 32 ? launch_int4<T, 32>(p, q, s) : p.group == 64 ? launch_int4<T, 64>(p, q, s) : launch_int4<T, 128>(p, q, s);
 }

@@ -511,7 +511,8 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
         }
         __syncwarp();
       }
-      cluster_sync_all();                        // the others may go on
+      cluster_arrive_relaxed_all();              // what was read has been used: the others may go on
+      cluster_wait_all();
       if (rank == 0 && g.top > 0) {
         const int n = candidate_count;
         if (tid < LP_MAX_TOP) best[tid] = 0ull;
