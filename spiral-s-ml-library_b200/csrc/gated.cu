@@ -16,10 +16,22 @@ enum GatedAct { ACT_SILU = SB_ACT_SILU, ACT_GELU = SB_ACT_GELU, ACT_RELU = SB_AC
 
 __device__ __forceinline__ float gated_sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
+// The normal distribution's P(g) and exp(-g^2 / 2), which its tails are made of: erfc(x) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2) with
+// t = 1 / (1 + p x), off by at most 1.5e-7 (M. Abramowitz, I. A. Stegun, Handbook of Mathematical Functions, 7.1.26).
+__device__ __forceinline__ float2 gated_normal(float g) {
+  const float x = fabsf(g) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f)), e = __expf(-x * x);
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  q *= 0.5f * t * e;
+  return make_float2(g > 0.f ? 1.f - q : q, e);
+}
+
 template <int ACT>
 __device__ __forceinline__ float gated_act(float g) {
   if (ACT == ACT_SILU) return g * gated_sigmoid(g);
-  if (ACT == ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  if (ACT == ACT_GELU) return g * gated_normal(g).x;
   return g > 0.f ? g : (g != g ? g : 0.f);
 }
 // The activation and its derivative.
@@ -30,8 +42,8 @@ __device__ __forceinline__ float2 gated_act_grad(float g) {
     return make_float2(g * s, s * (1.f + g * (1.f - s)));
   }
   if (ACT == ACT_GELU) {
-    const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-    return make_float2(g * p, p + g * __expf(-0.5f * g * g) * 0.39894228040143268f);
+    const float2 n = gated_normal(g);
+    return make_float2(g * n.x, fmaf(g * 0.39894228040143268f, n.y, n.x));
   }
   return make_float2(gated_act<ACT_RELU>(g), g > 0.f ? 1.f : 0.f);
 }

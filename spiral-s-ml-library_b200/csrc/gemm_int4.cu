@@ -369,6 +369,84 @@ __global__ void __launch_bounds__(32 * WARPS) gemm_int4_kernel(Int4Args p, Int4F
   }
 }
 
+// Fewest rows of a (at most 8): a block has 16 rows of w, whose groups its eight warps take in turn, all that a lane needs of UNROLL of
+// them on its way to registers at a time and nothing through shared memory but the warps' sums.  Whole groups, codes that start on the
+// words of a lane, rows of a that start on 16 bytes.
+template <typename T, int G>
+__global__ void __launch_bounds__(256, 2) gemm_int4_fewest_kernel(Int4Args p, int scale_dtype) {
+  constexpr int V = G / 32, UNROLL = V == 4 ? 2 : 4;
+  __shared__ float part[8][16][9];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int r0 = blockIdx.x * 16;
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  // Rows that are not there give sums that are not written: they read the last one.
+  const int row_a = min(r0 + g, p.n - 1), row_b = min(r0 + g + 8, p.n - 1);
+  const uint8_t* codes_a = p.codes + (long long)row_a * p.ldw + 4 * V * t;
+  const uint8_t* codes_b = p.codes + (long long)row_b * p.ldw + 4 * V * t;
+  const uint16_t* scales = reinterpret_cast<const uint16_t*>(p.scales);
+  const T* x = reinterpret_cast<const T*>(p.a) + (long long)g * p.lda + 8 * V * t;
+  const bool there = g < p.m;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int groups = p.k / G;
+  for (int b0 = warp; b0 < groups; b0 += 8 * UNROLL) {
+    SbWords<4 * V> wa[UNROLL], wb[UNROLL];
+    SbWords<2> sa[UNROLL], sb[UNROLL];
+    SbWords<16> e[UNROLL][V];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int b = b0 + 8 * u;
+      const bool in = b < groups;
+      memset(&wa[u], 0, 4 * V);
+      memset(&wb[u], 0, 4 * V);
+      sa[u].v = sb[u].v = 0;
+      sb_load_words(wa[u], codes_a + (long long)b * (G / 2), in);
+      sb_load_words(wb[u], codes_b + (long long)b * (G / 2), in);
+      sb_load_kept(sa[u], scales + (long long)b * p.n + row_a, in);
+      sb_load_kept(sb[u], scales + (long long)b * p.n + row_b, in);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        e[u][v].v = make_uint4(0u, 0u, 0u, 0u);
+        sb_load_kept(e[u][v], x + b * G + 8 * v, in && there);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      uint32_t ca[V], cb[V];
+      memcpy(ca, &wa[u], 4 * V);
+      memcpy(cb, &wb[u], 4 * V);
+      float sum[4];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        uint32_t a[4], c[4];
+        int4_pairs<T>(ca[v], a);
+        int4_pairs<T>(cb[v], c);
+        const uint4 y = e[u][v].v;
+        const uint32_t x04 = __byte_perm(y.x, y.z, 0x5410), x15 = __byte_perm(y.x, y.z, 0x7632), x26 = __byte_perm(y.y, y.w, 0x5410),
+                       x37 = __byte_perm(y.y, y.w, 0x7632);
+        if (v == 0) mma_16x8x16_first<T>(sum, a[0], c[0], a[1], c[1], x04, x15);
+        else mma_16x8x16<T>(sum, a[0], c[0], a[1], c[1], x04, x15);
+        mma_16x8x16<T>(sum, a[2], c[2], a[3], c[3], x26, x37);
+      }
+      const float scale_a = int4_scale(sa[u].v, scale_dtype), scale_b = int4_scale(sb[u].v, scale_dtype);
+      acc[0] = fmaf(scale_a, sum[0], acc[0]);
+      acc[1] = fmaf(scale_a, sum[1], acc[1]);
+      acc[2] = fmaf(scale_b, sum[2], acc[2]);
+      acc[3] = fmaf(scale_b, sum[3], acc[3]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) part[warp][g + 8 * (j >> 1)][2 * t + (j & 1)] = acc[j];
+  __syncthreads();
+  const int row = threadIdx.x % 16, col = threadIdx.x / 16;
+  if (col < p.m && r0 + row < p.n) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += part[w][row][col];
+    int4_store(p, col, r0 + row, sum, p.bias ? p.bias[r0 + row] : 0.f);
+  }
+}
+
 int int4_args_ok(const char* who, long long n, int k, int group, int scale_dtype) {
   if (n < 0 || k < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
   if (group != 32 && group != 64 && group != 128) return sb_fail(SB_ERR_UNSUPPORTED, "%s: groups of 32, 64 or 128 (got %d)", who, group);
@@ -402,6 +480,14 @@ int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
 
 template <typename T, int G>
 int launch_int4(const Int4Args& p, const Int4Few& q, cudaStream_t s) {
+  // Small matrices of weights, whose time is that of the way there: 1 x 4096 x 4096 in groups of 128 4.8 us, through rings 6.1; 1 x 256 x 512
+  // 2.1 / 4.5; 8 x 4096 x 4096 6.5 / 6.5.  Not long rows (1 x 1024 x 16384 27 / 12) nor more blocks than there is room for (1 x 8192 x 8192
+  // 17.5 / 14.2).
+  if (p.m <= 8 && p.k <= 4096 && p.n <= 32 * sb_sm_count() && p.k % G == 0 && q.code_piece >= G / 8 && q.whole_rows) {
+    SB_CUDA(sb_launch(gemm_int4_fewest_kernel<T, G>, dim3((unsigned)(((long long)p.n + 15) / 16)), dim3(256), 0, s, 1, p, q.scale_dtype));
+    SB_COUNT_LAUNCH();
+    return SB_OK;
+  }
   if (p.m <= 8) return launch_int4<T, G, 1, 8, 4>(p, q, s);
   if (p.m <= 16) return launch_int4<T, G, 2, 16, 4>(p, q, s);
   if (p.m <= 32) return launch_int4<T, G, 4, 16, 4>(p, q, s);
