@@ -216,6 +216,7 @@ struct RowShape {
   __device__ __forceinline__ int single(int i) const { return i < head ? i : packs * V + i; }
 };
 
+// The largest of a pack's logits, NaN left out.
 template <typename T>
 __device__ __forceinline__ float lp_largest(const SbWords<16>& w);
 template <>
@@ -236,12 +237,207 @@ __device__ __forceinline__ float lp_largest<__half>(const SbWords<16>& w) {
   const float2 m = __half22float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
   return fmaxf(m.x, m.y);
 }
+// What a logit counts as at least in the fast sums, so that no product of them is 0 times infinity: -2^100, in f16 the lowest number.
+template <typename T>
+__device__ __forceinline__ float lp_low() { return std::is_same<T, __half>::value ? -65504.f : -1.2676506002282294e30f; }
+template <typename T>
+__device__ __forceinline__ void lp_lift(SbWords<16>& w);
+template <>
+__device__ __forceinline__ void lp_lift<float>(SbWords<16>& w) {
+  const float low = lp_low<float>();
+  w.v.x = __float_as_uint(max_nan(__uint_as_float(w.v.x), low));
+  w.v.y = __float_as_uint(max_nan(__uint_as_float(w.v.y), low));
+  w.v.z = __float_as_uint(max_nan(__uint_as_float(w.v.z), low));
+  w.v.w = __float_as_uint(max_nan(__uint_as_float(w.v.w), low));
+}
+template <>
+__device__ __forceinline__ void lp_lift<__nv_bfloat16>(SbWords<16>& w) {
+  const __nv_bfloat162 low = __float2bfloat162_rn(lp_low<__nv_bfloat16>());
+  __nv_bfloat162 v[4];
+  memcpy(v, &w, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __hmax2_nan(v[i], low);
+  memcpy(&w, v, 16);
+}
+template <>
+__device__ __forceinline__ void lp_lift<__half>(SbWords<16>& w) {
+  const __half2 low = __float2half2_rn(lp_low<__half>());
+  __half2 v[4];
+  memcpy(v, &w, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __hmax2_nan(v[i], low);
+  memcpy(&w, v, 16);
+}
 
+// The pairs of a pack as fp32.
+template <typename T>
+__device__ __forceinline__ void lp_pairs(const SbWords<16>& w, unsigned long long* x) {
+  float v[RowShape<T>::V];
+  sb_unpack_words<T, RowShape<T>::V>(w, v);
+#pragma unroll
+  for (int i = 0; i < RowShape<T>::V / 2; ++i) x[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+}
+
+// The sums of a thread's share of a row of legal logits, in powers of two: with c = s / ln 2 and the reference R = c top, rounded,
+//   sum = sum 2^(c x - R)   dist = sum 2^(c x - R) (c x - R),
+// one fused multiply-add, one exponential and two additions per logit, two at a time.  The rounding of R is made good at the end.  Four batches
+// of packs are on their way; a batch raises the reference first.  top_a and top_b: the largest of the even and of the odd packs.
+template <typename T>
+struct FastSums {
+  float c, top_a, top_b, ref;
+  unsigned long long sum, dist;
+};
+template <typename T>
+__device__ __forceinline__ void lp_fast_raise(FastSums<T>& f) {
+  const float ref = fmaxf(f.top_a, f.top_b) * f.c, d = f.ref - ref, e = exp2_approx(d);
+  const unsigned long long d2 = pack_f32x2(d, d), e2 = pack_f32x2(e, e);
+  fma_f32x2(f.dist, f.sum, d2);
+  f.dist = mul_f32x2(f.dist, e2);
+  f.sum = mul_f32x2(f.sum, e2);
+  f.ref = ref;
+}
+template <typename T>
+__device__ __forceinline__ void lp_fast_pack(FastSums<T>& f, const SbWords<16>& w) {
+  unsigned long long x[RowShape<T>::V / 2];
+  lp_pairs<T>(w, x);
+  const unsigned long long c2 = pack_f32x2(f.c, f.c), ref2 = pack_f32x2(-f.ref, -f.ref);
+#pragma unroll
+  for (int i = 0; i < RowShape<T>::V / 2; ++i) {
+    unsigned long long a2 = ref2;
+    fma_f32x2(a2, x[i], c2);
+    float a0, a1;
+    unpack_f32x2(a2, a0, a1);
+    const unsigned long long e2 = pack_f32x2(exp2_approx(a0), exp2_approx(a1));
+    f.sum = add_f32x2(f.sum, e2);
+    fma_f32x2(f.dist, e2, a2);
+  }
+}
+template <typename T>
+__device__ __forceinline__ RowSums lp_fast_sums(const T* x, const RowShape<T>& shape, int first, int stride, float c, float& top_a, float& top_b) {
+  constexpr int UNROLL = 4;
+  const float low = lp_low<T>();
+  FastSums<T> f = {c, low, low, low * c, 0ull, 0ull};
+  if (first < shape.head + shape.tail) {
+    const float v = max_nan(sb_to_f32<T>(x[shape.single(first)]), low);
+    f.top_a = fmaxf(low, v);
+    f.ref = f.top_a * c;
+    const float a = fmaf(v, c, -f.ref), e = exp2_approx(a);
+    f.sum = pack_f32x2(e, 0.f);
+    f.dist = pack_f32x2(e * a, 0.f);
+  }
+  const T* from = x + shape.head;
+  // Packs that are not there hold -inf.
+  auto load = [&](SbWords<16>* w, int p) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      w[u].v.x = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+      w[u].v.y = w[u].v.z = w[u].v.w = w[u].v.x;
+      sb_load_words(w[u], from + (long long)(p + u * stride) * RowShape<T>::V, p + u * stride < shape.packs);
+    }
+  };
+  SbWords<16> now[UNROLL], next[UNROLL];
+  load(now, first);
+  for (int p = first; p < shape.packs; p += UNROLL * stride) {
+    load(next, p + UNROLL * stride);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      lp_lift<T>(now[u]);
+      if (u % 2 == 0) f.top_a = fmaxf(f.top_a, lp_largest<T>(now[u]));
+      else f.top_b = fmaxf(f.top_b, lp_largest<T>(now[u]));
+    }
+    lp_fast_raise(f);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) lp_fast_pack(f, now[u]);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) now[u] = next[u];
+  }
+  top_a = f.top_a;
+  top_b = f.top_b;
+  float s0, s1, d0, d1;
+  unpack_f32x2(f.sum, s0, s1);
+  unpack_f32x2(f.dist, d0, d1);
+  RowSums r;
+  r.top = fmaxf(f.top_a, f.top_b);
+  // c top is ref + rest.  (Far from zero the rest is large: such a share counts only in rows that take the exact sums, or not at all.)
+  const float rest = fminf(fmaxf(fmaf(r.top, c, -f.ref), -60.f), 60.f), back = exp2_approx(-rest);
+  r.sum = (s0 + s1) * back;
+  r.dist = (d0 + d1 - rest * (s0 + s1)) * back * __fdividef(1.f, c);
+  return r;
+}
+// The fast sums of a row are right where its largest logit is neither so low (first) that what was lifted has weight beside it nor so far
+// up (second) that the reference's rounding, 2^-4 of a power of two, is not made good to the last bits.
+constexpr float LP_FAST_MOST = 1048576.f;
+template <typename T>
+__device__ __forceinline__ bool lp_not_low(float top, float c) { return (top - lp_low<T>()) * c >= 60.f && top * c >= -LP_FAST_MOST; }
+__device__ __forceinline__ bool lp_too_high(float top, float c) { return top * c > LP_FAST_MOST || c > LP_FAST_MOST; }
+
+// -inf where the bytes of a mask forbid a pack's columns.
 template <typename T>
 __device__ __forceinline__ void lp_mask_pack(float* x, const uint8_t* mask) {
+  constexpr int V = RowShape<T>::V;
+  uint8_t m[V];
+  if (reinterpret_cast<uintptr_t>(mask) % V == 0) {
+    SbWords<V> w;
+    sb_load_words(w, mask, true);
+    memcpy(m, &w, V);
+  } else {
 #pragma unroll
-  for (int i = 0; i < RowShape<T>::V; ++i)
-    if (mask[i] == 0) x[i] = -INFINITY;
+    for (int i = 0; i < V; ++i) m[i] = mask[i];
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (m[i] == 0) x[i] = -INFINITY;
+}
+
+// The same sums one logit at a time, under a mask or where the fast ones do not hold.
+template <typename T>
+__device__ __noinline__ RowSums lp_exact_sums(const T* x, const uint8_t* mask, const RowShape<T>& shape, int first, int stride, float c, float& top_a, float& top_b) {
+  constexpr int V = RowShape<T>::V;
+  RowSums r = {LP_LOWEST, 0.f, 0.f};
+  top_a = top_b = LP_LOWEST;
+  if (first < shape.head + shape.tail) {
+    const float v = lp_logit<T>(x, mask, shape.single(first));
+    r.top = top_a = fmaxf(r.top, v);
+    lp_take<1>(r, &v, c);
+  }
+  constexpr int UNROLL = 4;
+  const bool whole = mask && reinterpret_cast<uintptr_t>(mask + shape.head) % V == 0;
+  for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
+    SbWords<16> w[UNROLL];
+    SbWords<V> m[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int p = p0 + u * stride;
+      w[u].v = make_uint4(0u, 0u, 0u, 0u);
+      sb_load_words(w[u], x + shape.column(p < shape.packs ? p : p0), true);
+      memset(&m[u], 1, V);
+      sb_load_words(m[u], mask + shape.column(p < shape.packs ? p : p0), whole);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int p = p0 + u * stride;
+      if (p >= shape.packs) break;
+      float v[V];
+      sb_unpack_words<T, V>(w[u], v);
+      if (mask && !whole) {
+        lp_mask_pack<T>(v, mask + shape.column(p));
+      } else {
+        uint8_t legal[V];
+        memcpy(legal, &m[u], V);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (legal[i] == 0) v[i] = -INFINITY;
+      }
+      float most = LP_LOWEST;
+#pragma unroll
+      for (int i = 0; i < V; ++i) most = fmaxf(most, v[i]);
+      if (u % 2 == 0) top_a = fmaxf(top_a, most);
+      else top_b = fmaxf(top_b, most);
+      lp_raise(r, fmaxf(r.top, most), c);
+      lp_take<V>(r, v, c);
+    }
+  }
+  return r;
 }
 
 // An order of floats as unsigned numbers.
@@ -262,8 +458,8 @@ __device__ __forceinline__ int lp_place_column(unsigned long long place) { retur
 
 constexpr int LP_CANDIDATES = 512;
 // The `top` best of n candidates in their order: each counts those before it. 
-__device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, unsigned long long* best, int top, int threads) {
-  for (int i = threadIdx.x; i < n; i += threads) {
+__device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, unsigned long long* best, int top, int first, int threads) {
+  for (int i = first; i < n; i += threads) {
     const unsigned long long mine = candidates[i];
     int before = 0, k = 0;
     for (; k + 8 <= n; k += 8) {
@@ -285,8 +481,8 @@ __device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, u
 // the threads that reach it hold alternatives; the block reads their share of the row once more, from L2, and ranks what reaches
 // the bound.  Rows with more of those than there is room for (long runs of equal logits) find them one after the other.
 template <typename T, int NT, bool MASKED, bool CLUSTER>
-__global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
-  constexpr int V = RowShape<T>::V, WARPS = NT / 32, UNROLL = 4;
+__global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_kernel(LogProbArgs g) {
+  constexpr int V = RowShape<T>::V, WARPS = NT / 32;
   __shared__ RowSums part[WARPS];
   __shared__ RowSums whole;                      // of this block's share
   __shared__ float largest[NT];
@@ -306,48 +502,20 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
     const RowShape<T> shape(x, g.cols);
     const int stride = NT * blocks, first = rank * NT + tid;
     const int singles = shape.head + shape.tail;               // fewer than 2 V: the first threads of the first block have one each
-    RowSums r = {LP_LOWEST, 0.f, 0.f};
-    if (first < singles) {
-      const float v = lp_logit<T>(x, mask, shape.single(first));
-      r.top = fmaxf(r.top, v);
-      lp_take<1>(r, &v, c);
+    long long token = -1;
+    float token_logit = 0.f;
+    if (g.out && first == 0) {
+      token = lp_token(g.tokens, g.wide_tokens, row);
+      if (token >= 0 && token < g.cols) token_logit = lp_logit<T>(x, mask, (int)token);
     }
-    for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
-      SbWords<16> w[UNROLL];
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        // Packs that are not there hold -inf.
-        w[u].v = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
-                 : std::is_same<T, __half>::value ? make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u)
-                                                  : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-        sb_load_words(w[u], x + shape.column(p0 + u * stride < shape.packs ? p0 + u * stride : 0), p0 + u * stride < shape.packs);
-      }
-      float top = r.top;
-      if constexpr (!MASKED) {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) top = fmaxf(top, lp_largest<T>(w[u]));
-        lp_raise(r, top, c);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          float v[V];
-          sb_unpack_words<T, V>(w[u], v);
-          lp_take<V>(r, v, c);
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-          float v[V];
-          sb_unpack_words<T, V>(w[u], v);
-          if (p0 + u * stride < shape.packs) lp_mask_pack<T>(v, mask + shape.column(p0 + u * stride));
-          float most = r.top;
-#pragma unroll
-          for (int i = 0; i < V; ++i) most = fmaxf(most, v[i]);
-          lp_raise(r, most, c);
-          lp_take<V>(r, v, c);
-        }
-      }
+    float top_a, top_b;
+    RowSums r = MASKED ? lp_exact_sums<T>(x, mask, shape, first, stride, c, top_a, top_b) : lp_fast_sums<T>(x, shape, first, stride, c, top_a, top_b);
+    if (!MASKED) {
+      // The same decision in all blocks of a row: one whose own share has no logit to speak of lets the others have theirs.
+      const bool low = !__syncthreads_or(lp_not_low<T>(r.top, c));
+      if (__syncthreads_or(lp_too_high(r.top, c)) || low) r = lp_exact_sums<T>(x, nullptr, shape, first, stride, c, top_a, top_b);
     }
-    const float mine = r.top;
+    const float mine = fmaxf(top_a, top_b);
     float top = r.top;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -397,12 +565,12 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
           reach = (int)__reduce_add_sync(0xffffffffu, (unsigned)reach);
           if (reach >= g.top) {
             key = tried;
-            if (reach <= g.top + 4) break;
+            if (reach <= g.top + 8) break;
           }
         }
-        // The key as a number; below the lowest number's (fewer threads than alternatives have a logit) everything counts.
+        // The key as a number; where fewer threads than alternatives have a logit to speak of everything counts.
         const float b = __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-        if (lane == 0) bound = key <= lp_key(LP_LOWEST) ? LP_LOWEST : b;
+        if (lane == 0) bound = key <= lp_key(lp_low<T>()) ? LP_LOWEST : b;
       }
       __syncthreads();
       const float least = bound;
@@ -440,7 +608,7 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
       __syncthreads();
       const int n = candidate_count;
       if (n <= LP_CANDIDATES) {
-        lp_rank(candidates, n, best, g.top, NT);
+        lp_rank(candidates, n, best, g.top, tid, NT);
         __syncthreads();
       } else {
         unsigned long long last = ~0ull;
@@ -517,18 +685,141 @@ __global__ void __launch_bounds__(NT) log_probs_long_kernel(LogProbArgs g) {
         const int n = candidate_count;
         if (tid < LP_MAX_TOP) best[tid] = 0ull;
         __syncthreads();
-        lp_rank(candidates, n, best, g.top, NT);
+        lp_rank(candidates, n, best, g.top, tid, NT);
         __syncthreads();
       }
     }
     if (rank == 0) {
       const float log_sum = all.sum == 0.f ? INFINITY : logf(all.sum);
-      if (tid == 0) {
-        const long long token = g.out ? lp_token(g.tokens, g.wide_tokens, row) : -1;
-        lp_finish(g, row, all, log_sum, token >= 0 && token < g.cols ? lp_logit<T>(x, mask, (int)token) : 0.f, token);
-      }
+      if (tid == 0) lp_finish(g, row, all, log_sum, token_logit, token);
       if (tid < g.top) lp_alternative(g, row, tid, lp_place_logit(best[tid]), best[tid] == 0ull ? -1 : lp_place_column(best[tid]), all.top, log_sum);
     }
+  }
+}
+
+// Rows of middle length, and long ones where there are many: a warp per row, which needs no barrier.  The same steps; a lane's even and odd
+// packs have a largest logit each, so that there are 64 to bound the alternatives by.
+constexpr int LP_WARP_CANDIDATES = 160;
+template <typename T, bool MASKED>
+__global__ void __launch_bounds__(128, 8) log_probs_warp_kernel(LogProbArgs g) {
+  constexpr int V = RowShape<T>::V;
+  __shared__ __align__(16) unsigned long long all_candidates[4][LP_WARP_CANDIDATES];
+  __shared__ unsigned long long all_best[4][LP_MAX_TOP];
+  __shared__ uint8_t all_hot[4][64];
+  __shared__ int counts[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long* candidates = all_candidates[warp];
+  unsigned long long* best = all_best[warp];
+  uint8_t* hot = all_hot[warp];
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const float c = g.scale * LP_LOG2E;
+  for (long long row = (long long)blockIdx.x * 4 + warp; row < g.rows; row += (long long)gridDim.x * 4) {
+    const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
+    const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
+    const RowShape<T> shape(x, g.cols);
+    const int singles = shape.head + shape.tail;
+    long long token = -1;
+    float token_logit = 0.f;
+    if (g.out && lane == 0) {
+      token = lp_token(g.tokens, g.wide_tokens, row);
+      if (token >= 0 && token < g.cols) token_logit = lp_logit<T>(x, mask, (int)token);
+    }
+    float top_a, top_b;
+    RowSums r = MASKED ? lp_exact_sums<T>(x, mask, shape, lane, 32, c, top_a, top_b) : lp_fast_sums<T>(x, shape, lane, 32, c, top_a, top_b);
+    if (!MASKED) {
+      const bool low = !__any_sync(0xffffffffu, lp_not_low<T>(r.top, c));
+      if (__any_sync(0xffffffffu, lp_too_high(r.top, c)) || low) r = lp_exact_sums<T>(x, nullptr, shape, lane, 32, c, top_a, top_b);
+    }
+    float top = r.top;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    lp_raise(r, top, c);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+      r.dist += __shfl_xor_sync(0xffffffffu, r.dist, o);
+    }
+    const float log_sum = r.sum == 0.f ? INFINITY : logf(r.sum);
+    if (lane == 0) lp_finish(g, row, r, log_sum, token_logit, token);
+    if (g.top == 0) continue;
+    const uint32_t key_a = lp_key(top_a), key_b = lp_key(top_b);
+    const uint32_t low = __reduce_min_sync(0xffffffffu, min(key_a, key_b)), high = __reduce_max_sync(0xffffffffu, max(key_a, key_b));
+    const int alike = __clz((int)(low ^ high));
+    uint32_t key = alike == 32 ? low : low & ~(0xffffffffu >> alike);
+    for (int bit = 31 - alike; bit >= 0; --bit) {
+      const uint32_t tried = key | 1u << bit;
+      const int reach = __popc(__ballot_sync(0xffffffffu, key_a >= tried)) + __popc(__ballot_sync(0xffffffffu, key_b >= tried));
+      if (reach >= g.top) {
+        key = tried;
+        if (reach <= g.top + 2) break;
+      }
+    }
+    const float least = key <= lp_key(lp_low<T>()) ? LP_LOWEST : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    const uint32_t hot_a = __ballot_sync(0xffffffffu, top_a >= least), hot_b = __ballot_sync(0xffffffffu, top_b >= least);
+    __syncwarp();                                // what the row before left has been read
+    if (hot_a >> lane & 1u) hot[__popc(hot_a & ((1u << lane) - 1u))] = (uint8_t)lane;
+    if (hot_b >> lane & 1u) hot[__popc(hot_a) + __popc(hot_b & ((1u << lane) - 1u))] = (uint8_t)(32 + lane);
+    if (lane == 0) counts[warp] = 0;
+    for (int i = lane; i < g.top; i += 32) best[i] = 0ull;
+    __syncwarp();
+    auto candidate = [&](float v, int j) {
+      if (v >= least && v > -INFINITY) {
+        const int at = atomicAdd(&counts[warp], 1);
+        if (at < LP_WARP_CANDIDATES) candidates[at] = lp_place(v, j);
+      }
+    };
+    // A share: every second pack of a lane's; the single element goes with the even ones.
+    const int each = ((shape.packs + 31) / 32 + 1) / 2 + 1, items = (__popc(hot_a) + __popc(hot_b)) * each;
+    for (int item = lane; item < items; item += 32) {
+      const int who = hot[item / each], k = item % each, pack = 32 * (2 * k + (who >> 5)) + (who & 31);
+      if (k == each - 1) {
+        if (who < singles) candidate(lp_logit<T>(x, mask, shape.single(who)), shape.single(who));
+      } else if (pack < shape.packs) {
+        SbWords<16> w;
+        sb_load_kept(w, x + shape.column(pack), true);
+        if (MASKED || lp_largest<T>(w) >= least) {
+          float v[V];
+          sb_unpack_words<T, V>(w, v);
+          if (MASKED) lp_mask_pack<T>(v, mask + shape.column(pack));
+#pragma unroll
+          for (int i = 0; i < V; ++i) candidate(v[i], shape.column(pack) + i);
+        }
+      }
+    }
+    __syncwarp();
+    const int n = counts[warp];
+    if (n <= LP_WARP_CANDIDATES) {
+      lp_rank(candidates, n, best, g.top, lane, 32);
+    } else {
+      unsigned long long last = ~0ull;
+      for (int i = 0; i < g.top; ++i) {
+        unsigned long long next = 0ull;
+        auto look = [&](float v, int j) {
+          const unsigned long long place = lp_place(v, j);
+          if (v > -INFINITY && place < last && place > next) next = place;
+        };
+        if (lane < singles) look(lp_logit<T>(x, mask, shape.single(lane)), shape.single(lane));
+        for (int p = lane; p < shape.packs; p += 32) {
+          SbWords<16> w;
+          sb_load_kept(w, x + shape.column(p), true);
+          float v[V];
+          sb_unpack_words<T, V>(w, v);
+          if (MASKED) lp_mask_pack<T>(v, mask + shape.column(p));
+#pragma unroll
+          for (int e = 0; e < V; ++e) look(v[e], shape.column(p) + e);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, next, o);
+          next = other > next ? other : next;
+        }
+        if (lane == 0) best[i] = next;
+        last = next;
+      }
+    }
+    __syncwarp();
+    for (int i = lane; i < g.top; i += 32) lp_alternative(g, row, i, lp_place_logit(best[i]), best[i] == 0ull ? -1 : lp_place_column(best[i]), top, log_sum);
   }
 }
 
@@ -603,14 +894,18 @@ __global__ void __launch_bounds__(256) log_probs_grad_short_kernel(LogProbGradAr
   }
 }
 
-// Long rows: packs of 16 bytes, several on their way; the blocks of a column of the grid share the rows.
-template <typename T, bool MASKED>
+// Long rows, NT threads each: packs of 16 bytes, several on their way; the blocks of a column of the grid share the rows.  With c = s / ln 2 and
+// log p_j / ln 2 = c x_j - (ref + rest), where ref is rounded, a logit takes a fused multiply-add, an exponential, another multiply-add and a product, two at a
+// time: the constants have the rest and all factors in them.
+template <typename T, bool MASKED, int NT>
 __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArgs g) {
   constexpr int V = RowShape<T>::V, UNROLL = 4;
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const int first = blockIdx.x * 256 + threadIdx.x, stride = gridDim.x * 256;
-  for (long long row = blockIdx.y; row < g.rows; row += gridDim.y) {
+  const int first = NT == 256 ? blockIdx.x * 256 + threadIdx.x : threadIdx.x % NT, stride = NT == 256 ? gridDim.x * 256 : NT;
+  const float c = g.scale * LP_LOG2E;
+  for (long long row = NT == 256 ? blockIdx.y : (long long)blockIdx.x * (256 / NT) + threadIdx.x / NT; row < g.rows;
+       row += NT == 256 ? gridDim.y : (long long)gridDim.x * (256 / NT)) {
     const RowGrad r = lp_row_grad(g, row);
     const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
     const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
@@ -619,35 +914,38 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
     const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
     if (first < shape.head + shape.tail) lp_grad_one<T>(r, x, mask, d, shape.single(first), g.cols);
     for (int j = g.cols + first; j < g.mask_cols; j += stride) d[j] = sb_from_f32<T>(0.f);
+    // The short way holds where the lifted logits come out as 0 and no product leaves fp32's range.
+    const bool fast = fabsf(r.top) * c <= LP_FAST_MOST && c <= LP_FAST_MOST && (r.top - lp_low<T>()) * c >= 200.f && r.log_sum <= LP_FAST_MOST &&
+                      fabsf(r.h) < 1e6f && fabsf(r.c) < 1e30f;
+    const float ref = fmaf(r.top, c, r.log_sum * LP_LOG2E), rest = fmaf(r.top, c, -ref) + r.log_sum * LP_LOG2E, back = -r.scale * exp2_approx(-rest);
+    const float h = back * r.h * (1.f / LP_LOG2E), k = back * fmaf(r.h, -rest * (1.f / LP_LOG2E), r.c);
+    const unsigned long long c2 = pack_f32x2(c, c), ref2 = pack_f32x2(-ref, -ref), h2 = pack_f32x2(h, h), k2 = pack_f32x2(k, k);
     for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
       SbWords<16> w[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        w[u].v = make_uint4(0u, 0u, 0u, 0u);
-        const bool there = p0 + u * stride < shape.packs;
-        lp_load_once(w[u], x + shape.column(there ? p0 + u * stride : 0), there);
-      }
+      for (int u = 0; u < UNROLL; ++u) lp_load_once(w[u], x + shape.column(p0 + u * stride < shape.packs ? p0 + u * stride : p0), true);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         if (p0 + u * stride >= shape.packs) break;
         const int j = shape.column(p0 + u * stride);
         float v[V];
-        sb_unpack_words<T, V>(w[u], v);
-        const unsigned long long top2 = pack_f32x2(r.top, r.top), scale2 = pack_f32x2(r.scale, r.scale), sum2 = pack_f32x2(-r.log_sum, -r.log_sum),
-                                 log2 = pack_f32x2(LP_LOG2E, LP_LOG2E), h2 = pack_f32x2(r.h, r.h), c2 = pack_f32x2(r.c, r.c),
-                                 minus2 = pack_f32x2(-r.scale, -r.scale);
+        if (fast) {
+          unsigned long long pairs[V / 2];
+          lp_lift<T>(w[u]);
+          lp_pairs<T>(w[u], pairs);
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          unsigned long long lp2 = sum2;
-          fma_f32x2(lp2, scale2, sub_f32x2(pack_f32x2(v[i], v[i + 1]), top2));
-          float l0, l1;
-          unpack_f32x2(lp2, l0, l1);
-          lp2 = pack_f32x2(max_nan(l0, LP_NOTHING), max_nan(l1, LP_NOTHING));
-          unpack_f32x2(mul_f32x2(lp2, log2), l0, l1);
-          unsigned long long q2 = c2;
-          fma_f32x2(q2, h2, lp2);
-          q2 = mul_f32x2(mul_f32x2(pack_f32x2(exp2_approx(l0), exp2_approx(l1)), q2), minus2);
-          unpack_f32x2(q2, v[i], v[i + 1]);
+          for (int i = 0; i < V / 2; ++i) {
+            unsigned long long a2 = ref2, q2 = k2;
+            fma_f32x2(a2, pairs[i], c2);
+            fma_f32x2(q2, a2, h2);
+            float a0, a1;
+            unpack_f32x2(a2, a0, a1);
+            unpack_f32x2(mul_f32x2(pack_f32x2(exp2_approx(a0), exp2_approx(a1)), q2), v[2 * i], v[2 * i + 1]);
+          }
+        } else {
+          sb_unpack_words<T, V>(w[u], v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[i] = lp_grad(r, v[i]);
         }
         if ((unsigned)(r.token - j) < (unsigned)V) {
 #pragma unroll
@@ -655,9 +953,10 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
             if (j + i == r.token) v[i] += r.a;
         }
         if (MASKED) {
+          float legal[V] = {};
+          lp_mask_pack<T>(legal, mask + j);
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (mask[j + i] == 0) v[i] = 0.f;
+          for (int i = 0; i < V; ++i) v[i] = legal[i] == 0.f ? v[i] : 0.f;
         }
         if (alike) {
           sb_store_f32<T, V>(d + j, v);
@@ -711,26 +1010,46 @@ int launch_log_probs_long(const LogProbArgs& g, int blocks, cudaStream_t s) {
 
 template <typename T>
 int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
+  // us, 2^17 rows of bf16 unless it says otherwise.  Rounds among the lanes of a row cost by the alternative, a bound costs once: 200 columns with 5
+  // alternatives (10^5 rows) 110 in registers, 133 by warps; with 8 of them 201 / 185; 1000 columns with none 105 / 85, with 8 488 / 232.
   if (g.cols <= 16) return launch_log_probs_short<T, 4, 4>(g, s);
   if (g.cols <= 64) return launch_log_probs_short<T, 8, 8>(g, s);
-  if (g.cols <= 256) return launch_log_probs_short<T, 32, 8>(g, s);
-  if (g.cols <= 1024) return launch_log_probs_short<T, 32, 32>(g, s);
+  if (g.cols <= 256 && g.top <= 7) return launch_log_probs_short<T, 32, 8>(g, s);
+  // Warps or blocks, 8 alternatives: 32768 x 2048 69 / 152, 16384 x 8192 94 / 98, 8192 x 16384 93 / 80, 600 x 4096 11.7 / 9.3.
+  if (g.cols <= 1024 || (g.cols <= 8192 && g.rows >= 16LL * sb_sm_count())) {
+    const long long blocks = (g.rows + 3) / 4, most = 64LL * sb_sm_count();
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    if (g.mask) SB_CUDA(sb_launch(log_probs_warp_kernel<T, true>, grid, dim3(128), 0, s, 1, g));
+    else SB_CUDA(sb_launch(log_probs_warp_kernel<T, false>, grid, dim3(128), 0, s, 1, g));
+    SB_COUNT_LAUNCH();
+    return SB_OK;
+  }
   int blocks = 1;
   while (blocks < 8 && g.rows * blocks * 2 <= 2LL * sb_sm_count() && g.cols / (2 * blocks) >= 4096) blocks *= 2;
   if (blocks > 1) return launch_log_probs_long<T, 512, true>(g, blocks, s);
-  if (g.cols <= 4096) return launch_log_probs_long<T, 128, false>(g, 1, s);
-  return launch_log_probs_long<T, 256, false>(g, 1, s);
+  // Threads of a row, 8 alternatives, 128 / 256 / 512: 4096 x 20000 53 / 61 / 114, 4096 x 50001 114 / 103 / 139, 1024 x 130000 80 / 73 / 66.
+  if (g.cols <= 24576) return launch_log_probs_long<T, 128, false>(g, 1, s);
+  if (g.cols <= 98304) return launch_log_probs_long<T, 256, false>(g, 1, s);
+  return launch_log_probs_long<T, 512, false>(g, 1, s);
 }
 
 template <typename T>
 int launch_log_probs_grad(const LogProbGradArgs& g, cudaStream_t s) {
-  if (g.mask_cols <= 256) {
-    const int lanes = g.mask_cols <= 16 ? 4 : g.mask_cols <= 64 ? 8 : 32;
+  if (g.mask_cols <= 64) {
+    const int lanes = g.mask_cols <= 16 ? 4 : 8;
     const long long blocks = (g.rows * lanes + 255) / 256, most = 32LL * sb_sm_count();
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
     if (lanes == 4) SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 4>, grid, dim3(256), 0, s, 1, g));
-    else if (lanes == 8) SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 8>, grid, dim3(256), 0, s, 1, g));
-    else SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 32>, grid, dim3(256), 0, s, 1, g));
+    else SB_CUDA(sb_launch(log_probs_grad_short_kernel<T, 8>, grid, dim3(256), 0, s, 1, g));
+    SB_COUNT_LAUNCH();
+    return SB_OK;
+  }
+  // A warp per row where that keeps the chip busy.
+  if (g.mask_cols <= 4096 && g.rows * 8 >= (long long)sb_sm_count() * (g.mask_cols / 64)) {
+    const long long blocks = (g.rows + 7) / 8, most = 64LL * sb_sm_count();
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    if (g.mask) SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, true, 32>, grid, dim3(256), 0, s, 1, g));
+    else SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, false, 32>, grid, dim3(256), 0, s, 1, g));
     SB_COUNT_LAUNCH();
     return SB_OK;
   }
@@ -739,8 +1058,8 @@ int launch_log_probs_grad(const LogProbGradArgs& g, cudaStream_t s) {
   long long across = (8LL * sb_sm_count() + g.rows - 1) / g.rows;
   if (across > (g.mask_cols + batch - 1) / batch) across = (g.mask_cols + batch - 1) / batch;
   const dim3 grid((unsigned)across, (unsigned)(g.rows < 65535 ? g.rows : 65535));
-  if (g.mask) SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, true>, grid, dim3(256), 0, s, 1, g));
-  else SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, false>, grid, dim3(256), 0, s, 1, g));
+  if (g.mask) SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, true, 256>, grid, dim3(256), 0, s, 1, g));
+  else SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, false, 256>, grid, dim3(256), 0, s, 1, g));
   SB_COUNT_LAUNCH();
   return SB_OK;
 }

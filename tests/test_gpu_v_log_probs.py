@@ -88,6 +88,14 @@ def check(gpu, logits, tokens, mask=None, prefix=-1, scale=1.0, top=0, stream=No
     assert gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats, top=top_values, top_tokens=top_tokens, mask=mask,
                                     prefix=prefix, scale=scale, stream=stream) is out
     torch.cuda.synchronize()
+    return compare(out, entropy, stats, top_values, top_tokens, logits, tokens, mask, prefix, scale)
+
+
+def compare(out, entropy, stats, top_values, top_tokens, logits, tokens, mask=None, prefix=-1, scale=1.0):
+    """What a call left against the definitions."""
+    torch = _torch()
+    rows, cols = logits.shape
+    top = top_tokens.shape[1] if top_tokens is not None else 0
     lp, want_entropy, largest, log_sum = definition(logits, mask, prefix, scale)
     t = tokens.long()
     held = (t >= 0) & (t < cols)
@@ -118,6 +126,13 @@ def check_grad(gpu, logits, tokens, stats, entropy, dout, dentropy, mask=None, p
     gpu.primitives.log_probs_grad(logits, tokens, stats, dlogits, dout=dout, dentropy=dentropy, entropy=entropy, mask=mask, prefix=prefix,
                                   scale=scale, stream=stream)
     torch.cuda.synchronize()
+    return compare_grad(dlogits, name, x, tokens, stats, entropy, dout, dentropy, scale)
+
+
+def compare_grad(dlogits, name, x, tokens, stats, entropy, dout, dentropy, scale=1.0):
+    """A gradient against the definition for legal logits x."""
+    torch = _torch()
+    rows, cols = x.shape
     top, log_sum = stats[:, :1].double(), stats[:, 1:].double()
     lp = (x - top) * scale - log_sum
     p = torch.exp(lp)
@@ -284,14 +299,12 @@ def test_places_beyond_32_bits(gpu):
     out, entropy, stats = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros((rows, 2), device="cuda")
     gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats)
     torch.cuda.synchronize()
-    got = check(gpu, logits[-2:], tokens[-2:])
-    assert torch.equal(out[-2:], got[0]) and torch.equal(entropy[-2:], got[1]) and torch.equal(stats[-2:], got[2])
+    compare(out[-2:], entropy[-2:], stats[-2:], None, None, logits[-2:], tokens[-2:])
     assert (out[:-2] == out[0]).all()
-    ones = torch.ones(rows, device="cuda")
-    last = check_grad(gpu, logits[-2:], tokens[-2:], stats[-2:], entropy[-2:], ones[-2:], ones[-2:])
+    ones, x = torch.ones(rows, device="cuda"), logits[-2:].double()
     gpu.primitives.log_probs_grad(logits, tokens, stats, logits, dout=ones, dentropy=ones, entropy=entropy)
     torch.cuda.synchronize()
-    assert torch.equal(logits[-2:], last)
+    compare_grad(logits[-2:], "bf16", x, tokens[-2:], stats[-2:], entropy[-2:], ones[-2:], ones[-2:])
 
 
 @pytest.mark.parametrize("rows,cols", [(128, 12), (6, 700), (2, 9000)])
