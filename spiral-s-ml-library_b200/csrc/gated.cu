@@ -162,20 +162,24 @@ constexpr int GU_STAGING = GU_EPI_WARPS * GU_BOXES * GU_BOX;
 constexpr int GU_SMEM = 225 * 1024;
 
 struct GatedMaps {
-  CUtensorMap x, gate, up, h, g, u;
+  CUtensorMap x, w, w_half, h, g, u;            // w_half: boxes of half as many rows, for the half tiles; g, u: the halves of saved
 };
 struct GatedPlan {
-  int bf, tiles_m, tiles_f, tiles, k_blocks, stages, acc_stride, tmem_cols;
-  uint32_t idesc, b_bytes;                      // of w per stage and CTA
+  int bf, tiles_m, tiles_f, k_blocks, stages, acc_stride, tmem_cols;
+  int items, half_first;                        // items from half_first on are the halves of tiles
+  uint32_t idesc, idesc_half, b_bytes;          // of w per stage and CTA
   int boxes_out;                                // 1: outputs leave as TMA boxes
 };
 
-__device__ __forceinline__ void gated_tile(const GatedPlan& q, int tile, int& mb, int& fb) {
+// An item's row block, first column of h and columns.
+__device__ __forceinline__ void gated_item(const GatedPlan& q, int item, int& mb, int& f0, int& bf) {
+  const int tile = item < q.half_first ? item : q.half_first + (item - q.half_first) / 2;
+  bf = item < q.half_first ? q.bf : q.bf / 2;
   // Eight row blocks at a time: the CTAs that run together share rows of w and of x in L2.
   const int per_group = 8 * q.tiles_f, group = tile / per_group, first = 8 * group;
   const int rows = min(8, q.tiles_m - first), r = tile - group * per_group;
   mb = first + r % rows;
-  fb = r / rows;
+  f0 = r / rows * q.bf + (item < q.half_first ? 0 : (item - q.half_first) % 2 * bf);
 }
 
 template <typename T>
@@ -228,8 +232,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
     abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&maps.x);
-    tma_prefetch_desc(&maps.gate);
-    tma_prefetch_desc(&maps.up);
+    tma_prefetch_desc(&maps.w);
   }
   if (warp == 1) {
     if (PAIR) {
@@ -252,14 +255,15 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
   if (warp == 0 || warp == 2 + GU_EPI_WARPS) {
     const bool do_x = warp == 0;
     const uint32_t full_local = smem_u32(&bar_full[0]), full0 = PAIR ? map_to_cta(full_local, 0u) : full_local, empty0 = smem_u32(&bar_empty[0]);
-    const uint32_t tx = (PAIR ? 2u : 1u) * stage_bytes;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = worker; ok && tile < q.tiles; tile += workers) {
-      int mb, fb;
-      gated_tile(q, tile, mb, fb);
-      const int m0 = mb * TILE_M + (int)rank * 128, f0 = fb * q.bf;
+    for (int item = worker; ok && item < q.items; item += workers) {
+      int mb, f0, bf;
+      gated_item(q, item, mb, f0, bf);
+      const int m0 = mb * TILE_M + (int)rank * 128;
+      const CUtensorMap* w = bf == q.bf ? &maps.w : &maps.w_half;
+      const uint32_t b_bytes = bf == q.bf ? q.b_bytes : q.b_bytes / 2u, tx = (PAIR ? 2u : 1u) * (A_BYTES + b_bytes);
       for (int kb = 0; kb < q.k_blocks; ++kb) {
         if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) {
           ok = false;
@@ -272,10 +276,11 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
           if (PAIR) tma_load_2d_pair(dst, &maps.x, kb * 64, m0, full, one);
           else tma_load_2d(dst, &maps.x, kb * 64, m0, full, one);
         } else if (PAIR) {
-          tma_load_2d_pair(dst + A_BYTES, rank == 0u ? &maps.gate : &maps.up, kb * 64, f0, full, one);
+          // (Rows of the gate beyond f are the other projection's: outputs that are not written.)
+          tma_load_2d_pair(dst + A_BYTES, w, kb * 64, rank == 0u ? f0 : p.f + f0, full, one);
         } else {
-          tma_load_2d(dst + A_BYTES, &maps.gate, kb * 64, f0, full, one);
-          tma_load_2d(dst + A_BYTES + (uint32_t)q.bf * 128u, &maps.up, kb * 64, f0, full, one);
+          tma_load_2d(dst + A_BYTES, w, kb * 64, f0, full, one);
+          tma_load_2d(dst + A_BYTES + (uint32_t)bf * 128u, w, kb * 64, p.f + f0, full, one);
         }
         if (++stage == q.stages) {
           stage = 0;
@@ -291,7 +296,8 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
       uint32_t a_lo = a_lo0, b_lo = b_lo0, phase = 0, acc_phase = 0;
       int stage = 0, acc = 0;
       bool ok = true;
-      for (int tile = worker; ok && tile < q.tiles; tile += workers) {
+      for (int item = worker; ok && item < q.items; item += workers) {
+        const uint32_t idesc = item < q.half_first ? q.idesc : q.idesc_half;
         if (!mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY)) break;
         tc_fence_after_sync();
         const uint32_t d = tmem + (uint32_t)(acc * q.acc_stride);
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
           }
           tc_fence_after_sync();
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) umma_issue<PAIR, false>(d, a_lo + 2u * i, a_hi, b_lo + 2u * i, b_hi, q.idesc, kb > 0 || i > 0 ? 1u : 0u, one);
+          for (uint32_t i = 0; i < 4; ++i) umma_issue<PAIR, false>(d, a_lo + 2u * i, a_hi, b_lo + 2u * i, b_hi, idesc, kb > 0 || i > 0 ? 1u : 0u, one);
           if (PAIR) tc_commit_pair(empty0 + 8u * (uint32_t)stage, (uint16_t)3, one);
           else tc_commit(empty0 + 8u * (uint32_t)stage, one);
           a_lo += step;
@@ -327,27 +333,25 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
     const bool keep = p.saved != nullptr;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int tile = worker; tile < q.tiles; tile += workers) {
-      int mb, fb;
-      gated_tile(q, tile, mb, fb);
-      const int row0 = mb * TILE_M + (int)rank * 128 + quad * 32, f0 = fb * q.bf;
+    for (int item = worker; item < q.items; item += workers) {
+      int mb, f0, bf;
+      gated_item(q, item, mb, f0, bf);
+      const int row0 = mb * TILE_M + (int)rank * 128 + quad * 32;
       const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * q.acc_stride);
       if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abortp, SB_SITE_EPI_TMEM_FULL)) break;
       tc_fence_after_sync();
-      bool released = false;
-      for (int c = 32 * half; c < q.bf; c += 64) {
+      for (int c = 32 * half; c < bf; c += 64) {
         uint32_t raw_g[32], raw_u[32];
         tmem_ld32(t_row + (uint32_t)c, raw_g);
-        tmem_ld32(t_row + (uint32_t)(q.bf + c), raw_u);
+        tmem_ld32(t_row + (uint32_t)(bf + c), raw_u);
         tmem_ld_wait();
-        if (c + 64 >= q.bf) {                     // this warp's last: the accumulator is free
+        if (c + 64 >= bf) {                       // this warp's last: the accumulator is free
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) {
             if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0u));
             else mbar_arrive(smem_u32(&bar_acc_empty[acc]));
           }
-          released = true;
         }
         const int col0 = f0 + c;
         if (row0 >= p.m || col0 >= p.f) continue;
@@ -385,14 +389,6 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
                 saved[p.f + j] = sb_from_f32<T>(u[j]);
               }
             }
-        }
-      }
-      if (!released) {                            // a tile of 32 columns is one warp's
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0u));
-          else mbar_arrive(smem_u32(&bar_acc_empty[acc]));
         }
       }
       acc ^= 1;
@@ -578,25 +574,29 @@ int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
   GatedPlan q;
   memset(&q, 0, sizeof(q));
   const int tile_m = PAIR ? 256 : 128;
+  const int most = PAIR ? sb_sm_count() / 2 : sb_sm_count();
   q.bf = bf;
   q.tiles_m = (p.m + tile_m - 1) / tile_m;
   q.tiles_f = (p.f + bf - 1) / bf;
   if ((long long)q.tiles_m * q.tiles_f > 0x3fffffff) return sb_fail(SB_ERR_TOO_LARGE, "sb_gated: too many outputs");
-  q.tiles = q.tiles_m * q.tiles_f;
+  const int tiles = q.tiles_m * q.tiles_f, rest = tiles % most;
+  // A last wave of at most half the workers is cut into halves.
+  q.half_first = PAIR && tiles > most && 2 * rest <= most ? tiles - rest : tiles;
+  q.items = 2 * tiles - q.half_first;
   q.k_blocks = (p.k + 63) / 64;
   q.acc_stride = bf > 64 ? 256 : 2 * bf;
   q.tmem_cols = 2 * q.acc_stride;
   q.b_bytes = (uint32_t)bf * 128u * (PAIR ? 1u : 2u);
   q.idesc = sb_umma_idesc(gated_code<T>(), 0, 0, tile_m, 2 * bf);
+  q.idesc_half = sb_umma_idesc(gated_code<T>(), 0, 0, tile_m, bf);
   q.stages = (GU_SMEM - 1024 - GU_STAGING) / (int)(128 * 128 + q.b_bytes);
   if (q.stages > GU_MAX_STAGES) q.stages = GU_MAX_STAGES;
-  const T* w = reinterpret_cast<const T*>(p.w);
   T* saved = reinterpret_cast<T*>(p.saved);
   GatedMaps maps;
   memset(&maps, 0, sizeof(maps));
   int rc = sb_tensor_map(&maps.x, type, 2, p.x, p.m, p.k, p.ldx, 128, 64);
-  if (rc == SB_OK) rc = sb_tensor_map(&maps.gate, type, 2, w, p.f, p.k, p.ldw, bf, 64);
-  if (rc == SB_OK) rc = sb_tensor_map(&maps.up, type, 2, w + (long long)p.f * p.ldw, p.f, p.k, p.ldw, bf, 64);
+  if (rc == SB_OK) rc = sb_tensor_map(&maps.w, type, 2, p.w, 2LL * p.f, p.k, p.ldw, bf, 64);
+  if (rc == SB_OK && q.items > tiles) rc = sb_tensor_map(&maps.w_half, type, 2, p.w, 2LL * p.f, p.k, p.ldw, bf / 2, 64);
   q.boxes_out = gated_rows16(p.h, p.ldh, gated_code<T>()) && (!saved || (gated_rows16(saved, p.lds, gated_code<T>()) && p.f % 8 == 0)) ? 1 : 0;
   if (q.boxes_out) {
     if (rc == SB_OK) rc = sb_tensor_map(&maps.h, type, 2, p.h, p.m, p.f, p.ldh, 32, 32);
@@ -606,7 +606,7 @@ int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
   static std::atomic<bool> ready[64];
   if (rc == SB_OK) rc = sb_allow_smem(gated_umma_kernel<PAIR, T, ACT>, GU_SMEM, ready);
   if (rc != SB_OK) return rc;
-  const int most = PAIR ? sb_sm_count() / 2 : sb_sm_count(), workers = q.tiles < most ? q.tiles : most;
+  const int workers = q.items < most ? q.items : most;
   const size_t smem = 1024 + (size_t)q.stages * (128 * 128 + q.b_bytes) + GU_STAGING;
   SB_CUDA(sb_launch(gated_umma_kernel<PAIR, T, ACT>, dim3((unsigned)(PAIR ? 2 * workers : workers)), dim3(GU_THREADS), smem, s, PAIR ? 2 : 1, maps, p, q));
   SB_COUNT_LAUNCH();
@@ -626,12 +626,16 @@ int launch_gated(const GatedArgs& p, cudaStream_t s) {
   if (p.k > 0 && gated_rows16(p.x, p.m == 1 ? 8 : p.ldx, gated_code<T>()) && gated_rows16(p.w, p.ldw, gated_code<T>())) {
     if (p.m <= 8) return launch_gated_few<T, ACT, 1>(p, s);
     if (p.m <= 16) return launch_gated_few<T, ACT, 2>(p, s);
-    const int sms = sb_sm_count();
-    // Tiles as wide as still fill the chip.
-    if (p.m > 128 && (long long)((p.m + 255) / 256) * ((p.f + 127) / 128) >= sms / 4) return launch_gated_umma<true, T, ACT>(p, 128, s);
-    for (int bf = 128; bf > 32; bf /= 2)
-      if ((long long)((p.m + 127) / 128) * ((p.f + bf - 1) / bf) >= sms / 2) return launch_gated_umma<false, T, ACT>(p, bf, s);
-    return launch_gated_umma<false, T, ACT>(p, 32, s);
+    // Pairs of CTAs on 256 rows and 128 columns of h, or CTAs on 128 rows and 128 or 64 columns: the least of waves x time of a tile, in us as
+    // measured.  Pairs / 128 / 64: 16384 x 4096 x 1024 176 / 198 / 238, 16384 x 512 x 512 23.2 / 23.2 / 19.5, 512 x 4096 x 1024 12.0 / 10.6 / 11.4,
+    // 256 x 4096 x 1024 11.5 / 10.0 / 9.7, 1000^3 13.3 / 14.7 / 10.7, 128 x 512 x 4096 28 / 29 / 16.
+    const int sms = sb_sm_count(), blocks = (p.k + 63) / 64;
+    const long long wide = (p.f + 127) / 128, tall = (p.m + 127) / 128, pairs = (p.m + 255) / 256 * wide, half = sms / 2;
+    const double pair_waves = (double)(pairs / half) + (pairs % half == 0 ? 0.0 : pairs > half && 2 * (pairs % half) <= half ? 0.5 : 1.0);
+    const double pair = 6.0 + pair_waves * (2.9 + 0.21 * blocks), single = 4.0 + (double)((tall * wide + sms - 1) / sms) * (2.55 + 0.28 * blocks),
+                 narrow = 4.0 + (double)((tall * ((p.f + 63) / 64) + sms - 1) / sms) * (0.15 + 0.256 * blocks);
+    if (p.m > 128 && pair <= single && pair <= narrow) return launch_gated_umma<true, T, ACT>(p, 128, s);
+    return launch_gated_umma<false, T, ACT>(p, single <= narrow ? 128 : 64, s);
   }
   const dim3 grid((unsigned)((p.m + GS_TILE - 1) / GS_TILE), (unsigned)((p.f + GS_TILE - 1) / GS_TILE));
   SB_CUDA(sb_launch(gated_simple_kernel<T, ACT>, grid, dim3(256), 0, s, 1, p));
