@@ -55,6 +55,11 @@ __device__ __forceinline__ long long lp_token(const void* tokens, int wide, long
 struct RowSums {
   float top, sum, dist;
 };
+// And the largest logits of a thread's even and odd packs.
+struct ShareSums {
+  RowSums r;
+  float top_a, top_b;
+};
 // The same, seen from `top`, which is not below its own.
 __device__ __forceinline__ void lp_raise(RowSums& r, float top, float c) {
   const float d = fmaxf(r.top - top, LP_FAR), f = exp2_approx(d * c);
@@ -313,7 +318,7 @@ __device__ __forceinline__ void lp_fast_pack(FastSums<T>& f, const SbWords<16>& 
   }
 }
 template <typename T>
-__device__ __forceinline__ RowSums lp_fast_sums(const T* x, const RowShape<T>& shape, int first, int stride, float c, float& top_a, float& top_b) {
+__device__ __forceinline__ ShareSums lp_fast_sums(const T* x, const RowShape<T>& shape, int first, int stride, float c) {
   constexpr int UNROLL = 4;
   const float low = lp_low<T>();
   FastSums<T> f = {c, low, low, low * c, 0ull, 0ull};
@@ -335,24 +340,25 @@ __device__ __forceinline__ RowSums lp_fast_sums(const T* x, const RowShape<T>& s
       sb_load_words(w[u], from + (long long)(p + u * stride) * RowShape<T>::V, p + u * stride < shape.packs);
     }
   };
+  auto take = [&](SbWords<16>* w) {
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      lp_lift<T>(w[u]);
+      if (u % 2 == 0) f.top_a = fmaxf(f.top_a, lp_largest<T>(w[u]));
+      else f.top_b = fmaxf(f.top_b, lp_largest<T>(w[u]));
+    }
+    lp_fast_raise(f);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) lp_fast_pack(f, w[u]);
+  };
   SbWords<16> now[UNROLL], next[UNROLL];
   load(now, first);
   for (int p = first; p < shape.packs; p += UNROLL * stride) {
     load(next, p + UNROLL * stride);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      lp_lift<T>(now[u]);
-      if (u % 2 == 0) f.top_a = fmaxf(f.top_a, lp_largest<T>(now[u]));
-      else f.top_b = fmaxf(f.top_b, lp_largest<T>(now[u]));
-    }
-    lp_fast_raise(f);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) lp_fast_pack(f, now[u]);
+    take(now);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) now[u] = next[u];
   }
-  top_a = f.top_a;
-  top_b = f.top_b;
   float s0, s1, d0, d1;
   unpack_f32x2(f.sum, s0, s1);
   unpack_f32x2(f.dist, d0, d1);
@@ -362,7 +368,7 @@ __device__ __forceinline__ RowSums lp_fast_sums(const T* x, const RowShape<T>& s
   const float rest = fminf(fmaxf(fmaf(r.top, c, -f.ref), -60.f), 60.f), back = exp2_approx(-rest);
   r.sum = (s0 + s1) * back;
   r.dist = (d0 + d1 - rest * (s0 + s1)) * back * __fdividef(1.f, c);
-  return r;
+  return {r, f.top_a, f.top_b};
 }
 // The fast sums of a row are right where its largest logit is neither so low (first) that what was lifted has weight beside it nor so far
 // up (second) that the reference's rounding, 2^-4 of a power of two, is not made good to the last bits.
@@ -391,10 +397,11 @@ __device__ __forceinline__ void lp_mask_pack(float* x, const uint8_t* mask) {
 
 // The same sums one logit at a time, under a mask or where the fast ones do not hold.
 template <typename T>
-__device__ __noinline__ RowSums lp_exact_sums(const T* x, const uint8_t* mask, const RowShape<T>& shape, int first, int stride, float c, float& top_a, float& top_b) {
+__device__ __noinline__ ShareSums lp_exact_sums(const T* x, const uint8_t* mask, int cols, int first, int stride, float c) {
+  const RowShape<T> shape(x, cols);
   constexpr int V = RowShape<T>::V;
   RowSums r = {LP_LOWEST, 0.f, 0.f};
-  top_a = top_b = LP_LOWEST;
+  float top_a = LP_LOWEST, top_b = LP_LOWEST;
   if (first < shape.head + shape.tail) {
     const float v = lp_logit<T>(x, mask, shape.single(first));
     r.top = top_a = fmaxf(r.top, v);
@@ -437,7 +444,7 @@ __device__ __noinline__ RowSums lp_exact_sums(const T* x, const uint8_t* mask, c
       lp_take<V>(r, v, c);
     }
   }
-  return r;
+  return {r, top_a, top_b};
 }
 
 // An order of floats as unsigned numbers.
@@ -508,14 +515,14 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_
       token = lp_token(g.tokens, g.wide_tokens, row);
       if (token >= 0 && token < g.cols) token_logit = lp_logit<T>(x, mask, (int)token);
     }
-    float top_a, top_b;
-    RowSums r = MASKED ? lp_exact_sums<T>(x, mask, shape, first, stride, c, top_a, top_b) : lp_fast_sums<T>(x, shape, first, stride, c, top_a, top_b);
+    ShareSums mine = MASKED ? lp_exact_sums<T>(x, mask, g.cols, first, stride, c) : lp_fast_sums<T>(x, shape, first, stride, c);
     if (!MASKED) {
       // The same decision in all blocks of a row: one whose own share has no logit to speak of lets the others have theirs.
-      const bool low = !__syncthreads_or(lp_not_low<T>(r.top, c));
-      if (__syncthreads_or(lp_too_high(r.top, c)) || low) r = lp_exact_sums<T>(x, nullptr, shape, first, stride, c, top_a, top_b);
+      const bool low = !__syncthreads_or(lp_not_low<T>(mine.r.top, c));
+      if (__syncthreads_or(lp_too_high(mine.r.top, c)) || low) mine = lp_exact_sums<T>(x, nullptr, g.cols, first, stride, c);
     }
-    const float mine = fmaxf(top_a, top_b);
+    RowSums r = mine.r;
+    const float own = r.top;
     float top = r.top;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -527,7 +534,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_
     }
     __syncthreads();                             // what the row before left has been read
     if (lane == 0) part[warp] = r;
-    if (g.top > 0) largest[tid] = mine;
+    if (g.top > 0) largest[tid] = own;
     if (tid == 0) hot_count = candidate_count = 0;
     __syncthreads();
     if (warp == 0) {
@@ -574,7 +581,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_
       }
       __syncthreads();
       const float least = bound;
-      if (mine >= least) hot[atomicAdd(&hot_count, 1)] = tid;
+      if (own >= least) hot[atomicAdd(&hot_count, 1)] = tid;
       __syncthreads();
       // A thread's share: its packs, then its single element.
       const int each = (shape.packs + stride - 1) / stride + 1, items = hot_count * each;
@@ -725,12 +732,13 @@ __global__ void __launch_bounds__(128, 8) log_probs_warp_kernel(LogProbArgs g) {
       token = lp_token(g.tokens, g.wide_tokens, row);
       if (token >= 0 && token < g.cols) token_logit = lp_logit<T>(x, mask, (int)token);
     }
-    float top_a, top_b;
-    RowSums r = MASKED ? lp_exact_sums<T>(x, mask, shape, lane, 32, c, top_a, top_b) : lp_fast_sums<T>(x, shape, lane, 32, c, top_a, top_b);
+    ShareSums mine = MASKED ? lp_exact_sums<T>(x, mask, g.cols, lane, 32, c) : lp_fast_sums<T>(x, shape, lane, 32, c);
     if (!MASKED) {
-      const bool low = !__any_sync(0xffffffffu, lp_not_low<T>(r.top, c));
-      if (__any_sync(0xffffffffu, lp_too_high(r.top, c)) || low) r = lp_exact_sums<T>(x, nullptr, shape, lane, 32, c, top_a, top_b);
+      const bool low = !__any_sync(0xffffffffu, lp_not_low<T>(mine.r.top, c));
+      if (__any_sync(0xffffffffu, lp_too_high(mine.r.top, c)) || low) mine = lp_exact_sums<T>(x, nullptr, g.cols, lane, 32, c);
     }
+    RowSums r = mine.r;
+    const float top_a = mine.top_a, top_b = mine.top_b;
     float top = r.top;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

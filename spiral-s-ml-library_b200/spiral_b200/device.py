@@ -278,9 +278,11 @@ def array_ptr(x, n, tag, what):
     if x is None:
         return None
     if type(x) is not DeviceArray:
-        numel = getattr(x, "numel", None)
-        if numel is not None and numel() == n and _TAG_OF.get(x.dtype) == tag and x.is_contiguous():
-            return x.data_ptr()
+        try:                                       # torch
+            if x.numel() == n and x.is_contiguous() and _TAG_OF[x.dtype] == tag:
+                return x.data_ptr()
+        except (AttributeError, KeyError, TypeError):
+            pass
     if dtype_tag(x) != tag or flat_size(x, what) != n:
         raise ValueError("%s must be %d contiguous %s values" % (what, n, tag))
     return device_ptr(x)

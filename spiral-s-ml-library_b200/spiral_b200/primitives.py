@@ -257,10 +257,10 @@ def _row_args(who, logits, tokens, mask):
 
 def _places(who, x, rows, n, tag, what):
     """Alternatives per row of a matrix that takes them; `n` is that of the other one, if there is one."""
-    shape = x.shape
+    shape = tuple(x.shape)
     if len(shape) != 2 or shape[0] != rows or (n is not None and shape[1] != n):
-        raise ValueError("%s: %s must be [%d, %s], got %s" % (who, what, rows, "n" if n is None else n, tuple(shape)))
-    return int(shape[1]), array_ptr(x, rows * shape[1], tag, what)
+        raise ValueError("%s: %s must be [%d, %s], got %s" % (who, what, rows, "n" if n is None else n, shape))
+    return shape[1], array_ptr(x, rows * shape[1], tag, what)
 
 
 def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None, top_tokens=None, mask=None, prefix=-1, scale=1.0,
