@@ -428,6 +428,12 @@ int sb_mlp_backward(int n_layers, const int* sizes, int batch, float inv_global_
                     float* grads, int with_bias, void* scratch, size_t scratch_bytes, float* loss,
                     void* stream);
 
+/* The same pass from a gradient of the logits [batch, n_out] that the caller computed (fp32; sb_log_probs_grad, for a policy gradient), after sb_mlp_forward
+ * with head 0, whose `out` are the logits. */
+int sb_mlp_backward_logits(int n_layers, const int* sizes, int batch, int in_dtype, const void* x, const void* w_compute,
+                           void* const* activations, void* const* relu_bits, const float* dlogits, float* grads, int with_bias,
+                           void* scratch, size_t scratch_bytes, void* stream);
+
 /* Where the backward pass keeps d(loss)/d(output of layer `layer`) inside `scratch`: byte offset
  * of a [batch, round_up(sizes[layer+1], 8)] matrix in the storage type.  The two dY buffers
  * alternate from layer to layer, so the matrix is intact from the moment layer `layer` has been

@@ -57,6 +57,21 @@ void param_offsets(int n_layers, const int* sizes, long long* off) {
   off[2 * n_layers] = cur;
 }
 
+// d logits that the caller computed, rounded to the storage type, rows padded with zeros.
+template <typename DyT, bool ROUND_TF32>
+__global__ void given_dy_kernel(const float* __restrict__ dlogits, DyT* __restrict__ dy, int rows, int n, int ld) {
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const long long total = (long long)rows * ld;
+  for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
+    const long long r = e / ld;
+    const int j = (int)(e - r * ld);
+    float v = j < n ? dlogits[r * n + j] : 0.f;
+    if (ROUND_TF32) v = round_tf32_rn(v);
+    dy[e] = (DyT)v;
+  }
+}
+
 // d logits of cross-entropy(masked softmax): (p * sum(t) - t) / global_batch on
 // legal entries, 0 elsewhere; also accumulates the loss.  One thread per row.
 // LD > 0: the padded row width is the compile-time LD and the column sums of
@@ -746,7 +761,7 @@ static int backward_impl(int n_layers, const int* sizes, int batch, float inv_gl
                          void* const* relu_bits, const float* probs, const uint8_t* mask,
                          const float* target, float* grads, int with_bias, void* scratch,
                          size_t scratch_bytes, float* loss, int first_layer, int last_layer, void* stream,
-                         float* const* grads_peers, int world);
+                         float* const* grads_peers, int world, const float* dlogits = nullptr);
 
 int sb_mlp_backward_range(int n_layers, const int* sizes, int batch, float inv_global_batch, int in_dtype,
                           const void* x, const void* w_compute, void* const* activations,
@@ -778,7 +793,7 @@ static int backward_impl(int n_layers, const int* sizes, int batch, float inv_gl
                          void* const* relu_bits, const float* probs, const uint8_t* mask,
                          const float* target, float* grads, int with_bias, void* scratch,
                          size_t scratch_bytes, float* loss, int first_layer, int last_layer, void* stream,
-                         float* const* grads_peers, int world) {
+                         float* const* grads_peers, int world, const float* dlogits) {
   int rc = check_layout("sb_mlp_backward", n_layers, sizes, batch, in_dtype);
   if (rc != SB_OK) return rc;
   if (!grads) return sb_fail(SB_ERR_BAD_ARG, "sb_mlp_backward: grads is null");
@@ -807,7 +822,7 @@ static int backward_impl(int n_layers, const int* sizes, int batch, float inv_gl
     if (from_top) return zero_grads();
     return SB_OK;
   }
-  if (!x || !w_compute || !probs || !target || !scratch)
+  if (!x || !w_compute || (!dlogits && (!probs || !target)) || !scratch)
     return sb_fail(SB_ERR_BAD_ARG, "sb_mlp_backward: null pointer");
   if (n_layers > 1 && !activations) return sb_fail(SB_ERR_BAD_ARG, "sb_mlp_backward: activations is null");
   for (int i = 1; i < n_layers; ++i)
@@ -840,7 +855,14 @@ static int backward_impl(int n_layers, const int* sizes, int batch, float inv_gl
   const int n_out = sizes[n_layers];
   const int ld_out = padded_out(n_out);
   bool head_bias_done = false;
-  if (from_top) {
+  if (from_top && dlogits) {
+    const dim3 blocks((unsigned)blocks_for((long long)batch * ld_out, 256));
+    if (in_dtype == SB_BF16) SB_CUDA(sb_launch(given_dy_kernel<__nv_bfloat16, false>, blocks, dim3(256), 0, s, 1, dlogits, (__nv_bfloat16*)dy_cur, batch, n_out, ld_out));
+    else if (in_dtype == SB_F16) SB_CUDA(sb_launch(given_dy_kernel<__half, false>, blocks, dim3(256), 0, s, 1, dlogits, (__half*)dy_cur, batch, n_out, ld_out));
+    else SB_CUDA(sb_launch(given_dy_kernel<float, true>, blocks, dim3(256), 0, s, 1, dlogits, (float*)dy_cur, batch, n_out, ld_out));
+    SB_COUNT_LAUNCH();
+    SB_CUDA(cudaGetLastError());
+  } else if (from_top) {
     const int blocks = blocks_for(batch, 256);
     // The head layer's bias gradient is summed by this kernel when its padded width is 8 or 16.
     head_bias_done = with_bias && first_layer == n_layers - 1 && (ld_out == 8 || ld_out == 16);
@@ -952,6 +974,14 @@ int sb_mlp_backward(int n_layers, const int* sizes, int batch, float inv_global_
   return sb_mlp_backward_range(n_layers, sizes, batch, inv_global_batch, in_dtype, x, w_compute, activations,
                                relu_bits, probs, mask, target, grads, with_bias, scratch, scratch_bytes, loss,
                                n_layers - 1, 0, stream);
+}
+
+int sb_mlp_backward_logits(int n_layers, const int* sizes, int batch, int in_dtype, const void* x, const void* w_compute,
+                           void* const* activations, void* const* relu_bits, const float* dlogits, float* grads, int with_bias,
+                           void* scratch, size_t scratch_bytes, void* stream) {
+  if (batch > 0 && !dlogits) return sb_fail(SB_ERR_BAD_ARG, "sb_mlp_backward_logits: null pointer");
+  return backward_impl(n_layers, sizes, batch, 0.f, in_dtype, x, w_compute, activations, relu_bits, nullptr, nullptr, nullptr, grads, with_bias,
+                       scratch, scratch_bytes, nullptr, n_layers - 1, 0, stream, nullptr, 1, dlogits);
 }
 
 int sb_sgd_update(float* params, const float* grads, void* w_compute, long long n, float lr,

@@ -11,9 +11,9 @@ import ctypes
 import numpy as np
 
 from . import _lib, primitives
-from .device import DeviceArray, device_ptr, stream_ptr
+from .device import DeviceArray, device_ptr, stream_ptr, values_ptr
 from . import dtypes
-from .matmul import matmul, matmul_fp8, quantize_fp8
+from .matmul import ACTIVATIONS, gated, gated_grad, matmul, matmul_fp8, matmul_int4, quantize_fp8, quantize_int4
 from .optim import AdamW
 
 HEAD_FLAGS = {"masked_softmax": _lib.EPI_MASKED_SOFTMAX, "regret_matching": _lib.EPI_REGRET_MATCHING,
@@ -194,6 +194,15 @@ class PolicyMLP:
                   self.probs.ptr,
                   device_ptr(mask), device_ptr(target), device_ptr(self.grads), int(self.with_bias),
                   self.scratch.ptr, self.scratch.nbytes, self.loss.ptr, stream_ptr(stream))
+        return self.grads
+
+    def backward_logits(self, x, dlogits, stream=None):
+        """grads <- the gradient whose part at the logits is ``dlogits`` (fp32 [batch, n_out]), after ``forward(x, head_flags=0)``,
+        which leaves the logits in ``probs``: for losses of the caller's own, a policy gradient among them
+        (``primitives.log_probs_grad``)."""
+        _lib.call("sb_mlp_backward_logits", self.n_layers, self._sizes_c, self.batch, _lib.DTYPE_CODES[self.in_dtype], device_ptr(x),
+                  self.w_compute.ptr, self._acts_c, self._bits_c, values_ptr(dlogits, self.batch * self.sizes[-1], "dlogits"),
+                  device_ptr(self.grads), int(self.with_bias), self.scratch.ptr, self.scratch.nbytes, stream_ptr(stream))
         return self.grads
 
     def backward_dp(self, x, mask, target, grads_table, world_size, rank, global_batch=None, stream=None):
@@ -399,66 +408,135 @@ class TokenPolicy:
     """A policy net whose states are sequences of ``n_tokens`` small integers (cards, actions, history; anything outside the
     vocabulary means "none"): embedding -> layer normalisation over the whole state -> a ``PolicyMLP`` with a masked-softmax
     head.  ``train_step`` is one AdamW step on the mean cross-entropy; ``forward_8bit`` answers with the dense layers in
-    8-bit floating point: ``quantize`` first.  After a step, an upload or a checkpoint the next answer quantises them anew; a
-    caller who writes ``mlp.params`` in another way calls ``quantize`` again.
+    8-bit floating point: ``quantize`` first; ``forward_4bit`` has their weights in 4 bits, for few states: ``quantize_4bit`` first.
+    After a step, an upload or a checkpoint the next answer quantises them anew; a caller who writes ``mlp.params`` in another
+    way calls ``quantize`` or ``quantize_4bit`` again.
 
-    Buffers: ``table`` fp32 [vocab, dim], ``norm_weight`` and ``norm_bias`` fp32 [n_tokens * dim], ``mlp.params``; all are
-    stepped by one ``AdamW`` (``optimizer``, states in fp32 or 'e4m3')."""
+    ``evaluate`` gives the log probabilities of actions that were taken, the entropy and the likeliest actions, and
+    ``policy_gradients`` the gradient of a loss of these two: the parts of a policy-gradient step.
 
-    def __init__(self, vocab, n_tokens, dim, hidden, n_actions, batch, in_dtype="bf16", training=False, state="f32"):
+    ``gated``: the columns, a multiple of 8, of a gated layer (``activation``) between the normalisation and the MLP, none by default.
+
+    Buffers: ``table`` fp32 [vocab, dim], ``norm_weight`` and ``norm_bias`` fp32 [n_tokens * dim], ``gated_weight`` fp32 [2 * gated,
+    n_tokens * dim], ``mlp.params``; all are stepped by one ``AdamW`` (``optimizer``, states in fp32 or 'e4m3')."""
+
+    def __init__(self, vocab, n_tokens, dim, hidden, n_actions, batch, in_dtype="bf16", training=False, state="f32", gated=None,
+                 activation="silu"):
         if in_dtype not in ("bf16", "f16"):
             raise ValueError("in_dtype must be 'bf16' or 'f16'")
         self.vocab, self.n_tokens, self.dim, self.batch = int(vocab), int(n_tokens), int(dim), int(batch)
         self.width = self.n_tokens * self.dim
         self.in_dtype = in_dtype
         self.scale = self.dim ** -0.5
-        self.mlp = PolicyMLP([self.width] + list(hidden) + [n_actions], batch, in_dtype=in_dtype, training=training)
+        self.gated = None if gated is None else int(gated)
+        self.activation = activation
+        if self.gated is not None and (self.gated < 8 or self.gated % 8 or activation not in ACTIVATIONS):
+            raise ValueError("gated must be a multiple of 8 columns (the MLP's rows are on 16 bytes) and its activation one of %s"
+                             % ", ".join(sorted(ACTIVATIONS)))
+        features = self.width if self.gated is None else self.gated
+        self.mlp = PolicyMLP([features] + list(hidden) + [n_actions], batch, in_dtype=in_dtype, training=training)
         self.table = DeviceArray.zeros((self.vocab, self.dim), "f32")
         self.norm_weight = DeviceArray.from_numpy(np.ones(self.width, np.float32))
         self.norm_bias = DeviceArray.zeros((self.width,), "f32")
         self.embedded = DeviceArray((self.batch, self.width), in_dtype)
         self.x = DeviceArray((self.batch, self.width), in_dtype)
         self.mean, self.rstd = DeviceArray((self.batch,), "f32"), DeviceArray((self.batch,), "f32")
+        self.features = self.x                    # what the MLP reads
+        if self.gated is not None:
+            self.gated_weight = DeviceArray.zeros((2 * self.gated, self.width), "f32")
+            self.gated_compute = DeviceArray.zeros((2 * self.gated, self.width), in_dtype)
+            self.gated_saved = DeviceArray((self.batch, 2 * self.gated), in_dtype) if training else None
+            self.features = DeviceArray((self.batch, self.gated), in_dtype)
         self.optimizer = None
-        self._codes = self._codes_of = None
+        self._codes = self._codes_of = self._codes4 = self._codes4_of = self._evaluated = None
+        self._logits_ready = False                # mlp.probs holds what evaluate() left
         if training:
             self.dx = DeviceArray((self.batch, self.width), in_dtype)
             self.dembedded = DeviceArray((self.batch, self.width), in_dtype)
             self.dtable = DeviceArray((self.vocab, self.dim), "f32")
             self.dnorm_weight, self.dnorm_bias = DeviceArray((self.width,), "f32"), DeviceArray((self.width,), "f32")
-            self.optimizer = AdamW([self.mlp.params, self.table, self.norm_weight, self.norm_bias],
-                                   [self.mlp.grads, self.dtable, self.dnorm_weight, self.dnorm_bias],
-                                   copies=[self.mlp.w_compute.view((self.mlp.n_params,)), None, None, None], state=state)
+            params, grads = [self.mlp.params, self.table, self.norm_weight, self.norm_bias], [self.mlp.grads, self.dtable, self.dnorm_weight, self.dnorm_bias]
+            copies = [self.mlp.w_compute.view((self.mlp.n_params,)), None, None, None]
+            if self.gated is not None:
+                self.dfeatures = DeviceArray((self.batch, self.gated), in_dtype)
+                self.dgated_weight = DeviceArray((2 * self.gated, self.width), "f32")
+                params, grads, copies = params + [self.gated_weight], grads + [self.dgated_weight], copies + [self.gated_compute]
+            self.optimizer = AdamW(params, grads, copies=copies, state=state)
 
-    def load_weights(self, table, weights, biases=None, norm_weight=None, norm_bias=None):
-        """Uploads fp32 host weights: the table, the layers' [out, in] matrices (and biases), the normalisation's vectors."""
+    def load_weights(self, table, weights, biases=None, norm_weight=None, norm_bias=None, gated=None):
+        """Uploads fp32 host weights: the table, the layers' [out, in] matrices (and biases), the normalisation's vectors, the
+        gated layer's matrix."""
         self.table.upload(np.asarray(table, np.float32))
         self.mlp.load_weights(weights, biases)
         if norm_weight is not None:
             self.norm_weight.upload(np.asarray(norm_weight, np.float32))
         if norm_bias is not None:
             self.norm_bias.upload(np.asarray(norm_bias, np.float32))
+        if gated is not None:
+            if self.gated is None:
+                raise ValueError("the net has no gated layer")
+            self.gated_weight.upload(np.asarray(gated, np.float32))
+            self.gated_compute.upload(np.asarray(gated, np.float32))
         return self
 
     def _input(self, tokens, stream):
+        self._logits_ready = False
         by_token = (self.batch * self.n_tokens, self.dim)
         primitives.embedding(tokens, self.table, self.embedded.view(by_token), scale=self.scale, stream=stream)
         primitives.layer_norm(self.embedded, self.x, self.norm_weight, self.norm_bias, mean=self.mean, rstd=self.rstd, stream=stream)
+        if self.gated is not None:
+            gated(self.x, self.gated_compute, self.features, activation=self.activation, saved=self.gated_saved, stream=stream)
 
     def forward(self, tokens, mask=None, stream=None):
         """Action probabilities fp32 [batch, n_actions] for ``tokens`` (int32 or int64, [batch, n_tokens])."""
         self._input(tokens, stream)
-        return self.mlp.forward(self.x, mask, stream=stream)
+        return self.mlp.forward(self.features, mask, stream=stream)
+
+    def evaluate(self, tokens, actions, mask=None, top=0, scale=1.0, stream=None):
+        """Log probabilities of ``actions`` (int32 or int64 [batch]) under the policy at the temperature 1 / ``scale``: a dict of ``log_probs`` and
+        ``entropy`` fp32 [batch] and, where ``top`` > 0, ``top_log_probs`` fp32 and ``top_actions`` int32 [batch, top], the likeliest.  The
+        logits stay in ``mlp.probs`` for ``policy_gradients``."""
+        held = self._evaluated
+        if held is None or held["top_actions"].shape[1] != top:
+            held = self._evaluated = {"log_probs": DeviceArray((self.batch,), "f32"), "entropy": DeviceArray((self.batch,), "f32"),
+                                      "stats": DeviceArray((self.batch, 2), "f32"), "top_log_probs": DeviceArray((self.batch, top), "f32"),
+                                      "top_actions": DeviceArray((self.batch, top), "i32")}
+        self._input(tokens, stream)
+        logits = self.mlp.forward(self.features, head_flags=0, stream=stream)
+        primitives.log_probs(logits, actions, held["log_probs"], entropy=held["entropy"], stats=held["stats"], top=held["top_log_probs"],
+                             top_tokens=held["top_actions"], mask=mask, scale=scale, stream=stream)
+        self._logits_ready = True
+        return {k: v for k, v in held.items() if k != "stats" and (top or not k.startswith("top"))}
+
+    def policy_gradients(self, tokens, actions, dlog_probs, dentropy=None, mask=None, scale=1.0, stream=None):
+        """Gradient of a loss whose derivatives by the log probabilities and the entropies of ``evaluate`` are ``dlog_probs`` and ``dentropy``
+        (fp32 [batch]; a PPO or REINFORCE step's advantages times its ratios, over the batch): fills the gradients that ``optimizer``
+        steps by.  Called after ``evaluate`` of the same states, actions, mask and scale, once: the gradient takes the logits' place."""
+        if not self.mlp.training:
+            raise ValueError("the net was not built for training")
+        if not self._logits_ready:
+            raise ValueError("evaluate() the states first: the logits are not, or no longer, those of this batch")
+        held, self._logits_ready = self._evaluated, False
+        primitives.log_probs_grad(self.mlp.probs, actions, held["stats"], self.mlp.probs, dout=dlog_probs, dentropy=dentropy,
+                                  entropy=held["entropy"], mask=mask, scale=scale, stream=stream)
+        self.mlp.backward_logits(self.features, self.mlp.probs, stream=stream)
+        self._input_gradients(tokens, stream)
 
     def gradients(self, tokens, mask, target, stream=None):
         """Forward and backward pass: fills ``mlp.grads``, ``dtable``, ``dnorm_weight`` and ``dnorm_bias`` with the gradient of
         the mean cross-entropy and adds that to ``mlp.loss``."""
         self.forward(tokens, mask, stream=stream)
-        self.mlp.backward(self.x, mask, target, stream=stream)
+        self.mlp.backward(self.features, mask, target, stream=stream)
+        self._input_gradients(tokens, stream)
+
+    def _input_gradients(self, tokens, stream):
         # Into the input: what the first layer left behind times its weights (rows padded alike to multiples of 8).
         dy = self.mlp.layer_dy(0)
-        w = self.mlp.w_compute.view((dy.shape[1], self.width), self.in_dtype, self.mlp.offsets[0] * 2)
-        matmul(False, False, 1.0, dy, w, 0.0, self.dx, stream=stream)
+        w = self.mlp.w_compute.view((dy.shape[1], self.mlp.sizes[0]), self.in_dtype, self.mlp.offsets[0] * 2)
+        matmul(False, False, 1.0, dy, w, 0.0, self.dx if self.gated is None else self.dfeatures, stream=stream)
+        if self.gated is not None:
+            gated_grad(self.dfeatures, self.x, self.gated_compute, self.gated_saved, dx=self.dx, dw=self.dgated_weight, activation=self.activation,
+                       stream=stream)
         primitives.layer_norm_grad(self.dx, self.embedded, self.mean, self.rstd, self.dembedded, self.norm_weight,
                                    self.dnorm_weight, self.dnorm_bias, stream=stream)
         primitives.embedding_grad(tokens, self.dembedded.view((self.batch * self.n_tokens, self.dim)), self.dtable,
@@ -493,7 +571,7 @@ class TokenPolicy:
         if self._codes_of != self._weight_changes():
             self.quantize(stream=stream)
         self._input(tokens, stream)
-        x = self.x
+        x = self.features
         for layer, (codes, scales, x_codes, x_scales) in enumerate(self._codes):
             last = layer == self.mlp.n_layers - 1
             out = self.mlp.probs if last else self.mlp.activations[layer]
@@ -501,5 +579,33 @@ class TokenPolicy:
             quantize_fp8(x, x_codes, x_scales, stream=stream)
             matmul_fp8(x_codes, x_scales, codes, scales, out, epilogue=("bias",) if last else ("bias", "relu"), bias=bias,
                        stream=stream)
+            x = out
+        return primitives.softmax(self.mlp.probs, mask=mask, stream=stream)
+
+    def quantize_4bit(self, group=128, stream=None):
+        """4-bit codes of the dense layers' weights, a scale per ``group`` columns of a row, for ``forward_4bit``."""
+        sizes = self.mlp.sizes
+        if self._codes4 is None or self._codes4[0] != group:
+            self._codes4 = group, [(DeviceArray((o, (i + 1) // 2), "u8"), DeviceArray((-(-i // group), o), self.in_dtype)) for i, o in zip(sizes, sizes[1:])]
+        for layer, (codes, scales) in enumerate(self._codes4[1]):
+            w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
+            quantize_int4(w, codes, scales, group=group, stream=stream)
+        self._codes4_of = self._weight_changes()
+        return self
+
+    def forward_4bit(self, tokens, mask=None, stream=None):
+        """``forward`` with the MLP's weights in 4 bits: for few states, whose answer waits for the weights."""
+        if self._codes4 is None:
+            raise ValueError("quantize_4bit() the weights first")
+        group, layers = self._codes4
+        if self._codes4_of != self._weight_changes():
+            self.quantize_4bit(group, stream=stream)
+        self._input(tokens, stream)
+        x = self.features
+        for layer, (codes, scales) in enumerate(layers):
+            last = layer == self.mlp.n_layers - 1
+            out = self.mlp.probs if last else self.mlp.activations[layer]
+            bias = self.mlp.params.view((self.mlp.sizes[layer + 1],), "f32", self.mlp.offsets[2 * layer + 1] * 4)
+            matmul_int4(x, codes, scales, out, group=group, epilogue=("bias",) if last else ("bias", "relu"), bias=bias, stream=stream)
             x = out
         return primitives.softmax(self.mlp.probs, mask=mask, stream=stream)
