@@ -81,10 +81,6 @@ struct SbPeerOut {
   int n;
   void* c[8];
 };
-// Elements between the rows of a product's matrices, where they are not packed (split-K partials are).
-struct SbPitches {
-  long long a, b, c;
-};
 // True when a GEMM with an [M, N] fp32 output can add its rows to n ranks' copies (sb_umma_gemm_launch
 // with peer_out): whole 128-row blocks per rank, at most 8 ranks, rows that can leave as TMA boxes.
 bool sb_umma_peer_out_ok(int M, int N, int n);
@@ -93,7 +89,7 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
                         int epi, const float* bias, const uint8_t* mask, const void* aux_in,
                         void* aux_out, cudaStream_t stream, int splits = 1, int* splits_used = nullptr,
                         const SbRowHead* head = nullptr, void* split_partials = nullptr,
-                        const SbPeerOut* peer_out = nullptr, bool three_products = false, const SbPitches* pitches = nullptr);
+                        const SbPeerOut* peer_out = nullptr, bool three_products = false);
 // `three_products` (SB_TF32 only): A and B are [2, ...] stacks of two matrices each, a high and a low part, and the
 // product is Ah Bh + Ah Bl + Al Bh.
 // True when a row head over N columns (legal columns j < prefix when prefix >= 0) runs inside the GEMM.

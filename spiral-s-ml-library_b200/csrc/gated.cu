@@ -207,6 +207,18 @@ __device__ __forceinline__ void gated_to_box(uint32_t box, int lane, const float
                                                     gated_pack<T>(v[8 * q + 4], v[8 * q + 5]), gated_pack<T>(v[8 * q + 6], v[8 * q + 7])));
 }
 
+// For outputs that no box takes: lanes' rows of 32 values to 4 KB of shared memory, from where the lanes take a row's columns.
+__device__ __forceinline__ void gated_turn(uint32_t to, int lane, const float* v) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 128u * (uint32_t)lane + 4u * (uint32_t)(j ^ lane)), "f"(v[j]) : "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ float gated_turned(uint32_t at, int lane, int row) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + 128u * (uint32_t)row + 4u * (uint32_t)(lane ^ row)) : "memory");
+  return v;
+}
+
 template <bool PAIR, typename T, int ACT>
 __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_constant__ GatedMaps maps, const GatedArgs p, const GatedPlan q) {
   extern __shared__ uint8_t gu_smem[];
@@ -377,18 +389,33 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
             }
             bulk_commit_group();
           }
-        } else if (row0 + lane < p.m) {
-          T* h = reinterpret_cast<T*>(p.h) + (long long)(row0 + lane) * p.ldh + col0;
-          T* saved = keep ? reinterpret_cast<T*>(p.saved) + (long long)(row0 + lane) * p.lds + col0 : nullptr;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col0 + j < p.f) {
-              h[j] = sb_from_f32<T>(gated_act<ACT>(g[j]) * u[j]);
-              if (saved) {
-                saved[j] = sb_from_f32<T>(g[j]);
-                saved[p.f + j] = sb_from_f32<T>(u[j]);
-              }
+        } else {
+          const bool mine = col0 + lane < p.f;
+          const int rows = min(32, p.m - row0);
+          T* saved = reinterpret_cast<T*>(p.saved) + (long long)row0 * p.lds + col0 + lane;
+          T* h = reinterpret_cast<T*>(p.h) + (long long)row0 * p.ldh + col0 + lane;
+          if (keep) {
+            gated_turn(boxes, lane, g);
+            for (int i = 0; i < rows; ++i) {
+              const float v = gated_turned(boxes, lane, i);
+              if (mine) saved[(long long)i * p.lds] = sb_from_f32<T>(v);
             }
+            __syncwarp();
+            gated_turn(boxes, lane, u);
+            for (int i = 0; i < rows; ++i) {
+              const float v = gated_turned(boxes, lane, i);
+              if (mine) saved[(long long)i * p.lds + p.f] = sb_from_f32<T>(v);
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) g[j] = gated_act<ACT>(g[j]) * u[j];
+          gated_turn(boxes, lane, g);
+          for (int i = 0; i < rows; ++i) {
+            const float v = gated_turned(boxes, lane, i);
+            if (mine) h[(long long)i * p.ldh] = sb_from_f32<T>(v);
+          }
+          __syncwarp();
         }
       }
       acc ^= 1;
@@ -537,18 +564,319 @@ __global__ void __launch_bounds__(256) gated_act_grad_kernel(GatedGradArgs p) {
   }
 }
 
-// out (+)= the sum of `splits` packed [rows, cols] matrices, in their order.
-template <typename Out>
-__global__ void __launch_bounds__(256) gated_join_kernel(const float* partial, Out* out, long long ld, long long rows, int cols, int splits, int accumulate) {
+// ---- the gradient's products -----------------------------------------------------------------------------------
+// dx = d w (d [m, 2 f], w [2 f, k]) and dw (+)= d^T x in one persistent launch of pairs of CTAs on tiles of 256 x bn, 128 of K per stage.  B has
+// rows of K in both; A does in dw alone.  As many tiles as fill the workers are whole; the rest are cut into parts of K, which leave fp32 sums for
+// the launch that joins them: one wave of short parts where two launches would have had a wave of few tiles each.  Bound by the tensor cores: 0.78 us
+// per 128 of K and 256 x 256 sums, 1.6 PFLOP/s over the card.  With the launch before and the join, against a launch for each product with K cut
+// there (us): 8192 x 4096 x 1024 249 -> 230, 4001 x 3000 x 1000 122 -> 110, 2048^3 73 -> 65, 4096 x 512 x 2048 62 -> 44, 4096 x 2048 x 512 88 -> 50,
+// 512^3 24 -> 17, 65536 x 256 x 216 87 -> 89, 128 x 4096 x 1024 35 -> 35.
+//   warp 0: TMA of A      warp 10: TMA of B      warp 1: MMAs      warps 2 .. 9: epilogue, as above
+constexpr int GP_BOX = 32 * 128;                // 32 rows of 32 fp32 columns on their way to memory
+constexpr int GP_STAGING = GU_EPI_WARPS * GP_BOX;
+constexpr uint32_t GP_A_BYTES = 128 * 256;      // of a stage and CTA: 128 rows (or columns) by 128 of K
+
+struct ProductsMaps {
+  CUtensorMap a[2], b[2], out[2];               // dx, dw
+};
+struct GatedProduct {
+  void* out;
+  long long ld;
+  int rows, cols;
+  int tiles_m, tiles_n, whole, parts;           // tiles from `whole` on are cut into `parts`
+  int k_blocks;
+  int a_mn, f32, accumulate, boxes;             // boxes: outputs leave as TMA boxes
+  uint32_t idesc;
+};
+struct ProductsPlan {
+  GatedProduct p[2];
+  int bn, stages, items;
+  uint32_t b_bytes;                             // of a stage and CTA
+  float* partial;
+};
+struct ProductsItem {
+  int which, tile, kb0, kb1;
+  long long part;                               // of all parts, -1: a whole tile
+};
+
+__device__ __forceinline__ ProductsItem products_item(const ProductsPlan& q, int item) {
+  ProductsItem t;
+  const int w0 = q.p[0].whole, w1 = q.p[1].whole;
+  if (item < w0 + w1) {
+    t.which = item < w0 ? 0 : 1;
+    t.tile = t.which == 0 ? item : item - w0;
+    t.kb0 = 0;
+    t.kb1 = q.p[t.which].k_blocks;
+    t.part = -1;
+    return t;
+  }
+  int r = item - w0 - w1;
+  const int first = (q.p[0].tiles_m * q.p[0].tiles_n - w0) * q.p[0].parts;
+  t.which = r < first ? 0 : 1;
+  t.part = r;
+  if (t.which == 1) r -= first;
+  const GatedProduct& p = q.p[t.which];
+  t.tile = p.whole + r / p.parts;
+  const int part = r % p.parts;
+  t.kb0 = (int)((long long)p.k_blocks * part / p.parts);
+  t.kb1 = (int)((long long)p.k_blocks * (part + 1) / p.parts);
+  if (p.parts == 1) t.part = -1;
+  return t;
+}
+// Eight row blocks at a time, as above.
+__device__ __forceinline__ void products_tile(const GatedProduct& p, int bn, int tile, int& row0, int& col0) {
+  const int per_group = 8 * p.tiles_n, group = tile / per_group, first = 8 * group;
+  const int rows = min(8, p.tiles_m - first), r = tile - group * per_group;
+  row0 = (first + r % rows) * 256;
+  col0 = r / rows * bn;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(GU_THREADS, 1) gated_products_kernel(const __grid_constant__ ProductsMaps maps, const __grid_constant__ ProductsPlan q) {
+  extern __shared__ uint8_t gu_smem[];
+  __shared__ __align__(8) uint64_t bar_full[GU_MAX_STAGES], bar_empty[GU_MAX_STAGES], bar_acc_full[2], bar_acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_cta_rank();
+  const int worker = (int)(blockIdx.x >> 1), workers = (int)(gridDim.x >> 1);
+  const uint32_t base = (smem_u32(gu_smem) + 1023u) & ~1023u;
+  const uint32_t stage_bytes = GP_A_BYTES + q.b_bytes;
+  if (tid == 0) {
+    for (int i = 0; i < q.stages; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 1);
+      mbar_init(smem_u32(&bar_acc_empty[i]), 2 * GU_EPI_WARPS);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(&tmem_slot), (uint32_t)(2 * q.bn));
+    tmem_relinquish_pair();
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &abort_flag;
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const long long total = rows * cols;
-  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-    float sum = 0.f;
-    for (int i = 0; i < splits; ++i) sum += partial[i * total + e];
-    const long long r = e / cols;
-    Out* o = out + r * ld + (e - r * cols);
-    *o = sb_from_f32<Out>(accumulate ? sum + sb_to_f32<Out>(*o) : sum);
+
+  const bool one = elect_one_lane();
+  if (warp == 0 || warp == 2 + GU_EPI_WARPS) {
+    const bool do_a = warp == 0;
+    const uint32_t full_local = smem_u32(&bar_full[0]), full0 = map_to_cta(full_local, 0u), empty0 = smem_u32(&bar_empty[0]);
+    const uint32_t tx = 2u * stage_bytes;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = worker; ok && item < q.items; item += workers) {
+      const ProductsItem t = products_item(q, item);
+      const GatedProduct& p = q.p[t.which];
+      int m0, n0;
+      products_tile(p, q.bn, t.tile, m0, n0);
+      m0 += (int)rank * 128;
+      n0 += (int)rank * (q.bn / 2);
+      const CUtensorMap *a = &maps.a[t.which], *b = &maps.b[t.which];
+      for (int kb = t.kb0; kb < t.kb1; ++kb) {
+        if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) {
+          ok = false;
+          break;
+        }
+        const uint32_t full = full0 + 8u * (uint32_t)stage, dst = base + (uint32_t)stage * stage_bytes;
+        if (do_a) {
+          // The leader arms its barrier with the bytes of both CTAs.
+          if (one && rank == 0u) mbar_arrive_expect_tx(full_local + 8u * (uint32_t)stage, tx);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tma_load_2d_pair(dst + (uint32_t)i * (GP_A_BYTES / 2), a, p.a_mn ? m0 + 64 * i : kb * 128 + 64 * i, p.a_mn ? kb * 128 : m0, full, one);
+        } else {
+          for (int i = 0; i < q.bn / 128; ++i)
+            tma_load_2d_pair(dst + GP_A_BYTES + (uint32_t)i * 16384u, b, n0 + 64 * i, kb * 128, full, one);
+        }
+        if (++stage == q.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0u) {
+      // Rows of K: segments of 64 columns 16384 bytes apart, 16 of K 2048.  Otherwise 16 of K are 32 bytes apart, 64 a slab.
+      const uint64_t a_cols = umma_smem_desc(base, 16u, 1024u, 2u), a_rows = umma_smem_desc(base, 16384u, 1024u, 2u),
+                     b_rows = umma_smem_desc(base + GP_A_BYTES, 16384u, 1024u, 2u);
+      const uint32_t hi = (uint32_t)(a_cols >> 32);            // the same in all three
+      const uint32_t step = stage_bytes >> 4, full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+      uint32_t phase = 0, acc_phase = 0, at = 0;
+      int stage = 0, acc = 0;
+      bool ok = true;
+      for (int item = worker; ok && item < q.items; item += workers) {
+        const ProductsItem t = products_item(q, item);
+        const bool mn = q.p[t.which].a_mn != 0;
+        const uint32_t idesc = q.p[t.which].idesc, a_lo0 = mn ? (uint32_t)a_rows : (uint32_t)a_cols, near = mn ? 128u : 2u, far = mn ? 512u : 1024u;
+        if (!mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), acc_phase ^ 1u, abortp, SB_SITE_MMA_TMEM_EMPTY)) break;
+        tc_fence_after_sync();
+        const uint32_t d = tmem + (uint32_t)(acc * q.bn);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!mbar_wait_warp(full0 + 8u * (uint32_t)stage, phase, abortp, SB_SITE_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a_lo = a_lo0 + at, b_lo = (uint32_t)b_rows + at;
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i)
+            umma_issue<true, false>(d, a_lo + (i / 4) * far + (i % 4) * near, hi, b_lo + 128u * i, hi, idesc, kb > t.kb0 || i > 0 ? 1u : 0u, one);
+          tc_commit_pair(empty0 + 8u * (uint32_t)stage, (uint16_t)3, one);
+          at += step;
+          if (++stage == q.stages) {
+            stage = 0;
+            phase ^= 1u;
+            at = 0;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(smem_u32(&bar_acc_full[acc]), (uint16_t)3, one);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+    }
+  } else if (warp < 2 + GU_EPI_WARPS) {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t box = base + (uint32_t)q.stages * stage_bytes + (uint32_t)(warp - 2) * GP_BOX;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int item = worker; item < q.items; item += workers) {
+      const ProductsItem t = products_item(q, item);
+      const GatedProduct& p = q.p[t.which];
+      int row0, n0;
+      products_tile(p, q.bn, t.tile, row0, n0);
+      row0 += (int)rank * 128 + quad * 32;
+      const uint32_t t_row = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * q.bn);
+      if (!mbar_wait(smem_u32(&bar_acc_full[acc]), acc_phase, abortp, SB_SITE_EPI_TMEM_FULL)) break;
+      tc_fence_after_sync();
+      for (int c = 32 * half; c < q.bn; c += 64) {
+        uint32_t raw[32];
+        tmem_ld32(t_row + (uint32_t)c, raw);
+        tmem_ld_wait();
+        if (c + 64 >= q.bn) {                     // this warp's last: the accumulator is free
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[acc]), 0u));
+        }
+        const int col0 = n0 + c;
+        if (row0 >= p.rows || col0 >= p.cols) continue;
+        float* v = reinterpret_cast<float*>(raw);
+        if (t.part >= 0) {                        // by columns, so that the lanes' stores are neighbours
+          float* to = q.partial + ((2 * t.part + rank) * q.bn + c) * 128 + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) to[128 * j] = v[j];
+          continue;
+        }
+        // Sums in fp32 are added by the memory system, one addition per element; 16-bit ones here, rounded once.
+        if (p.accumulate && !p.f32 && row0 + lane < p.rows) {
+          const T* old = reinterpret_cast<const T*>(p.out) + (long long)(row0 + lane) * p.ld + col0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col0 + j < p.cols) v[j] += sb_to_f32<T>(old[j]);
+        }
+        if (p.boxes) {
+          if (lane == 0) bulk_wait_group_read<0>();            // the box of the chunk before has been read
+          __syncwarp();
+          if (p.f32) {
+            const uint32_t row = box + 128u * (uint32_t)lane, key = (uint32_t)lane & 7u;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) st_shared_v4(row + ((i ^ key) << 4), make_uint4(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]));
+          } else {
+            gated_to_box<T>(box, lane, v);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (p.accumulate && p.f32) tma_reduce_add_2d(&maps.out[t.which], box, col0, row0);
+            else tma_store_2d(&maps.out[t.which], box, col0, row0);
+            bulk_commit_group();
+          }
+        } else {
+          gated_turn(box, lane, v);
+          for (int i = 0; i < 32 && row0 + i < p.rows; ++i) {
+            const float value = gated_turned(box, lane, i);
+            if (col0 + lane >= p.cols) continue;
+            const long long e = (long long)(row0 + i) * p.ld + col0 + lane;
+            if (p.f32) reinterpret_cast<float*>(p.out)[e] = p.accumulate ? reinterpret_cast<float*>(p.out)[e] + value : value;
+            else reinterpret_cast<T*>(p.out)[e] = sb_from_f32<T>(value);
+          }
+          __syncwarp();
+        }
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if (lane == 0) bulk_wait_group<0>();
+    __syncwarp();
+  }
+  // The end, as above.
+  tc_fence_before_sync();
+  cluster_sync_all();
+  if (*abortp != 0) {
+    const unsigned long long t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) { }
+  }
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, (uint32_t)(2 * q.bn));
+  }
+}
+
+// Tiles cut into parts: their sums, in the order of the parts.  A block has 32 rows of 32 columns, read along the parts' columns and written along
+// the rows.
+template <typename T>
+__global__ void __launch_bounds__(256) gated_join_kernel(const __grid_constant__ ProductsPlan q) {
+  __shared__ float tile[32][33];
+  sb_grid_dependency_wait();
+  sb_grid_dependents_launch();
+  const int chunks = q.bn / 32, cut0 = q.p[0].parts > 1 ? q.p[0].tiles_m * q.p[0].tiles_n - q.p[0].whole : 0;
+  const long long first1 = (long long)(q.p[0].tiles_m * q.p[0].tiles_n - q.p[0].whole) * q.p[0].parts;
+  const int c = (int)(blockIdx.x % chunks) * 32, sub = (int)(blockIdx.x / chunks) & 7;          // the eighths of a tile's rows, four to a CTA
+  int r = (int)(blockIdx.x / chunks) >> 3;
+  const int which = r < cut0 ? 0 : 1;
+  if (which == 1) r -= cut0;
+  const GatedProduct& p = q.p[which];
+  int row0, col0;
+  products_tile(p, q.bn, p.whole + r, row0, col0);
+  row0 += 32 * sub;
+  col0 += c;
+  if (row0 >= p.rows || col0 >= p.cols) return;
+  const long long part0 = (which == 1 ? first1 : 0) + (long long)r * p.parts;
+  const int row = threadIdx.x % 32, first = threadIdx.x / 32 * 4;
+  const float* from = q.partial + ((2 * part0 + sub / 4) * q.bn + c + first) * 128 + sub % 4 * 32 + row;
+  float sum[4] = {};
+#pragma unroll 8
+  for (int i = 0; i < p.parts; ++i) {
+    const float* part = from + (long long)i * (2 * q.bn * 128);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] += __ldcs(part + 128 * j);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tile[first + j][row] = sum[j];
+  __syncthreads();
+  const int lane = threadIdx.x % 32;
+  if (col0 + lane >= p.cols) return;
+  for (int i = threadIdx.x / 32; i < 32 && row0 + i < p.rows; i += 8) {
+    const long long at = (long long)(row0 + i) * p.ld + col0 + lane;
+    const float v = tile[lane][i];
+    if (p.f32) {
+      float* o = reinterpret_cast<float*>(p.out) + at;
+      *o = p.accumulate ? *o + v : v;
+    } else {
+      T* o = reinterpret_cast<T*>(p.out) + at;
+      *o = sb_from_f32<T>(p.accumulate ? v + sb_to_f32<T>(*o) : v);
+    }
   }
 }
 
@@ -657,47 +985,63 @@ int launch_gated_act_grad(const GatedGradArgs& p, cudaStream_t s) {
   return wide ? launch_gated_act_grad<T, ACT, 8>(p, s) : launch_gated_act_grad<T, ACT, 1>(p, s);
 }
 
-// How many parts K is cut into for a product of tiles of 256 x 256, in us as measured: a tile takes 0.4 per 64 of K and 4 besides; parts are
-// written in fp32 and joined by a launch of its own.
-int gated_splits(long long rows, long long cols, long long k) {
-  const long long tiles = ((rows + 255) / 256) * ((cols + 255) / 256), blocks = (k + 63) / 64, workers = sb_sm_count() / 2;
-  int best = 1;
+// What is whole and what is cut, for the products that are not empty (rows, cols and the length of K of each; 0 rows: none): the least of the modelled
+// times, in us as measured (74 tiles of 2 / 8 / 64 times 128 of K: 9.7 / 14.4 / 73 with 256 columns, 8.2 / 10.9 / 66 with 128).  A tile takes 1.5 and
+// per 128 of K 0.78 or 0.45; parts another 4 for the launch that joins them, and their bytes to memory and back.  Returns the parts' bytes.
+struct ProductSize {
+  long long rows, cols, k;
+};
+long long gated_products_plan(const ProductSize* size, ProductsPlan* q) {
+  const long long workers = sb_sm_count() / 2;
+  long long bytes = 0;
   double least = 1e30;
-  for (int i = 1; i <= 32 && 8 * (i - 1) < blocks; ++i) {
-    const double parts = i == 1 ? 0.0 : 3.0 + 8e-6 * (double)rows * cols * i / 4.0;
-    const double t = (double)((tiles * i + workers - 1) / workers) * (0.4 * ((blocks + i - 1) / i) + 4.0) + parts;
-    if (t < least) {
-      least = t;
-      best = i;
+  for (int bn = 256; bn >= 128; bn -= 128) {
+    const double block = bn == 256 ? 0.78 : 0.45;
+    long long tiles[2], blocks[2];
+    for (int i = 0; i < 2; ++i) {
+      tiles[i] = (size[i].rows + 255) / 256 * ((size[i].cols + bn - 1) / bn);
+      blocks[i] = (size[i].k + 127) / 128;
+    }
+    const long long full = (tiles[0] + tiles[1]) / workers, most = blocks[0] > blocks[1] ? blocks[0] : blocks[1];
+    for (int first = 0; first < 2; ++first) {     // the product whose tiles are whole first
+      long long whole[2];
+      whole[first] = tiles[first] < full * workers ? tiles[first] : full * workers;
+      whole[1 - first] = full * workers - whole[first];
+      const int slow = blocks[0] >= blocks[1] ? 0 : 1;
+      const long long slow_waves = (whole[slow] + workers - 1) / workers;
+      const double waves = slow_waves * (1.5 + block * blocks[slow]) + (full - slow_waves) * (1.5 + block * blocks[1 - slow]);
+      for (int s = 1; s <= 128 && (s == 1 || 2 * s <= most); s += s < 32 ? 1 : 16) {
+        long long parts[2], items = 0, cut = 0;
+        double longest = 0.0, sum = 0.0;
+        for (int i = 0; i < 2; ++i) {
+          parts[i] = most > 0 ? (blocks[i] * s + most - 1) / most : 1;
+          if (parts[i] < 1) parts[i] = 1;
+          const long long left = tiles[i] - whole[i];
+          const double t = 1.5 + block * ((blocks[i] + parts[i] - 1) / parts[i]);
+          items += left * parts[i];
+          sum += t * left * parts[i];
+          if (parts[i] > 1) cut += left * parts[i];
+          if (left > 0 && t > longest) longest = t;
+        }
+        const double rest = items > 0 ? sum / items * ((items + workers - 1) / workers) : 0.0;
+        const double t = waves + (rest > longest ? rest : longest) + (cut > 0 ? 4.0 + 2.0e-6 * 256 * bn * cut : 0.0);
+        if (t >= least) continue;
+        least = t;
+        bytes = cut > 0 ? items * 256 * bn * 4 : 0;            // (a rest that is whole has its places in the order)
+        q->bn = bn;
+        for (int i = 0; i < 2; ++i) {
+          GatedProduct& p = q->p[i];
+          p.tiles_m = (int)((size[i].rows + 255) / 256);
+          p.tiles_n = (int)((size[i].cols + bn - 1) / bn);
+          p.k_blocks = (int)blocks[i];
+          p.whole = (int)whole[i];
+          p.parts = (int)parts[i];
+        }
+        q->items = (int)(full * workers + items);
+      }
     }
   }
-  return best;
-}
-
-template <typename Out>
-int launch_gated_join(const float* partial, void* out, long long ld, long long rows, int cols, int splits, int accumulate, cudaStream_t s) {
-  const long long blocks = (rows * cols + 255) / 256, most = 16LL * sb_sm_count();
-  SB_CUDA(sb_launch(gated_join_kernel<Out>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, s, 1, partial, reinterpret_cast<Out*>(out), ld,
-                    rows, cols, splits, accumulate));
-  SB_COUNT_LAUNCH();
-  return SB_OK;
-}
-
-// out [rows, cols] (+)= op(a) b on the tensor cores, in parts of K where that is faster.
-template <typename T>
-int gated_product(bool a_trans, const void* a, const void* b, void* out, int rows, int cols, int k, const SbPitches& ld, int out_dtype, int accumulate,
-                  float* partial, cudaStream_t s) {
-  const int splits = gated_splits(rows, cols, k);
-  if (splits == 1)
-    return sb_umma_gemm_launch(a_trans ? 1 : 0, 0, 1.f, a, b, accumulate ? 1.f : 0.f, out, rows, cols, k, gated_code<T>(), out_dtype, 0, nullptr, nullptr,
-                               nullptr, nullptr, s, 1, nullptr, nullptr, nullptr, nullptr, false, &ld);
-  int used = splits;
-  const SbPitches packed = {ld.a, ld.b, cols};
-  int rc = sb_umma_gemm_launch(a_trans ? 1 : 0, 0, 1.f, a, b, 0.f, partial, rows, cols, k, gated_code<T>(), SB_F32, 0, nullptr, nullptr, nullptr, nullptr, s,
-                               splits, &used, nullptr, nullptr, nullptr, false, &packed);
-  if (rc != SB_OK) return rc;
-  return out_dtype == SB_F32 ? launch_gated_join<float>(partial, out, ld.c, rows, cols, used, accumulate, s)
-                             : launch_gated_join<T>(partial, out, ld.c, rows, cols, used, accumulate, s);
+  return bytes;
 }
 
 template <typename T, typename Out>
@@ -718,20 +1062,69 @@ struct GatedGradOut {
   float* partial;
 };
 
+// dx and dw, those that are wanted and whose operands have rows on 16 bytes, on the tensor cores.
+template <typename T>
+int launch_gated_products(const GatedGradArgs& g, const GatedGradOut& o, bool dx, bool dw, cudaStream_t s) {
+  constexpr int CODE = gated_code<T>();
+  const CUtensorMapDataType type = CODE == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const long long f2 = 2LL * g.f, ldx = g.m == 1 ? (o.k + 7) / 8 * 8 : o.ldx;
+  const ProductSize size[2] = {{dx ? g.m : 0, o.k, f2}, {dw ? f2 : 0, o.k, g.m}};
+  ProductsPlan q;
+  ProductsMaps maps;
+  memset(&q, 0, sizeof(q));
+  memset(&maps, 0, sizeof(maps));
+  if ((size[0].rows + 255) / 256 * ((o.k + 127) / 128) + (size[1].rows + 255) / 256 * ((o.k + 127) / 128) > 0x1fffffff)
+    return sb_fail(SB_ERR_TOO_LARGE, "sb_gated_grad: too many outputs");
+  gated_products_plan(size, &q);
+  q.partial = o.partial;
+  q.b_bytes = (uint32_t)q.bn * 128u;
+  q.stages = (GU_SMEM - 1024 - GP_STAGING) / (int)(GP_A_BYTES + q.b_bytes);
+  int rc = SB_OK;
+  for (int i = 0; i < 2; ++i) {
+    GatedProduct& p = q.p[i];
+    p.rows = (int)size[i].rows;
+    p.cols = o.k;
+    if (p.rows == 0) continue;
+    p.out = i == 0 ? o.dx : o.dw;
+    p.ld = i == 0 ? o.lddx : o.lddw;
+    p.a_mn = i;
+    p.f32 = i == 1 && o.dw_dtype == SB_F32 ? 1 : 0;
+    p.accumulate = i == 1 ? o.accumulate : 0;
+    p.boxes = gated_rows16(p.out, p.ld, p.f32 ? SB_F32 : CODE) ? 1 : 0;
+    p.idesc = sb_umma_idesc(CODE, p.a_mn, 1, 256, q.bn);
+    if (rc == SB_OK) rc = sb_tensor_map(&maps.a[i], type, 2, g.d, g.m, f2, g.ldd, 128, 64);
+    if (rc == SB_OK) rc = i == 0 ? sb_tensor_map(&maps.b[i], type, 2, o.w, f2, o.k, o.ldw, 128, 64) : sb_tensor_map(&maps.b[i], type, 2, o.x, g.m, o.k, ldx, 128, 64);
+    if (rc == SB_OK && p.boxes)
+      rc = p.f32 ? sb_tensor_map(&maps.out[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.out, p.rows, p.cols, p.ld, 32, 32)
+                 : sb_tensor_map(&maps.out[i], type, 2, p.out, p.rows, p.cols, p.ld, 32, 32);
+  }
+  static std::atomic<bool> ready[64];
+  if (rc == SB_OK) rc = sb_allow_smem(gated_products_kernel<T>, GU_SMEM, ready);
+  if (rc != SB_OK) return rc;
+  const int most = sb_sm_count() / 2, workers = q.items < most ? q.items : most;
+  const size_t smem = 1024 + (size_t)q.stages * (GP_A_BYTES + q.b_bytes) + GP_STAGING;
+  SB_CUDA(sb_launch(gated_products_kernel<T>, dim3((unsigned)(2 * workers)), dim3(GU_THREADS), smem, s, 2, maps, q));
+  SB_COUNT_LAUNCH();
+  long long cut = 0;
+  for (const GatedProduct& p : q.p) cut += p.parts > 1 ? p.tiles_m * p.tiles_n - p.whole : 0;
+  if (cut > 0) {
+    SB_CUDA(sb_launch(gated_join_kernel<T>, dim3((unsigned)(cut * 8 * (q.bn / 32))), dim3(256), 0, s, 1, q));
+    SB_COUNT_LAUNCH();
+  }
+  return SB_OK;
+}
+
 template <typename T>
 int gated_grad_products(const GatedGradArgs& g, const GatedGradOut& o, cudaStream_t s) {
   constexpr int CODE = gated_code<T>();
   const int f2 = 2 * g.f;
+  if (o.k == 0) return SB_OK;
+  const bool dx = o.dx && g.m > 0, dw = o.dw && f2 > 0;
+  const bool fast_dx = dx && f2 > 0 && gated_rows16(o.w, o.ldw, CODE), fast_dw = dw && g.m > 0 && gated_rows16(o.x, g.m == 1 ? 8 : o.ldx, CODE);
   int rc = SB_OK;
-  if (o.k == 0) return rc;
-  if (o.dx && g.m > 0) {
-    if (f2 > 0 && gated_rows16(o.w, o.ldw, CODE))
-      rc = gated_product<T>(false, g.d, o.w, o.dx, g.m, o.k, f2, {g.ldd, o.ldw, o.lddx}, CODE, 0, o.partial, s);
-    else rc = launch_product_simple<T, T>({g.d, g.ldd, 1}, {o.w, 1, o.ldw}, o.dx, o.lddx, g.m, o.k, f2, 0, s);
-  }
-  if (rc != SB_OK || !o.dw || f2 == 0) return rc;
-  if (g.m > 0 && gated_rows16(o.x, g.m == 1 ? 8 : o.ldx, CODE))
-    return gated_product<T>(true, g.d, o.x, o.dw, f2, o.k, g.m, {g.ldd, g.m == 1 ? (o.ldx + 7) / 8 * 8 : o.ldx, o.lddw}, o.dw_dtype, o.accumulate, o.partial, s);
+  if (fast_dx || fast_dw) rc = launch_gated_products<T>(g, o, fast_dx, fast_dw, s);
+  if (rc == SB_OK && dx && !fast_dx) rc = launch_product_simple<T, T>({g.d, g.ldd, 1}, {o.w, 1, o.ldw}, o.dx, o.lddx, g.m, o.k, f2, 0, s);
+  if (rc != SB_OK || !dw || fast_dw) return rc;
   const Strided a = {g.d, 1, g.ldd}, b = {o.x, 1, o.ldx};
   return o.dw_dtype == SB_F32 ? launch_product_simple<T, float>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s)
                               : launch_product_simple<T, T>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s);
@@ -766,9 +1159,14 @@ int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes) {
   const char* who = "sb_gated_grad_workspace_bytes";
   if (!bytes) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
   if (m < 0 || f < 0 || k < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
-  const int a = gated_splits(m, k, 2LL * f), b = gated_splits(2LL * f, k, m);
-  const size_t dx = a > 1 ? (size_t)a * m * k * 4 : 0, dw = b > 1 ? (size_t)b * 2 * f * k * 4 : 0;
-  *bytes = gated_grad_first(m, f) + (dx > dw ? dx : dw);
+  long long most = 0;                             // of both products or either
+  for (int want = 1; want < 4; ++want) {
+    const ProductSize size[2] = {{want & 1 ? m : 0, k, 2LL * f}, {want & 2 ? 2LL * f : 0, k, m}};
+    ProductsPlan q;
+    const long long parts = m > 0 && f > 0 && k > 0 ? gated_products_plan(size, &q) : 0;
+    if (parts > most) most = parts;
+  }
+  *bytes = gated_grad_first(m, f) + (size_t)most;
   return SB_OK;
 }
 

@@ -1304,11 +1304,11 @@ EncodeTiledFn get_encode_tiled() {
 // 128-byte swizzle (box_cols * elem size must be 128 bytes), zero fill outside.
 // `swz`: SWZ_128 (16-byte chunks), SWZ_128_CHUNK32 (32-byte chunks, MN-major
 // TF32 operands) or SWZ_64 (64-byte rows, 16-bit output boxes).  `parts` > 1: that many such tensors one behind the
-// other, the part as a third coordinate of the map.  `pitch` > 0: elements between rows.
+// other, the part as a third coordinate of the map.
 enum TmapSwizzle { SWZ_128 = 0, SWZ_128_CHUNK32 = 1, SWZ_64 = 2 };
 
 int make_tmap_2d(CUtensorMap* map, const void* base, int in_dtype, long long rows, long long cols,
-                 int box_rows, int box_cols, int swz, int parts = 1, long long pitch = 0) {
+                 int box_rows, int box_cols, int swz, int parts = 1) {
   EncodeTiledFn enc = get_encode_tiled();
   if (!enc) return sb_fail(SB_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const int es = sb_dtype_size(in_dtype);
@@ -1316,8 +1316,7 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int in_dtype, long long row
                            : in_dtype == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   cuuint64_t gdim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)parts};
-  const cuuint64_t row_bytes = (cuuint64_t)(pitch > 0 ? pitch : cols) * (cuuint64_t)es;
-  cuuint64_t gstride[2] = {row_bytes, row_bytes * (cuuint64_t)rows};
+  cuuint64_t gstride[2] = {(cuuint64_t)cols * (cuuint64_t)es, (cuuint64_t)cols * (cuuint64_t)es * (cuuint64_t)rows};
   cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1u};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, dt, parts > 1 ? 3 : 2, const_cast<void*>(base), gdim, gstride, box, estr,
@@ -1546,7 +1545,7 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
                         float beta, void* C, int M, int N, int K, int in_dtype, int out_dtype,
                         int epi, const float* bias, const uint8_t* mask, const void* aux_in,
                         void* aux_out, cudaStream_t stream, int splits, int* splits_used, const SbRowHead* head,
-                        void* split_partials, const SbPeerOut* peer_out, bool three_products, const SbPitches* pitches) {
+                        void* split_partials, const SbPeerOut* peer_out, bool three_products) {
   const bool to_peers = peer_out && peer_out->n > 1;
   if (to_peers) {
     if (!sb_umma_peer_out_ok(M, N, peer_out->n) || out_dtype != SB_F32 || epi != 0 || beta != 0.0f || alpha != 1.0f)
@@ -1583,12 +1582,12 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
   plan_for_epilogue(p, in_dtype, cached_sm_count(), epi, beta, out_dtype, splits, (split_partials && splits > 1) || to_peers);
   p.N = N;
   p.alpha = alpha; p.beta = beta;
-  p.C = C; p.ldc = pitches ? pitches->c : N; p.out_dtype = out_dtype;
+  p.C = C; p.ldc = N; p.out_dtype = out_dtype;
   p.epi = epi; p.bias = bias; p.mask = mask; p.aux_in = aux_in; p.aux_out = aux_out;
 
   // TMA needs 16-byte aligned bases and row pitches.
-  const long long lda = pitches ? pitches->a : a_trans ? M : K;
-  const long long ldb = pitches ? pitches->b : b_trans ? K : N;
+  const long long lda = a_trans ? M : K;
+  const long long ldb = b_trans ? K : N;
   if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15))
     return sb_fail(SB_ERR_MISALIGNED, "GEMM operand base pointers must be 16-byte aligned");
   if ((lda * es) % 16 != 0 || (ldb * es) % 16 != 0)
@@ -1599,11 +1598,11 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
   CUtensorMap ta, tb;
   int rc;
   const int parts = p.three ? 2 : 1;
-  if (!p.a_mn) rc = make_tmap_2d(&ta, A, in_dtype, M, K, UG_BLOCK_M, p.mn_box_elems, SWZ_128, parts, lda);
-  else rc = make_tmap_2d(&ta, A, in_dtype, K, M, p.block_k, p.mn_box_elems, p.a_layout == 1u ? SWZ_128_CHUNK32 : SWZ_128, parts, lda);
+  if (!p.a_mn) rc = make_tmap_2d(&ta, A, in_dtype, M, K, UG_BLOCK_M, p.mn_box_elems, SWZ_128, parts);
+  else rc = make_tmap_2d(&ta, A, in_dtype, K, M, p.block_k, p.mn_box_elems, p.a_layout == 1u ? SWZ_128_CHUNK32 : SWZ_128, parts);
   if (rc != SB_OK) return rc;
-  if (!p.b_mn) rc = make_tmap_2d(&tb, B, in_dtype, N, K, p.pair ? p.block_n / 2 : p.block_n, p.mn_box_elems, SWZ_128, parts, ldb);
-  else rc = make_tmap_2d(&tb, B, in_dtype, K, N, p.block_k, p.mn_box_elems, p.b_layout == 1u ? SWZ_128_CHUNK32 : SWZ_128, parts, ldb);
+  if (!p.b_mn) rc = make_tmap_2d(&tb, B, in_dtype, N, K, p.pair ? p.block_n / 2 : p.block_n, p.mn_box_elems, SWZ_128, parts);
+  else rc = make_tmap_2d(&tb, B, in_dtype, K, N, p.block_k, p.mn_box_elems, p.b_layout == 1u ? SWZ_128_CHUNK32 : SWZ_128, parts);
   if (rc != SB_OK) return rc;
 
   if (splits > 1) {
@@ -1637,7 +1636,7 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
   // Row-contiguous (coalesced) stores need a 16-byte aligned base and row pitch;
   // anything else falls back to per-thread stores.  Row heads write directly.
   const int es_out = out_dtype == SB_BF16 || out_dtype == SB_F16 ? 2 : 4;
-  p.coalesced = (!(epi & EPI_HEAD_MASK) && ((long long)N * es_out) % 16 == 0 && (p.ldc * es_out) % 16 == 0 &&
+  p.coalesced = (!(epi & EPI_HEAD_MASK) && ((long long)N * es_out) % 16 == 0 &&
                  (reinterpret_cast<uintptr_t>(C) & 15) == 0 &&
                  (!(epi & SB_EPI_RELU_GRAD) || (reinterpret_cast<uintptr_t>(aux_in) & 15) == 0)) ? 1 : 0;
 
@@ -1666,7 +1665,7 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
     p.wide = (es_out == 2 && p.block_n % 64 == 0 && !(epi & SB_EPI_LN_L2) && p.epi_warps == 8) ? 1 : 0;
     for (int r = 0; r < (to_peers ? peer_out->n : 1); ++r) {
       rc = make_tmap_2d(&tc.m[r], to_peers ? peer_out->c[r] : C, cdt, p.reduce_add ? (long long)M : (long long)M * p.splits, N,
-                        32, p.wide ? 64 : 32, (es_out == 4 || p.wide) ? SWZ_128 : SWZ_64, 1, p.splits > 1 && !p.reduce_add ? 0 : p.ldc);
+                        32, p.wide ? 64 : 32, (es_out == 4 || p.wide) ? SWZ_128 : SWZ_64);
       if (rc != SB_OK) return rc;
     }
     p.tma_store = 1;
@@ -1686,7 +1685,7 @@ int sb_umma_gemm_launch(int a_trans, int b_trans, float alpha, const void* A, co
       p.num_work = p.num_tiles + rem;
       p.idesc_tail = sb_umma_idesc(in_dtype, p.a_mn, p.b_mn, 2 * UG_BLOCK_M, p.block_n / 2);
       if (!p.b_mn) {
-        rc = make_tmap_2d(&tc.b_tail, B, in_dtype, N, K, p.block_n / 4, p.mn_box_elems, SWZ_128, parts, ldb);
+        rc = make_tmap_2d(&tc.b_tail, B, in_dtype, N, K, p.block_n / 4, p.mn_box_elems, SWZ_128, parts);
         if (rc != SB_OK) return rc;
       }
     }
