@@ -574,7 +574,8 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
  *   g = x w[0 .. f)^T   u = x w[f .. 2 f)^T   h = act(g) * u
  * x [m, k], w [2 f, k] (the gate's rows, then the other projection's), h [m, f] and, where not NULL, saved [m, 2 f] = (g, u) for the
  * gradient; SB_BF16 or SB_F16, the same for all, fp32 sums, each output rounded once.  Rows of x and w that start on
- * 16 bytes run on the tensor cores, others on the CUDA cores at about 1 % of their rate.  f and k of at most 2^21. */
+ * 16 bytes run on the tensor cores, others on the CUDA cores at about 1 % of their rate.  f and k of at most 2^21, m of at most
+ * 2^30.  No output may be one of the inputs. */
 enum { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* g (1 + erf(g / sqrt 2)) / 2 */, SB_ACT_RELU = 2 };
 int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h, long long ldh, void* saved, long long lds, int m, int f,
              int k, int dtype, int activation, void* stream);
@@ -582,7 +583,7 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
  *   dg = dh u act'(g)   du = dh act(g)   dx = [dg du] w   dw = [dg du]^T x
  * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
  * the old dw.  dg and du are rounded to the storage type for the products, whose sums are fp32 in a fixed order.  workspace:
- * 256-byte aligned, at least sb_gated_grad_workspace_bytes. */
+ * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  Both products run at once: where both are wanted dx may not be x, nor dw w. */
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
 int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,
                   void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, int accumulate, int m, int f, int k, int dtype,
@@ -599,7 +600,7 @@ int sb_dequantize_int4(const uint8_t* codes, long long ldw, const void* scales, 
                        long long n, int k, int group, void* stream);
 /* c [m, n] = a w^T (+ bias) (relu) for few rows of a [m, k] (SB_BF16 or SB_F16); c in SB_F32, SB_BF16 or SB_F16, fp32 sums; epilogue:
  * SB_EPI_BIAS (fp32 [n]), SB_EPI_RELU (a NaN gives 0, as in the other products).  Made for up to 64 rows, which read the weights once;
- * more rows are right, and with many of them sb_dequantize_int4 and sb_matmul_ex are faster. */
+ * more rows, 2^22 - 64 at most, are right, and with many of them sb_dequantize_int4 and sb_matmul_ex are faster.  c may not be a. */
 int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes, long long ldw, const void* scales, int scale_dtype, void* c,
                    long long ldc, int m, int n, int k, int group, int out_dtype, int epilogue, const float* bias, void* stream);
 

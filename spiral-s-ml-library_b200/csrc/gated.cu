@@ -1146,6 +1146,7 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
   if (!h || (k > 0 && (!x || !w))) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if (ldh < f || (saved && lds < 2LL * f) || (k > 0 && (ldx < k || ldw < k)))
     return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  if (h == x || h == w || h == saved || (saved && (saved == x || saved == w))) return sb_fail(SB_ERR_BAD_ARG, "%s: outputs in the place of an input", who);
   if (!gated_element_aligned(x, dtype) || !gated_element_aligned(w, dtype) || !gated_element_aligned(h, dtype) || !gated_element_aligned(saved, dtype))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
   const GatedArgs p = {x, w, h, saved, ldx, ldw, ldh, lds, m, f, k};
@@ -1182,6 +1183,7 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
   if (any && ((dx && k > 0 && !w) || (dw && k > 0 && !x))) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if ((any && (lddh < f || lds < 2LL * f)) || (x && ldx < k) || (w && ldw < k) || (dx && lddx < k) || (dw && lddw < k))
     return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  if (dx && dw && (dx == x || dw == w || dx == dw)) return sb_fail(SB_ERR_BAD_ARG, "%s: dx or dw in the place of what the other is made from", who);
   if (!gated_element_aligned(dh, dtype) || !gated_element_aligned(saved, dtype) || !gated_element_aligned(x, dtype) || !gated_element_aligned(w, dtype) ||
       !gated_element_aligned(dx, dtype) || (dw && !gated_element_aligned(dw, dw_dtype)) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size, or the workspace not to 256 bytes", who);

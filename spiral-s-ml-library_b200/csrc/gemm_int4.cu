@@ -586,6 +586,7 @@ int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes
   if (m == 0 || n == 0) return SB_OK;
   if (!c || ((epilogue & SB_EPI_BIAS) && !bias) || (k > 0 && (!a || !codes || !scales))) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if (ldc < n || (k > 0 && (lda < k || ldw < (k + 1) / 2))) return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  if (c == a) return sb_fail(SB_ERR_BAD_ARG, "%s: c in the place of a", who);
   if (!int4_aligned(a, dtype) || !int4_aligned(scales, scale_dtype) || !int4_aligned(c, out_dtype) || !int4_aligned(bias, SB_F32))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
   Int4Args p;

@@ -495,7 +495,7 @@ class TokenPolicy:
     def evaluate(self, tokens, actions, mask=None, top=0, scale=1.0, stream=None):
         """Log probabilities of ``actions`` (int32 or int64 [batch]) under the policy at the temperature 1 / ``scale``: a dict of ``log_probs`` and
         ``entropy`` fp32 [batch] and, where ``top`` > 0, ``top_log_probs`` fp32 and ``top_actions`` int32 [batch, top], the likeliest.  The
-        logits stay in ``mlp.probs`` for ``policy_gradients``."""
+        logits stay in ``mlp.probs`` for ``policy_gradients``, and what is returned until the next call."""
         held = self._evaluated
         if held is None or held["top_actions"].shape[1] != top:
             held = self._evaluated = {"log_probs": DeviceArray((self.batch,), "f32"), "entropy": DeviceArray((self.batch,), "f32"),

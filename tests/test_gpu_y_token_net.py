@@ -254,3 +254,31 @@ def test_refusals(gpu):
         policy.policy_gradients(dt, da, D(np.zeros(8, np.float32)))              # not built for training
     with pytest.raises(ValueError):
         policy.quantize_4bit(group=48)
+
+
+@pytest.mark.parametrize("in_dtype,sizes,batch,with_bias", [("bf16", [64, 128, 64, 5], 300, True), ("f16", [40, 72, 9], 77, True), ("tf32", [36, 64, 32, 13], 200, True),
+                                                            ("bf16", [16, 40, 1], 1, True), ("f16", [64, 128], 50, False)])
+def test_backward_from_logits(gpu, in_dtype, sizes, batch, with_bias):
+    """``backward_logits`` of the cross-entropy's gradient at the logits is ``backward``."""
+    rng = np.random.default_rng(batch)
+    weights = [rng.standard_normal((o, i)) * np.sqrt(2 / i) for i, o in zip(sizes, sizes[1:])]
+    biases = [0.1 * rng.standard_normal(o) for o in sizes[1:]] if with_bias else None
+    D = gpu.DeviceArray.from_numpy
+    x = gpu.DeviceArray((batch, sizes[0]), in_dtype)
+    x.upload(rng.standard_normal((batch, sizes[0])).astype(np.float32))
+    mask = np.ones((batch, sizes[-1]), np.uint8)
+    target = softmax(rng.standard_normal((batch, sizes[-1])), mask).astype(np.float32)
+    net = gpu.PolicyMLP(sizes, batch, in_dtype=in_dtype, training=True, with_bias=with_bias).load_weights(weights, biases)
+    p = net.forward(x, D(mask)).numpy().astype(np.float64)
+    net.backward(x, D(mask), D(target))
+    want = net.grads.numpy().astype(np.float64).copy()
+    net.forward(x, head_flags=0)
+    net.backward_logits(x, D(((p * target.sum(1, keepdims=True) - target) / batch).astype(np.float32)))
+    got = net.grads.numpy().astype(np.float64)
+    # The same values at the logits but for fp32's last places, which move a rounding to the storage type here and there: 2^-8 of a value
+    # (tf32, f16: 2^-11), and so at most that of a norm.
+    for (aw, ab), (bw, bb) in zip(net.split_flat(got), net.split_flat(want)):
+        for a, b in ((aw, bw), (ab, bb)):
+            assert np.linalg.norm(a - b) <= 2 ** -8 * np.linalg.norm(b) + 1e-9
+    with pytest.raises(ValueError):
+        net.backward_logits(x, D(np.zeros((batch, sizes[-1] + 1), np.float32)))

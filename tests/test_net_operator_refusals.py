@@ -83,6 +83,8 @@ def test_gated(sb):
     for pitch in ("ldx", "ldw", "ldh"):
         refused(sb, BAD, *go(**{pitch: 7}))
     refused(sb, BAD, *go(saved=0x4000, lds=15))
+    for place in ("x", "w"):
+        refused(sb, BAD, *go(**{place: 0x3000, "h": 0x3000}))
     refused(sb, UNSUPPORTED, *go(dt=0))
     refused(sb, UNSUPPORTED, *go(act=3))
     refused(sb, LARGE, *go(f=1 << 22, ldh=1 << 22))
@@ -99,6 +101,8 @@ def test_gated_grad(sb):
     for pitch in ("lddh", "ldx", "ldw", "lds", "lddx", "lddw"):
         refused(sb, BAD, *go(**{pitch: 7}))
     refused(sb, BAD, *go(nws=100))
+    refused(sb, BAD, *go(dx=0x2000))
+    refused(sb, BAD, *go(dw=0x3000))
     refused(sb, BAD, *go(m=-1))
     refused(sb, UNSUPPORTED, *go(dwt=3))
     refused(sb, UNSUPPORTED, *go(dt=1))
