@@ -185,12 +185,26 @@ __device__ __noinline__ void int4_ask_pieces(uint32_t to, const uint8_t* from, l
   }
 }
 
+// Asks for a whole stage of 16 rows, each row's 128 bytes by neighbouring lanes.
+template <int PIECE>
+__device__ __forceinline__ void int4_ask_rows(uint32_t to, const uint8_t* lane_from, long long pitch, int lane) {
+  constexpr int ACROSS = 128 / PIECE, DOWN = 32 / ACROSS;
+  const int row = lane / ACROSS, b = lane % ACROSS * PIECE;
+#pragma unroll
+  for (int i = 0; i < 16 / DOWN; ++i, lane_from += DOWN * pitch) int4_copy<PIECE>(to + int4_code_at(row + DOWN * i, b / 16) + b % 16, lane_from, PIECE);
+}
+
+__device__ __noinline__ void int4_ask_narrow(uint32_t to, const uint8_t* lane_from, long long pitch, int lane, int piece) {
+  if (piece == 8) int4_ask_rows<8>(to, lane_from, pitch, lane);
+  else int4_ask_rows<4>(to, lane_from, pitch, lane);
+}
+
 // A warp has 16 rows of w, whose codes come to it through a ring of STAGES steps in shared memory; a block's warps share up to 8 NT
 // rows of a there, and the blocks of a cluster share K.  The V = G / 32 words of a lane (8 codes each) are of one group in all four lanes
 // of a row, so the products of a group are summed as whole numbers times elements of a, and the sums are scaled.  The blocks' sums are
 // joined in their order.
 template <typename T, int G, int NT, int WARPS, int STAGES>
-__global__ void __launch_bounds__(32 * WARPS) gemm_int4_kernel(Int4Args p, Int4Few q) {
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) gemm_int4_kernel(Int4Args p, Int4Few q) {
   constexpr int V = G / 32, PER = I4_STEP / G, COLS = 8 * NT, PITCH = COLS + 2, ROWS = 16 * WARPS;
   extern __shared__ __align__(16) uint8_t i4_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -205,16 +219,17 @@ __global__ void __launch_bounds__(32 * WARPS) gemm_int4_kernel(Int4Args p, Int4F
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const int steps = (end - begin + I4_STEP - 1) / I4_STEP, groups = (p.k + G - 1) / G, rows = min(16, p.n - r0);
-  const uint8_t* lane_codes = p.codes + (long long)(r0 + (lane >> 3)) * p.ldw + begin / 2 + 16 * (lane & 7);
+  const int across = 128 / q.code_piece;                                  // lanes that copy a row of a step
+  const uint8_t* lane_codes = p.codes + (long long)(r0 + lane / across) * p.ldw + begin / 2 + q.code_piece * (lane % across);
   // Asks for the codes of a step.
   auto ask = [&](int step, int slot) {
     if (step < steps && rows > 0) {
       const int k0 = begin + step * I4_STEP;
       const uint32_t at = ring_at + (uint32_t)(slot * I4_STAGE);
-      if (q.code_piece == 16 && rows == 16 && k0 + I4_STEP <= p.k) {
+      if (q.code_piece >= 4 && rows == 16 && k0 + I4_STEP <= p.k) {
         const uint8_t* from = lane_codes + step * (I4_STEP / 2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) int4_copy<16>(at + int4_code_at((lane >> 3) + 4 * i, lane & 7), from + i * (4 * p.ldw), 16);
+        if (q.code_piece == 16) int4_ask_rows<16>(at, from, p.ldw, lane);
+        else int4_ask_narrow(at, from, p.ldw, lane, q.code_piece);
       } else {
         // What lies beyond k meets zeros of a; rows that are not there are zero.
         const uint8_t* from = p.codes + (long long)r0 * p.ldw + k0 / 2;
@@ -462,9 +477,9 @@ int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
   constexpr int ROWS = 16 * WARPS, COLS = 8 * NT, MOST = int4_chunk<NT>, RING = WARPS * STAGES * I4_STAGE, SUMS = ROWS * (COLS + 2) * 4, LIMIT = RING + MOST * COLS * 2 + MOST / G * ROWS * 4 + SUMS;
   static_assert(LIMIT <= 227 * 1024, "more shared memory than an SM has");
   const long long tiles = ((long long)p.n + ROWS - 1) / ROWS, down = ((long long)p.m + COLS - 1) / COLS;
-  // Blocks that share K until every SM has the warps it can hold, each with 512 columns at least.
+  // Blocks that share K until every SM has the warps it can hold, each with 256 columns at least.
   int blocks = 1;
-  while (blocks < 8 && tiles * down * blocks * (WARPS / 8) <= sb_sm_count() && p.k >= 1024 * blocks) blocks *= 2;
+  while (blocks < 8 && tiles * down * blocks * (WARPS / 8) <= sb_sm_count() && p.k >= 512 * blocks) blocks *= 2;
   q.blocks = blocks;
   q.range = ((p.k + blocks - 1) / blocks + I4_STEP - 1) / I4_STEP * I4_STEP;
   q.chunk = q.range < MOST ? q.range : MOST;
