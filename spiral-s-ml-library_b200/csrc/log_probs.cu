@@ -1018,11 +1018,17 @@ int launch_log_probs_long(const LogProbArgs& g, int blocks, cudaStream_t s) {
 
 template <typename T>
 int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
-  // us, 2^17 rows of bf16 unless it says otherwise.  Rounds among the lanes of a row cost by the alternative, a bound costs once: 200 columns with 5
-  // alternatives (10^5 rows) 110 in registers, 133 by warps; with 8 of them 201 / 185; 1000 columns with none 105 / 85, with 8 488 / 232.
-  if (g.cols <= 16) return launch_log_probs_short<T, 4, 4>(g, s);
-  if (g.cols <= 64) return launch_log_probs_short<T, 8, 8>(g, s);
-  if (g.cols <= 256 && g.top <= 7) return launch_log_probs_short<T, 32, 8>(g, s);
+  // Few lanes with many columns each: their rounds cost by the lane.  us, 65536 rows: 10 columns (fp32, 2 alternatives) with 4 / 2 lanes 7.5 / 5.5; 20 with
+  // 8 / 4 14.7 / 8.1; 64 (bf16, 2) with 8 / 4 / 2 15.0 / 12.3 / 13.5; 100000 rows: 128 (bf16, none) with 32 / 8 / 4 46.8 / 20.8 / 14.9, with 32
+  // alternatives by warps, as below / 8 / 4 413 / 212 / 172; 200 (2) with 32 / 16 / 8 84.5 / 66.6 / 46.7.
+  if (g.cols <= 16) return launch_log_probs_short<T, 2, 8>(g, s);
+  if (g.cols <= 32) return launch_log_probs_short<T, 4, 8>(g, s);
+  if (g.cols <= 64) return launch_log_probs_short<T, 4, 16>(g, s);
+  if (g.cols <= 128) return launch_log_probs_short<T, 4, 32>(g, s);
+  // Rounds cost by the alternative, the warps' bound costs once: 250 columns with 16 alternatives 237 (16 lanes) / 168; 500 columns with none, 2 or 7 of
+  // them 28 / 41, 53 / 88, 59 / 41 (32768 rows of fp32); 1000 with 2 of them 54 / 45.
+  if (g.cols <= 256 && g.top <= 7) return launch_log_probs_short<T, 8, 32>(g, s);
+  if (g.cols <= 512 && g.top <= 3) return launch_log_probs_short<T, 16, 32>(g, s);
   // Warps or blocks, 8 alternatives: 32768 x 2048 69 / 152, 16384 x 8192 94 / 98, 8192 x 16384 93 / 80, 600 x 4096 11.7 / 9.3.
   if (g.cols <= 1024 || (g.cols <= 8192 && g.rows >= 16LL * sb_sm_count())) {
     const long long blocks = (g.rows + 3) / 4, most = 64LL * sb_sm_count();
@@ -1032,8 +1038,10 @@ int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
     SB_COUNT_LAUNCH();
     return SB_OK;
   }
+  // A cluster per row where rows are few, all of them resident at once: 35 x 41654 with 3 alternatives in clusters of 8, which the chip's parts hold 32
+  // of, 16.3, of 4 9.5; 70 rows 12.1 (4), 9.1 (2).
   int blocks = 1;
-  while (blocks < 8 && g.rows * blocks * 2 <= 2LL * sb_sm_count() && g.cols / (2 * blocks) >= 4096) blocks *= 2;
+  while (blocks < 8 && g.rows * blocks * 2 <= 3LL * sb_sm_count() / 2 && g.cols / (2 * blocks) >= 4096) blocks *= 2;
   if (blocks > 1) return launch_log_probs_long<T, 512, true>(g, blocks, s);
   // Threads of a row, 8 alternatives, 128 / 256 / 512: 4096 x 20000 53 / 61 / 114, 4096 x 50001 114 / 103 / 139, 1024 x 130000 80 / 73 / 66.
   if (g.cols <= 24576) return launch_log_probs_long<T, 128, false>(g, 1, s);
