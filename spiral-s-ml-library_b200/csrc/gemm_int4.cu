@@ -479,7 +479,9 @@ int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
   const long long tiles = ((long long)p.n + ROWS - 1) / ROWS, down = ((long long)p.m + COLS - 1) / COLS;
   // Blocks that share K until every SM has the warps it can hold, each with 256 columns at least.
   int blocks = 1;
-  while (blocks < 8 && tiles * down * blocks * (WARPS / 8) <= sb_sm_count() && p.k >= 512 * blocks) blocks *= 2;
+  // Not in clusters of 8 that the chip's parts have no room for at once: 16 x 4096 x 4096 in 16 of them 14.5 us, in clusters of 4 10.4.
+  const long long room = (16 / WARPS) * sb_sm_count(), room8 = WARPS == 16 ? 3 * room / 4 : 7 * room / 8;
+  while (blocks < 8 && tiles * down * blocks * 2 <= (blocks < 4 ? room : room8) && p.k >= 512 * blocks) blocks *= 2;
   q.blocks = blocks;
   q.range = ((p.k + blocks - 1) / blocks + I4_STEP - 1) / I4_STEP * I4_STEP;
   q.chunk = q.range < MOST ? q.range : MOST;
@@ -503,8 +505,12 @@ int launch_int4(const Int4Args& p, const Int4Few& q, cudaStream_t s) {
     SB_COUNT_LAUNCH();
     return SB_OK;
   }
-  if (p.m <= 8) return launch_int4<T, G, 1, 8, 4>(p, q, s);
-  if (p.m <= 16) return launch_int4<T, G, 2, 16, 4>(p, q, s);
+  // Where all blocks run at once (or, of 16 rows, nearly), fewer rows of a in each and more blocks: 48 x 201 x 12728 with 64 / 16 / 8 rows of a in a
+  // block 53 / 20.5 / 12.2 us, 64 x 1024 x 1024 15.1 / 6.5 / 5.6, 64 x 2048 x 2048 15.6 / 8.0 / 8.8, 64 x 4096 x 4096 32 / 18.6 / 23, 16 x 3000 x 6000
+  // 9.9 (16) / 14.1; larger ones read their weights again for nothing: 32 x 8192 x 8192 30 (32) / 33 / 43.
+  const long long shares = p.k >= 2048 ? 8 : p.k >= 1024 ? 4 : p.k >= 512 ? 2 : 1, sms = sb_sm_count();
+  if (p.m <= 8 || ((long long)p.n + 127) / 128 * (((long long)p.m + 7) / 8) * shares <= 2 * sms) return launch_int4<T, G, 1, 8, 4>(p, q, s);
+  if (p.m <= 16 || ((long long)p.n + 255) / 256 * (((long long)p.m + 15) / 16) * shares <= 4 * sms) return launch_int4<T, G, 2, 16, 4>(p, q, s);
   if (p.m <= 32) return launch_int4<T, G, 4, 16, 4>(p, q, s);
   return launch_int4<T, G, 8, 16, 3>(p, q, s);
 }
