@@ -582,7 +582,8 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
 /* Its gradient from dh [m, f] and what was saved:
  *   dg = dh u act'(g)   du = dh act(g)   dx = [dg du] w   dw = [dg du]^T x
  * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
- * the old dw.  dg and du are rounded to the storage type for the products, whose sums are fp32 in a fixed order.  workspace:
+ * the old dw.  dg and du are rounded to the storage type for the products (up to 64 rows and rows on 16 bytes: to two numbers of it),
+ * whose sums are fp32 in a fixed order.  workspace:
  * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  Both products run at once: where both are wanted dx may not be x, nor dw w. */
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
 int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,

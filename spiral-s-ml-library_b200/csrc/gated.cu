@@ -530,6 +530,7 @@ struct GatedGradArgs {
   const void* dh;
   const void* saved;
   void* d;                        // [m, 2 f]: dg, du
+  void* lo;                       // what their rounding left off, where it is kept
   long long lddh, lds, ldd;
   int m, f;
 };
@@ -561,6 +562,17 @@ __global__ void __launch_bounds__(256) gated_act_grad_kernel(GatedGradArgs p) {
     T* d = reinterpret_cast<T*>(p.d) + r * p.ldd + c;
     sb_store_f32<T, V>(d, g);
     sb_store_f32<T, V>(d + p.f, u);
+    if (p.lo) {
+      T* lo = reinterpret_cast<T*>(p.lo) + r * p.ldd + c;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float hg = sb_to_f32<T>(sb_from_f32<T>(g[i])), hu = sb_to_f32<T>(sb_from_f32<T>(u[i]));
+        g[i] = fabsf(hg) < INFINITY ? g[i] - hg : 0.f;
+        u[i] = fabsf(hu) < INFINITY ? u[i] - hu : 0.f;
+      }
+      sb_store_f32<T, V>(lo, g);
+      sb_store_f32<T, V>(lo + p.f, u);
+    }
   }
 }
 
@@ -577,7 +589,7 @@ constexpr int GP_STAGING = GU_EPI_WARPS * GP_BOX;
 constexpr uint32_t GP_A_BYTES = 128 * 256;      // of a stage and CTA: 128 rows (or columns) by 128 of K
 
 struct ProductsMaps {
-  CUtensorMap a[2], b[2], out[2];               // dx, dw
+  CUtensorMap a[2], a_lo[2], b[2], out[2];      // dx, dw
 };
 struct GatedProduct {
   void* out;
@@ -591,6 +603,7 @@ struct GatedProduct {
 struct ProductsPlan {
   GatedProduct p[2];
   int bn, stages, items;
+  int twice;                                    // 1: every block of K once with d and once with what its rounding left off
   uint32_t b_bytes;                             // of a stage and CTA
   float* partial;
 };
@@ -681,8 +694,10 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_products_kernel(const __g
       products_tile(p, q.bn, t.tile, m0, n0);
       m0 += (int)rank * 128;
       n0 += (int)rank * (q.bn / 2);
-      const CUtensorMap *a = &maps.a[t.which], *b = &maps.b[t.which];
-      for (int kb = t.kb0; kb < t.kb1; ++kb) {
+      const CUtensorMap* b = &maps.b[t.which];
+      for (int block = t.kb0; block < t.kb1; ++block) {
+        const int kb = block >> q.twice;
+        const CUtensorMap* a = block & q.twice ? &maps.a_lo[t.which] : &maps.a[t.which];
         if (!mbar_wait_warp(empty0 + 8u * (uint32_t)stage, phase ^ 1u, abortp, SB_SITE_PRODUCER_EMPTY)) {
           ok = false;
           break;
@@ -991,7 +1006,7 @@ int launch_gated_act_grad(const GatedGradArgs& p, cudaStream_t s) {
 struct ProductSize {
   long long rows, cols, k;
 };
-long long gated_products_plan(const ProductSize* size, ProductsPlan* q) {
+long long gated_products_plan(const ProductSize* size, int twice, ProductsPlan* q) {
   const long long workers = sb_sm_count() / 2;
   long long bytes = 0;
   double least = 1e30;
@@ -1000,7 +1015,7 @@ long long gated_products_plan(const ProductSize* size, ProductsPlan* q) {
     long long tiles[2], blocks[2];
     for (int i = 0; i < 2; ++i) {
       tiles[i] = (size[i].rows + 255) / 256 * ((size[i].cols + bn - 1) / bn);
-      blocks[i] = (size[i].k + 127) / 128;
+      blocks[i] = ((size[i].k + 127) / 128) << twice;
     }
     const long long full = (tiles[0] + tiles[1]) / workers, most = blocks[0] > blocks[1] ? blocks[0] : blocks[1];
     for (int first = 0; first < 2; ++first) {     // the product whose tiles are whole first
@@ -1075,7 +1090,8 @@ int launch_gated_products(const GatedGradArgs& g, const GatedGradOut& o, bool dx
   memset(&maps, 0, sizeof(maps));
   if ((size[0].rows + 255) / 256 * ((o.k + 127) / 128) + (size[1].rows + 255) / 256 * ((o.k + 127) / 128) > 0x1fffffff)
     return sb_fail(SB_ERR_TOO_LARGE, "sb_gated_grad: too many outputs");
-  gated_products_plan(size, &q);
+  q.twice = g.lo ? 1 : 0;
+  gated_products_plan(size, q.twice, &q);
   q.partial = o.partial;
   q.b_bytes = (uint32_t)q.bn * 128u;
   q.stages = (GU_SMEM - 1024 - GP_STAGING) / (int)(GP_A_BYTES + q.b_bytes);
@@ -1093,6 +1109,7 @@ int launch_gated_products(const GatedGradArgs& g, const GatedGradOut& o, bool dx
     p.boxes = gated_rows16(p.out, p.ld, p.f32 ? SB_F32 : CODE) ? 1 : 0;
     p.idesc = sb_umma_idesc(CODE, p.a_mn, 1, 256, q.bn);
     if (rc == SB_OK) rc = sb_tensor_map(&maps.a[i], type, 2, g.d, g.m, f2, g.ldd, 128, 64);
+    if (rc == SB_OK && q.twice) rc = sb_tensor_map(&maps.a_lo[i], type, 2, g.lo, g.m, f2, g.ldd, 128, 64);
     if (rc == SB_OK) rc = i == 0 ? sb_tensor_map(&maps.b[i], type, 2, o.w, f2, o.k, o.ldw, 128, 64) : sb_tensor_map(&maps.b[i], type, 2, o.x, g.m, o.k, ldx, 128, 64);
     if (rc == SB_OK && p.boxes)
       rc = p.f32 ? sb_tensor_map(&maps.out[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.out, p.rows, p.cols, p.ld, 32, 32)
@@ -1132,7 +1149,11 @@ int gated_grad_products(const GatedGradArgs& g, const GatedGradOut& o, cudaStrea
 
 // The workspace: dg and du [m, 2 f] with rows on 16 bytes, and behind them the parts of a product.
 long long gated_grad_pitch(int f) { return (2LL * f + 7) / 8 * 8; }
-size_t gated_grad_first(int m, int f) { return ((size_t)m * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
+// Rounding dg and du to 16 bits adds as much to the error of a gradient as rounding that itself does: sqrt(2) of it in all.  With few rows, whose few
+// values of dg and du need not average, it was up to twice: there what their rounding left off is kept too and multiplied beside them, at the time of
+// the launches (64 rows at most: no more than one block of K more for dw, and every block of w twice, the second time from L2).
+int gated_grad_twice(int m) { return m <= 64 ? 1 : 0; }
+size_t gated_grad_first(int m, int f) { return (((size_t)m << gated_grad_twice(m)) * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -1164,7 +1185,7 @@ int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes) {
   for (int want = 1; want < 4; ++want) {
     const ProductSize size[2] = {{want & 1 ? m : 0, k, 2LL * f}, {want & 2 ? 2LL * f : 0, k, m}};
     ProductsPlan q;
-    const long long parts = m > 0 && f > 0 && k > 0 ? gated_products_plan(size, &q) : 0;
+    const long long parts = m > 0 && f > 0 && k > 0 ? gated_products_plan(size, gated_grad_twice(m), &q) : 0;
     if (parts > most) most = parts;
   }
   *bytes = gated_grad_first(m, f) + (size_t)most;
@@ -1191,7 +1212,8 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
   if ((rc = sb_gated_grad_workspace_bytes(m, f, k, &need)) != SB_OK) return rc;
   if (any && workspace_bytes < need) return sb_fail(SB_ERR_BAD_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
   if (!dx && !dw) return SB_OK;
-  const GatedGradArgs g = {dh, saved, workspace, lddh, lds, gated_grad_pitch(f), m, f};
+  char* const lo = gated_grad_twice(m) ? reinterpret_cast<char*>(workspace) + (size_t)m * (size_t)gated_grad_pitch(f) * 2 : nullptr;
+  const GatedGradArgs g = {dh, saved, workspace, lo, lddh, lds, gated_grad_pitch(f), m, f};
   const GatedGradOut o = {x, w, dx, dw, ldx, ldw, lddx, lddw, dw_dtype, accumulate, k, reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + gated_grad_first(m, f))};
   cudaStream_t s = (cudaStream_t)stream;
 #define SB_GATED_CALL(ACT) (dtype == SB_BF16 ? launch_gated_act_grad<__nv_bfloat16, ACT>(g, s) : launch_gated_act_grad<__half, ACT>(g, s))

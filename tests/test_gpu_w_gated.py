@@ -310,3 +310,27 @@ def test_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for _, _, _, _, _, dx, dw, want in jobs:
         assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+
+
+@pytest.mark.parametrize("m,f,k", [(1, 64, 64), (3, 432, 104), (5, 33, 40), (64, 200, 136)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ACTS)
+def test_few_rows_keep_what_rounding_leaves_off(gpu, m, f, k, dtype, kind):
+    """Up to 64 rows the products see dg and du as two numbers of the storage type each: the gradients are off by their own rounding and by
+    next to nothing else."""
+    torch = _torch()
+    x, w = inputs(m, f, k, dtype, 3)
+    saved = (x.float() @ w.float().t()).to(x.dtype)
+    dout = torch.randn((m, f), generator=generator(4), device="cuda").to(x.dtype)
+    dx, dw = torch.empty_like(x), torch.empty_like(w)
+    gpu.gated_grad(dout, x, w, saved, dx=dx, dw=dw, activation=kind)
+    g, u = saved.double().chunk(2, 1)
+    d, wide = dout.double(), torch.cat([dout.double(), dout.double()], 1)
+    exact = torch.cat([d * u * act_grad(kind, g), d * act(kind, g)], 1)
+    # Of dg and du: the activation's, the rounding of the second number (the first leaves at most ROUND of the value, which is rounded by ROUND again),
+    # and in f16 what lies below its least number.
+    slack = act_error(torch.cat([g, g], 1)) * wide.abs() * torch.cat([u.abs(), torch.ones_like(u)], 1) + (ROUND[dtype] ** 2 + 2.0 ** -23) * exact.abs() + LEAST[dtype]
+    for got, want, size, least in ((dx, exact @ w.double(), exact.abs() @ w.double().abs() * product_error(4 * f), slack @ w.double().abs()),
+                                   (dw, exact.t() @ x.double(), exact.abs().t() @ x.double().abs() * product_error(2 * m), slack.t() @ x.double().abs())):
+        tol = size + least
+        within(got, want, tol + ROUND[dtype] * (want.abs() + tol) + LEAST[dtype])
