@@ -688,8 +688,8 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_
         }
         __syncwarp();
       }
-      cluster_arrive_relaxed_all();              // what was read has been used: the others may go on
-      cluster_wait_all();
+      // What was read of the others has arrived before they go on, and what this block's warps counted is seen by all of them.
+      cluster_sync_all();
       if (rank == 0 && g.top > 0) {
         const int n = candidate_count;
         if (tid < LP_MAX_TOP) best[tid] = 0ull;

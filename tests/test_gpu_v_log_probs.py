@@ -370,3 +370,22 @@ def test_device_arrays(gpu):
     out = gpu.DeviceArray((30,), "f32")
     gpu.primitives.log_probs(gpu.DeviceArray.from_numpy(logits.cpu().numpy()), gpu.DeviceArray.from_numpy(tokens.cpu().numpy()), out)
     assert np.array_equal(out.numpy(), check(gpu, logits, tokens)[0].cpu().numpy())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,cols,top", [(100, 8209, 64), (50, 16411, 33), (27, 32771, 64), (3, 131072, 64), (9, 50001, 1)])
+def test_alternatives_of_rows_that_blocks_share(gpu, rows, cols, top, dtype):
+    """The first block of a cluster ranks what all of them offer: the same places, the same bits, one call behind the other."""
+    torch = _torch()
+    logits, tokens, _, _, _ = inputs(rows, cols, dtype, cols)
+    check(gpu, logits, tokens, top=top)
+    held = []
+    for _ in range(12):
+        out = torch.empty(rows, device="cuda")
+        values, places = torch.empty((rows, top), device="cuda"), torch.empty((rows, top), dtype=torch.int32, device="cuda")
+        gpu.primitives.log_probs(logits, tokens, out, top=values, top_tokens=places)
+        held.append((out, values, places))
+    torch.cuda.synchronize()
+    assert torch.equal(held[0][2].long(), alternatives(logits.double(), top))
+    for again in held[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(held[0], again))
