@@ -584,7 +584,8 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
  * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
  * the old dw.  dg and du are rounded to the storage type for the products (up to 64 rows and rows on 16 bytes: to two numbers of it),
  * whose sums are fp32 in a fixed order.  workspace:
- * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  Both products run at once: where both are wanted dx may not be x, nor dw w. */
+ * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  dx may not be w, nor dw x.  Both products run at once: where both are wanted dx may
+ * not be x either, nor dw w. */
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
 int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,
                   void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, int accumulate, int m, int f, int k, int dtype,

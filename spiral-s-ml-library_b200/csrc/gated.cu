@@ -1206,7 +1206,11 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
   if (any && ((dx && k > 0 && !w) || (dw && k > 0 && !x))) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if ((any && (lddh < f || lds < 2LL * f)) || (x && ldx < k) || (w && ldw < k) || (dx && lddx < k) || (dw && lddw < k))
     return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  // Tiles of both products are written while others are still made.
+  if (any && ((dx && dx == w) || (dw && dw == x))) return sb_fail(SB_ERR_BAD_ARG, "%s: dx or dw in the place of what it is made from", who);
   if (dx && dw && (dx == x || dw == w || dx == dw)) return sb_fail(SB_ERR_BAD_ARG, "%s: dx or dw in the place of what the other is made from", who);
+  if (any && (workspace == dh || workspace == saved || workspace == x || workspace == w || workspace == dx || workspace == dw))
+    return sb_fail(SB_ERR_BAD_ARG, "%s: the workspace in the place of an input or output", who);
   if (!gated_element_aligned(dh, dtype) || !gated_element_aligned(saved, dtype) || !gated_element_aligned(x, dtype) || !gated_element_aligned(w, dtype) ||
       !gated_element_aligned(dx, dtype) || (dw && !gated_element_aligned(dw, dw_dtype)) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size, or the workspace not to 256 bytes", who);

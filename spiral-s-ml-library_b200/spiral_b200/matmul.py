@@ -260,7 +260,8 @@ def gated(x, w, out, activation="silu", saved=None, stream=None):
 def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulate=False, workspace=None, stream=None):
     """Gradient of ``gated`` from ``dout`` [m, f] and what it ``saved``: ``dx`` (like ``x``) and ``dw`` (like ``w``, or fp32), each where given;
     ``accumulate`` adds to the old ``dw``.  ``workspace``: device memory of ``gated_grad_workspace`` bytes; by default one is kept per device,
-    stream and host thread.  Both products run at once: ``dx`` is not ``x`` and ``dw`` not ``w``.  Returns (dx, dw)."""
+    stream and host thread.  ``dx`` may not be ``w``, nor ``dw`` ``x``; where both are wanted ``dx`` may not be ``x`` either, nor ``dw`` ``w``.
+    Returns (dx, dw)."""
     m, f, k, x, ldx, w, ldw, tag, act = _gated_sizes("gated_grad", x, w, activation)
     dh, lddh = _gated_matrix("gated_grad", dout, "dout", tag, m, f)
     saved, lds = _gated_matrix("gated_grad", saved, "saved", tag, m, 2 * f)

@@ -199,3 +199,13 @@ def test_int4_arrays(sb):
         sb.quantize_int4(Fake((7, 64)), codes, scales, group=64)
     with pytest.raises(ValueError):
         sb.dequantize_int4(codes, scales, Fake((7, 64)), group=64)
+
+
+@pytest.mark.parametrize("places", [{"dx": 0x3000}, {"dx": 0x3000, "dw": None}, {"dw": 0x2000}, {"dw": 0x2000, "dx": None}, {"dx": 0x2000}, {"dw": 0x3000},
+                                    {"dx": 0x6000}, {"ws": 0x1000}, {"ws": 0x2000}, {"ws": 0x3000}, {"ws": 0x4000}, {"ws": 0x5000}, {"ws": 0x6000}])
+def test_gradients_of_gated_layers_in_the_place_of_what_they_are_made_from(sb, places):
+    """m = 2 f: dx is as large as w, and dw as x."""
+    a = dict(dh=0x1000, x=0x2000, w=0x3000, saved=0x4000, dx=0x5000, dw=0x6000, ws=0x10000)
+    a.update(places)
+    refused(sb, BAD, "sb_gated_grad", a["dh"], 8, a["x"], 16, a["w"], 16, a["saved"], 16, a["dx"], 16, a["dw"], 16, 2, 0, 16, 8, 16, 2, 0, a["ws"],
+            1 << 20, None)
