@@ -602,7 +602,8 @@ int sb_dequantize_int4(const uint8_t* codes, long long ldw, const void* scales, 
                        long long n, int k, int group, void* stream);
 /* c [m, n] = a w^T (+ bias) (relu) for few rows of a [m, k] (SB_BF16 or SB_F16); c in SB_F32, SB_BF16 or SB_F16, fp32 sums; epilogue:
  * SB_EPI_BIAS (fp32 [n]), SB_EPI_RELU (a NaN gives 0, as in the other products).  Made for up to 64 rows, which read the weights once;
- * more rows, 2^22 - 64 at most, are right, and with many of them sb_dequantize_int4 and sb_matmul_ex are faster.  c may not be a. */
+ * more rows, 2^22 - 64 at most, are right, and with many of them sb_dequantize_int4 and sb_matmul_ex are faster.  In none of the three an output may be
+ * one of the inputs. */
 int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes, long long ldw, const void* scales, int scale_dtype, void* c,
                    long long ldc, int m, int n, int k, int group, int out_dtype, int epilogue, const float* bias, void* stream);
 

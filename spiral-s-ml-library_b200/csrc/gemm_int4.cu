@@ -569,6 +569,7 @@ int sb_quantize_int4(const void* x, long long ldx, int dtype, long long n, int k
   if (n == 0 || k == 0) return SB_OK;
   if (!x || !codes || !scales) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if (ldx < k || ldc < (k + 1) / 2) return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  if ((const void*)codes == x || scales == x || scales == (const void*)codes) return sb_fail(SB_ERR_BAD_ARG, "%s: codes and scales have places of their own", who);
   if (!int4_aligned(x, dtype) || !int4_aligned(scales, scale_dtype))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
   const QuantInt4Args p = {x, codes, scales, ldx, ldc, n, (k + group - 1) / group, k, group};
@@ -587,6 +588,7 @@ int sb_dequantize_int4(const uint8_t* codes, long long ldw, const void* scales, 
   if (n == 0 || k == 0) return SB_OK;
   if (!codes || !scales || !out) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if (ldw < (k + 1) / 2 || ldo < k) return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
+  if (out == (const void*)codes || out == scales) return sb_fail(SB_ERR_BAD_ARG, "%s: the output in the place of codes or scales", who);
   if (!int4_aligned(out, out_dtype) || !int4_aligned(scales, scale_dtype))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
   cudaStream_t s = (cudaStream_t)stream;
@@ -608,7 +610,8 @@ int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes
   if (m == 0 || n == 0) return SB_OK;
   if (!c || ((epilogue & SB_EPI_BIAS) && !bias) || (k > 0 && (!a || !codes || !scales))) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
   if (ldc < n || (k > 0 && (lda < k || ldw < (k + 1) / 2))) return sb_fail(SB_ERR_BAD_ARG, "%s: a row pitch is shorter than its rows", who);
-  if (c == a) return sb_fail(SB_ERR_BAD_ARG, "%s: c in the place of a", who);
+  if (k > 0 && (c == a || c == (const void*)codes || c == scales)) return sb_fail(SB_ERR_BAD_ARG, "%s: c in the place of what it is made from", who);
+  if ((epilogue & SB_EPI_BIAS) && c == (const void*)bias) return sb_fail(SB_ERR_BAD_ARG, "%s: c in the place of the bias", who);
   if (!int4_aligned(a, dtype) || !int4_aligned(scales, scale_dtype) || !int4_aligned(c, out_dtype) || !int4_aligned(bias, SB_F32))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
   Int4Args p;

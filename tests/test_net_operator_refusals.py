@@ -209,3 +209,12 @@ def test_gradients_of_gated_layers_in_the_place_of_what_they_are_made_from(sb, p
     a.update(places)
     refused(sb, BAD, "sb_gated_grad", a["dh"], 8, a["x"], 16, a["w"], 16, a["saved"], 16, a["dx"], 16, a["dw"], 16, 2, 0, 16, 8, 16, 2, 0, a["ws"],
             1 << 20, None)
+
+
+def test_4_bit_outputs_in_the_place_of_what_they_are_made_from(sb):
+    for c in (0x1000, 0x2000, 0x3000, 0x5000):
+        refused(sb, BAD, "sb_matmul_int4", 0x1000, 64, 2, 0x2000, 32, 0x3000, 2, c, 8, 2, 8, 64, 64, 0, 1, 0x5000, None)
+    for codes, scales in ((0x1000, 0x3000), (0x2000, 0x1000), (0x2000, 0x2000)):
+        refused(sb, BAD, "sb_quantize_int4", 0x1000, 64, 0, 4, 64, 32, codes, 32, scales, 2, None)
+    for out in (0x1000, 0x2000):
+        refused(sb, BAD, "sb_dequantize_int4", 0x1000, 32, 0x2000, 2, out, 64, 2, 4, 64, 64, None)
