@@ -273,10 +273,13 @@ def values_ptr(x, n, what):
     return device_ptr(x)
 
 
-def array_ptr(x, n, tag, what):
-    """Address of n contiguous values of the storage type ``tag`` (None -> NULL)."""
+def array_ptr(x, n, tag, what, cols=None):
+    """Address of n contiguous values of the storage type ``tag`` (None -> NULL).  ``cols``: of a matrix, whose rows have so many; in one
+    dimension its values stand row by row."""
     if x is None:
         return None
+    if cols is not None and len(x.shape) > 1 and x.shape[-1] != cols:
+        raise ValueError("%s must have rows of %d, got %s" % (what, cols, tuple(x.shape)))
     if type(x) is not DeviceArray:
         try:                                       # torch
             if x.numel() == n and x.is_contiguous() and _TAG_OF[x.dtype] == tag:

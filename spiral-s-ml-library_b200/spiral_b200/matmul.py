@@ -301,7 +301,7 @@ def _int4_weights(who, codes, scales, k, group):
     tag = dtype_tag(scales)
     if tag not in _GATED:
         raise TypeError("%s: scales must hold bf16 or f16, not %s" % (who, tag))
-    return n, codes, ldw, array_ptr(scales, -(-k // group) * n, tag, "scales"), _GATED[tag]
+    return n, codes, ldw, array_ptr(scales, -(-k // group) * n, tag, "scales", n), _GATED[tag]
 
 
 def quantize_int4(x, codes, scales, group=128, stream=None):

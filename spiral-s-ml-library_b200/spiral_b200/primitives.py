@@ -244,7 +244,7 @@ def _row_args(who, logits, tokens, mask):
     if code is None:
         raise TypeError("logits must hold %s, not %s" % (" / ".join(_FLOATS), tag))
     if mask is not None:
-        mask = array_ptr(mask, rows * cols, "u8", "mask")
+        mask = array_ptr(mask, rows * cols, "u8", "mask", cols)
     index = _lib.I32
     if tokens is not None:
         tag = dtype_tag(tokens)
@@ -283,7 +283,7 @@ def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None,
     if not n:
         n, top, top_tokens = 0, None, None
     _lib.call("sb_log_probs", ptr, ld, code, rows, cols, mask, prefix, scale, tokens, index, array_ptr(out, rows, "f32", "out"),
-              array_ptr(entropy, rows, "f32", "entropy"), array_ptr(stats, 2 * rows, "f32", "stats"), n, top, top_tokens,
+              array_ptr(entropy, rows, "f32", "entropy"), array_ptr(stats, 2 * rows, "f32", "stats", 2), n, top, top_tokens,
               stream_ptr(stream))
     return out
 
@@ -296,7 +296,7 @@ def log_probs_grad(logits, tokens, stats, dlogits, dout=None, dentropy=None, ent
     drows, dcols, ldd, dptr, dtag = typed_matrix(dlogits, "dlogits")
     if drows != rows or dcols != cols or _FLOATS.get(dtag) != code:
         raise ValueError("log_probs_grad: dlogits must be like logits, %dx%d" % (rows, cols))
-    _lib.call("sb_log_probs_grad", ptr, ld, code, rows, cols, mask, prefix, scale, tokens, index, array_ptr(stats, 2 * rows, "f32", "stats"),
+    _lib.call("sb_log_probs_grad", ptr, ld, code, rows, cols, mask, prefix, scale, tokens, index, array_ptr(stats, 2 * rows, "f32", "stats", 2),
               array_ptr(dout, rows, "f32", "dout"), array_ptr(entropy, rows, "f32", "entropy"), array_ptr(dentropy, rows, "f32", "dentropy"),
               dptr, ldd, stream_ptr(stream))
     return keep_tf32(dlogits, stream)

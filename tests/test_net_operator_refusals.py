@@ -218,3 +218,30 @@ def test_4_bit_outputs_in_the_place_of_what_they_are_made_from(sb):
         refused(sb, BAD, "sb_quantize_int4", 0x1000, 64, 0, 4, 64, 32, codes, 32, scales, 2, None)
     for out in (0x1000, 0x2000):
         refused(sb, BAD, "sb_dequantize_int4", 0x1000, 32, 0x2000, 2, out, 64, 2, 4, 64, 64, None)
+
+
+def test_matrices_that_are_turned_over(sb):
+    """The right number of values in the wrong layout."""
+    b, p = "bfloat16", sb.primitives
+    codes, scales, a, c = Fake((8, 64), "uint8"), Fake((8, 4), b), Fake((2, 128), b), Fake((2, 8))          # scales are [4, 8]
+    with pytest.raises(ValueError):
+        sb.matmul_int4(a, codes, scales, c, group=32)
+    with pytest.raises(ValueError):
+        sb.quantize_int4(Fake((8, 128)), codes, scales, group=32)
+    with pytest.raises(ValueError):
+        sb.dequantize_int4(codes, scales, Fake((8, 128)), group=32)
+    x, t, v = Fake((4, 8)), Fake((4,), "int32"), Fake((4,))
+    for more in ({"mask": Fake((8, 4), "uint8")}, {"stats": Fake((2, 4))}):
+        with pytest.raises(ValueError):
+            p.log_probs(x, t, v, **more)
+    with pytest.raises(ValueError):
+        p.log_probs_grad(x, t, Fake((2, 4)), Fake((4, 8)), dout=v)
+    with pytest.raises(ValueError):
+        p.log_probs_grad(x, t, Fake((4, 2)), Fake((4, 8)), dout=v, mask=Fake((8, 4), "uint8"))
+
+
+def test_matrices_in_one_dimension(sb):
+    """Row by row is what they are: accepted."""
+    from spiral_b200.device import array_ptr
+    assert array_ptr(Fake((32,), "uint8"), 32, "u8", "mask", 8) == array_ptr(Fake((4, 8), "uint8"), 32, "u8", "mask", 8) == 0x1000
+    assert array_ptr(Fake((2, 2, 8), "uint8"), 32, "u8", "mask", 8) == 0x1000 and array_ptr(None, 32, "u8", "mask", 8) is None
