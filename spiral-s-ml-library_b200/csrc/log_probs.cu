@@ -12,7 +12,7 @@
 namespace {
 
 constexpr int LP_MAX_TOP = 64;
-constexpr float LP_LOG2E = 1.4426950408889634f;
+constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.69314718055994531f;
 
 struct LogProbArgs {
   const void* logits;
@@ -43,15 +43,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 constexpr float LP_LOWEST = -3.402823466e38f;
-// What a distance from the largest logit counts as at least where it is multiplied by its own probability: 0, not NaN, for -inf.
-constexpr float LP_FAR = -1e30f;
+// What the logarithm of a probability (by any base) counts as at least where it is multiplied by that probability, which is 0 in fp32 from
+// -150 on: 0, not NaN, for -inf.  It is bounded behind the multiplication by the scale, which may be as small as fp32 has it.
+constexpr float LP_NOTHING = -1e4f;
+// s / ln 2, finite for every scale.
+__device__ __forceinline__ float lp_factor(float scale) { return fminf(scale * LP_LOG2E, -LP_LOWEST); }
 
 __device__ __forceinline__ long long lp_token(const void* tokens, int wide, long long row) {
   return wide ? reinterpret_cast<const long long*>(tokens)[row] : (long long)reinterpret_cast<const int*>(tokens)[row];
 }
 
-// Largest logit so far (NaN left out: it shows in the sum), sum = S and dist = sum exp(s (x - top)) (x - top).  Of nothing: the lowest
-// number, which no -inf reaches, and zeros.
+// Largest logit so far (NaN left out: it shows in the sum), sum = S and with c = s / ln 2 dist = sum 2^(c (x - top)) c (x - top).  Of
+// nothing: the lowest number, which no -inf reaches, and zeros.
 struct RowSums {
   float top, sum, dist;
 };
@@ -62,8 +65,8 @@ struct ShareSums {
 };
 // The same, seen from `top`, which is not below its own.
 __device__ __forceinline__ void lp_raise(RowSums& r, float top, float c) {
-  const float d = fmaxf(r.top - top, LP_FAR), f = exp2_approx(d * c);
-  r.dist = fmaf(r.sum, d, r.dist) * f;
+  const float a = fmaxf((r.top - top) * c, LP_NOTHING), f = exp2_approx(a);
+  r.dist = fmaf(r.sum, a, r.dist) * f;
   r.sum *= f;
   r.top = top;
 }
@@ -75,13 +78,13 @@ __device__ __forceinline__ void lp_take(RowSums& r, const float* x, float c) {
     unsigned long long sum2 = 0ull, dist2 = 0ull;
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      float d0, d1, a0, a1;
-      unpack_f32x2(sub_f32x2(pack_f32x2(x[i], x[i + 1]), top2), d0, d1);
-      const unsigned long long d2 = pack_f32x2(max_nan(d0, LP_FAR), max_nan(d1, LP_FAR));
-      unpack_f32x2(mul_f32x2(d2, c2), a0, a1);
+      float a0, a1;
+      unpack_f32x2(mul_f32x2(sub_f32x2(pack_f32x2(x[i], x[i + 1]), top2), c2), a0, a1);
+      a0 = max_nan(a0, LP_NOTHING);
+      a1 = max_nan(a1, LP_NOTHING);
       const unsigned long long e2 = pack_f32x2(exp2_approx(a0), exp2_approx(a1));
       sum2 = add_f32x2(sum2, e2);
-      fma_f32x2(dist2, e2, d2);
+      fma_f32x2(dist2, e2, pack_f32x2(a0, a1));
     }
     float s0, s1, d0, d1;
     unpack_f32x2(sum2, s0, s1);
@@ -91,9 +94,9 @@ __device__ __forceinline__ void lp_take(RowSums& r, const float* x, float c) {
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = max_nan(x[i] - r.top, LP_FAR), e = exp2_approx(d * c);
+      const float a = max_nan((x[i] - r.top) * c, LP_NOTHING), e = exp2_approx(a);
       r.sum += e;
-      r.dist = fmaf(e, d, r.dist);
+      r.dist = fmaf(e, a, r.dist);
     }
   }
 }
@@ -103,7 +106,7 @@ __device__ __forceinline__ void lp_finish(const LogProbArgs& g, long long row, c
   const bool empty = r.sum == 0.f;
   if (g.out)
     g.out[row] = token < 0 || token >= g.mask_cols ? 0.f : token >= g.cols || empty ? -INFINITY : g.scale * (token_logit - r.top) - log_sum;
-  if (g.entropy) g.entropy[row] = empty ? 0.f : log_sum - g.scale * (r.dist / r.sum);
+  if (g.entropy) g.entropy[row] = empty ? 0.f : log_sum - LP_LN2 * (r.dist / r.sum);
   if (g.stats) {
     g.stats[2 * row] = empty ? 0.f : r.top;
     g.stats[2 * row + 1] = log_sum;
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(128) log_probs_short_kernel(LogProbArgs g) {
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const int lane = threadIdx.x % G;
-  const float c = g.scale * LP_LOG2E;
+  const float c = lp_factor(g.scale);
   const long long groups = (long long)gridDim.x * (128 / G);
   // Whole warps go round together.
   const long long first = (long long)blockIdx.x * (128 / G) + threadIdx.x / G, warp_first = first - (threadIdx.x % 32) / G;
@@ -367,7 +370,7 @@ __device__ __forceinline__ ShareSums lp_fast_sums(const T* x, const RowShape<T>&
   // c top is ref + rest.  (Far from zero the rest is large: such a share counts only in rows that take the exact sums, or not at all.)
   const float rest = fminf(fmaxf(fmaf(r.top, c, -f.ref), -60.f), 60.f), back = exp2_approx(-rest);
   r.sum = (s0 + s1) * back;
-  r.dist = (d0 + d1 - rest * (s0 + s1)) * back * __fdividef(1.f, c);
+  r.dist = (d0 + d1 - rest * (s0 + s1)) * back;
   return {r, f.top_a, f.top_b};
 }
 // The fast sums of a row are right where its largest logit is neither so low (first) that what was lifted has weight beside it nor so far
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_
   const int blocks = CLUSTER ? (int)gridDim.x : 1, rank = CLUSTER ? (int)blockIdx.x : 0;
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const float c = g.scale * LP_LOG2E;
+  const float c = lp_factor(g.scale);
   for (long long row = blockIdx.y; row < g.rows; row += gridDim.y) {
     const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
     const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
@@ -722,7 +725,7 @@ __global__ void __launch_bounds__(128, 8) log_probs_warp_kernel(LogProbArgs g) {
   uint8_t* hot = all_hot[warp];
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
-  const float c = g.scale * LP_LOG2E;
+  const float c = lp_factor(g.scale);
   for (long long row = (long long)blockIdx.x * 4 + warp; row < g.rows; row += (long long)gridDim.x * 4) {
     const T* x = reinterpret_cast<const T*>(g.logits) + row * g.ld;
     const uint8_t* mask = MASKED ? g.mask + row * g.mask_cols : nullptr;
@@ -866,8 +869,6 @@ __device__ __forceinline__ RowGrad lp_row_grad(const LogProbGradArgs& g, long lo
   r.token = t >= 0 && t < g.cols && r.log_sum != INFINITY ? (int)t : -1;
   return r;
 }
-// Logarithms of probabilities at least this far from 1, whose probabilities are 0 in fp32.
-constexpr float LP_NOTHING = -1e4f;
 __device__ __forceinline__ float lp_grad(const RowGrad& r, float x) {
   const float lp = max_nan(fmaf(r.scale, x - r.top, -r.log_sum), LP_NOTHING);
   return exp2_approx(lp * LP_LOG2E) * fmaf(r.h, lp, r.c) * -r.scale;
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
   sb_grid_dependency_wait();
   sb_grid_dependents_launch();
   const int first = NT == 256 ? blockIdx.x * 256 + threadIdx.x : threadIdx.x % NT, stride = NT == 256 ? gridDim.x * 256 : NT;
-  const float c = g.scale * LP_LOG2E;
+  const float c = lp_factor(g.scale);
   for (long long row = NT == 256 ? blockIdx.y : (long long)blockIdx.x * (256 / NT) + threadIdx.x / NT; row < g.rows;
        row += NT == 256 ? gridDim.y : (long long)gridDim.x * (256 / NT)) {
     const RowGrad r = lp_row_grad(g, row);

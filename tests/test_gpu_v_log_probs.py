@@ -389,3 +389,38 @@ def test_alternatives_of_rows_that_blocks_share(gpu, rows, cols, top, dtype):
     assert torch.equal(held[0][2].long(), alternatives(logits.double(), top))
     for again in held[1:]:
         assert all(torch.equal(a, b) for a, b in zip(held[0], again))
+
+
+@pytest.mark.parametrize("scale", [1e-20, 1e-30, 1e-37, 2.0 ** -140])
+@pytest.mark.parametrize("rows,cols", [(40, 7), (30, 40), (20, 300), (10, 900), (3000, 1500), (8, 6000), (4, 50001)])
+def test_a_column_that_is_not_legal_has_no_weight_at_the_smallest_scales(gpu, rows, cols, scale):
+    """As good as uniform over the legal columns, whether a mask or -inf forbids the others."""
+    torch = _torch()
+    logits, tokens, mask, dout, dentropy = inputs(rows, cols, "f32", cols, mask=0.3)
+    mask[:, 0] = 1
+    mask[1, 1:] = 0
+    by_value = torch.where(mask != 0, logits, -math.inf)
+    _, entropy, stats = check(gpu, logits, tokens, mask=mask, scale=scale, top=3)
+    check_grad(gpu, logits, tokens, stats, entropy, dout, dentropy, mask=mask, scale=scale)
+    _, entropy, stats = check(gpu, by_value, tokens, scale=scale, top=3)
+    dlogits = torch.full_like(logits, 7.0)
+    gpu.primitives.log_probs_grad(by_value, tokens, stats, dlogits, dout=dout, dentropy=dentropy, entropy=entropy, scale=scale)
+    # Without a mask a token at -inf is a legal one: its own column has scale dout, which the definition for legal columns above does not count.
+    at, held = tokens.long().clamp(0, cols - 1)[:, None], ((tokens >= 0) & (tokens < cols))[:, None]
+    own = torch.where(held & (by_value.gather(1, at) == -math.inf), dout[:, None] * torch.tensor(scale, dtype=torch.float32, device="cuda"), 0.0)
+    compare_grad(dlogits.scatter_add(1, at, -own), "f32", legal(by_value, None, -1), tokens, stats, entropy, dout, dentropy, scale)
+    lowest = torch.finfo(torch.float32).min          # a number, and legal
+    logits[:, 1::2] = lowest
+    check(gpu, logits, tokens, scale=scale)
+
+
+@pytest.mark.parametrize("cols", [7, 40, 300, 900, 6000, 50001])
+def test_the_largest_scale(gpu, cols):
+    """One column has it all; the logarithms of the others are beyond fp32."""
+    torch = _torch()
+    logits, _, _, _, _ = inputs(4, cols, "f32", cols)
+    tokens = logits.argmax(1).to(torch.int32)
+    scale = torch.finfo(torch.float32).max
+    out, entropy, stats = torch.full((4,), 7.0, device="cuda"), torch.full((4,), 7.0, device="cuda"), torch.full((4, 2), 7.0, device="cuda")
+    gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats, scale=scale)
+    assert not out.any() and not entropy.any() and not stats[:, 1].any() and torch.equal(stats[:, 0], logits.amax(1))
