@@ -926,11 +926,12 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
     const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
     if (first < shape.head + shape.tail) lp_grad_one<T>(r, x, mask, d, shape.single(first), g.cols);
     for (int j = g.cols + first; j < g.mask_cols; j += stride) d[j] = sb_from_f32<T>(0.f);
-    // The short way holds where the lifted logits come out as 0 and no product leaves fp32's range.
-    const bool fast = fabsf(r.top) * c <= LP_FAST_MOST && c <= LP_FAST_MOST && (r.top - lp_low<T>()) * c >= 200.f && r.log_sum <= LP_FAST_MOST &&
-                      fabsf(r.h) < 1e6f && fabsf(r.c) < 1e30f;
     const float ref = fmaf(r.top, c, r.log_sum * LP_LOG2E), rest = fmaf(r.top, c, -ref) + r.log_sum * LP_LOG2E, back = -r.scale * exp2_approx(-rest);
     const float h = back * r.h * (1.f / LP_LOG2E), k = back * fmaf(r.h, -rest * (1.f / LP_LOG2E), r.c);
+    // The short way holds where the lifted logits come out as 0 and no product leaves fp32's range: not that of a lifted logit's logarithm, which
+    // is the largest, and h either, as it would be infinite beside a probability of 0.
+    const bool fast = fabsf(r.top) * c <= LP_FAST_MOST && c <= LP_FAST_MOST && (r.top - lp_low<T>()) * c >= 200.f && r.log_sum <= LP_FAST_MOST &&
+                      -lp_low<T>() * c * fabsf(h) < 1e37f && fabsf(r.c) < 1e30f;
     const unsigned long long c2 = pack_f32x2(c, c), ref2 = pack_f32x2(-ref, -ref), h2 = pack_f32x2(h, h), k2 = pack_f32x2(k, k);
     for (int p0 = first; p0 < shape.packs; p0 += UNROLL * stride) {
       SbWords<16> w[UNROLL];

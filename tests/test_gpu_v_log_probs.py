@@ -424,3 +424,22 @@ def test_the_largest_scale(gpu, cols):
     out, entropy, stats = torch.full((4,), 7.0, device="cuda"), torch.full((4,), 7.0, device="cuda"), torch.full((4, 2), 7.0, device="cuda")
     gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats, scale=scale)
     assert not out.any() and not entropy.any() and not stats[:, 1].any() and torch.equal(stats[:, 0], logits.amax(1))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale,weight", [(100.0, 65536.0), (1000.0, 300.0), (1e4, 3.0), (1.0, 1e9), (20.0, 1e6)])
+@pytest.mark.parametrize("rows,cols", [(30, 100), (4, 5000), (3, 70000)])
+def test_gradients_of_large_entropies_weights_where_logits_are_forbidden_by_value(gpu, rows, cols, scale, weight, dtype):
+    """Columns at -inf have no gradient, whatever the scale and the weight of the entropy."""
+    torch = _torch()
+    logits, tokens, mask, dout, dentropy = inputs(rows, cols, dtype, cols, std=0.5 / scale, mask=0.5)
+    mask[:, 0] = 1
+    tokens[:] = 0
+    logits = torch.where(mask != 0, logits, -math.inf)
+    _, entropy, stats = check(gpu, logits, tokens, scale=scale)
+    if dtype != "f16":
+        check_grad(gpu, logits, tokens, stats, entropy, dout, weight * dentropy, scale=scale)
+        return
+    dlogits = torch.full_like(logits, 7.0)           # other columns' gradients may be beyond f16, which the definition in 64 bits does not know
+    gpu.primitives.log_probs_grad(logits, tokens, stats, dlogits, dout=dout, dentropy=weight * dentropy, entropy=entropy, scale=scale)
+    assert not dlogits[mask == 0].any() and not torch.isnan(dlogits).any()
