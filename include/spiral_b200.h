@@ -565,7 +565,7 @@ int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, in
  *   dlogits_j = scale (dout ([j = token] - p_j) - dentropy p_j (log p_j + entropy))
  * in the type of the logits; 0 in columns that are not legal and in rows without a legal logit, and no dout where there is no token.
  * The token of a row that is not legal is a constant -inf: its dout reaches the logits through -p_j only.  stats and entropy are
- * those that sb_log_probs left.  dlogits may be the logits. */
+ * those that sb_log_probs left.  dlogits may be the logits, with their pitch. */
 int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
                       const void* tokens, int index_dtype, const float* stats, const float* dout, const float* entropy,
                       const float* dentropy, void* dlogits, long long ldd, void* stream);

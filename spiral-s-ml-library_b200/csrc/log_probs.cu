@@ -982,9 +982,8 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
   }
 }
 
-int lp_args_ok(const char* who, const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
-               const void* tokens, int index_dtype) {
-  (void)mask;
+int lp_args_ok(const char* who, const void* logits, long long ld, int dtype, long long rows, int cols, int prefix, float scale, const void* tokens,
+               int index_dtype) {
   if (rows < 0 || cols < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
   if (prefix > cols) return sb_fail(SB_ERR_BAD_ARG, "%s: prefix %d beyond the %d columns", who, prefix, cols);
   if (dtype != SB_F32 && dtype != SB_BF16 && dtype != SB_F16)
@@ -1093,7 +1092,7 @@ int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, in
                  const void* tokens, int index_dtype, float* out, float* entropy, float* stats, int top, float* top_values,
                  int32_t* top_tokens, void* stream) {
   const char* who = "sb_log_probs";
-  int rc = lp_args_ok(who, logits, ld, dtype, rows, cols, mask, prefix, scale, tokens, index_dtype);
+  int rc = lp_args_ok(who, logits, ld, dtype, rows, cols, prefix, scale, tokens, index_dtype);
   if (rc != SB_OK) return rc;
   if (top < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
   if (top > LP_MAX_TOP) return sb_fail(SB_ERR_TOO_LARGE, "%s: at most %d alternatives (got %d)", who, LP_MAX_TOP, top);
@@ -1102,6 +1101,8 @@ int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, in
   if (top > 0 && !top_values && !top_tokens) return sb_fail(SB_ERR_BAD_ARG, "%s: nowhere to put %d alternatives", who, top);
   if (!lp_words(out) || !lp_words(entropy) || !lp_words(stats) || !lp_words(top_values) || !lp_words(top_tokens))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
+  for (const void* o : {(const void*)out, (const void*)entropy, (const void*)stats, (const void*)top_values, (const void*)top_tokens})
+    if (o && cols > 0 && (o == logits || o == (const void*)mask)) return sb_fail(SB_ERR_BAD_ARG, "%s: an output in the place of the logits or the mask", who);
   LogProbArgs g;
   memset(&g, 0, sizeof(g));
   g.logits = logits; g.ld = ld; g.rows = rows; g.cols = prefix >= 0 ? prefix : cols; g.mask_cols = cols;
@@ -1116,7 +1117,7 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
                       const void* tokens, int index_dtype, const float* stats, const float* dout, const float* entropy,
                       const float* dentropy, void* dlogits, long long ldd, void* stream) {
   const char* who = "sb_log_probs_grad";
-  int rc = lp_args_ok(who, logits, ld, dtype, rows, cols, mask, prefix, scale, tokens, index_dtype);
+  int rc = lp_args_ok(who, logits, ld, dtype, rows, cols, prefix, scale, tokens, index_dtype);
   if (rc != SB_OK) return rc;
   if (rows == 0 || cols == 0) return SB_OK;
   if (!dlogits || !stats) return sb_fail(SB_ERR_BAD_ARG, "%s: null pointer", who);
@@ -1126,6 +1127,9 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
   if (reinterpret_cast<uintptr_t>(dlogits) % (size_t)sb_dtype_size(dtype) != 0 || !lp_words(stats) || !lp_words(dout) || !lp_words(entropy) ||
       !lp_words(dentropy))
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size", who);
+  if (dlogits == logits && rows > 1 && ldd != ld) return sb_fail(SB_ERR_BAD_ARG, "%s: gradients in the place of the logits have their row pitch", who);
+  for (const void* i : {(const void*)mask, tokens, (const void*)stats, (const void*)dout, (const void*)entropy, (const void*)dentropy})
+    if (i == dlogits) return sb_fail(SB_ERR_BAD_ARG, "%s: gradients in the place of another input than the logits", who);
   LogProbGradArgs g;
   memset(&g, 0, sizeof(g));
   g.logits = logits; g.ld = ld; g.rows = rows; g.cols = prefix >= 0 ? prefix : cols; g.mask_cols = cols;

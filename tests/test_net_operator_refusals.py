@@ -245,3 +245,14 @@ def test_matrices_in_one_dimension(sb):
     from spiral_b200.device import array_ptr
     assert array_ptr(Fake((32,), "uint8"), 32, "u8", "mask", 8) == array_ptr(Fake((4, 8), "uint8"), 32, "u8", "mask", 8) == 0x1000
     assert array_ptr(Fake((2, 2, 8), "uint8"), 32, "u8", "mask", 8) == 0x1000 and array_ptr(None, 32, "u8", "mask", 8) is None
+
+
+def test_log_probs_in_the_place_of_what_they_are_made_from(sb):
+    for place in (0x1000, 0x8000):
+        for name in range(5):
+            outs = [0x3000, 0x4000, 0x5000, 0x6000, 0x7000]
+            outs[name] = place
+            out, h, stats, values, places = outs
+            refused(sb, BAD, "sb_log_probs", 0x1000, 8, 0, 4, 8, 0x8000, -1, 1.0, 0x2000, 4, out, h, stats, 2, values, places, None)
+    for d, ldd in ((0x1000, 16), (0x2000, 8), (0x3000, 8), (0x4000, 8), (0x5000, 8), (0x6000, 8), (0x8000, 8)):
+        refused(sb, BAD, "sb_log_probs_grad", 0x1000, 8, 2, 4, 8, 0x8000, -1, 1.0, 0x2000, 4, 0x3000, 0x4000, 0x5000, 0x6000, d, ldd, None)
