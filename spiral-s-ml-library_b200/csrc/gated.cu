@@ -16,15 +16,19 @@ enum GatedAct { ACT_SILU = SB_ACT_SILU, ACT_GELU = SB_ACT_GELU, ACT_RELU = SB_AC
 
 __device__ __forceinline__ float gated_sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
-// The normal distribution's P(g) and exp(-g^2 / 2), which its tails are made of: erfc(x) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2) with
-// t = 1 / (1 + p x), off by at most 1.5e-7 (M. Abramowitz, I. A. Stegun, Handbook of Mathematical Functions, 7.1.26).
+// The normal distribution's P(g) and exp(-g^2 / 2), which its tails are made of: with t = 1 / (1 + |g| / sqrt 8) P(-|g|) = t (a1 + t (a2 + ... + t
+// a7)) exp(-g^2 / 2).  The coefficients are a fit of this file's own, the least largest error on 0 <= |g| <= 14.4 relative to exp(g^2 / 2) P(-|g|), which
+// falls like 1 / |g|: with all roundings 6e-7 up to |g| = 1, 1e-6 up to 2, 7e-6 up to 12, so that the smallest values have all the digits of the storage
+// types.
 __device__ __forceinline__ float2 gated_normal(float g) {
-  const float x = fabsf(g) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f)), e = __expf(-x * x);
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  q *= 0.5f * t * e;
+  const float t = __fdividef(1.f, fmaf(0.35355339059327376f, fabsf(g), 1.f)), e = __expf(-0.5f * g * g);
+  float q = fmaf(t, 0.04597611858848591f, -0.18459764335694676f);
+  q = fmaf(t, q, 0.20273347957186824f);
+  q = fmaf(t, q, 0.013682007891541514f);
+  q = fmaf(t, q, 0.1425210676958373f);
+  q = fmaf(t, q, 0.13850115379783598f);
+  q = fmaf(t, q, 0.14118375197936758f);
+  q *= t * e;
   return make_float2(g > 0.f ? 1.f - q : q, e);
 }
 

@@ -334,3 +334,48 @@ def test_few_rows_keep_what_rounding_leaves_off(gpu, m, f, k, dtype, kind):
                                    (dw, exact.t() @ x.double(), exact.abs().t() @ x.double().abs() * product_error(2 * m), slack.t() @ x.double().abs())):
         tol = size + least
         within(got, want, tol + ROUND[dtype] * (want.abs() + tol) + LEAST[dtype])
+
+
+def far_gates(dtype, m, span):
+    """Gates of the storage type, most of them far below zero, and a power of two that keeps their activations in its range."""
+    torch = _torch()
+    g = (torch.rand(m, generator=generator(m), device="cuda") * (span + 2) - span).to(dtype_of(dtype))
+    g[0], g[-1] = -span, 0.0
+    return g, 2.0 ** 14 if dtype == "f16" else 2.0 ** 60
+
+
+# What the kernels' exponential and the tails' fit are off by, relative to themselves: 7e-6, and 2 + 1.2 |x| units of 2^-24 of exp(x), |x| <= 100.
+FAR = 2.0 ** -16
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m,f,k", [(3, 24, 8), (16, 24, 8), (300, 136, 8), (300, 24, 9)])
+def test_activations_keep_their_digits_far_below_zero(gpu, m, f, k, kind, dtype):
+    """One gate per row, as it is: the layer's output is its activation times a power of two, rounded once."""
+    torch = _torch()
+    g, up = far_gates(dtype, m, 5.0 if dtype == "f16" else 12.0)
+    x, w = torch.zeros((m, k), dtype=g.dtype, device="cuda"), torch.zeros((2 * f, k), dtype=g.dtype, device="cuda")
+    x[:, 0], x[:, 1], w[:f, 0], w[f:, 1] = g, up, 1.0, 1.0
+    out = torch.full((m, f), 7.0, dtype=g.dtype, device="cuda")
+    gpu.gated(x, w, out, activation=kind)
+    want = (act(kind, g.double()) * up)[:, None].expand(m, f)
+    within(out, want, (ROUND[dtype] * 1.01 + FAR) * want.abs() + LEAST[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m,f", [(5, 8), (64, 24), (300, 24)])
+def test_derivatives_keep_their_digits_far_below_zero(gpu, m, f, kind, dtype):
+    """The gradients of the projections themselves, through a unit matrix."""
+    torch = _torch()
+    g, up = far_gates(dtype, m, 5.0 if dtype == "f16" else 12.0)
+    saved = torch.cat([g[:, None].expand(m, f), torch.full((m, f), up, dtype=g.dtype, device="cuda")], 1).contiguous()
+    dout, x, w = torch.ones((m, f), dtype=g.dtype, device="cuda"), torch.zeros((m, 2 * f), dtype=g.dtype, device="cuda"), torch.eye(2 * f, dtype=g.dtype, device="cuda")
+    dx = torch.full((m, 2 * f), 7.0, dtype=g.dtype, device="cuda")
+    gpu.gated_grad(dout, x, w, saved, dx=dx, activation=kind)
+    z = g.double()
+    terms = act(kind, z).abs() / z.abs().clamp_min(1e-300) + (z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)).abs() if kind == "gelu" else act_grad(kind, z).abs()
+    for got, want, size in ((dx[:, :f], act_grad(kind, z) * up, terms * up), (dx[:, f:], act(kind, z), act(kind, z).abs())):
+        want, size = want[:, None].expand(m, f), size[:, None].expand(m, f)
+        within(got, want, ROUND[dtype] * 1.01 * want.abs() + FAR * size + LEAST[dtype])
