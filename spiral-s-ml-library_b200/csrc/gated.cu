@@ -14,7 +14,11 @@ namespace {
 
 enum GatedAct { ACT_SILU = SB_ACT_SILU, ACT_GELU = SB_ACT_GELU, ACT_RELU = SB_ACT_RELU };
 
-__device__ __forceinline__ float gated_sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+// 1 / (1 + exp(-g)), from exp(-|g|), which no g takes out of range: the quick division gives 0 for divisors above 2^126.
+__device__ __forceinline__ float gated_sigmoid(float g) {
+  const float e = __expf(-fabsf(g)), r = __fdividef(1.f, 1.f + e);
+  return g < 0.f ? e * r : r;
+}
 
 // The normal distribution's P(g) and exp(-g^2 / 2), which its tails are made of: with t = 1 / (1 + |g| / sqrt 8) P(-|g|) = t (a1 + t (a2 + ... + t
 // a7)) exp(-g^2 / 2).  The coefficients are a fit of this file's own, the least largest error on 0 <= |g| <= 14.4 relative to exp(g^2 / 2) P(-|g|), which

@@ -379,3 +379,21 @@ def test_derivatives_keep_their_digits_far_below_zero(gpu, m, f, kind, dtype):
     for got, want, size in ((dx[:, :f], act_grad(kind, z) * up, terms * up), (dx[:, f:], act(kind, z), act(kind, z).abs())):
         want, size = want[:, None].expand(m, f), size[:, None].expand(m, f)
         within(got, want, ROUND[dtype] * 1.01 * want.abs() + FAR * size + LEAST[dtype])
+
+
+@pytest.mark.parametrize("m", [4, 300])
+def test_silu_to_the_end_of_its_range(gpu, m):
+    """exp(-88) is a number of bf16 and fp32, and so are the activation and its derivative there."""
+    torch = _torch()
+    g = torch.linspace(-88.0, -84.0, m, device="cuda").to(torch.bfloat16)
+    f, k, up = 24, 8, 2.0 ** 100
+    x, w = torch.zeros((m, k), dtype=g.dtype, device="cuda"), torch.zeros((2 * f, k), dtype=g.dtype, device="cuda")
+    x[:, 0], x[:, 1], w[:f, 0], w[f:, 1] = g, up, 1.0, 1.0
+    out, saved = torch.zeros((m, f), dtype=g.dtype, device="cuda"), torch.zeros((m, 2 * f), dtype=g.dtype, device="cuda")
+    gpu.gated(x, w, out, saved=saved)
+    want = (act("silu", g.double()) * up)[:, None].expand(m, f)
+    within(out, want, (ROUND["bf16"] * 1.01 + FAR) * want.abs())
+    dx = torch.zeros((m, 2 * f), dtype=g.dtype, device="cuda")
+    gpu.gated_grad(torch.ones_like(out), torch.zeros_like(dx), torch.eye(2 * f, dtype=g.dtype, device="cuda"), saved, dx=dx)
+    want = (act_grad("silu", g.double()) * up)[:, None].expand(m, f)
+    within(dx[:, :f], want, (ROUND["bf16"] * 1.01 + FAR) * want.abs())
