@@ -457,6 +457,18 @@ __device__ __forceinline__ void tmem_ld_head(uint32_t taddr, uint32_t* r) {
   }
 }
 
+// The larger and the smaller of two numbers, NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // --------------------------- packed arithmetic ------------------------------
 // Two fp32 operations in one instruction (the packed forms that sm_100 adds); each half rounds as the scalar form.
 __device__ __forceinline__ unsigned long long pack_f32x2(float lo, float hi) {

@@ -42,9 +42,12 @@ __device__ __forceinline__ float gated_act(float g) {
   if (ACT == ACT_GELU) return g * gated_normal(g).x;
   return g > 0.f ? g : (g != g ? g : 0.f);
 }
-// The activation and its derivative.
+// The activation and its derivative.  A gate that the storage type rounded to an infinity counts as the number next to it: far below zero both are 0,
+// not 0 times infinity (the layer's output was finite there), and far above the derivative is 1.
 template <int ACT>
 __device__ __forceinline__ float2 gated_act_grad(float g) {
+  constexpr float MOST = 3.402823466e38f;
+  g = min_nan(max_nan(g, -MOST), MOST);
   if (ACT == ACT_SILU) {
     const float s = gated_sigmoid(g);
     return make_float2(g * s, s * (1.f + g * (1.f - s)));

@@ -397,3 +397,27 @@ def test_silu_to_the_end_of_its_range(gpu, m):
     gpu.gated_grad(torch.ones_like(out), torch.zeros_like(dx), torch.eye(2 * f, dtype=g.dtype, device="cuda"), saved, dx=dx)
     want = (act_grad("silu", g.double()) * up)[:, None].expand(m, f)
     within(dx[:, :f], want, (ROUND["bf16"] * 1.01 + FAR) * want.abs())
+
+
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("m", [3, 300])
+def test_gates_beyond_f16(gpu, m, kind):
+    """A gate below -65504 is saved as -inf; the layer's output is 0 there, and so are the gradients of both projections."""
+    torch = _torch()
+    f, k = 24, 48
+    x, w = inputs(m, f, k, "f16", 5)
+    x[:, 0], w[:, 0] = 280.0, 0.0
+    w[7, 0] = -250.0                                 # the gate of column 7: some -70000
+    out, saved = check(gpu, x, w, "f16", kind, with_saved=False)[0], torch.zeros((m, 2 * f), dtype=torch.float16, device="cuda")
+    gpu.gated(x, w, torch.zeros_like(out), activation=kind, saved=saved)
+    assert not out[:, 7].any() and (saved[:, 7] == -math.inf).all() and int(torch.isinf(saved).sum()) == m
+    dout = torch.randn((m, f), generator=generator(7), device="cuda").to(torch.float16)
+    kept = saved.clone()
+    kept[:, 7] = -60000.0                            # as far as the gradient goes, the same
+    want = check_grad(gpu, dout, x, w, kept, "f16", kind)
+    got = gpu.gated_grad(dout, x, w, saved, dx=torch.zeros_like(x), dw=torch.zeros_like(w), activation=kind)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    saved[:, 3], kept[:, 3], dout[:, 3] = math.inf, 60000.0, 0.0       # and above, where nothing comes back
+    want = check_grad(gpu, dout, x, w, kept, "f16", kind)
+    got = gpu.gated_grad(dout, x, w, saved, dx=torch.zeros_like(x), dw=torch.zeros_like(w), activation=kind)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
