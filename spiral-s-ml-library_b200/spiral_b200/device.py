@@ -315,10 +315,13 @@ class Workspaces:
     """Device memory for one call's intermediate results: kept per device, host thread and stream, grown on demand (the C ABI
     itself allocates nothing).  A thread's calls on one stream share it in their order.  Calls of other threads, whose launches
     may come between those of one call, on other streams or on other devices (whose default streams share a handle) never do.
-    A thread that ends leaves its own to the next one of its number: its launches, or a graph that holds them, may yet run."""
+    A thread that ends leaves its own to the next one of its number: its launches, or a graph that holds them, may yet run.  For
+    the same reason one that has become too small stays beside the larger one, which is half as large again where there is room:
+    all together then hold at most three times the last."""
 
     def __init__(self):
         self.held = {}
+        self.outgrown = []
 
     @staticmethod
     def _key(stream):
@@ -335,9 +338,18 @@ class Workspaces:
         key = self._key(stream)
         ws = self.held.get(key)
         if ws is None or ws.nbytes < nbytes:
+            nbytes, larger = int(nbytes), None
             if ws is not None:
-                _lib.call("sb_stream_sync", stream_ptr(stream))      # the old buffer may still be in use
-            ws = self.held[key] = DeviceArray((int(nbytes),), "u8")
+                _lib.call("sb_stream_sync", stream_ptr(stream))
+                if nbytes < ws.nbytes + ws.nbytes // 2:
+                    try:
+                        larger = DeviceArray((ws.nbytes + ws.nbytes // 2,), "u8")
+                    except _lib.SpiralError:                         # no room: what is asked for
+                        pass
+            larger = larger or DeviceArray((nbytes,), "u8")
+            if ws is not None:
+                self.outgrown.append(ws)
+            ws = self.held[key] = larger
         return ws
 
 

@@ -115,3 +115,19 @@ def test_split_operands_of_the_fp32_class(sb, library, monkeypatch):
     thread.start()
     thread.join()
     assert others[0].ptr not in {w.ptr for w in held} | {grown.ptr}
+
+
+def test_outgrown_workspaces_stay(sb, library):
+    """A graph that was captured with a workspace may be replayed after a larger call of the same stream."""
+    import gc
+    from spiral_b200.device import stream_workspace
+    sizes, at = [100000, 100001, 150000, 400000, 390000, 1200000], []
+    for n in sizes:
+        ws = stream_workspace(n, 0x71)
+        assert ws.nbytes >= n
+        at.append((ws.ptr, ws.nbytes))
+        del ws
+    gc.collect()
+    assert not library.freed
+    places = dict(at)
+    assert len(places) == 4 and sum(places.values()) <= 3 * at[-1][1]       # 100000, 150000, 400000, 1200000
