@@ -410,7 +410,7 @@ class TokenPolicy:
     head.  ``train_step`` is one AdamW step on the mean cross-entropy; ``forward_8bit`` answers with the dense layers in
     8-bit floating point: ``quantize`` first; ``forward_4bit`` has their weights in 4 bits, for few states: ``quantize_4bit`` first.
     After a step, an upload or a checkpoint the next answer quantises them anew; a caller who writes ``mlp.params`` in another
-    way calls ``quantize`` or ``quantize_4bit`` again.
+    way, as a replayed graph of a step does, calls ``quantize`` or ``quantize_4bit`` again.
 
     ``evaluate`` gives the log probabilities of actions that were taken, the entropy and the likeliest actions, and
     ``policy_gradients`` the gradient of a loss of these two: the parts of a policy-gradient step.
@@ -449,6 +449,8 @@ class TokenPolicy:
             self.features = DeviceArray((self.batch, self.gated), in_dtype)
         self.optimizer = None
         self._codes = self._codes_of = self._codes4 = self._codes4_of = self._evaluated = None
+        # Per group, and per number of alternatives: what one call left may be in a caller's graph when the next wants another.
+        self._codes4_held, self._alternatives = {}, {}
         self._logits_ready = False                # mlp.probs holds what evaluate() left
         if training:
             self.dx = DeviceArray((self.batch, self.width), in_dtype)
@@ -496,17 +498,21 @@ class TokenPolicy:
         """Log probabilities of ``actions`` (int32 or int64 [batch]) under the policy at the temperature 1 / ``scale``: a dict of ``log_probs`` and
         ``entropy`` fp32 [batch] and, where ``top`` > 0, ``top_log_probs`` fp32 and ``top_actions`` int32 [batch, top], the likeliest.  The
         logits stay in ``mlp.probs`` for ``policy_gradients``, and what is returned until the next call."""
-        held = self._evaluated
-        if held is None or held["top_actions"].shape[1] != top:
-            held = self._evaluated = {"log_probs": DeviceArray((self.batch,), "f32"), "entropy": DeviceArray((self.batch,), "f32"),
-                                      "stats": DeviceArray((self.batch, 2), "f32"), "top_log_probs": DeviceArray((self.batch, top), "f32"),
-                                      "top_actions": DeviceArray((self.batch, top), "i32")}
+        if self._evaluated is None:
+            self._evaluated = {"log_probs": DeviceArray((self.batch,), "f32"), "entropy": DeviceArray((self.batch,), "f32"),
+                               "stats": DeviceArray((self.batch, 2), "f32")}
+        held, best, places = self._evaluated, None, None
+        if top:
+            if top not in self._alternatives:
+                self._alternatives[top] = DeviceArray((self.batch, top), "f32"), DeviceArray((self.batch, top), "i32")
+            best, places = self._alternatives[top]
         self._input(tokens, stream)
         logits = self.mlp.forward(self.features, head_flags=0, stream=stream)
-        primitives.log_probs(logits, actions, held["log_probs"], entropy=held["entropy"], stats=held["stats"], top=held["top_log_probs"],
-                             top_tokens=held["top_actions"], mask=mask, scale=scale, stream=stream)
+        primitives.log_probs(logits, actions, held["log_probs"], entropy=held["entropy"], stats=held["stats"], top=best, top_tokens=places,
+                             mask=mask, scale=scale, stream=stream)
         self._logits_ready = True
-        return {k: v for k, v in held.items() if k != "stats" and (top or not k.startswith("top"))}
+        got = {"log_probs": held["log_probs"], "entropy": held["entropy"]}
+        return {**got, "top_log_probs": best, "top_actions": places} if top else got
 
     def policy_gradients(self, tokens, actions, dlog_probs, dentropy=None, mask=None, scale=1.0, stream=None):
         """Gradient of a loss whose derivatives by the log probabilities and the entropies of ``evaluate`` are ``dlog_probs`` and ``dentropy``
@@ -585,8 +591,9 @@ class TokenPolicy:
     def quantize_4bit(self, group=128, stream=None):
         """4-bit codes of the dense layers' weights, a scale per ``group`` columns of a row, for ``forward_4bit``."""
         sizes = self.mlp.sizes
-        if self._codes4 is None or self._codes4[0] != group:
-            self._codes4 = group, [(DeviceArray((o, (i + 1) // 2), "u8"), DeviceArray((-(-i // group), o), self.in_dtype)) for i, o in zip(sizes, sizes[1:])]
+        if group not in self._codes4_held:
+            self._codes4_held[group] = [(DeviceArray((o, (i + 1) // 2), "u8"), DeviceArray((-(-i // group), o), self.in_dtype)) for i, o in zip(sizes, sizes[1:])]
+        self._codes4 = group, self._codes4_held[group]
         for layer, (codes, scales) in enumerate(self._codes4[1]):
             w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
             quantize_int4(w, codes, scales, group=group, stream=stream)
