@@ -561,6 +561,8 @@ int sb_matmul_fp8_plan(int m, int n, int k, int* plan);
 int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,
                  const void* tokens, int index_dtype, float* out, float* entropy, float* stats, int top, float* top_values,
                  int32_t* top_tokens, void* stream);
+/* What sb_log_probs takes a row with: plan = {threads, columns of each in registers (0: in one pass over memory), blocks that share a row}. */
+int sb_log_probs_plan(long long rows, int cols, int top, int* plan);
 /* Its gradient: with dout and dentropy the gradients of `out` and `entropy` (fp32 [rows], NULL: none),
  *   dlogits_j = scale (dout ([j = token] - p_j) - dentropy p_j (log p_j + entropy))
  * in the type of the logits; 0 in columns that are not legal and in rows without a legal logit, and no dout where there is no token.
@@ -579,6 +581,9 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
 enum { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* g (1 + erf(g / sqrt 2)) / 2 */, SB_ACT_RELU = 2 };
 int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h, long long ldh, void* saved, long long lds, int m, int f,
              int k, int dtype, int activation, void* stream);
+/* The tiles that sb_gated takes for rows of x and w that start on 16 bytes: plan = {rows, columns of h, tiles, tiles of half the columns behind
+ * them}; 8 or 16 rows are the form for few rows, 256 a pair of CTAs. */
+int sb_gated_plan(int m, int f, int k, int* plan);
 /* Its gradient from dh [m, f] and what was saved:
  *   dg = dh u act'(g)   du = dh act(g)   dx = [dg du] w   dw = [dg du]^T x
  * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
@@ -587,6 +592,9 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
  * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  dx may not be w, nor dw x.  Both products run at once: where both are wanted dx may
  * not be x either, nor dw w. */
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
+/* The tiles of its products where rows start on 16 bytes (which: 1 dx, 2 dw, 3 both): plan = {columns, and for dx and then dw: tiles of all K, tiles in
+ * parts of K, parts}; tiles have 256 rows. */
+int sb_gated_grad_plan(int m, int f, int k, int which, int* plan);
 int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,
                   void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, int accumulate, int m, int f, int k, int dtype,
                   int activation, void* workspace, size_t workspace_bytes, void* stream);
@@ -606,6 +614,9 @@ int sb_dequantize_int4(const uint8_t* codes, long long ldw, const void* scales, 
  * one of the inputs. */
 int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes, long long ldw, const void* scales, int scale_dtype, void* c,
                    long long ldc, int m, int n, int k, int group, int out_dtype, int epilogue, const float* bias, void* stream);
+/* Its form for contiguous matrices that start on 16 bytes: plan = {rows of a that a block has (0: up to 8, through registers alone), blocks that
+ * share K}. */
+int sb_matmul_int4_plan(int m, int n, int k, int group, int* plan);
 
 /* ---- data-parallel update over peer memory ---------------------------------
  * No reference counterpart (the reference is single-device, corecuda/base.spi:7);

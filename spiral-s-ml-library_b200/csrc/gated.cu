@@ -924,6 +924,22 @@ int gated_args_ok(const char* who, int m, int f, int k, int dtype, int activatio
 template <typename T>
 constexpr int gated_code() { return std::is_same<T, __half>::value ? SB_F16 : SB_BF16; }
 
+// Tiles of `rows` x `columns`: whole ones, and behind them halves of columns for the rest.
+struct GatedTiles {
+  int tiles_m, tiles_f, half_first, items;
+};
+GatedTiles gated_tiles(long long m, long long f, int rows, int columns) {
+  const int most = rows == 256 ? sb_sm_count() / 2 : sb_sm_count();
+  GatedTiles t;
+  t.tiles_m = (int)((m + rows - 1) / rows);
+  t.tiles_f = (int)((f + columns - 1) / columns);
+  const int tiles = t.tiles_m * t.tiles_f, rest = tiles % most;
+  // A last wave of at most half the workers is cut into halves.
+  t.half_first = rows == 256 && tiles > most && 2 * rest <= most ? tiles - rest : tiles;
+  t.items = 2 * tiles - t.half_first;
+  return t;
+}
+
 template <bool PAIR, typename T, int ACT>
 int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
   const CUtensorMapDataType type = gated_code<T>() == SB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -932,13 +948,12 @@ int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
   const int tile_m = PAIR ? 256 : 128;
   const int most = PAIR ? sb_sm_count() / 2 : sb_sm_count();
   q.bf = bf;
-  q.tiles_m = (p.m + tile_m - 1) / tile_m;
-  q.tiles_f = (p.f + bf - 1) / bf;
-  if ((long long)q.tiles_m * q.tiles_f > 0x3fffffff) return sb_fail(SB_ERR_TOO_LARGE, "sb_gated: too many outputs");
-  const int tiles = q.tiles_m * q.tiles_f, rest = tiles % most;
-  // A last wave of at most half the workers is cut into halves.
-  q.half_first = PAIR && tiles > most && 2 * rest <= most ? tiles - rest : tiles;
-  q.items = 2 * tiles - q.half_first;
+  if (((long long)p.m + tile_m - 1) / tile_m * (((long long)p.f + bf - 1) / bf) > 0x3fffffff) return sb_fail(SB_ERR_TOO_LARGE, "sb_gated: too many outputs");
+  const GatedTiles t = gated_tiles(p.m, p.f, tile_m, bf);
+  q.tiles_m = t.tiles_m;
+  q.tiles_f = t.tiles_f;
+  q.half_first = t.half_first;
+  q.items = t.items;
   q.k_blocks = (p.k + 63) / 64;
   q.acc_stride = bf > 64 ? 256 : 2 * bf;
   q.tmem_cols = 2 * q.acc_stride;
@@ -952,7 +967,7 @@ int launch_gated_umma(const GatedArgs& p, int bf, cudaStream_t s) {
   memset(&maps, 0, sizeof(maps));
   int rc = sb_tensor_map(&maps.x, type, 2, p.x, p.m, p.k, p.ldx, 128, 64);
   if (rc == SB_OK) rc = sb_tensor_map(&maps.w, type, 2, p.w, 2LL * p.f, p.k, p.ldw, bf, 64);
-  if (rc == SB_OK && q.items > tiles) rc = sb_tensor_map(&maps.w_half, type, 2, p.w, 2LL * p.f, p.k, p.ldw, bf / 2, 64);
+  if (rc == SB_OK && q.items > q.half_first) rc = sb_tensor_map(&maps.w_half, type, 2, p.w, 2LL * p.f, p.k, p.ldw, bf / 2, 64);
   q.boxes_out = gated_rows16(p.h, p.ldh, gated_code<T>()) && (!saved || (gated_rows16(saved, p.lds, gated_code<T>()) && p.f % 8 == 0)) ? 1 : 0;
   if (q.boxes_out) {
     if (rc == SB_OK) rc = sb_tensor_map(&maps.h, type, 2, p.h, p.m, p.f, p.ldh, 32, 32);
@@ -977,21 +992,31 @@ int launch_gated_few(const GatedArgs& p, cudaStream_t s) {
   return SB_OK;
 }
 
+// Rows and columns of h that a block, or a pair of them, makes where rows of x and w start on 16 bytes; up to 16 rows are for the few.
+struct GatedForm {
+  int rows, columns;
+};
+GatedForm gated_form(int m, int f, int k) {
+  if (m <= 16) return {m <= 8 ? 8 : 16, GF_ROWS};
+  // Pairs of CTAs on 256 rows and 128 columns of h, or CTAs on 128 rows and 128 or 64 columns: the least of waves x time of a tile, in us as
+  // measured.  Pairs / 128 / 64: 16384 x 4096 x 1024 176 / 198 / 238, 16384 x 512 x 512 23.2 / 23.2 / 19.5, 512 x 4096 x 1024 12.0 / 10.6 / 11.4,
+  // 256 x 4096 x 1024 11.5 / 10.0 / 9.7, 1000^3 13.3 / 14.7 / 10.7, 128 x 512 x 4096 28 / 29 / 16.
+  const int sms = sb_sm_count(), blocks = (k + 63) / 64;
+  const long long wide = (f + 127) / 128, tall = (m + 127) / 128, pairs = (m + 255) / 256 * wide, half = sms / 2;
+  const double pair_waves = (double)(pairs / half) + (pairs % half == 0 ? 0.0 : pairs > half && 2 * (pairs % half) <= half ? 0.5 : 1.0);
+  const double pair = 6.0 + pair_waves * (2.9 + 0.21 * blocks), single = 4.0 + (double)((tall * wide + sms - 1) / sms) * (2.55 + 0.28 * blocks),
+               narrow = 4.0 + (double)((tall * ((f + 63) / 64) + sms - 1) / sms) * (0.15 + 0.256 * blocks);
+  if (m > 128 && pair <= single && pair <= narrow) return {256, 128};
+  return {128, single <= narrow ? 128 : 64};
+}
+
 template <typename T, int ACT>
 int launch_gated(const GatedArgs& p, cudaStream_t s) {
   if (p.k > 0 && gated_rows16(p.x, p.m == 1 ? 8 : p.ldx, gated_code<T>()) && gated_rows16(p.w, p.ldw, gated_code<T>())) {
-    if (p.m <= 8) return launch_gated_few<T, ACT, 1>(p, s);
-    if (p.m <= 16) return launch_gated_few<T, ACT, 2>(p, s);
-    // Pairs of CTAs on 256 rows and 128 columns of h, or CTAs on 128 rows and 128 or 64 columns: the least of waves x time of a tile, in us as
-    // measured.  Pairs / 128 / 64: 16384 x 4096 x 1024 176 / 198 / 238, 16384 x 512 x 512 23.2 / 23.2 / 19.5, 512 x 4096 x 1024 12.0 / 10.6 / 11.4,
-    // 256 x 4096 x 1024 11.5 / 10.0 / 9.7, 1000^3 13.3 / 14.7 / 10.7, 128 x 512 x 4096 28 / 29 / 16.
-    const int sms = sb_sm_count(), blocks = (p.k + 63) / 64;
-    const long long wide = (p.f + 127) / 128, tall = (p.m + 127) / 128, pairs = (p.m + 255) / 256 * wide, half = sms / 2;
-    const double pair_waves = (double)(pairs / half) + (pairs % half == 0 ? 0.0 : pairs > half && 2 * (pairs % half) <= half ? 0.5 : 1.0);
-    const double pair = 6.0 + pair_waves * (2.9 + 0.21 * blocks), single = 4.0 + (double)((tall * wide + sms - 1) / sms) * (2.55 + 0.28 * blocks),
-                 narrow = 4.0 + (double)((tall * ((p.f + 63) / 64) + sms - 1) / sms) * (0.15 + 0.256 * blocks);
-    if (p.m > 128 && pair <= single && pair <= narrow) return launch_gated_umma<true, T, ACT>(p, 128, s);
-    return launch_gated_umma<false, T, ACT>(p, single <= narrow ? 128 : 64, s);
+    const GatedForm form = gated_form(p.m, p.f, p.k);
+    if (form.rows == 8) return launch_gated_few<T, ACT, 1>(p, s);
+    if (form.rows == 16) return launch_gated_few<T, ACT, 2>(p, s);
+    return form.rows == 256 ? launch_gated_umma<true, T, ACT>(p, form.columns, s) : launch_gated_umma<false, T, ACT>(p, form.columns, s);
   }
   const dim3 grid((unsigned)((p.m + GS_TILE - 1) / GS_TILE), (unsigned)((p.f + GS_TILE - 1) / GS_TILE));
   SB_CUDA(sb_launch(gated_simple_kernel<T, ACT>, grid, dim3(256), 0, s, 1, p));
@@ -1188,6 +1213,42 @@ int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h
 #define SB_GATED_CALL(ACT) (dtype == SB_BF16 ? launch_gated<__nv_bfloat16, ACT>(p, s) : launch_gated<__half, ACT>(p, s))
   return activation == SB_ACT_SILU ? SB_GATED_CALL(ACT_SILU) : activation == SB_ACT_GELU ? SB_GATED_CALL(ACT_GELU) : SB_GATED_CALL(ACT_RELU);
 #undef SB_GATED_CALL
+}
+
+int sb_gated_plan(int m, int f, int k, int* plan) {
+  const char* who = "sb_gated_plan";
+  int rc = gated_args_ok(who, m, f, k, SB_BF16, SB_ACT_SILU);
+  if (rc != SB_OK) return rc;
+  if (!plan) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
+  if (m == 0 || f == 0 || k == 0) return sb_fail(SB_ERR_BAD_ARG, "%s: sizes of nothing", who);
+  const GatedForm form = gated_form(m, f, k);
+  if (((long long)m + form.rows - 1) / form.rows * (((long long)f + form.columns - 1) / form.columns) > 0x3fffffff) return sb_fail(SB_ERR_TOO_LARGE, "%s: too many outputs", who);
+  const GatedTiles t = gated_tiles(m, f, form.rows, form.columns);
+  plan[0] = form.rows;
+  plan[1] = form.columns;
+  plan[2] = t.half_first;
+  plan[3] = t.items - t.half_first;
+  return SB_OK;
+}
+
+int sb_gated_grad_plan(int m, int f, int k, int which, int* plan) {
+  const char* who = "sb_gated_grad_plan";
+  int rc = gated_args_ok(who, m, f, k, SB_BF16, SB_ACT_SILU);
+  if (rc != SB_OK) return rc;
+  if (!plan) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
+  if (m == 0 || f == 0 || k == 0 || which < 1 || which > 3) return sb_fail(SB_ERR_BAD_ARG, "%s: sizes of nothing, or neither product", who);
+  if (((long long)m + 255) / 256 * ((k + 127) / 128) + (2LL * f + 255) / 256 * ((k + 127) / 128) > 0x1fffffff) return sb_fail(SB_ERR_TOO_LARGE, "%s: too many outputs", who);
+  const ProductSize size[2] = {{which & 1 ? m : 0, k, 2LL * f}, {which & 2 ? 2LL * f : 0, k, m}};
+  ProductsPlan q;
+  memset(&q, 0, sizeof(q));
+  gated_products_plan(size, gated_grad_twice(m), &q);
+  plan[0] = q.bn;
+  for (int i = 0; i < 2; ++i) {
+    plan[1 + 3 * i] = q.p[i].whole;
+    plan[2 + 3 * i] = q.p[i].tiles_m * q.p[i].tiles_n - q.p[i].whole;
+    plan[3 + 3 * i] = q.p[i].parts;
+  }
+  return SB_OK;
 }
 
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes) {

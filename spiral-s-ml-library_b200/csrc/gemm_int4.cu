@@ -473,16 +473,38 @@ int int4_args_ok(const char* who, long long n, int k, int group, int scale_dtype
 
 bool int4_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (size_t)sb_dtype_size(dtype) == 0; }
 
+// The form of a product: rows of a that a block has (0: the fewest, straight to registers), and blocks that share K.
+struct Int4Form {
+  int rows, blocks;
+};
+Int4Form int4_form(long long m, long long n, int k, int group, int code_piece, bool whole_rows) {
+  const long long sms = sb_sm_count();
+  // Small matrices of weights, whose time is that of the way there: 1 x 4096 x 4096 in groups of 128 4.8 us, through rings 6.1; 1 x 256 x 512
+  // 2.1 / 4.5; 8 x 4096 x 4096 6.5 / 6.5.  Not long rows (1 x 1024 x 16384 27 / 12) nor more blocks than there is room for (1 x 8192 x 8192
+  // 17.5 / 14.2).
+  if (m <= 8 && k <= 4096 && n <= 32 * sms && k % group == 0 && code_piece >= group / 8 && whole_rows) return {0, 1};
+  // Where all blocks run at once (or, of 16 rows, nearly), fewer rows of a in each and more blocks: 48 x 201 x 12728 with 64 / 16 / 8 rows of a in a
+  // block 53 / 20.5 / 12.2 us, 64 x 1024 x 1024 15.1 / 6.5 / 5.6, 64 x 2048 x 2048 15.6 / 8.0 / 8.8, 64 x 4096 x 4096 32 / 18.6 / 23, 16 x 3000 x 6000
+  // 9.9 (16) / 14.1; larger ones read their weights again for nothing: 32 x 8192 x 8192 30 (32) / 33 / 43.
+  const long long shares = k >= 2048 ? 8 : k >= 1024 ? 4 : k >= 512 ? 2 : 1;
+  int rows = m <= 32 ? 32 : 64;
+  if (m <= 8 || (n + 127) / 128 * ((m + 7) / 8) * shares <= 2 * sms) rows = 8;
+  else if (m <= 16 || (n + 255) / 256 * ((m + 15) / 16) * shares <= 4 * sms) rows = 16;
+  // Blocks that share K until every SM has the warps it can hold, each with 256 columns at least.
+  const int warps = rows == 8 ? 8 : 16;
+  const long long tiles = (n + 16 * warps - 1) / (16 * warps), down = (m + rows - 1) / rows;
+  int blocks = 1;
+  // Not in clusters of 8 that the chip's parts have no room for at once: 16 x 4096 x 4096 in 16 of them 14.5 us, in clusters of 4 10.4.
+  const long long room = (16 / warps) * sms, room8 = warps == 16 ? 3 * room / 4 : 7 * room / 8;
+  while (blocks < 8 && tiles * down * blocks * 2 <= (blocks < 4 ? room : room8) && k >= 512 * blocks) blocks *= 2;
+  return {rows, blocks};
+}
+
 template <typename T, int G, int NT, int WARPS, int STAGES>
-int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
+int launch_int4(const Int4Args& p, Int4Few q, int blocks, cudaStream_t s) {
   constexpr int ROWS = 16 * WARPS, COLS = 8 * NT, MOST = int4_chunk<NT>, RING = WARPS * STAGES * I4_STAGE, SUMS = ROWS * (COLS + 2) * 4, LIMIT = RING + MOST * COLS * 2 + MOST / G * ROWS * 4 + SUMS;
   static_assert(LIMIT <= 227 * 1024, "more shared memory than an SM has");
   const long long tiles = ((long long)p.n + ROWS - 1) / ROWS, down = ((long long)p.m + COLS - 1) / COLS;
-  // Blocks that share K until every SM has the warps it can hold, each with 256 columns at least.
-  int blocks = 1;
-  // Not in clusters of 8 that the chip's parts have no room for at once: 16 x 4096 x 4096 in 16 of them 14.5 us, in clusters of 4 10.4.
-  const long long room = (16 / WARPS) * sb_sm_count(), room8 = WARPS == 16 ? 3 * room / 4 : 7 * room / 8;
-  while (blocks < 8 && tiles * down * blocks * 2 <= (blocks < 4 ? room : room8) && p.k >= 512 * blocks) blocks *= 2;
   q.blocks = blocks;
   q.range = ((p.k + blocks - 1) / blocks + I4_STEP - 1) / I4_STEP * I4_STEP;
   q.chunk = q.range < MOST ? q.range : MOST;
@@ -498,22 +520,16 @@ int launch_int4(const Int4Args& p, Int4Few q, cudaStream_t s) {
 
 template <typename T, int G>
 int launch_int4(const Int4Args& p, const Int4Few& q, cudaStream_t s) {
-  // Small matrices of weights, whose time is that of the way there: 1 x 4096 x 4096 in groups of 128 4.8 us, through rings 6.1; 1 x 256 x 512
-  // 2.1 / 4.5; 8 x 4096 x 4096 6.5 / 6.5.  Not long rows (1 x 1024 x 16384 27 / 12) nor more blocks than there is room for (1 x 8192 x 8192
-  // 17.5 / 14.2).
-  if (p.m <= 8 && p.k <= 4096 && p.n <= 32 * sb_sm_count() && p.k % G == 0 && q.code_piece >= G / 8 && q.whole_rows) {
+  const Int4Form form = int4_form(p.m, p.n, p.k, G, q.code_piece, q.whole_rows != 0);
+  if (form.rows == 0) {
     SB_CUDA(sb_launch(gemm_int4_fewest_kernel<T, G>, dim3((unsigned)(((long long)p.n + 15) / 16)), dim3(256), 0, s, 1, p, q.scale_dtype));
     SB_COUNT_LAUNCH();
     return SB_OK;
   }
-  // Where all blocks run at once (or, of 16 rows, nearly), fewer rows of a in each and more blocks: 48 x 201 x 12728 with 64 / 16 / 8 rows of a in a
-  // block 53 / 20.5 / 12.2 us, 64 x 1024 x 1024 15.1 / 6.5 / 5.6, 64 x 2048 x 2048 15.6 / 8.0 / 8.8, 64 x 4096 x 4096 32 / 18.6 / 23, 16 x 3000 x 6000
-  // 9.9 (16) / 14.1; larger ones read their weights again for nothing: 32 x 8192 x 8192 30 (32) / 33 / 43.
-  const long long shares = p.k >= 2048 ? 8 : p.k >= 1024 ? 4 : p.k >= 512 ? 2 : 1, sms = sb_sm_count();
-  if (p.m <= 8 || ((long long)p.n + 127) / 128 * (((long long)p.m + 7) / 8) * shares <= 2 * sms) return launch_int4<T, G, 1, 8, 4>(p, q, s);
-  if (p.m <= 16 || ((long long)p.n + 255) / 256 * (((long long)p.m + 15) / 16) * shares <= 4 * sms) return launch_int4<T, G, 2, 16, 4>(p, q, s);
-  if (p.m <= 32) return launch_int4<T, G, 4, 16, 4>(p, q, s);
-  return launch_int4<T, G, 8, 16, 3>(p, q, s);
+  if (form.rows == 8) return launch_int4<T, G, 1, 8, 4>(p, q, form.blocks, s);
+  if (form.rows == 16) return launch_int4<T, G, 2, 16, 4>(p, q, form.blocks, s);
+  if (form.rows == 32) return launch_int4<T, G, 4, 16, 4>(p, q, form.blocks, s);
+  return launch_int4<T, G, 8, 16, 3>(p, q, form.blocks, s);
 }
 
 // The widest pieces in which rows can be copied.
@@ -621,6 +637,18 @@ int sb_matmul_int4(const void* a, long long lda, int dtype, const uint8_t* codes
   p.out_dtype = out_dtype;
   cudaStream_t s = (cudaStream_t)stream;
   return dtype == SB_BF16 ? launch_int4<__nv_bfloat16>(p, scale_dtype, s) : launch_int4<__half>(p, scale_dtype, s);
+}
+
+int sb_matmul_int4_plan(int m, int n, int k, int group, int* plan) {
+  const char* who = "sb_matmul_int4_plan";
+  int rc = int4_args_ok(who, n, k, group, SB_BF16);
+  if (rc != SB_OK) return rc;
+  if (!plan) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
+  if (m <= 0 || n == 0 || k == 0) return sb_fail(SB_ERR_BAD_ARG, "%s: sizes of nothing", who);
+  const Int4Form form = int4_form(m, n, k, group, int4_piece(nullptr, n == 1 ? 16 : (k + 1) / 2, 1), int4_piece(nullptr, m == 1 ? 16 : 2LL * k, 2) == 16);
+  plan[0] = form.rows;
+  plan[1] = form.blocks;
+  return SB_OK;
 }
 
 }  // extern "C"

@@ -1015,21 +1015,43 @@ int launch_log_probs_long(const LogProbArgs& g, int blocks, cudaStream_t s) {
   return SB_OK;
 }
 
-template <typename T>
-int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
+// What takes a row: `threads` of a warp with `columns` each in registers (0: in one pass over memory), or a block of them, and `blocks` that share a row.
+struct LogProbForm {
+  int threads, columns, blocks;
+};
+LogProbForm log_probs_form(long long rows, int cols, int top) {
   // Few lanes with many columns each: their rounds cost by the lane.  us, 65536 rows: 10 columns (fp32, 2 alternatives) with 4 / 2 lanes 7.5 / 5.5; 20 with
   // 8 / 4 14.7 / 8.1; 64 (bf16, 2) with 8 / 4 / 2 15.0 / 12.3 / 13.5; 100000 rows: 128 (bf16, none) with 32 / 8 / 4 46.8 / 20.8 / 14.9, with 32
   // alternatives by warps, as below / 8 / 4 413 / 212 / 172; 200 (2) with 32 / 16 / 8 84.5 / 66.6 / 46.7.
-  if (g.cols <= 16) return launch_log_probs_short<T, 2, 8>(g, s);
-  if (g.cols <= 32) return launch_log_probs_short<T, 4, 8>(g, s);
-  if (g.cols <= 64) return launch_log_probs_short<T, 4, 16>(g, s);
-  if (g.cols <= 128) return launch_log_probs_short<T, 4, 32>(g, s);
+  if (cols <= 16) return {2, 8, 1};
+  if (cols <= 32) return {4, 8, 1};
+  if (cols <= 64) return {4, 16, 1};
+  if (cols <= 128) return {4, 32, 1};
   // Rounds cost by the alternative, the warps' bound costs once: 250 columns with 16 alternatives 237 (16 lanes) / 168; 500 columns with none, 2 or 7 of
   // them 28 / 41, 53 / 88, 59 / 41 (32768 rows of fp32); 1000 with 2 of them 54 / 45.
-  if (g.cols <= 256 && g.top <= 7) return launch_log_probs_short<T, 8, 32>(g, s);
-  if (g.cols <= 512 && g.top <= 3) return launch_log_probs_short<T, 16, 32>(g, s);
+  if (cols <= 256 && top <= 7) return {8, 32, 1};
+  if (cols <= 512 && top <= 3) return {16, 32, 1};
   // Warps or blocks, 8 alternatives: 32768 x 2048 69 / 152, 16384 x 8192 94 / 98, 8192 x 16384 93 / 80, 600 x 4096 11.7 / 9.3.
-  if (g.cols <= 1024 || (g.cols <= 8192 && g.rows >= 16LL * sb_sm_count())) {
+  if (cols <= 1024 || (cols <= 8192 && rows >= 16LL * sb_sm_count())) return {32, 0, 1};
+  // A cluster per row where rows are few, all of them resident at once: 35 x 41654 with 3 alternatives in clusters of 8, which the chip's parts hold 32
+  // of, 16.3, of 4 9.5; 70 rows 12.1 (4), 9.1 (2).
+  int blocks = 1;
+  while (blocks < 8 && rows * blocks * 2 <= 3LL * sb_sm_count() / 2 && cols / (2 * blocks) >= 4096) blocks *= 2;
+  if (blocks > 1) return {512, 0, blocks};
+  // Threads of a row, 8 alternatives, 128 / 256 / 512: 4096 x 20000 53 / 61 / 114, 4096 x 50001 114 / 103 / 139, 1024 x 130000 80 / 73 / 66.
+  return {cols <= 24576 ? 128 : cols <= 98304 ? 256 : 512, 0, 1};
+}
+
+template <typename T>
+int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
+  const LogProbForm form = log_probs_form(g.rows, g.cols, g.top);
+  if (form.columns > 0) {
+    if (form.threads == 2) return launch_log_probs_short<T, 2, 8>(g, s);
+    if (form.threads == 4)
+      return form.columns == 8 ? launch_log_probs_short<T, 4, 8>(g, s) : form.columns == 16 ? launch_log_probs_short<T, 4, 16>(g, s) : launch_log_probs_short<T, 4, 32>(g, s);
+    return form.threads == 8 ? launch_log_probs_short<T, 8, 32>(g, s) : launch_log_probs_short<T, 16, 32>(g, s);
+  }
+  if (form.threads == 32) {
     const long long blocks = (g.rows + 3) / 4, most = 64LL * sb_sm_count();
     const dim3 grid((unsigned)(blocks < most ? blocks : most));
     if (g.mask) SB_CUDA(sb_launch(log_probs_warp_kernel<T, true>, grid, dim3(128), 0, s, 1, g));
@@ -1037,14 +1059,9 @@ int launch_log_probs(const LogProbArgs& g, cudaStream_t s) {
     SB_COUNT_LAUNCH();
     return SB_OK;
   }
-  // A cluster per row where rows are few, all of them resident at once: 35 x 41654 with 3 alternatives in clusters of 8, which the chip's parts hold 32
-  // of, 16.3, of 4 9.5; 70 rows 12.1 (4), 9.1 (2).
-  int blocks = 1;
-  while (blocks < 8 && g.rows * blocks * 2 <= 3LL * sb_sm_count() / 2 && g.cols / (2 * blocks) >= 4096) blocks *= 2;
-  if (blocks > 1) return launch_log_probs_long<T, 512, true>(g, blocks, s);
-  // Threads of a row, 8 alternatives, 128 / 256 / 512: 4096 x 20000 53 / 61 / 114, 4096 x 50001 114 / 103 / 139, 1024 x 130000 80 / 73 / 66.
-  if (g.cols <= 24576) return launch_log_probs_long<T, 128, false>(g, 1, s);
-  if (g.cols <= 98304) return launch_log_probs_long<T, 256, false>(g, 1, s);
+  if (form.blocks > 1) return launch_log_probs_long<T, 512, true>(g, form.blocks, s);
+  if (form.threads == 128) return launch_log_probs_long<T, 128, false>(g, 1, s);
+  if (form.threads == 256) return launch_log_probs_long<T, 256, false>(g, 1, s);
   return launch_log_probs_long<T, 512, false>(g, 1, s);
 }
 
@@ -1106,6 +1123,17 @@ int sb_log_probs(const void* logits, long long ld, int dtype, long long rows, in
   cudaStream_t s = (cudaStream_t)stream;
   return dtype == SB_F32 ? launch_log_probs<float>(g, s)
          : dtype == SB_BF16 ? launch_log_probs<__nv_bfloat16>(g, s) : launch_log_probs<__half>(g, s);
+}
+
+int sb_log_probs_plan(long long rows, int cols, int top, int* plan) {
+  const char* who = "sb_log_probs_plan";
+  if (!plan) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
+  if (rows <= 0 || cols <= 0 || top < 0 || top > LP_MAX_TOP) return sb_fail(SB_ERR_BAD_ARG, "%s: sizes of nothing, or more than %d alternatives", who, LP_MAX_TOP);
+  const LogProbForm form = log_probs_form(rows, cols, top);
+  plan[0] = form.threads;
+  plan[1] = form.columns;
+  plan[2] = form.blocks;
+  return SB_OK;
 }
 
 int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long rows, int cols, const uint8_t* mask, int prefix, float scale,

@@ -170,12 +170,16 @@ SIGNATURES = {
     "sb_matmul_fp8": (_I, [_P, _L, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _P, _P]),
     "sb_matmul_fp8_plan": (_I, [_I, _I, _I, _IP]),
     "sb_log_probs": (_I, [_P, _L, _I, _L, _I, _P, _I, _F, _P, _I, _P, _P, _P, _I, _P, _P, _P]),
+    "sb_log_probs_plan": (_I, [_L, _I, _I, _IP]),
     "sb_log_probs_grad": (_I, [_P, _L, _I, _L, _I, _P, _I, _F, _P, _I, _P, _P, _P, _P, _P, _L, _P]),
     "sb_gated": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _P]),
+    "sb_gated_plan": (_I, [_I, _I, _I, _IP]),
+    "sb_gated_grad_plan": (_I, [_I, _I, _I, _I, _IP]),
     "sb_gated_grad_workspace_bytes": (_I, [_I, _I, _I, POINTER(c_size_t)]),
     "sb_gated_grad": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "sb_quantize_int4": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _I, _P]),
     "sb_dequantize_int4": (_I, [_P, _L, _P, _I, _P, _L, _I, _L, _I, _I, _P]),
+    "sb_matmul_int4_plan": (_I, [_I, _I, _I, _I, _IP]),
     "sb_matmul_int4": (_I, [_P, _L, _I, _P, _L, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _P, _P]),
     "sb_sgd_update": (_I, [_P, _P, _P, ctypes.c_longlong, _F, _I, _P]),
     "sb_mlp_train_step": (_I, [_I, _IP, _I, _I, _P, _P, _P, _PP, _PP, _P, _P, _P, _P, _I, _F, _P, _Z, _P, _P]),

@@ -282,6 +282,22 @@ def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulat
     return dx, keep_tf32(dw, stream)
 
 
+def gated_plan(m, f, k):
+    """What ``gated`` takes for rows of x and w that start on 16 bytes: rows and columns of h in a tile (8 or 16 rows: the form for few
+    rows; 256: a pair of CTAs), tiles, and tiles of half the columns behind them."""
+    plan = (ctypes.c_int * 4)()
+    _lib.call("sb_gated_plan", int(m), int(f), int(k), plan)
+    return dict(zip(("rows", "columns", "tiles", "half_tiles"), list(plan)))
+
+
+def gated_grad_plan(m, f, k, dx=True, dw=True):
+    """What the products of ``gated_grad`` take where rows start on 16 bytes: columns of a tile (of 256 rows), and for dx and dw the tiles of
+    all K, those in parts of K, and the parts."""
+    plan = (ctypes.c_int * 7)()
+    _lib.call("sb_gated_grad_plan", int(m), int(f), int(k), int(bool(dx)) + 2 * int(bool(dw)), plan)
+    return {"columns": plan[0], "dx": tuple(plan[1:4]), "dw": tuple(plan[4:7])}
+
+
 def gated_grad_workspace(m, f, k):
     """Bytes of device memory that ``gated_grad`` needs for m rows and a [2 f, k] weight matrix."""
     nbytes = ctypes.c_size_t(0)
@@ -352,3 +368,11 @@ def matmul_int4(a, codes, scales, c, group=128, epilogue=(), bias=None, stream=N
     _lib.call("sb_matmul_int4", a, lda, _GATED[a_tag], codes, ldw, scales, scale_code, c_ptr, ldc, m, n, k, group, _FP8_FLOATS[tag], epi,
               array_ptr(bias, n, "f32", "bias") if epi & _lib.EPI_BIAS else None, stream_ptr(stream))
     return keep_tf32(c, stream)
+
+
+def matmul_int4_plan(m, n, k, group=128):
+    """What ``matmul_int4`` takes for contiguous matrices that start on 16 bytes: rows of a in a block (0: up to 8, through registers
+    alone) and blocks that share K."""
+    plan = (ctypes.c_int * 2)()
+    _lib.call("sb_matmul_int4_plan", int(m), int(n), int(k), int(group), plan)
+    return dict(zip(("rows", "blocks"), list(plan)))

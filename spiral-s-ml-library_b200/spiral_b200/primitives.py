@@ -288,6 +288,13 @@ def log_probs(logits, tokens=None, out=None, entropy=None, stats=None, top=None,
     return out
 
 
+def log_probs_plan(rows, cols, top=0):
+    """What ``log_probs`` takes a row with: threads, columns of each in registers (0: in one pass over memory), blocks that share a row."""
+    plan = (ctypes.c_int * 3)()
+    _lib.call("sb_log_probs_plan", int(rows), int(cols), int(top), plan)
+    return dict(zip(("threads", "columns", "blocks"), list(plan)))
+
+
 def log_probs_grad(logits, tokens, stats, dlogits, dout=None, dentropy=None, entropy=None, mask=None, prefix=-1, scale=1.0, stream=None):
     """Gradient of ``log_probs``: ``dlogits`` (like ``logits``, and may be them) from ``dout`` and ``dentropy``, the gradients of
     ``out`` and ``entropy`` (fp32 [rows], None: none), with the ``stats`` and, for ``dentropy``, the ``entropy`` that the forward call
