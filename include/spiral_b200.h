@@ -117,6 +117,8 @@ int sb_memset(void* dst, int value, size_t bytes, void* stream);
 int sb_stream_create(void** stream);
 int sb_stream_destroy(void* stream);
 int sb_stream_sync(void* stream);               /* corecuda/base.spi:45 device_sync */
+/* 1 while launches on `stream` are captured into a graph and do not run, else 0. */
+int sb_stream_capturing(void* stream, int* capturing);
 int sb_device_sync(void);
 int sb_event_create(void** event);
 int sb_event_destroy(void* event);

@@ -209,6 +209,14 @@ int sb_stream_sync(void* stream) {
   return SB_OK;
 }
 
+int sb_stream_capturing(void* stream, int* capturing) {
+  if (!capturing) return sb_fail(SB_ERR_BAD_ARG, "sb_stream_capturing: null output");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  SB_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &status));
+  *capturing = status != cudaStreamCaptureStatusNone ? 1 : 0;
+  return SB_OK;
+}
+
 int sb_device_sync(void) {
   SB_CUDA(cudaDeviceSynchronize());
   return SB_OK;

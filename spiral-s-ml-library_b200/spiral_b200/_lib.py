@@ -99,6 +99,7 @@ SIGNATURES = {
     "sb_stream_create": (_I, [_PP]),
     "sb_stream_destroy": (_I, [_P]),
     "sb_stream_sync": (_I, [_P]),
+    "sb_stream_capturing": (_I, [_P, _IP]),
     "sb_device_sync": (_I, []),
     "sb_event_create": (_I, [_PP]),
     "sb_event_destroy": (_I, [_P]),

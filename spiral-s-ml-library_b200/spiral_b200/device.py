@@ -396,6 +396,13 @@ class Stream:
             pass
 
 
+def capturing(stream=None):
+    """Whether launches on ``stream`` are captured into a graph, and do not run."""
+    n = ctypes.c_int(0)
+    _lib.call("sb_stream_capturing", stream_ptr(stream), ctypes.byref(n))
+    return bool(n.value)
+
+
 def wait_event(stream, event):
     """Work submitted to `stream` (None = default stream) after this call waits for `event`."""
     _lib.call("sb_stream_wait_event", stream_ptr(stream), event.ptr)

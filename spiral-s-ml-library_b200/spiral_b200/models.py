@@ -11,7 +11,7 @@ import ctypes
 import numpy as np
 
 from . import _lib, primitives
-from .device import DeviceArray, device_ptr, stream_ptr, values_ptr
+from .device import DeviceArray, capturing, device_ptr, stream_ptr, values_ptr
 from . import dtypes
 from .matmul import ACTIVATIONS, gated, gated_grad, matmul, matmul_fp8, matmul_int4, quantize_fp8, quantize_int4
 from .optim import AdamW
@@ -410,7 +410,8 @@ class TokenPolicy:
     head.  ``train_step`` is one AdamW step on the mean cross-entropy; ``forward_8bit`` answers with the dense layers in
     8-bit floating point: ``quantize`` first; ``forward_4bit`` has their weights in 4 bits, for few states: ``quantize_4bit`` first.
     After a step, an upload or a checkpoint the next answer quantises them anew; a caller who writes ``mlp.params`` in another
-    way, as a replayed graph of a step does, calls ``quantize`` or ``quantize_4bit`` again.
+    way, as a replayed graph of a step does, calls ``quantize`` or ``quantize_4bit`` again.  A graph of an answer quantises in every
+    replay if the weights had changed when it was captured, else never: then its caller quantises.
 
     ``evaluate`` gives the log probabilities of actions that were taken, the entropy and the likeliest actions, and
     ``policy_gradients`` the gradient of a loss of these two: the parts of a policy-gradient step.
@@ -563,11 +564,15 @@ class TokenPolicy:
         for layer, (codes, scales, _, _) in enumerate(self._codes):
             w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
             quantize_fp8(w, codes, scales, block_rows=128, stream=stream)
-        self._codes_of = self._weight_changes()
+        self._codes_of = self._weights_now(stream)
         return self
 
     def _weight_changes(self):
         return self.mlp.weight_changes, self.optimizer.calls if self.optimizer else 0
+
+    def _weights_now(self, stream):
+        """The weights whose codes a call on ``stream`` has just made; none while it is captured, as nothing has been made yet."""
+        return None if capturing(stream) else self._weight_changes()
 
     def forward_8bit(self, tokens, mask=None, stream=None):
         """``forward`` with the dense layers in 8 bits: activations quantised per row and 128 columns, products of codes (on the
@@ -597,7 +602,7 @@ class TokenPolicy:
         for layer, (codes, scales) in enumerate(self._codes4[1]):
             w = self.mlp.params.view((sizes[layer + 1], sizes[layer]), "f32", self.mlp.offsets[2 * layer] * 4)
             quantize_int4(w, codes, scales, group=group, stream=stream)
-        self._codes4_of = self._weight_changes()
+        self._codes4_of = self._weights_now(stream)
         return self
 
     def forward_4bit(self, tokens, mask=None, stream=None):

@@ -282,3 +282,28 @@ def test_backward_from_logits(gpu, in_dtype, sizes, batch, with_bias):
             assert np.linalg.norm(a - b) <= 2 ** -8 * np.linalg.norm(b) + 1e-9
     with pytest.raises(ValueError):
         net.backward_logits(x, D(np.zeros((batch, sizes[-1] + 1), np.float32)))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_captured_answer_quantises_nothing_before_it_is_replayed(gpu, bits):
+    torch = pytest.importorskip("torch")
+    batch = 16
+    net, tokens, mask, _ = make(np.random.default_rng(8), batch)
+    policy = load(gpu, net, batch)
+    dt, dm = gpu.DeviceArray.from_numpy(tokens), gpu.DeviceArray.from_numpy(mask)
+    quantize, answer = (policy.quantize_4bit, policy.forward_4bit) if bits == 4 else (policy.quantize, policy.forward_8bit)
+    side = torch.cuda.Stream()
+    quantize()
+    old = answer(dt, dm).numpy().copy()
+    answer(dt, dm, stream=side).numpy(stream=side)
+    policy.mlp.load_weights([w[::-1] for w in net["weights"]], net["biases"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        answer(dt, dm, stream=torch.cuda.current_stream())
+    got = answer(dt, dm).numpy().copy()                     # of the new weights, although the graph has not run
+    quantize()
+    want = answer(dt, dm).numpy().copy()
+    assert np.array_equal(got, want) and np.abs(got - old).max() > 1e-3
+    graph.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(policy.mlp.probs.numpy(), want)
