@@ -920,7 +920,8 @@ __global__ void __launch_bounds__(256) log_probs_grad_long_kernel(LogProbGradArg
     const RowShape<T> shape(x, g.cols);
     const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(d)) & 15u) == 0;
     if (first < shape.head + shape.tail) lp_grad_one<T>(r, x, mask, d, shape.single(first), g.cols);
-    for (int j = g.cols + first; j < g.mask_cols; j += stride) d[j] = sb_from_f32<T>(0.f);
+    // (Up to 2^31 - 1 columns: a step behind the last one is beyond 32 bits.)
+    for (long long j = (long long)g.cols + first; j < g.mask_cols; j += stride) d[j] = sb_from_f32<T>(0.f);
     const float ref = fmaf(r.top, c, r.log_sum * LP_LOG2E), rest = fmaf(r.top, c, -ref) + r.log_sum * LP_LOG2E, back = -r.scale * exp2_approx(-rest);
     const float h = back * r.h * (1.f / LP_LOG2E), k = back * fmaf(r.h, -rest * (1.f / LP_LOG2E), r.c);
     // The short way holds where the lifted logits come out as 0 and no product leaves fp32's range: not that of a lifted logit's logarithm, which
@@ -1088,7 +1089,8 @@ int launch_log_probs_grad(const LogProbGradArgs& g, cudaStream_t s) {
   // Enough blocks for the chip where rows are few, each with a batch of packs per thread at least.
   const int batch = 256 * 4 * (16 / (int)sizeof(T));
   long long across = (8LL * sb_sm_count() + g.rows - 1) / g.rows;
-  if (across > (g.mask_cols + batch - 1) / batch) across = (g.mask_cols + batch - 1) / batch;
+  const long long most_across = ((long long)g.mask_cols + batch - 1) / batch;
+  if (across > most_across) across = most_across;
   const dim3 grid((unsigned)across, (unsigned)(g.rows < 65535 ? g.rows : 65535));
   if (g.mask) SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, true, 256>, grid, dim3(256), 0, s, 1, g));
   else SB_CUDA(sb_launch(log_probs_grad_long_kernel<T, false, 256>, grid, dim3(256), 0, s, 1, g));

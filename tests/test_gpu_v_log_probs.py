@@ -443,3 +443,29 @@ def test_gradients_of_large_entropies_weights_where_logits_are_forbidden_by_valu
     dlogits = torch.full_like(logits, 7.0)           # other columns' gradients may be beyond f16, which the definition in 64 bits does not know
     gpu.primitives.log_probs_grad(logits, tokens, stats, dlogits, dout=dout, dentropy=weight * dentropy, entropy=entropy, scale=scale)
     assert not dlogits[mask == 0].any() and not torch.isnan(dlogits).any()
+
+
+def test_the_longest_row(gpu):
+    """2^31 - 1 columns, and a prefix of them: no step of the loops leaves 32 bits."""
+    torch = _torch()
+    cols = 2 ** 31 - 1
+    logits = torch.zeros((1, cols), dtype=torch.float16, device="cuda")
+    logits[0, cols - 1], logits[0, cols - 9], logits[0, 1] = 3.0, 4.0, 4.0
+    tokens = torch.full((1,), cols - 1, dtype=torch.int32, device="cuda")
+    out, entropy, stats = torch.zeros(1, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros((1, 2), device="cuda")
+    top, places = torch.zeros((1, 4), device="cuda"), torch.zeros((1, 4), dtype=torch.int32, device="cuda")
+    gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats, top=top, top_tokens=places)
+    total = math.log(cols - 3 + 2 * math.exp(4.0) + math.exp(3.0))
+    # Sums of a thread: 2^31 / 2^12 equal terms, each addition off by half a last place of a sum of up to 2^19 terms; relative 2^-24 * 2^19 / 2 at the
+    # very most, were all of them in one direction: 2^-6, and its logarithm as much.
+    assert abs(float(out[0]) - (3.0 - total)) < 2.0 ** -6 and abs(float(entropy[0]) - total) < 2.0 ** -5
+    assert places[0].tolist() == [1, cols - 9, cols - 1, 0]
+    prefix, ones = 1000, torch.ones(1, device="cuda")
+    dlogits = torch.full_like(logits, 7.0)
+    gpu.primitives.log_probs(logits, tokens, out, entropy=entropy, stats=stats, prefix=prefix)
+    gpu.primitives.log_probs_grad(logits, tokens, stats, dlogits, dout=ones, dentropy=ones, entropy=entropy, prefix=prefix)
+    assert not dlogits[0, prefix:].any()
+    # The token is not legal: its dout is in all columns by their probabilities, and has none of its own.
+    lp = torch.log_softmax(logits[0, :prefix].double(), 0)
+    want = -torch.exp(lp) * (1.0 + lp - (torch.exp(lp) * lp).sum())
+    same(dlogits[0, :prefix], want, (ROUND["f16"] + 2.0 ** -17) * want.abs() + 2.0 ** -20 * torch.exp(lp) + LEAST["f16"])
