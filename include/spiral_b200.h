@@ -580,7 +580,7 @@ int sb_log_probs_grad(const void* logits, long long ld, int dtype, long long row
  * gradient; SB_BF16 or SB_F16, the same for all, fp32 sums, each output rounded once.  Rows of x and w that start on
  * 16 bytes run on the tensor cores, others on the CUDA cores at about 1 % of their rate.  f and k of at most 2^21, m of at most
  * 2^30.  No output may be one of the inputs. */
-enum { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* g (1 + erf(g / sqrt 2)) / 2 */, SB_ACT_RELU = 2 };
+enum { SB_ACT_SILU = 0, SB_ACT_GELU = 1 /* g (1 + erf(g / sqrt 2)) / 2 */, SB_ACT_RELU = 2, SB_GATED_EXACT = 16 /* of sb_gated_grad */ };
 int sb_gated(const void* x, long long ldx, const void* w, long long ldw, void* h, long long ldh, void* saved, long long lds, int m, int f,
              int k, int dtype, int activation, void* stream);
 /* The tiles that sb_gated takes for rows of x and w that start on 16 bytes: plan = {rows, columns of h, tiles, tiles of half the columns behind
@@ -589,11 +589,13 @@ int sb_gated_plan(int m, int f, int k, int* plan);
 /* Its gradient from dh [m, f] and what was saved:
  *   dg = dh u act'(g)   du = dh act(g)   dx = [dg du] w   dw = [dg du]^T x
  * dx [m, k] in the storage type, dw [2 f, k] in the storage type or SB_F32, each NULL where it is not wanted; accumulate != 0 adds to
- * the old dw.  dg and du are rounded to the storage type for the products (up to 64 rows and rows on 16 bytes: to two numbers of it),
- * whose sums are fp32 in a fixed order.  workspace:
- * 256-byte aligned, at least sb_gated_grad_workspace_bytes.  dx may not be w, nor dw x.  Both products run at once: where both are wanted dx may
+ * the old dw.  dg and du are rounded to the storage type for the products, whose sums are fp32 in a fixed order: that is as large an error as
+ * the rounding of a 16-bit gradient itself, and all of that of a dw in SB_F32.  Up to 64 rows, and with SB_GATED_EXACT beside the activation for any
+ * number, what their rounding leaves off is multiplied too, and the gradients are as near as products of fp32 (with many rows at about twice the
+ * time).  workspace: 256-byte aligned, at least sb_gated_grad_workspace_bytes, with SB_GATED_EXACT sb_gated_grad_exact_workspace_bytes.  dx may not be w, nor dw x.  Both products run at once: where both are wanted dx may
  * not be x either, nor dw w. */
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes);
+int sb_gated_grad_exact_workspace_bytes(int m, int f, int k, size_t* bytes);
 /* The tiles of its products where rows start on 16 bytes (which: 1 dx, 2 dw, 3 both): plan = {columns, and for dx and then dw: tiles of all K, tiles in
  * parts of K, parts}; tiles have 256 rows. */
 int sb_gated_grad_plan(int m, int f, int k, int which, int* plan);

@@ -62,15 +62,18 @@ __device__ __forceinline__ float2 gated_act_grad(float g) {
 // Any sizes, pitches and alignments, on the CUDA cores: 64 x 64 outputs per block, 16 of K at a time.
 constexpr int GS_TILE = 64, GS_K = 16;
 
-// A matrix by the distances of neighbours in a column and in a row.
+// A matrix by the distances of neighbours in a column and in a row; `lo`: what its rounding left off, laid out the same, where that is kept.
 struct Strided {
   const void* p;
   long long down, across;
+  const void* lo;
 };
 
 template <typename T>
 __device__ __forceinline__ float strided_at(const Strided& m, long long i, long long j) {
-  return sb_to_f32<T>(reinterpret_cast<const T*>(m.p)[i * m.down + j * m.across]);
+  const long long at = i * m.down + j * m.across;
+  const float v = sb_to_f32<T>(reinterpret_cast<const T*>(m.p)[at]);
+  return m.lo ? v + sb_to_f32<T>(reinterpret_cast<const T*>(m.lo)[at]) : v;
 }
 
 template <typename T>
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(256) gated_simple_kernel(GatedArgs p) {
   sb_grid_dependents_launch();
   const long long i0 = (long long)blockIdx.x * GS_TILE, j0 = (long long)blockIdx.y * GS_TILE;
   const int ti = threadIdx.x / 16 * 4, tj = threadIdx.x % 16 * 4;
-  const Strided x = {p.x, p.ldx, 1}, g = {p.w, p.ldw, 1}, u = {reinterpret_cast<const T*>(p.w) + (long long)p.f * p.ldw, p.ldw, 1};
+  const Strided x = {p.x, p.ldx, 1, nullptr}, g = {p.w, p.ldw, 1, nullptr}, u = {reinterpret_cast<const T*>(p.w) + (long long)p.f * p.ldw, p.ldw, 1, nullptr};
   float ag[4][4] = {}, au[4][4] = {};
   for (long long k0 = 0; k0 < p.k; k0 += GS_K) {
     simple_tile<T>(sx, x, i0, k0, p.m, p.k, false);
@@ -1178,9 +1181,9 @@ int gated_grad_products(const GatedGradArgs& g, const GatedGradOut& o, cudaStrea
   const bool fast_dx = dx && f2 > 0 && gated_rows16(o.w, o.ldw, CODE), fast_dw = dw && g.m > 0 && gated_rows16(o.x, g.m == 1 ? 8 : o.ldx, CODE);
   int rc = SB_OK;
   if (fast_dx || fast_dw) rc = launch_gated_products<T>(g, o, fast_dx, fast_dw, s);
-  if (rc == SB_OK && dx && !fast_dx) rc = launch_product_simple<T, T>({g.d, g.ldd, 1}, {o.w, 1, o.ldw}, o.dx, o.lddx, g.m, o.k, f2, 0, s);
+  if (rc == SB_OK && dx && !fast_dx) rc = launch_product_simple<T, T>({g.d, g.ldd, 1, g.lo}, {o.w, 1, o.ldw, nullptr}, o.dx, o.lddx, g.m, o.k, f2, 0, s);
   if (rc != SB_OK || !dw || fast_dw) return rc;
-  const Strided a = {g.d, 1, g.ldd}, b = {o.x, 1, o.ldx};
+  const Strided a = {g.d, 1, g.ldd, g.lo}, b = {o.x, 1, o.ldx, nullptr};
   return o.dw_dtype == SB_F32 ? launch_product_simple<T, float>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s)
                               : launch_product_simple<T, T>(a, b, o.dw, o.lddw, f2, o.k, g.m, o.accumulate, s);
 }
@@ -1189,9 +1192,24 @@ int gated_grad_products(const GatedGradArgs& g, const GatedGradOut& o, cudaStrea
 long long gated_grad_pitch(int f) { return (2LL * f + 7) / 8 * 8; }
 // Rounding dg and du to 16 bits adds as much to the error of a gradient as rounding that itself does: sqrt(2) of it in all.  With few rows, whose few
 // values of dg and du need not average, it was up to twice: there what their rounding left off is kept too and multiplied beside them, at the time of
-// the launches (64 rows at most: no more than one block of K more for dw, and every block of w twice, the second time from L2).
-int gated_grad_twice(int m) { return m <= 64 ? 1 : 0; }
-size_t gated_grad_first(int m, int f) { return (((size_t)m << gated_grad_twice(m)) * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
+// the launches (64 rows at most: no more than one block of K more for dw, and every block of w twice, the second time from L2).  With more rows it
+// takes as long again as the products themselves, and is the caller's choice.
+int gated_grad_twice(int m, bool exact) { return m <= 64 || exact ? 1 : 0; }
+size_t gated_grad_first(int m, int f, bool exact) { return (((size_t)m << gated_grad_twice(m, exact)) * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
+
+int gated_grad_bytes(const char* who, int m, int f, int k, bool exact, size_t* bytes) {
+  if (!bytes) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
+  if (m < 0 || f < 0 || k < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
+  long long most = 0;                             // of both products or either
+  for (int want = 1; want < 4; ++want) {
+    const ProductSize size[2] = {{want & 1 ? m : 0, k, 2LL * f}, {want & 2 ? 2LL * f : 0, k, m}};
+    ProductsPlan q;
+    const long long parts = m > 0 && f > 0 && k > 0 ? gated_products_plan(size, gated_grad_twice(m, exact), &q) : 0;
+    if (parts > most) most = parts;
+  }
+  *bytes = gated_grad_first(m, f, exact) + (size_t)most;
+  return SB_OK;
+}
 
 }  // namespace
 
@@ -1241,7 +1259,7 @@ int sb_gated_grad_plan(int m, int f, int k, int which, int* plan) {
   const ProductSize size[2] = {{which & 1 ? m : 0, k, 2LL * f}, {which & 2 ? 2LL * f : 0, k, m}};
   ProductsPlan q;
   memset(&q, 0, sizeof(q));
-  gated_products_plan(size, gated_grad_twice(m), &q);
+  gated_products_plan(size, gated_grad_twice(m, false), &q);
   plan[0] = q.bn;
   for (int i = 0; i < 2; ++i) {
     plan[1 + 3 * i] = q.p[i].whole;
@@ -1252,24 +1270,19 @@ int sb_gated_grad_plan(int m, int f, int k, int which, int* plan) {
 }
 
 int sb_gated_grad_workspace_bytes(int m, int f, int k, size_t* bytes) {
-  const char* who = "sb_gated_grad_workspace_bytes";
-  if (!bytes) return sb_fail(SB_ERR_BAD_ARG, "%s: null output", who);
-  if (m < 0 || f < 0 || k < 0) return sb_fail(SB_ERR_BAD_ARG, "%s: negative size", who);
-  long long most = 0;                             // of both products or either
-  for (int want = 1; want < 4; ++want) {
-    const ProductSize size[2] = {{want & 1 ? m : 0, k, 2LL * f}, {want & 2 ? 2LL * f : 0, k, m}};
-    ProductsPlan q;
-    const long long parts = m > 0 && f > 0 && k > 0 ? gated_products_plan(size, gated_grad_twice(m), &q) : 0;
-    if (parts > most) most = parts;
-  }
-  *bytes = gated_grad_first(m, f) + (size_t)most;
-  return SB_OK;
+  return gated_grad_bytes("sb_gated_grad_workspace_bytes", m, f, k, false, bytes);
+}
+
+int sb_gated_grad_exact_workspace_bytes(int m, int f, int k, size_t* bytes) {
+  return gated_grad_bytes("sb_gated_grad_exact_workspace_bytes", m, f, k, true, bytes);
 }
 
 int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, const void* w, long long ldw, const void* saved, long long lds,
                   void* dx, long long lddx, void* dw, long long lddw, int dw_dtype, int accumulate, int m, int f, int k, int dtype,
                   int activation, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "sb_gated_grad";
+  const bool exact = (activation & SB_GATED_EXACT) != 0;
+  activation &= ~SB_GATED_EXACT;
   int rc = gated_args_ok(who, m, f, k, dtype, activation);
   if (rc != SB_OK) return rc;
   if (dw && dw_dtype != dtype && dw_dtype != SB_F32) return sb_fail(SB_ERR_UNSUPPORTED, "%s: dw holds f32 or the storage type (got %d)", who, dw_dtype);
@@ -1287,12 +1300,12 @@ int sb_gated_grad(const void* dh, long long lddh, const void* x, long long ldx, 
       !gated_element_aligned(dx, dtype) || (dw && !gated_element_aligned(dw, dw_dtype)) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
     return sb_fail(SB_ERR_MISALIGNED, "%s: a pointer is not aligned to its element size, or the workspace not to 256 bytes", who);
   size_t need = 0;
-  if ((rc = sb_gated_grad_workspace_bytes(m, f, k, &need)) != SB_OK) return rc;
+  if ((rc = gated_grad_bytes(who, m, f, k, exact, &need)) != SB_OK) return rc;
   if (any && workspace_bytes < need) return sb_fail(SB_ERR_BAD_ARG, "%s: the workspace has %zu bytes, %zu are needed", who, workspace_bytes, need);
   if (!dx && !dw) return SB_OK;
-  char* const lo = gated_grad_twice(m) ? reinterpret_cast<char*>(workspace) + (size_t)m * (size_t)gated_grad_pitch(f) * 2 : nullptr;
+  char* const lo = gated_grad_twice(m, exact) ? reinterpret_cast<char*>(workspace) + (size_t)m * (size_t)gated_grad_pitch(f) * 2 : nullptr;
   const GatedGradArgs g = {dh, saved, workspace, lo, lddh, lds, gated_grad_pitch(f), m, f};
-  const GatedGradOut o = {x, w, dx, dw, ldx, ldw, lddx, lddw, dw_dtype, accumulate, k, reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + gated_grad_first(m, f))};
+  const GatedGradOut o = {x, w, dx, dw, ldx, ldw, lddx, lddw, dw_dtype, accumulate, k, reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + gated_grad_first(m, f, exact))};
   cudaStream_t s = (cudaStream_t)stream;
 #define SB_GATED_CALL(ACT) (dtype == SB_BF16 ? launch_gated_act_grad<__nv_bfloat16, ACT>(g, s) : launch_gated_act_grad<__half, ACT>(g, s))
   if (any) rc = activation == SB_ACT_SILU ? SB_GATED_CALL(ACT_SILU) : activation == SB_ACT_GELU ? SB_GATED_CALL(ACT_GELU) : SB_GATED_CALL(ACT_RELU);

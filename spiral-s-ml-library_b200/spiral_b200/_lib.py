@@ -28,6 +28,7 @@ EPI_SAMPLE, EPI_BINARIZE, EPI_LN_L2 = 512, 1024, 2048
 
 # activations of a gated layer
 ACT_SILU, ACT_GELU, ACT_RELU = 0, 1, 2
+GATED_EXACT = 16
 
 
 class HeadSpec(ctypes.Structure):
@@ -177,6 +178,7 @@ SIGNATURES = {
     "sb_gated_plan": (_I, [_I, _I, _I, _IP]),
     "sb_gated_grad_plan": (_I, [_I, _I, _I, _I, _IP]),
     "sb_gated_grad_workspace_bytes": (_I, [_I, _I, _I, POINTER(c_size_t)]),
+    "sb_gated_grad_exact_workspace_bytes": (_I, [_I, _I, _I, POINTER(c_size_t)]),
     "sb_gated_grad": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "sb_quantize_int4": (_I, [_P, _L, _I, _L, _I, _I, _P, _L, _P, _I, _P]),
     "sb_dequantize_int4": (_I, [_P, _L, _P, _I, _P, _L, _I, _L, _I, _I, _P]),

@@ -257,10 +257,12 @@ def gated(x, w, out, activation="silu", saved=None, stream=None):
     return out
 
 
-def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulate=False, workspace=None, stream=None):
+def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulate=False, workspace=None, stream=None, exact=False):
     """Gradient of ``gated`` from ``dout`` [m, f] and what it ``saved``: ``dx`` (like ``x``) and ``dw`` (like ``w``, or fp32), each where given;
-    ``accumulate`` adds to the old ``dw``.  ``workspace``: device memory of ``gated_grad_workspace`` bytes; by default one is kept per device,
-    stream and host thread.  ``dx`` may not be ``w``, nor ``dw`` ``x``; where both are wanted ``dx`` may not be ``x`` either, nor ``dw`` ``w``.
+    ``accumulate`` adds to the old ``dw``.  The projections' gradients are rounded to the storage type for the products, which is as large an error
+    as the rounding of a 16-bit gradient itself and all of that of an fp32 ``dw``; up to 64 rows, and with ``exact`` for any number, what that
+    rounding leaves off is multiplied too (with many rows at about twice the time).  ``workspace``: device memory of ``gated_grad_workspace`` bytes; by
+    default one is kept per device, stream and host thread.  ``dx`` may not be ``w``, nor ``dw`` ``x``; where both are wanted ``dx`` may not be ``x`` either, nor ``dw`` ``w``.
     Returns (dx, dw)."""
     m, f, k, x, ldx, w, ldw, tag, act = _gated_sizes("gated_grad", x, w, activation)
     dh, lddh = _gated_matrix("gated_grad", dout, "dout", tag, m, f)
@@ -274,7 +276,8 @@ def gated_grad(dout, x, w, saved, dx=None, dw=None, activation="silu", accumulat
             raise TypeError("gated_grad: dw must hold %s or f32, not %s" % (tag, dw_tag))
         if rows != 2 * f or cols != k:
             raise ValueError("gated_grad: dw must be like w, %dx%d" % (2 * f, k))
-    nbytes = gated_grad_workspace(m, f, k) if workspace is None else nbytes_of(workspace)
+    nbytes = gated_grad_workspace(m, f, k, exact) if workspace is None else nbytes_of(workspace)
+    act |= _lib.GATED_EXACT if exact else 0
     if workspace is None:
         workspace = stream_workspace(nbytes, stream)
     _lib.call("sb_gated_grad", dh, lddh, x, ldx, w, ldw, saved, lds, dx_ptr, lddx, dw_ptr, lddw, _GATED.get(dw_tag, _lib.F32),
@@ -298,10 +301,10 @@ def gated_grad_plan(m, f, k, dx=True, dw=True):
     return {"columns": plan[0], "dx": tuple(plan[1:4]), "dw": tuple(plan[4:7])}
 
 
-def gated_grad_workspace(m, f, k):
+def gated_grad_workspace(m, f, k, exact=False):
     """Bytes of device memory that ``gated_grad`` needs for m rows and a [2 f, k] weight matrix."""
     nbytes = ctypes.c_size_t(0)
-    _lib.call("sb_gated_grad_workspace_bytes", m, f, k, ctypes.byref(nbytes))
+    _lib.call("sb_gated_grad_exact_workspace_bytes" if exact else "sb_gated_grad_workspace_bytes", m, f, k, ctypes.byref(nbytes))
     return nbytes.value
 
 

@@ -421,3 +421,32 @@ def test_gates_beyond_f16(gpu, m, kind):
     want = check_grad(gpu, dout, x, w, kept, "f16", kind)
     got = gpu.gated_grad(dout, x, w, saved, dx=torch.zeros_like(x), dw=torch.zeros_like(w), activation=kind)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kind", ACTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m,f,k", [(1, 64, 64), (64, 200, 136), (65, 200, 136), (300, 264, 1000), (5000, 72, 64), (4001, 3000, 1000), (2050, 1032, 264), (5, 33, 41), (300, 65, 67)])
+def test_exact_gradients(gpu, m, f, k, dtype, kind):
+    """With ``exact`` the gradients are off by their own rounding and by next to nothing else, for any number of rows and any alignment; a dw in fp32
+    has none of the storage type's rounding."""
+    torch = _torch()
+    x, w = inputs(m, f, k, dtype, 3)
+    saved = (x.float() @ w.float().t()).to(x.dtype)
+    dout = torch.randn((m, f), generator=generator(4), device="cuda").to(x.dtype)
+    g, u = saved.double().chunk(2, 1)
+    d, wide = dout.double(), torch.cat([dout.double(), dout.double()], 1)
+    exact = torch.cat([d * u * act_grad(kind, g), d * act(kind, g)], 1)
+    # As for few rows: the activation's error, the rounding of the second number, and in f16 what lies below its least number.
+    slack = act_error(torch.cat([g, g], 1)) * wide.abs() * torch.cat([u.abs(), torch.ones_like(u)], 1) + (ROUND[dtype] ** 2 + 2.0 ** -23) * exact.abs() + LEAST[dtype]
+    need = gpu.gated_grad_workspace(m, f, k, exact=True)
+    assert need >= 8 * m * f and (need > gpu.gated_grad_workspace(m, f, k) or m <= 64)
+    for dw_type, accumulate, workspace in ((dtype, False, None), ("f32", True, torch.empty(need, dtype=torch.uint8, device="cuda"))):
+        dx, dw = torch.full_like(x, 7.0), torch.full_like(w, 0.5, dtype=dtype_of(dw_type))
+        gpu.gated_grad(dout, x, w, saved, dx=dx, dw=dw, activation=kind, accumulate=accumulate, exact=True, workspace=workspace)
+        again = gpu.gated_grad(dout, x, w, saved, dx=torch.empty_like(x), activation=kind, exact=True)[0]
+        assert torch.equal(dx, again) or f * k > 100000           # one product alone may be cut along K in another way
+        old = 0.5 if accumulate else 0.0
+        for got, want, size, off, name in ((dx, exact @ w.double(), exact.abs() @ w.double().abs(), slack @ w.double().abs(), dtype),
+                                           (dw, exact.t() @ x.double() + old, exact.abs().t() @ x.double().abs() + old, slack.t() @ x.double().abs(), dw_type)):
+            tol = size * product_error(4 * f if got is dx else 2 * m) + off
+            within(got, want, tol + ROUND[name] * (want.abs() + tol) + LEAST[name])

@@ -256,3 +256,16 @@ def test_log_probs_in_the_place_of_what_they_are_made_from(sb):
             refused(sb, BAD, "sb_log_probs", 0x1000, 8, 0, 4, 8, 0x8000, -1, 1.0, 0x2000, 4, out, h, stats, 2, values, places, None)
     for d, ldd in ((0x1000, 16), (0x2000, 8), (0x3000, 8), (0x4000, 8), (0x5000, 8), (0x6000, 8), (0x8000, 8)):
         refused(sb, BAD, "sb_log_probs_grad", 0x1000, 8, 2, 4, 8, 0x8000, -1, 1.0, 0x2000, 4, 0x3000, 0x4000, 0x5000, 0x6000, d, ldd, None)
+
+
+def test_workspaces_of_exact_gradients(sb):
+    from spiral_b200 import _lib
+    need, exact = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _lib.call("sb_gated_grad_workspace_bytes", 1000, 64, 32, ctypes.byref(need))
+    _lib.call("sb_gated_grad_exact_workspace_bytes", 1000, 64, 32, ctypes.byref(exact))
+    assert exact.value >= need.value + 1000 * 128 * 2 and sb.gated_grad_workspace(1000, 64, 32, exact=True) == exact.value
+    refused(sb, BAD, "sb_gated_grad_exact_workspace_bytes", 1, -1, 1, ctypes.byref(need))
+    args = [0x1000000, 64, 0x2000000, 32, 0x3000000, 32, 0x4000000, 128, 0x5000000, 32, 0x6000000, 32, 2, 0, 1000, 64, 32, 2]
+    refused(sb, BAD, "sb_gated_grad", *args, _lib.GATED_EXACT, 0x10000000, exact.value - 1, None)
+    refused(sb, UNSUPPORTED, "sb_gated_grad", *args, 32, 0x10000000, exact.value, None)
+    refused(sb, UNSUPPORTED, "sb_gated", 0x1000, 16, 0x2000, 16, 0x3000, 8, None, 16, 4, 8, 16, 2, _lib.GATED_EXACT, None)
