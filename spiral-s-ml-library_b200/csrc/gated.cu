@@ -166,9 +166,9 @@ __global__ void __launch_bounds__(256) gated_product_simple_kernel(Strided a, St
 // gate's and beside them the other projection's, from one sequence of MMAs with N = 2 bf whose B operand is bf rows of each half of w: in
 // a pair the leader brings the gate's and its peer the other's.  The epilogue finds both values of an output in one TMEM lane.
 //   warp 0: TMA of x      warp 10: TMA of w      warp 1: MMAs      warps 2 .. 9: epilogue, two per lane quadrant on alternate 32-column chunks
-// Two accumulators let the epilogue of a tile run beside the MMAs of the next.  Bound by the tensor cores where rows are on 32 bytes: 16384 x 4096 x
-// 1024 210 us in short bursts, 1.3 PFLOP/s (249 under the power cap), 4001 x 3000 x 1024 51; rows of 2000 bytes, whose pieces of 128 lie in five
-// sectors of L2 each, take 62 to 66 for 4001 x 3000 x 1000.
+// Two accumulators let the epilogue of a tile run beside the MMAs of the next.  Bound by the tensor cores where rows are on 32 bytes; calls one after
+// the other, all with saved: 16384 x 4096 x 1024 (silu) 233 to 249 us, 1.1 to 1.2 PFLOP/s under the power cap, 4001 x 3000 x 1024 (gelu) 52 to 58.
+// Rows of 2000 bytes, whose pieces of 128 lie in five sectors of L2 each, take 61 to 71 for 4001 x 3000 x 1000.
 constexpr int GU_EPI_WARPS = 8;
 constexpr int GU_THREADS = 96 + 32 * GU_EPI_WARPS;
 constexpr int GU_MAX_STAGES = 8;
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(GU_THREADS, 1) gated_umma_kernel(const __grid_
 
 // ---- few rows --------------------------------------------------------------------------------------------------
 // Up to 8 NT rows: a block has 16 columns of h, 16 rows of each half of w, and its eight warps share K, UNROLL blocks of 32 on their way at a
-// time.  Their sums are joined in the order of the warps.  1 x 4096 x 1024: 3.7 us, of which the 16.8 MB of weights take 2.6.
+// time.  Their sums are joined in the order of the warps.  1 x 4096 x 1024: 3.3 to 3.7 us, of which the 16.8 MB of weights take 2.6.
 constexpr int GF_ROWS = 16, GF_WARPS = 8;
 constexpr long long GF_NO_END = 1LL << 60;
 
@@ -596,8 +596,9 @@ __global__ void __launch_bounds__(256) gated_act_grad_kernel(GatedGradArgs p) {
 // dx = d w (d [m, 2 f], w [2 f, k]) and dw (+)= d^T x in one persistent launch of pairs of CTAs on tiles of 256 x bn, 128 of K per stage.  B has
 // rows of K in both; A does in dw alone.  As many tiles as fill the workers are whole; the rest are cut into parts of K, which leave fp32 sums for
 // the launch that joins them: one wave of short parts where two launches would have had a wave of few tiles each.  Bound by the tensor cores: 0.78 us
-// per 128 of K and 256 x 256 sums, 1.6 PFLOP/s over the card.  With the launch before and the join, against a launch for each product with K cut
-// there (us): 8192 x 4096 x 1024 249 -> 230, 4001 x 3000 x 1000 122 -> 110, 2048^3 73 -> 65, 4096 x 512 x 2048 62 -> 44, 4096 x 2048 x 512 88 -> 50,
+// per 128 of K and 256 x 256 sums, 1.6 PFLOP/s over the card.  With the launch before and the join one call after the other under the power cap: 8192 x
+// 4096 x 1024 279 to 305 us, 4001 x 3000 x 1000 122 to 129, 2048^3 59.  Against a launch for each product with K cut there, single launches at the
+// full clock (in series the largest gains nothing): 8192 x 4096 x 1024 249 -> 230, 4001 x 3000 x 1000 122 -> 110, 2048^3 73 -> 65, 4096 x 512 x 2048 62 -> 44, 4096 x 2048 x 512 88 -> 50,
 // 512^3 24 -> 17, 65536 x 256 x 216 87 -> 89, 128 x 4096 x 1024 35 -> 35.
 //   warp 0: TMA of A      warp 10: TMA of B      warp 1: MMAs      warps 2 .. 9: epilogue, as above
 constexpr int GP_BOX = 32 * 128;                // 32 rows of 32 fp32 columns on their way to memory
@@ -1193,7 +1194,8 @@ long long gated_grad_pitch(int f) { return (2LL * f + 7) / 8 * 8; }
 // Rounding dg and du to 16 bits adds as much to the error of a gradient as rounding that itself does: sqrt(2) of it in all.  With few rows, whose few
 // values of dg and du need not average, it was up to twice: there what their rounding left off is kept too and multiplied beside them, at the time of
 // the launches (64 rows at most: no more than one block of K more for dw, and every block of w twice, the second time from L2).  With more rows it
-// takes as long again as the products themselves, and is the caller's choice.
+// takes as long again as the products themselves, and is the caller's choice: 8192 x 4096 x 1024 281 -> 518 us, 4001 x 3000 x 1000 122 -> 220, 128 x
+// 4096 x 1024 25 -> 31; errors 0.0023 -> 0.0017 in bf16, 0.00029 -> 0.00021 in f16, and of an fp32 dw 0.0017 -> 0.00002.
 int gated_grad_twice(int m, bool exact) { return m <= 64 || exact ? 1 : 0; }
 size_t gated_grad_first(int m, int f, bool exact) { return (((size_t)m << gated_grad_twice(m, exact)) * (size_t)gated_grad_pitch(f) * 2 + 255) / 256 * 256; }
 

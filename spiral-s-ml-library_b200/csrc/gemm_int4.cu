@@ -24,7 +24,8 @@ struct QuantInt4Args {
   int k, group;
 };
 
-// One warp per group: the largest magnitude becomes 7 steps.
+// One warp per group: the largest magnitude becomes 7 steps.  Single elements and bytes: 4096 x 4096 from fp32 in groups of 128 41 us, where the bytes
+// take 12; 512 x 1024 3.2.
 template <typename T, typename S>
 __global__ void __launch_bounds__(256) quantize_int4_kernel(QuantInt4Args p) {
   sb_grid_dependency_wait();
@@ -63,6 +64,7 @@ struct Int4Args {
   int m, n, k, group, relu, out_dtype;
 };
 
+// A byte per thread: 4096 x 4096 to fp32 38 us, where the bytes take 12.
 template <typename S, typename Out>
 __global__ void __launch_bounds__(256) dequantize_int4_kernel(const uint8_t* codes, long long ldw, const S* scales, Out* out, long long ldo, long long n, int k, int group) {
   sb_grid_dependency_wait();
@@ -202,8 +204,9 @@ __device__ __noinline__ void int4_ask_narrow(uint32_t to, const uint8_t* lane_fr
 // A warp has 16 rows of w, whose codes come to it through a ring of STAGES steps in shared memory; a block's warps share up to 8 NT
 // rows of a there, and the blocks of a cluster share K.  The V = G / 32 words of a lane (8 codes each) are of one group in all four lanes
 // of a row, so the products of a group are summed as whole numbers times elements of a, and the sums are scaled.  The blocks' sums are
-// joined in their order.  Bound by its instructions, some 17 per lane and 8 codes, and by the way to the first and from the last of them: 16 x 8192 x
-// 8192 in groups of 64 17.7 us (issue 50 %), where the bytes take 5.5; 1 x 8192 x 8192 in groups of 128 11.7.
+// joined in their order.  Bound by its instructions, 34 per lane and 8 codes for 16 rows of a (nine of them unpack), and by the way to the first and from
+// the last of them: 16 x 8192 x 8192 in groups of 64 17.4 us (issue 50 %), where the bytes take 5.5; 1 x 8192 x 8192 in groups of 128 11.  At 128
+// registers the forms of 16, 32 and 64 rows of a spill some 10, 50 and 170 bytes a thread.
 template <typename T, int G, int NT, int WARPS, int STAGES>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) gemm_int4_kernel(Int4Args p, Int4Few q) {
   constexpr int V = G / 32, PER = I4_STEP / G, COLS = 8 * NT, PITCH = COLS + 2, ROWS = 16 * WARPS;
@@ -485,7 +488,7 @@ Int4Form int4_form(long long m, long long n, int k, int group, int code_piece, b
   if (m <= 8 && k <= 4096 && n <= 32 * sms && k % group == 0 && code_piece >= group / 8 && whole_rows) return {0, 1};
   // Where all blocks run at once (or, of 16 rows, nearly), fewer rows of a in each and more blocks: 48 x 201 x 12728 with 64 / 16 / 8 rows of a in a
   // block 53 / 20.5 / 12.2 us, 64 x 1024 x 1024 15.1 / 6.5 / 5.6, 64 x 2048 x 2048 15.6 / 8.0 / 8.8, 64 x 4096 x 4096 32 / 18.6 / 23, 16 x 3000 x 6000
-  // 9.9 (16) / 14.1; larger ones read their weights again for nothing: 32 x 8192 x 8192 30 (32) / 33 / 43.
+  // 9.9 (16) / 14.1.  At the rule's border 32 x 8192 x 8192 with 32 / 16 / 8 rows takes 32.5 / 32.3 / 49, behind it 48 x 8192 x 8192 with 64 / 16 58 / 60.
   const long long shares = k >= 2048 ? 8 : k >= 1024 ? 4 : k >= 512 ? 2 : 1;
   int rows = m <= 32 ? 32 : 64;
   if (m <= 8 || (n + 127) / 128 * ((m + 7) / 8) * shares <= 2 * sms) rows = 8;

@@ -485,7 +485,7 @@ __device__ __forceinline__ void lp_rank(unsigned long long* candidates, int n, u
 // Alternatives: the top-th largest of the threads' own largest logits is a bound that `top` logits at least reach and few others do.  Only
 // the threads that reach it hold alternatives; the block reads their share of the row once more, from L2, and ranks what reaches
 // the bound.  Rows with more of those than there is room for (long runs of equal logits) find them one after the other.
-// 4096 x 50001 in bf16 with 8 alternatives: 101 to 107 us where the bytes take 62.5; without alternatives 80, bound by the exponentials' unit (60 % busy)
+// 4096 x 50001 in bf16 with 8 alternatives: 97 to 107 us where the bytes take 62.5; without alternatives 80 to 82, bound by the exponentials' unit (60 % busy)
 // and the issue (57 %) as much as by memory.
 template <typename T, int NT, bool MASKED, bool CLUSTER>
 __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 1280 / NT) log_probs_long_kernel(LogProbArgs g) {
