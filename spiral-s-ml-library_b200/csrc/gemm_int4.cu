@@ -97,7 +97,7 @@ __device__ __forceinline__ uint32_t int4_pick(uint32_t w, uint32_t mask, uint32_
 }
 // Eight codes as four pairs of 16-bit numbers q - 8, (0, 4), (1, 5), (2, 6), (3, 7): with the bits of 1024 (f16) or 128 (bf16) above them a
 // code is the number 1024 + q or 128 + q, from which 1032 or 136 is taken without rounding.  Four bits further up, where f16 has room for
-// them, it is 1024 + 16 q.
+// them, it is 1024 + 16 q.  (A common way to unpack whole numbers: it follows from where the formats keep their last bit.)
 template <typename T>
 __device__ __forceinline__ void int4_pairs(uint32_t w, uint32_t* out) {
   if constexpr (std::is_same<T, __half>::value) {

@@ -416,7 +416,8 @@ class TokenPolicy:
     ``evaluate`` gives the log probabilities of actions that were taken, the entropy and the likeliest actions, and
     ``policy_gradients`` the gradient of a loss of these two: the parts of a policy-gradient step.
 
-    ``gated``: the columns, a multiple of 8, of a gated layer (``activation``) between the normalisation and the MLP, none by default.
+    ``gated``: the columns, a multiple of 8, of a gated layer (``activation``) between the normalisation and the MLP, none by default.  Its
+    products run on the tensor cores where ``n_tokens * dim`` is a multiple of 8, else on the CUDA cores at about 1 % of their rate.
 
     Buffers: ``table`` fp32 [vocab, dim], ``norm_weight`` and ``norm_bias`` fp32 [n_tokens * dim], ``gated_weight`` fp32 [2 * gated,
     n_tokens * dim], ``mlp.params``; all are stepped by one ``AdamW`` (``optimizer``, states in fp32 or 'e4m3')."""
